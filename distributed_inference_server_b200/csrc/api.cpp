@@ -297,6 +297,91 @@ int dis_k_attn_prefill(const uint16_t *q, const uint16_t *kv_pool, int64_t n_pag
 int dis_k_attn_prefill_block_tokens(int32_t n_heads, int32_t n_kv, int32_t d) {
   return dis::attn_prefill_block_tokens(n_heads, n_kv, d);
 }
+
+// What the calls on 8-bit pages and on shared prefixes ask of their arguments, beyond pointers; 0 or the refusal's code
+static int cache_shape(const char *who, int T, int n_heads, int n_kv, int d, int page_size, int max_pages) {
+  const char *what = nullptr;
+  const int G = n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0 ? n_heads / n_kv : 0;
+  if (T < 0) what = "a negative number of rows";
+  else if (G != 1 && G != 2 && G != 4 && G != 8) what = "n_heads must be 1, 2, 4 or 8 times n_kv";
+  else if (n_kv > 65536) what = "more than 65536 kv heads";
+  else if (d != 64 && d != 128) what = "head_dim must be 64 or 128";
+  else if (page_size < 8 || (page_size & (page_size - 1))) what = "page_size must be a power of two >= 8";
+  else if (max_pages < 1 || (long long)max_pages * page_size > 0x7fffffffll) what = "max_pages must be positive and a table's row end below position 2^31";
+  if (!what) return DIS_OK;
+  dis::set_last_error(std::string(who) + ": " + what);
+  return DIS_ERR_INVALID_ARGUMENT;
+}
+static int cache_refuse(const char *who, const char *what) {
+  dis::set_last_error(std::string(who) + ": " + what);
+  return DIS_ERR_INVALID_ARGUMENT;
+}
+static bool off(const void *p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p) & (align - 1)) != 0; }
+
+int dis_k_rope_kv_write_i8(const float *qkv, int32_t n_partial, int64_t partial_stride, uint16_t *q, int8_t *pool, float *scale,
+                           const int32_t *page_table, int32_t max_pages, const int32_t *pt_row, const int32_t *pos, const float *rope_cos,
+                           const float *rope_sin, int32_t T, int32_t n_heads, int32_t n_kv, int32_t d, int32_t page_size, void *stream) {
+  static const char *me = "rope_kv_write_i8";
+  if (int rc = need_gpu()) return rc;
+  if (int rc = cache_shape(me, T, n_heads, n_kv, d, page_size, max_pages)) return rc;
+  if (n_partial < 1) return cache_refuse(me, "n_partial must be positive");
+  if ((long long)T * (n_heads + 2 * n_kv) > 0x7fffffffll) return cache_refuse(me, "more than 2^31 rows of q, k and v");
+  if (T == 0) return DIS_OK;
+  if (!qkv || !q || !pool || !scale || !page_table || !pt_row || !pos || !rope_cos || !rope_sin) return cache_refuse(me, "null pointer");
+  if (off(qkv, 16) || off(rope_cos, 16) || off(rope_sin, 16) || (n_partial > 1 && partial_stride % 4) || off(q, 8) || off(pool, 4))
+    return cache_refuse(me, "qkv, its slices, rope_cos and rope_sin start on 16 bytes, q on 8, the pool on 4");
+  CallOverlap overlap(stream);
+  return k_ret(dis::launch_rope_kv_write_i8(qkv, n_partial, partial_stride, q, pool, scale, page_table, max_pages, pt_row, pos, rope_cos, rope_sin, T,
+                                            n_heads, n_kv, d, page_size, (cudaStream_t)stream));
+}
+int dis_k_kv_read_i8(const int8_t *pool, const float *scale, uint16_t *kv_pool, const int32_t *src_table, const int32_t *dst_table,
+                     int32_t max_pages, const int32_t *pt_row, const int32_t *first, const int32_t *ctx, int32_t n_rows, int32_t n_kv, int32_t d,
+                     int32_t page_size, void *stream) {
+  static const char *me = "kv_read_i8";
+  if (int rc = need_gpu()) return rc;
+  if (int rc = cache_shape(me, n_rows, n_kv, n_kv, d, page_size, max_pages)) return rc;
+  if (max_pages > 65535) return cache_refuse(me, "more than 65535 pages in a table's row");
+  if (n_rows == 0) return DIS_OK;
+  if (!pool || !scale || !kv_pool || !src_table || !dst_table || !pt_row || !ctx) return cache_refuse(me, "null pointer");
+  if (off(pool, 16) || off(kv_pool, 16)) return cache_refuse(me, "both pools start on 16 bytes");
+  CallOverlap overlap(stream);
+  return k_ret(dis::launch_kv_read_i8(pool, scale, kv_pool, src_table, dst_table, max_pages, pt_row, first, ctx, n_rows, n_kv, d, page_size,
+                                      (cudaStream_t)stream));
+}
+size_t dis_k_attn_paged_i8_scratch_elems(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d) {
+  return T > 0 ? dis::attn_stream_scratch_elems(n_heads, n_kv, d) : 0;
+}
+int dis_k_attn_paged_i8(const uint16_t *q, const int8_t *pool, const float *scale, const int32_t *page_table, int32_t max_pages, const int32_t *pt_row,
+                        const int32_t *ctx, uint16_t *out, float *scratch, int32_t T, int32_t n_heads, int32_t n_kv, int32_t d, int32_t page_size,
+                        void *stream) {
+  static const char *me = "attn_paged_i8";
+  if (int rc = need_gpu()) return rc;
+  if (int rc = cache_shape(me, T, n_heads, n_kv, d, page_size, max_pages)) return rc;
+  if (T == 0) return DIS_OK;
+  if (!q || !pool || !scale || !page_table || !pt_row || !ctx || !out || !scratch) return cache_refuse(me, "null pointer");
+  if (off(q, 16) || off(pool, 16) || off(scratch, 16) || off(out, 4)) return cache_refuse(me, "q, the pool and scratch start on 16 bytes, out on 4");
+  CallOverlap overlap(stream);
+  return k_ret(dis::launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, 0, out, nullptr, nullptr, scratch, false, T, n_heads, n_kv, d,
+                                       page_size, (cudaStream_t)stream));
+}
+size_t dis_k_attn_shared_scratch_elems(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d) {
+  return T > 0 ? dis::attn_shared_scratch_elems(T, n_heads, n_kv, d) : 0;
+}
+int dis_k_attn_shared(const uint16_t *q, const void *kv_pool, const float *scale, int64_t n_pages, const int32_t *page_table, int32_t max_pages,
+                      const int32_t *pt_row, const int32_t *ctx, int32_t prefix, uint16_t *out, float *scratch, int32_t T, int32_t n_heads,
+                      int32_t n_kv, int32_t d, int32_t page_size, void *stream) {
+  static const char *me = "attn_shared";
+  if (int rc = need_gpu()) return rc;
+  if (int rc = cache_shape(me, T, n_heads, n_kv, d, page_size, max_pages)) return rc;
+  if (prefix < 0 || prefix > (long long)max_pages * page_size) return cache_refuse(me, "prefix must lie between 0 and the positions of a table's row");
+  if (n_pages < 1 || n_pages * 2 * n_kv * page_size > 0x7fffffffll) return cache_refuse(me, "n_pages must be positive and the pool have fewer than 2^31 rows");
+  if (T == 0) return DIS_OK;
+  if (!q || !kv_pool || !page_table || !pt_row || !ctx || !out || !scratch) return cache_refuse(me, "null pointer");
+  if (off(q, 16) || off(kv_pool, 16) || off(scratch, 16) || off(out, 4)) return cache_refuse(me, "q, the pool and scratch start on 16 bytes, out on 4");
+  CallOverlap overlap(stream);
+  return k_ret(dis::launch_attn_shared(q, kv_pool, scale, n_pages, page_table, max_pages, pt_row, ctx, prefix, out, scratch, T, n_heads, n_kv, d, page_size,
+                                       (cudaStream_t)stream));
+}
 int dis_k_sample(const float *logits, int64_t ld, int32_t T, int32_t V, const float *temperature, const float *top_p,
                  const uint64_t *seeds, const uint64_t *steps, uint32_t *out_tokens, float *out_logprob, void *stream) {
   if (int rc = need_gpu()) return rc;

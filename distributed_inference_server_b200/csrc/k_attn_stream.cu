@@ -1,0 +1,628 @@
+// k_attn_stream.cu -- attention of single query tokens over paged keys and values, 8-bit (dis_k_attn_paged_i8) or bf16 (the own parts of
+// dis_k_attn_shared): softmax(q K^T / sqrt d) V for all query heads of a kv head at once.
+//
+// 8-bit rows: k = ks k8, v = vs v8 with whole numbers k8, v8 and one fp32 factor per token and kv head.  The factors stay outside the products:
+//   s_j = (q . k8_j) ks_j / sqrt d,   o = sum_j (p_j vs_j) v8_j / sum_j p_j,   p_j = 2^(s_j - m)
+// so the operands are exact in fp16 or nearly: k8 and v8 by themselves, q after a power of two per head that brings its largest entry to
+// [2^13, 2^14) (entries below 2^-28 of it lose bits), and p_j vs_j because m is the largest s_j + log2 vs_j instead of the largest s_j: no product
+// is above 1, the largest is 1, and each loses 2^-11 of itself at most (bf16: 2^-8) or, below 2^-14, 2^-25.  Which m a softmax is taken under
+// cancels; vs is at least 2^-87 or counted as that, so that sum p_j stays within fp32.  m, l, O and the scores are fp32.
+//
+// HBM-bound: 2 (d + 4) bytes (i8) or 4 d (bf16) per token and kv head, 4 G d operations on mma.sync m16n8k16 (tokens are its rows, the up to eight
+// heads its columns: S^T = K Q^T, O^T = V^T P^T).  Operands go from shared memory to registers by 16-byte loads without ldmatrix: which dim is
+// which k index of K Q^T is free as long as Q agrees, so a lane's 16 bytes of a K row are its operand of four k-steps; and a lane's 16 dims of two
+// V rows, bytes interleaved, are its operand of eight m-tiles, the transposition being part of the conversion.
+//
+// Work: the histories of all (token, kv head) pairs laid end to end in tiles of 16 tokens (32 for 8-bit heads of 64), cut into equal shares, one per
+// resident CTA, whatever the lengths are: lengths are read on the device, nothing depends on their maximum.  The CTA's four warps take its
+// tiles in turn, each with a ring of its own filled by cp.async (no barrier of the block per tile, nothing to spin on), and merge their states at
+// the end of a history's piece.  A history in several CTAs is finished by whichever of them ends last, which adds the pieces in the
+// order of the history: the result does not depend on who that is.
+#include <algorithm>
+
+#include <cuda_fp16.h>
+
+#include "attn_piece.cuh"
+
+namespace dis {
+
+constexpr int kStWarps = 4;
+constexpr int kStMaxT = 1024;           // tokens of one launch
+constexpr int kStMaxUnits = 1 << 16;    // (token, kv head) pairs of one launch: one counter each
+constexpr int kStMinShare = 2 * kStWarps;  // tiles of a CTA, at least
+
+template <int D, bool I8>
+struct StCfg {
+  static constexpr int kSub = I8 && D == 64 ? 2 : 1;      // groups of 16 tokens in a tile
+  static constexpr int kTok = 16 * kSub;
+  static constexpr int kRow = D * (I8 ? 1 : 2);           // bytes of a row
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kPart = kTok * kRow;               // K or V of a tile
+  static constexpr int kStage = 2 * kPart + (I8 ? 2 * kTok * 4 : 0);
+  static constexpr int kStages = 3;
+  static constexpr int kHead = 16 * (D / 16 + 1) + 4;     // floats between two heads' O in the merge: no bank twice in a half warp
+  static constexpr int kCtas = I8 ? 3 : 2;                // per SM
+  static constexpr int kRing = kStWarps * kStages * kStage;
+  static constexpr int meet(int G) { return G < 4 ? G : 4; }  // heads whose states meet in shared memory at a time
+  static constexpr int fixed(int G) { return kRing + kStWarps * meet(G) * kHead * 4; }
+};
+
+// Where row r's 16-byte chunk c of a tile lies, in chunks: a quarter warp's loads (K: two rows, four chunks; V: two chunks of four rows, every
+// second one) meet every bank once.
+template <int D, bool I8>
+__device__ __forceinline__ int st_k_chunk(int r, int c) {
+  if (I8 && D == 64) return r * 4 + c;
+  return r * StCfg<D, I8>::kChunks + (c ^ ((r & 1) << 2));
+}
+template <int D, bool I8>
+__device__ __forceinline__ int st_v_chunk(int r, int c) {
+  const int t = (r >> 1) & 3;
+  if (I8 && D == 64) return (r ^ (t & 1)) * 4 + (c ^ (t & 2));
+  if (!I8 && D == 128) return r * 16 + (c ^ ((t & 1) | ((t & 2) << 1)));
+  return r * 8 + (c ^ (t << 1));
+}
+
+__device__ __forceinline__ void st_copy_16(uint32_t dst, const void *src, bool in) {  // zeros where the row is not visible
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void st_copy_4(uint32_t dst, const void *src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void st_copy_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void st_copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint4 st_lds_16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 st_lds_8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float st_lds_f(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+template <bool I8>
+__device__ __forceinline__ void st_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (I8)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t st_transpose(uint32_t v) {  // an 8x8 matrix of pairs across the warp
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+struct StArgs {
+  const uint16_t *q;
+  const void *pool;
+  const float *scale;      // I8
+  const int *page_table;
+  int max_pages;
+  const int *pt_row, *ctx;
+  int first;               // keys in front of this position are somebody else's
+  uint16_t *out;           // the result, or nullptr: the states go to state_o, state_ml
+  float *state_o, *state_ml;
+  int *counters;           // [T * n_kv], zero between calls
+  float *piece_o, *piece_ml;  // [2 per CTA][G][D], [2 per CTA][G][2]
+  int T, n_kv, page_shift;
+  int late_wait;           // the kernel in front was told to let this one start once its own inputs were complete: wait for it at the end
+};
+
+template <int D, int G, bool I8>
+__global__ void __launch_bounds__(kStWarps * 32, StCfg<D, I8>::kCtas)
+attn_stream_kernel(const StArgs a) {
+  using Cfg = StCfg<D, I8>;
+  constexpr int KS = D / 16;
+  constexpr int kPer = D / 8;                    // dims of a lane's V operand
+  constexpr bool kTwice = !I8 && G <= 4;         // bf16 weights in two halves, the rest through columns of its own or (G = 8) a product of its own
+  constexpr int kCols = kTwice ? 2 * G : G, kMeet = Cfg::meet(G);
+  extern __shared__ __align__(16) uint8_t st_smem[];
+  float *s_o = reinterpret_cast<float *>(st_smem + Cfg::kRing);  // [warp][kMeet heads][kHead]
+  int *s_tiles = reinterpret_cast<int *>(s_o + kStWarps * kMeet * Cfg::kHead);  // [T + 1]: tiles of a kv head in front of token t
+  __shared__ float s_m[kStWarps][8], s_l[kStWarps][8];
+  __shared__ int s_scan[kStWarps], s_last;
+
+  const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  pdl_launch_dependents();
+  if (!a.late_wait) pdl_wait();
+  const int n_heads = a.n_kv * G, page_size = 1 << a.page_shift, base = a.first / Cfg::kTok * Cfg::kTok;
+  auto keys_of = [&](int t) { return min(a.ctx[t], a.max_pages << a.page_shift); };
+
+  // ---- tiles in front of each token; tokens without keys of their own get their result here
+  for (int t0 = 0, sum = 0; t0 < a.T; t0 += kStWarps * 32) {
+    const int t = t0 + threadIdx.x;
+    int n = 0;
+    if (t < a.T) {
+      const int keys = keys_of(t);
+      n = keys > a.first ? (keys - base + Cfg::kTok - 1) / Cfg::kTok : 0;
+    }
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_scan[warp] = x;
+    __syncthreads();
+    int before = sum;
+    for (int w = 0; w < kStWarps; w++) {
+      if (w < warp) before += s_scan[w];
+      sum += s_scan[w];
+    }
+    if (t < a.T) s_tiles[t + 1] = before + x;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) s_tiles[0] = 0;
+  __syncthreads();
+  for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
+    if (s_tiles[t + 1] > s_tiles[t]) continue;
+    for (int i = threadIdx.x; i < n_heads * D; i += kStWarps * 32) {
+      if (a.out) a.out[(size_t)t * n_heads * D + i] = 0;
+      else a.state_o[(size_t)t * n_heads * D + i] = 0.f;
+    }
+    if (!a.out)
+      for (int i = threadIdx.x; i < n_heads; i += kStWarps * 32) {
+        a.state_ml[((size_t)t * n_heads + i) * 2] = -INFINITY;
+        a.state_ml[((size_t)t * n_heads + i) * 2 + 1] = 0.f;
+      }
+  }
+
+  const int total = s_tiles[a.T] * a.n_kv;
+  const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kStMinShare);
+  const int lo = (int)min((long long)total, (long long)blockIdx.x * share), hi = min(total, lo + share);
+
+  // A walk over the (token, kv head) pairs; [u0, u1) are the pair's tiles
+  struct Cursor { int t, h, u0, u1; };
+  auto next_pair = [&](Cursor &c) {
+    c.u0 = c.u1;
+    if (++c.h == a.n_kv) {
+      c.h = 0;
+      do c.t++;
+      while (s_tiles[c.t + 1] == s_tiles[c.t]);
+    }
+    c.u1 = c.u0 + s_tiles[c.t + 1] - s_tiles[c.t];
+  };
+  Cursor cur{0, 0, 0, 0};
+  if (lo < hi) {
+    int b = 0, e = a.T;  // the last token with s_tiles[t] * n_kv <= lo
+    while (e - b > 1) {
+      const int mid = (b + e) >> 1;
+      if (s_tiles[mid] * a.n_kv <= lo) b = mid;
+      else e = mid;
+    }
+    const int n = s_tiles[b + 1] - s_tiles[b], at = s_tiles[b] * a.n_kv;
+    cur.t = b;
+    cur.h = (lo - at) / n;
+    cur.u0 = at + cur.h * n;
+    cur.u1 = cur.u0 + n;
+  }
+
+  // ---- the ring: this warp's tiles lo + warp, lo + warp + 4, ..
+  const uint32_t ring = smem_u32(st_smem) + warp * Cfg::kStages * Cfg::kStage;
+  Cursor ahead = cur;
+  int fetch = lo + warp, into = 0;                      // next tile to fetch, and its stage
+  int a_t = -1, a_keys = 0, win_first = 0, win = 0;     // of token a_t: keys, and 32 page numbers, one in each lane
+  const int *a_pt = nullptr;
+  auto fetch_next = [&] {
+    if (fetch < hi) {
+      while (fetch >= ahead.u1) next_pair(ahead);
+      if (ahead.t != a_t) {
+        a_t = ahead.t;
+        a_keys = keys_of(a_t);
+        a_pt = a.page_table + (size_t)a.pt_row[a_t] * a.max_pages;
+        win_first = 1 << 30;
+      }
+      const int pos0 = base + (fetch - ahead.u0) * Cfg::kTok, last_page = (a_keys - 1) >> a.page_shift;
+      const uint32_t dst = ring + into * Cfg::kStage;
+      long long row8[Cfg::kTok / 8];  // first row of every eight tokens' part of a page (pages are eight tokens or more)
+#pragma unroll
+      for (int e = 0; e < Cfg::kTok / 8; e++) {
+        const int pos = pos0 + 8 * e, pi = min(pos >> a.page_shift, last_page);
+        if (pi < win_first || pi - win_first >= 32) {
+          win_first = pi;
+          win = a_pt[min(pi + lane, last_page)];
+        }
+        const long long page = __shfl_sync(0xffffffffu, win, pi - win_first);
+        row8[e] = ((page * 2) * a.n_kv + ahead.h) * page_size + (pos & (page_size - 1));
+      }
+      const long long v_rows = (long long)a.n_kv * page_size;
+      const char *pool = reinterpret_cast<const char *>(a.pool);
+#pragma unroll
+      for (int i = 0; i < Cfg::kTok * Cfg::kChunks / 32; i++) {
+        const int id = i * 32 + lane, r = id / Cfg::kChunks, c = id % Cfg::kChunks;
+        const int e = i * (32 / Cfg::kChunks) / 8;
+        const long long row = row8[e] + (r & 7);
+        const bool in = pos0 + r >= a.first && pos0 + r < a_keys;
+        st_copy_16(dst + st_k_chunk<D, I8>(r, c) * 16, pool + row * Cfg::kRow + c * 16, in);
+        st_copy_16(dst + Cfg::kPart + st_v_chunk<D, I8>(r, c) * 16, pool + (row + v_rows) * Cfg::kRow + c * 16, in);
+      }
+      if (I8) {
+#pragma unroll
+        for (int i = 0; i < Cfg::kSub; i++) {  // lanes 0-15: K, 16-31: V
+          const int r = i * 16 + (lane & 15);
+          const long long row = ((lane & 15) < 8 ? row8[2 * i] : row8[2 * i + 1]) + (r & 7) + (lane < 16 ? 0 : v_rows);
+          const bool in = pos0 + r >= a.first && pos0 + r < a_keys;
+          st_copy_4(dst + 2 * Cfg::kPart + ((lane < 16 ? 0 : Cfg::kTok) + r) * 4, a.scale + row, in);
+        }
+      }
+      fetch += kStWarps;
+    }
+    into = into + 1 == Cfg::kStages ? 0 : into + 1;
+    st_copy_end();
+  };
+  if (lo < hi) {
+#pragma unroll
+    for (int i = 0; i < Cfg::kStages - 1; i++) fetch_next();
+  }
+
+  constexpr float kScale = (D == 128 ? 0.08838834764831845f : 0.125f) * 1.4426950408889634f;  // scores are kept in the log2 domain
+  int tile = lo + warp, stage = 0;
+  while (cur.u0 < hi && lo < hi) {
+    // ================= one piece: tiles [max(u0, lo), min(u1, hi)) of a pair
+    const int end = min(cur.u1, hi), keys = keys_of(cur.t);
+    // Q as the B operand: column g is head g (kTwice: the next G columns repeat it)
+    uint32_t qb[KS][2];
+    float qf[2] = {kScale, kScale};  // factor of the scores of columns 2 tq, 2 tq + 1
+    {
+      const bool has = g < kCols;
+      const uint4 *qp = reinterpret_cast<const uint4 *>(a.q + ((size_t)cur.t * n_heads + cur.h * G + (has ? g % G : 0)) * D);
+      if constexpr (I8) {
+        uint4 raw[D / 64][2];
+#pragma unroll
+        for (int i = 0; i < D / 64; i++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) raw[i][j] = has ? qp[(tq + 4 * i) * 2 + j] : make_uint4(0u, 0u, 0u, 0u);
+        uint32_t big = 0;  // largest magnitude's bits (a NaN's are above infinity's)
+#pragma unroll
+        for (int i = 0; i < D / 64; i++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const uint32_t w[4] = {raw[i][j].x, raw[i][j].y, raw[i][j].z, raw[i][j].w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) big = max(big, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+          }
+        big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        // exponent of the factor, kept where the factor and its inverse are normal numbers; infinities and NaN go through as they are
+        const int ex = min(max((int)(big >> 7) - 127 - 13, -100), 100);
+        const float down = __int_as_float((127 - ex) << 23), up = __int_as_float((127 + ex) << 23);
+#pragma unroll
+        for (int i = 0; i < D / 64; i++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const uint32_t w[4] = {raw[i][j].x, raw[i][j].y, raw[i][j].z, raw[i][j].w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const float2 f = bf16x2_to_float2(w[k]);
+              const __half2 h = __floats2half2_rn(f.x * down, f.y * down);
+              qb[i * 4 + j * 2 + (k >> 1)][k & 1] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+          }
+        qf[0] *= __shfl_sync(0xffffffffu, up, tq * 8);
+        qf[1] *= __shfl_sync(0xffffffffu, up, tq * 8 + 4);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+          const uint4 w = has ? qp[tq + 4 * i] : make_uint4(0u, 0u, 0u, 0u);
+          qb[2 * i][0] = w.x; qb[2 * i][1] = w.y; qb[2 * i + 1][0] = w.z; qb[2 * i + 1][1] = w.w;
+        }
+      }
+    }
+    float oacc[KS][4];  // O^T: dims g kPer + 2 m (+ 1) of columns 2 tq (+ 1): {dim, column}, {dim, column + 1}, {dim + 1, column}, ..
+#pragma unroll
+    for (int m = 0; m < KS; m++) { oacc[m][0] = 0.f; oacc[m][1] = 0.f; oacc[m][2] = 0.f; oacc[m][3] = 0.f; }
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+
+    for (; tile < end; tile += kStWarps) {
+      st_copy_wait<Cfg::kStages - 2>();
+      __syncwarp();
+      fetch_next();  // into the stage that was read last
+      const uint32_t at = ring + stage * Cfg::kStage;
+      stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
+      const int pos0 = base + (tile - cur.u0) * Cfg::kTok;
+#pragma unroll
+      for (int sub = 0; sub < Cfg::kSub; sub++) {
+        const int r0 = sub * 16 + g;
+        if (Cfg::kSub > 1 && sub > 0 && pos0 + sub * 16 >= keys) break;  // (uniform)
+        // ---- S^T = K Q^T: tokens r0, r0 + 8, columns 2 tq (+ 1); two accumulators halve the chain
+        float sa[2][4];
+#pragma unroll
+        for (int e = 0; e < 2; e++) { sa[e][0] = 0.f; sa[e][1] = 0.f; sa[e][2] = 0.f; sa[e][3] = 0.f; }
+#pragma unroll
+        for (int i = 0; i < Cfg::kChunks / 4; i++) {
+          const uint4 x4 = st_lds_16(at + st_k_chunk<D, I8>(r0, tq + 4 * i) * 16), y4 = st_lds_16(at + st_k_chunk<D, I8>(r0 + 8, tq + 4 * i) * 16);
+          const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
+          if constexpr (I8) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              uint32_t a0, a1, a2, a3;
+              bytes_to_half2(x[j] ^ 0x80808080u, a0, a2);
+              bytes_to_half2(y[j] ^ 0x80808080u, a1, a3);
+              st_mma<I8>(sa[j & 1], a0, a1, a2, a3, qb[i * 4 + j][0], qb[i * 4 + j][1]);
+            }
+          } else {
+            st_mma<I8>(sa[0], x[0], y[0], x[1], y[1], qb[2 * i][0], qb[2 * i][1]);
+            st_mma<I8>(sa[1], x[2], y[2], x[3], y[3], qb[2 * i + 1][0], qb[2 * i + 1][1]);
+          }
+        }
+        // ---- running maximum; the whole warp acts only where one of its maxima grows
+        float k_f[2] = {1.f, 1.f}, v_f[2] = {1.f, 1.f};
+        if (I8) {
+          const uint32_t sc = at + 2 * Cfg::kPart + r0 * 4;
+          k_f[0] = st_lds_f(sc); k_f[1] = st_lds_f(sc + 32);
+          v_f[0] = st_lds_f(sc + Cfg::kTok * 4); v_f[1] = st_lds_f(sc + Cfg::kTok * 4 + 32);
+        }
+        const int p0 = pos0 + r0, p1 = p0 + 8;
+        const bool in0 = p0 < keys && p0 >= a.first, in1 = p1 < keys && p1 >= a.first;
+        const float up0 = I8 ? piece_log2_scale(v_f[0]) : 0.f, up1 = I8 ? piece_log2_scale(v_f[1]) : 0.f;
+        float p[4], mx[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          p[e] = in0 ? (sa[0][e] + sa[1][e]) * (k_f[0] * qf[e]) : -INFINITY;
+          p[2 + e] = in1 ? (sa[0][2 + e] + sa[1][2 + e]) * (k_f[1] * qf[e]) : -INFINITY;
+          mx[e] = fmaxf(p[e] + up0, p[2 + e] + up1);
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m_run[0] || mx[1] > m_run[1])) {
+          float f[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float x = mx[e];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float m_new = fmaxf(m_run[e], x);
+            f[e] = piece_weight(m_run[e], m_new);
+            l_run[e] *= f[e];
+            m_run[e] = m_new;
+          }
+#pragma unroll
+          for (int m = 0; m < KS; m++) { oacc[m][0] *= f[0]; oacc[m][1] *= f[1]; oacc[m][2] *= f[0]; oacc[m][3] *= f[1]; }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          p[e] = piece_weight(p[e], m_run[e]);
+          p[2 + e] = piece_weight(p[2 + e], m_run[e]);
+          l_run[e] += p[e] + p[2 + e];
+        }
+        uint32_t pb0, pb1, pl0 = 0u, pl1 = 0u;
+        if constexpr (I8) {
+          const __half2 h0 = __floats2half2_rn(p[0] * v_f[0], p[1] * v_f[0]), h1 = __floats2half2_rn(p[2] * v_f[1], p[3] * v_f[1]);
+          pb0 = st_transpose(*reinterpret_cast<const uint32_t *>(&h0));
+          pb1 = st_transpose(*reinterpret_cast<const uint32_t *>(&h1));
+        } else {
+          const uint32_t p01 = float2_to_bf16x2(p[0], p[1]), p23 = float2_to_bf16x2(p[2], p[3]);
+          const float2 r01 = bf16x2_to_float2(p01), r23 = bf16x2_to_float2(p23);
+          const uint32_t q01 = float2_to_bf16x2(p[0] - r01.x, p[1] - r01.y), q23 = float2_to_bf16x2(p[2] - r23.x, p[3] - r23.y);
+          const bool rest = kTwice && tq * 2 >= G;
+          pb0 = st_transpose(G == 1 ? (p01 & 0xffffu) | (q01 & 0xffff0000u) : rest ? q01 : p01);
+          pb1 = st_transpose(G == 1 ? (p23 & 0xffffu) | (q23 & 0xffff0000u) : rest ? q23 : p23);
+          if (!kTwice) { pl0 = st_transpose(q01); pl1 = st_transpose(q23); }
+        }
+        // ---- O^T += V^T P^T: tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9, dims g kPer ..
+        const uint32_t va = at + Cfg::kPart;
+        const int t0 = sub * 16 + 2 * tq;
+        if constexpr (I8) {
+          uint32_t v[4][kPer / 4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const int r = t0 + (k & 1) + (k >> 1) * 8;
+            if constexpr (D == 128) {
+              const uint4 w = st_lds_16(va + st_v_chunk<D, I8>(r, g) * 16);
+              v[k][0] = w.x; v[k][1] = w.y; v[k][2] = w.z; v[k][3] = w.w;
+            } else {
+              const uint2 w = st_lds_8(va + st_v_chunk<D, I8>(r, g >> 1) * 16 + (g & 1) * 8);
+              v[k][0] = w.x; v[k][1] = w.y;
+            }
+#pragma unroll
+            for (int j = 0; j < kPer / 4; j++) v[k][j] ^= 0x80808080u;
+          }
+#pragma unroll
+          for (int j = 0; j < kPer / 4; j++) {
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+              uint32_t a0, a1, a2, a3;
+              bytes_to_half2(__byte_perm(v[0][j], v[1][j], hf ? 0x7362 : 0x5140), a0, a1);
+              bytes_to_half2(__byte_perm(v[2][j], v[3][j], hf ? 0x7362 : 0x5140), a2, a3);
+              st_mma<I8>(oacc[2 * j + hf], a0, a1, a2, a3, pb0, pb1);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int cc = 0; cc < kPer / 8; cc++) {
+            uint4 w[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) w[k] = st_lds_16(va + st_v_chunk<D, I8>(t0 + (k & 1) + (k >> 1) * 8, g * (kPer / 8) + cc) * 16);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              auto el = [&](int k) { return j == 0 ? w[k].x : j == 1 ? w[k].y : j == 2 ? w[k].z : w[k].w; };
+              const uint32_t a0 = __byte_perm(el(0), el(1), 0x5410), a1 = __byte_perm(el(0), el(1), 0x7632);
+              const uint32_t a2 = __byte_perm(el(2), el(3), 0x5410), a3 = __byte_perm(el(2), el(3), 0x7632);
+              st_mma<I8>(oacc[4 * cc + j], a0, a1, a2, a3, pb0, pb1);
+              if (!kTwice) st_mma<I8>(oacc[4 * cc + j], a0, a1, a2, a3, pl0, pl1);
+            }
+          }
+        }
+      }
+    }
+
+    // ================= the warps' states meet in shared memory, kMeet heads at a time
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 4);
+      l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 8);
+      l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 16);
+    }
+    if constexpr (kTwice) {  // the weights' halves: columns h and h + G
+#pragma unroll
+      for (int m = 0; m < KS; m++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          if (G == 1) { if (!(k & 1)) oacc[m][k] += oacc[m][k + 1]; }
+          else oacc[m][k] += __shfl_xor_sync(0xffffffffu, oacc[m][k], G / 2);
+        }
+    }
+    if (g == 0) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) { s_m[warp][2 * tq + e] = m_run[e]; s_l[warp][2 * tq + e] = l_run[e]; }
+    }
+    const int c_first = cur.u0 / share, c_last = (cur.u1 - 1) / share;  // the CTAs that have a piece of this history
+    const int slot = 2 * blockIdx.x + (cur.u0 >= lo ? 1 : 0);
+    const size_t row = (size_t)cur.t * n_heads + cur.h * G;
+    auto put = [&](int h, int i, float2 o, float m, float l) {  // dims 2 i, 2 i + 1 of head h
+      if (a.out) {
+        *reinterpret_cast<uint32_t *>(a.out + (row + h) * D + 2 * i) = float2_to_bf16x2(o.x / l, o.y / l);
+      } else {
+        *reinterpret_cast<float2 *>(a.state_o + (row + h) * D + 2 * i) = o;
+        if (i == 0) *reinterpret_cast<float2 *>(a.state_ml + (row + h) * 2) = make_float2(m, l);
+      }
+    };
+#pragma unroll
+    for (int h0 = 0; h0 < G; h0 += kMeet) {
+      if (h0) __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int col = 2 * tq + e - h0;
+        if (col >= 0 && col < kMeet) {
+          float2 *o = reinterpret_cast<float2 *>(s_o + (warp * kMeet + col) * Cfg::kHead + g * (kPer + 2));
+#pragma unroll
+          for (int m = 0; m < KS; m++) o[m] = make_float2(oacc[m][e], oacc[m][2 + e]);
+        }
+      }
+      __syncthreads();
+      for (int it = threadIdx.x; it < kMeet * (D / 2); it += kStWarps * 32) {
+        const int hh = it / (D / 2), h = h0 + hh, i = it % (D / 2), off = (2 * i) / kPer * (kPer + 2) + (2 * i) % kPer;
+        float M = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kStWarps; w++) M = fmaxf(M, s_m[w][h]);
+        float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kStWarps; w++) {
+          const float f = piece_weight(s_m[w][h], M);
+          const float2 x = *reinterpret_cast<const float2 *>(s_o + (w * kMeet + hh) * Cfg::kHead + off);
+          o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y);
+          l = fmaf(s_l[w][h], f, l);
+        }
+        if (c_first == c_last) {
+          put(h, i, o, M, l);
+        } else {
+          __stcg(reinterpret_cast<float2 *>(a.piece_o + ((size_t)slot * G + h) * D + 2 * i), o);
+          if (i == 0) __stcg(reinterpret_cast<float2 *>(a.piece_ml + ((size_t)slot * G + h) * 2), make_float2(M, l));
+        }
+      }
+    }
+    if (c_first != c_last) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        int *count = a.counters + cur.t * a.n_kv + cur.h;
+        s_last = atomicAdd(count, 1) == c_last - c_first;
+        if (s_last) *count = 0;  // as the next call wants it
+        __threadfence();
+      }
+      __syncthreads();
+      if (s_last) {
+        for (int it = threadIdx.x; it < G * (D / 2); it += kStWarps * 32) {
+          const int h = it / (D / 2), i = it % (D / 2);
+          float M = -INFINITY, l = 0.f;
+          float2 o = make_float2(0.f, 0.f);
+          for (int c0 = c_first; c0 <= c_last; c0 += 8) {  // eight pieces on their way at a time
+            float2 ml[8], x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              const int c = c0 + j;
+              if (c <= c_last) {
+                const size_t sl = ((size_t)2 * c + (c == c_first ? 1 : 0)) * G + h;
+                ml[j] = __ldcg(reinterpret_cast<const float2 *>(a.piece_ml + sl * 2));
+                x[j] = __ldcg(reinterpret_cast<const float2 *>(a.piece_o + sl * D + 2 * i));
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              if (c0 + j <= c_last) {
+                const float m_new = fmaxf(M, ml[j].x), f = piece_weight(M, m_new), fn = piece_weight(ml[j].x, m_new);
+                M = m_new;
+                l = l * f + ml[j].y * fn;
+                o.x = o.x * f + x[j].x * fn;
+                o.y = o.y * f + x[j].y * fn;
+              }
+            }
+          }
+          put(h, i, o, M, l);
+        }
+      }
+    }
+    __syncthreads();  // the next piece's states may come
+    if (cur.u1 >= hi) break;
+    next_pair(cur);
+  }
+  st_copy_wait<0>();
+  if (a.late_wait) pdl_wait();
+}
+
+// ---------------------------------------------------------------------------------------- host
+static size_t stream_slots(int per_sm) { return 2 * (size_t)kNumSMs * per_sm; }
+size_t attn_stream_scratch_elems(int n_heads, int n_kv, int d) {  // counters, then the pieces of every resident CTA
+  if (n_kv <= 0 || n_heads <= 0 || d <= 0) return 0;
+  return kStMaxUnits + stream_slots(3) * (size_t)(n_heads / n_kv) * (2 + (size_t)d);
+}
+
+template <int D, int G, bool I8>
+static cudaError_t stream_launch(const StArgs &a, cudaStream_t st) {
+  using Cfg = StCfg<D, I8>;
+  auto kern = attn_stream_kernel<D, G, I8>;
+  constexpr int kFixed = Cfg::fixed(G);
+  static DeviceOnce once;
+  DIS_CUDA_TRY(once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + (kStMaxT + 1) * 4); }));
+  return launch_k(kern, dim3(kNumSMs * Cfg::kCtas), dim3(kStWarps * 32), (size_t)kFixed + (a.T + 1) * 4, st, a);
+}
+
+template <bool I8>
+static cudaError_t stream_dispatch(const StArgs &a, int G, int d, cudaStream_t st) {
+#define DIS_ST_CASE(DD, GG) \
+  if (d == DD && G == GG) return stream_launch<DD, GG, I8>(a, st);
+  DIS_ST_CASE(128, 8) DIS_ST_CASE(128, 4) DIS_ST_CASE(128, 2) DIS_ST_CASE(128, 1)
+  DIS_ST_CASE(64, 8) DIS_ST_CASE(64, 4) DIS_ST_CASE(64, 2) DIS_ST_CASE(64, 1)
+#undef DIS_ST_CASE
+  set_last_error("attention over pieces: head_dim must be 64 or 128 and the GQA group 1, 2, 4 or 8");
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float *scale, const int *page_table, int max_pages, const int *pt_row,
+                               const int *ctx, int first, uint16_t *out, float *state_o, float *state_ml, float *scratch, bool late_wait, int T,
+                               int n_heads, int n_kv, int d, int page_size, cudaStream_t st) {
+  if (n_kv > kStMaxUnits) { set_last_error("attention over pieces: more than 65536 kv heads"); return cudaErrorInvalidValue; }
+  // a launch's tiles are counted in 32 bits
+  const long long most = ((long long)max_pages * page_size / 16 + 2) * n_kv;
+  const int G = n_heads / n_kv, step = (int)std::max(1ll, std::min({(long long)kStMaxT, (long long)kStMaxUnits / n_kv, 0x7fffffffll / most}));
+  StArgs a{};
+  a.pool = pool; a.scale = scale; a.page_table = page_table; a.max_pages = max_pages; a.first = first;
+  a.counters = reinterpret_cast<int *>(scratch);
+  a.piece_o = scratch + kStMaxUnits;
+  a.piece_ml = a.piece_o + stream_slots(3) * (size_t)G * d;
+  a.n_kv = n_kv;
+  a.late_wait = late_wait;
+  while ((1 << a.page_shift) < page_size) a.page_shift++;
+  for (int t = 0; t < T; t += step) {
+    a.T = std::min(step, T - t);
+    a.q = q + (size_t)t * n_heads * d;
+    a.pt_row = pt_row + t;
+    a.ctx = ctx + t;
+    a.out = out ? out + (size_t)t * n_heads * d : nullptr;
+    a.state_o = state_o ? state_o + (size_t)t * n_heads * d : nullptr;
+    a.state_ml = state_ml ? state_ml + (size_t)t * n_heads * 2 : nullptr;
+    DIS_CUDA_TRY(scale ? stream_dispatch<true>(a, G, d, st) : stream_dispatch<false>(a, G, d, st));
+  }
+  return cudaSuccess;
+}
+
+}  // namespace dis

@@ -114,6 +114,27 @@ cudaError_t launch_attn_prefill_tc(const TmaMap &kv_map, long long row0, const u
                                    const int *qb_ptrow, uint16_t *out, int n_blocks, int n_heads, int n_kv, int d,
                                    int page_size, long long mean_keys /* keys in front of and in a block, on average */, cudaStream_t st);
 
+// k_cache_i8.cu : keys and values in 8 bits, [page][2 (K, V)][n_kv][page_size][d] int8 beside [page][2][n_kv][page_size] fp32 scales
+cudaError_t launch_rope_kv_write_i8(const float *qkv, int n_partial, long long partial_stride, uint16_t *q, int8_t *pool, float *scale,
+                                    const int *page_table, int max_pages, const int *pt_row, const int *pos, const float *rope_cos,
+                                    const float *rope_sin, int T, int n_heads, int n_kv, int d, int page_size, cudaStream_t st);
+cudaError_t launch_kv_read_i8(const int8_t *pool, const float *scale, uint16_t *kv_pool, const int *src_table, const int *dst_table, int max_pages,
+                              const int *pt_row, const int *first, const int *ctx, int n_rows, int n_kv, int d, int page_size, cudaStream_t st);
+
+// k_attn_stream.cu : attention of single tokens over the keys from position `first` on, in equal shares whatever the lengths are.  scale: of the
+// 8-bit pool (nullptr: a bf16 pool).  out, or the states (m, l, O) in state_ml [T][n_heads][2] and state_o [T][n_heads][d].  scratch: its first
+// part is zero between calls.
+size_t attn_stream_scratch_elems(int n_heads, int n_kv, int d);
+cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float *scale, const int *page_table, int max_pages, const int *pt_row,
+                               const int *ctx, int first, uint16_t *out, float *state_o, float *state_ml, float *scratch, bool late_wait, int T,
+                               int n_heads, int n_kv, int d, int page_size, cudaStream_t st);
+
+// k_attn_shared.cu : the same where positions [0, prefix) are the same rows for every token
+size_t attn_shared_scratch_elems(int T, int n_heads, int n_kv, int d);
+cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float *scale, long long n_pages, const int *page_table, int max_pages,
+                               const int *pt_row, const int *ctx, int prefix, uint16_t *out, float *scratch, int T, int n_heads, int n_kv, int d,
+                               int page_size, cudaStream_t st);
+
 // k_gemm_tcgen05.cu
 cudaError_t make_tma_map_2d(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows);
 int gemm_token_tile(int T);  // 32 / 64 / 128: the UMMA N used for T tokens

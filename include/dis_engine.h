@@ -396,6 +396,45 @@ DIS_API int dis_k_attn_prefill(const uint16_t *q, const uint16_t *kv_pool, int64
                                int32_t max_pages, const int32_t *qb_tok0, const int32_t *qb_len,
                                const int32_t *qb_pos0, const int32_t *qb_ptrow, uint16_t *out, int32_t n_blocks,
                                int32_t n_heads, int32_t n_kv, int32_t d, int32_t page_size, void *stream);
+/* ---- keys and values in 8 bits, shared prefixes ---------------------------------------------------- *
+ * The same pages with half the bytes: a row (one token and kv head of K or V, d entries) is d whole numbers x8 in [-127, 127] and one
+ * fp32 scale s, and stands for x8 s.  pool: [page][2 (K,V)][nkv][page_size][d] int8; scale: [page][2][nkv][page_size] fp32.  s = max|x| / 127,
+ * x8 = x / s rounded to the nearest whole number; a row below 2^-80 is zeros with scale 0, a row with an infinity or NaN has the scale NaN and
+ * is NaN wherever it is read.  All of these take d = 64 or 128, n_heads / n_kv of 1, 2, 4 or 8, page sizes that are powers of two >= 8;
+ * anything else, null pointers and starts off the boundaries given are refused with DIS_ERR_INVALID_ARGUMENT before anything is launched.
+ * T = 0 (n_rows = 0) is a call without work.  Page numbers, positions and lengths are on the device and are not checked. */
+
+/* dis_k_rope_kv_write into 8-bit pages: qkv partials [S][T][(nh+2nkv)*d] fp32 -> RoPE(q) bf16 [T][nh*d]; RoPE(k), v -> pool and scale.  qkv,
+ * its slices, rope_cos and rope_sin start on 16 bytes, q on 8, the pool on 4. */
+DIS_API int dis_k_rope_kv_write_i8(const float *qkv, int32_t n_partial, int64_t partial_stride, uint16_t *q, int8_t *pool, float *scale,
+                                   const int32_t *page_table, int32_t max_pages, const int32_t *pt_row, const int32_t *pos,
+                                   const float *rope_cos, const float *rope_sin, int32_t T, int32_t n_heads, int32_t n_kv, int32_t d,
+                                   int32_t page_size, void *stream);
+/* Reads 8-bit pages back into a bf16 pool of the layout of dis_k_rope_kv_write, where prompt attention finds them.  Row r of n_rows: positions
+ * [first[r], ctx[r]) (first may be NULL: from 0) of page-table row pt_row[r]; page i of it comes from 8-bit page src_table[row][i] and goes to
+ * bf16 page dst_table[row][i] (the same table may serve as both).  Other positions of those pages are left as they are.  Two rows may map the
+ * same pages: both write the same values.  Both pools start on 16 bytes; max_pages <= 65535. */
+DIS_API int dis_k_kv_read_i8(const int8_t *pool, const float *scale, uint16_t *kv_pool, const int32_t *src_table, const int32_t *dst_table,
+                             int32_t max_pages, const int32_t *pt_row, const int32_t *first, const int32_t *ctx, int32_t n_rows,
+                             int32_t n_kv, int32_t d, int32_t page_size, void *stream);
+/* dis_k_attn_paged over 8-bit pages: out[t] = softmax(q[t] K^T / sqrt(d)) V over positions [0, ctx[t]) of row pt_row[t], bf16 [T][nh*d].  A token
+ * without keys (ctx <= 0) gets zeros; positions past ctx are never read.  The work is cut into equal shares whatever the lengths are.
+ * scratch: dis_k_attn_paged_i8_scratch_elems() floats, zero-filled once by the caller; every call leaves it so that the next, of any
+ * shape with the same or a smaller need, may use it.  Calls that can overlap on the GPU need a scratch each.  q, the pool and scratch start on
+ * 16 bytes, out on 4. */
+DIS_API size_t dis_k_attn_paged_i8_scratch_elems(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d);
+DIS_API int dis_k_attn_paged_i8(const uint16_t *q, const int8_t *pool, const float *scale, const int32_t *page_table, int32_t max_pages,
+                                const int32_t *pt_row, const int32_t *ctx, uint16_t *out, float *scratch, int32_t T, int32_t n_heads,
+                                int32_t n_kv, int32_t d, int32_t page_size, void *stream);
+/* The same for a batch whose requests share a prefix: positions [0, prefix) hold the same keys and values for every token and are read once for
+ * all of them, through the pages of the first token's row; positions [prefix, ctx[t]) are each token's own.  A token with ctx[t] <= prefix sees
+ * the first ctx[t] positions of the prefix.  kv_pool: bf16 pages (scale NULL) or 8-bit pages with their scales; n_pages pages.
+ * Rows of a bf16 prefix page past `prefix` must hold finite values, as for dis_k_attn_paged.  scratch: dis_k_attn_shared_scratch_elems()
+ * floats under the terms of dis_k_attn_paged_i8, whose scratch it may be too. */
+DIS_API size_t dis_k_attn_shared_scratch_elems(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d);
+DIS_API int dis_k_attn_shared(const uint16_t *q, const void *kv_pool, const float *scale, int64_t n_pages, const int32_t *page_table,
+                              int32_t max_pages, const int32_t *pt_row, const int32_t *ctx, int32_t prefix, uint16_t *out, float *scratch,
+                              int32_t T, int32_t n_heads, int32_t n_kv, int32_t d, int32_t page_size, void *stream);
 /* Sampler over fp32 logits [T][V] (row stride ld): temperature 0 -> argmax, lowest index wins ties;
  * else nucleus sampling as oracle/llama_oracle.c states it.  out_tokens[T]; out_logprob[T] (may be NULL) receives
  * the chosen token's log-probability (see dis_engine_last_logprobs). */
