@@ -374,7 +374,7 @@ int dis_k_attn_shared(const uint16_t *q, const void *kv_pool, const float *scale
   if (int rc = need_gpu()) return rc;
   if (int rc = cache_shape(me, T, n_heads, n_kv, d, page_size, max_pages)) return rc;
   if (prefix < 0 || prefix > (long long)max_pages * page_size) return cache_refuse(me, "prefix must lie between 0 and the positions of a table's row");
-  if (n_pages < 1 || n_pages * 2 * n_kv * page_size > 0x7fffffffll) return cache_refuse(me, "n_pages must be positive and the pool have fewer than 2^31 rows");
+  if (n_pages < 1 || n_pages > 0x7fffffffll || n_pages * 2 * n_kv * page_size > 0x7fffffffll) return cache_refuse(me, "n_pages must be positive and the pool have fewer than 2^31 rows");
   if (T == 0) return DIS_OK;
   if (!q || !kv_pool || !page_table || !pt_row || !ctx || !out || !scratch) return cache_refuse(me, "null pointer");
   if (off(q, 16) || off(kv_pool, 16) || off(scratch, 16) || off(out, 4)) return cache_refuse(me, "q, the pool and scratch start on 16 bytes, out on 4");

@@ -109,7 +109,7 @@ struct StArgs {
   const int *page_table;
   int max_pages;
   const int *pt_row, *ctx;
-  int first;               // keys in front of this position are somebody else's
+  int first;               // keys in front of this position are somebody else's, for the tokens that reach it
   uint16_t *out;           // the result, or nullptr: the states go to state_o, state_ml
   float *state_o, *state_ml;
   int *counters;           // [T * n_kv], zero between calls
@@ -135,8 +135,10 @@ attn_stream_kernel(const StArgs a) {
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   pdl_launch_dependents();
   if (!a.late_wait) pdl_wait();
-  const int n_heads = a.n_kv * G, page_size = 1 << a.page_shift, base = a.first / Cfg::kTok * Cfg::kTok;
+  const int n_heads = a.n_kv * G, page_size = 1 << a.page_shift, base0 = a.first / Cfg::kTok * Cfg::kTok;
   auto keys_of = [&](int t) { return min(a.ctx[t], a.max_pages << a.page_shift); };
+  auto first_of = [&](int keys) { return keys < a.first ? 0 : a.first; };  // a history that ends in front of it is all this kernel's
+  auto base_of = [&](int keys) { return keys < a.first ? 0 : base0; };
 
   // ---- tiles in front of each token; tokens without keys of their own get their result here
   for (int t0 = 0, sum = 0; t0 < a.T; t0 += kStWarps * 32) {
@@ -144,7 +146,7 @@ attn_stream_kernel(const StArgs a) {
     int n = 0;
     if (t < a.T) {
       const int keys = keys_of(t);
-      n = keys > a.first ? (keys - base + Cfg::kTok - 1) / Cfg::kTok : 0;
+      n = keys > first_of(keys) ? (keys - base_of(keys) + Cfg::kTok - 1) / Cfg::kTok : 0;
     }
     int x = n;
 #pragma unroll
@@ -222,7 +224,7 @@ attn_stream_kernel(const StArgs a) {
         a_pt = a.page_table + (size_t)a.pt_row[a_t] * a.max_pages;
         win_first = 1 << 30;
       }
-      const int pos0 = base + (fetch - ahead.u0) * Cfg::kTok, last_page = (a_keys - 1) >> a.page_shift;
+      const int first = first_of(a_keys), pos0 = base_of(a_keys) + (fetch - ahead.u0) * Cfg::kTok, last_page = (a_keys - 1) >> a.page_shift;
       const uint32_t dst = ring + into * Cfg::kStage;
       long long row8[Cfg::kTok / 8];  // first row of every eight tokens' part of a page (pages are eight tokens or more)
 #pragma unroll
@@ -242,7 +244,7 @@ attn_stream_kernel(const StArgs a) {
         const int id = i * 32 + lane, r = id / Cfg::kChunks, c = id % Cfg::kChunks;
         const int e = i * (32 / Cfg::kChunks) / 8;
         const long long row = row8[e] + (r & 7);
-        const bool in = pos0 + r >= a.first && pos0 + r < a_keys;
+        const bool in = pos0 + r >= first && pos0 + r < a_keys;
         st_copy_16(dst + st_k_chunk<D, I8>(r, c) * 16, pool + row * Cfg::kRow + c * 16, in);
         st_copy_16(dst + Cfg::kPart + st_v_chunk<D, I8>(r, c) * 16, pool + (row + v_rows) * Cfg::kRow + c * 16, in);
       }
@@ -251,7 +253,7 @@ attn_stream_kernel(const StArgs a) {
         for (int i = 0; i < Cfg::kSub; i++) {  // lanes 0-15: K, 16-31: V
           const int r = i * 16 + (lane & 15);
           const long long row = ((lane & 15) < 8 ? row8[2 * i] : row8[2 * i + 1]) + (r & 7) + (lane < 16 ? 0 : v_rows);
-          const bool in = pos0 + r >= a.first && pos0 + r < a_keys;
+          const bool in = pos0 + r >= first && pos0 + r < a_keys;
           st_copy_4(dst + 2 * Cfg::kPart + ((lane < 16 ? 0 : Cfg::kTok) + r) * 4, a.scale + row, in);
         }
       }
@@ -269,7 +271,7 @@ attn_stream_kernel(const StArgs a) {
   int tile = lo + warp, stage = 0;
   while (cur.u0 < hi && lo < hi) {
     // ================= one piece: tiles [max(u0, lo), min(u1, hi)) of a pair
-    const int end = min(cur.u1, hi), keys = keys_of(cur.t);
+    const int end = min(cur.u1, hi), keys = keys_of(cur.t), first = first_of(keys), base = base_of(keys);
     // Q as the B operand: column g is head g (kTwice: the next G columns repeat it)
     uint32_t qb[KS][2];
     float qf[2] = {kScale, kScale};  // factor of the scores of columns 2 tq, 2 tq + 1
@@ -363,7 +365,7 @@ attn_stream_kernel(const StArgs a) {
           v_f[0] = st_lds_f(sc + Cfg::kTok * 4); v_f[1] = st_lds_f(sc + Cfg::kTok * 4 + 32);
         }
         const int p0 = pos0 + r0, p1 = p0 + 8;
-        const bool in0 = p0 < keys && p0 >= a.first, in1 = p1 < keys && p1 >= a.first;
+        const bool in0 = p0 < keys && p0 >= first, in1 = p1 < keys && p1 >= first;
         const float up0 = I8 ? piece_log2_scale(v_f[0]) : 0.f, up1 = I8 ? piece_log2_scale(v_f[1]) : 0.f;
         float p[4], mx[2];
 #pragma unroll
@@ -610,10 +612,10 @@ cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float 
   a.piece_o = scratch + kStMaxUnits;
   a.piece_ml = a.piece_o + stream_slots(3) * (size_t)G * d;
   a.n_kv = n_kv;
-  a.late_wait = late_wait;
   while ((1 << a.page_shift) < page_size) a.page_shift++;
   for (int t = 0; t < T; t += step) {
     a.T = std::min(step, T - t);
+    a.late_wait = late_wait && t == 0;  // (the next launch uses the same scratch)
     a.q = q + (size_t)t * n_heads * d;
     a.pt_row = pt_row + t;
     a.ctx = ctx + t;

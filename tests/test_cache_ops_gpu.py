@@ -457,6 +457,21 @@ def test_shared_prefix_long_and_again(int8):
         assert torch.equal(out, first)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("T,group,d,prefix", [(64, 8, 128, 8000), (40, 4, 128, 5000), (64, 8, 64, 8000), (30, 4, 64, 9000)])
+def test_shared_prefix_many_steps_again(int8, T, group, d, prefix):
+    """Slices of many key tiles: every run has the same bits, whatever the scratch held."""
+    ctx = [prefix + 1 + 7 * t % 300 for t in range(T)]
+    c = Cache(ctx, 8, d, 64, T, int8, prefix)
+    q = queries(T, 8 * group, d, 5)
+    area = scratch(T, 8 * group, 8, d, True)
+    first = shared(c, q, 8 * group, prefix, area=area)
+    near(first, attention(c, q, 8 * group, 2.0 ** -8))
+    for k in range(10):
+        area[1 << 16:].fill_(float(k))
+        assert torch.equal(shared(c, q, 8 * group, prefix, area=area), first), k
+
+
 def test_shared_prefix_sizes():
     """Large scores (one key wins), and values' scales from 2^-60 to 2^40, in 8-bit pages."""
     ctx = [700 + t for t in range(20)]
