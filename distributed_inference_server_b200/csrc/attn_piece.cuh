@@ -1,7 +1,9 @@
 // attn_piece.cuh -- what the attention kernels that cut one history into pieces share: states (m, l, O) of pieces and their merge.
 //
 // The state of a set of keys under one query row: a reference m near its largest score (in the log2 domain), l = sum 2^(s - m), O = sum
-// 2^(s - m) v.  Two states join as (M = max m, sum l 2^(m - M), sum O 2^(m - M)); a set without keys is (-inf, 0, 0).
+// 2^(s - m) v.  Two states join as (M = max m, sum l 2^(m - M), sum O 2^(m - M)); a set without keys is (kPieceNone, 0, 0).  Raising a row's m
+// costs a pass over its O, so m follows the largest score only where that has grown by more than kPieceLazy: weights are then at most
+// 2^kPieceLazy instead of 1, and as far from it as before in the types they are kept in.
 #pragma once
 #include "kernels.h"
 #include "ptx.cuh"
@@ -14,9 +16,10 @@ __device__ __forceinline__ float piece_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// The factor that brings a state under maximum m to maximum M >= m.  A set without keys weighs nothing, also beside another such set; where
-// both are +inf or a score is NaN the state has NaN sums, which stay NaN.
-__device__ __forceinline__ float piece_weight(float m, float M) { return m == -INFINITY ? 0.f : piece_ex2(m - M); }
+// Finite, and below any score of finite rows: the difference of two references is a number.  A score of -inf weighs nothing, one of +inf or a NaN
+// makes the sums NaN.
+constexpr float kPieceNone = -1e30f;
+constexpr float kPieceLazy = 8.f;
 
 // log2 of a value row's scale, of 2^-87 for one below it (a row of zeros; the smallest scale otherwise) and for NaN
 __device__ __forceinline__ float piece_log2_scale(float s) {

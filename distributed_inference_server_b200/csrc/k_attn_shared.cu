@@ -20,7 +20,6 @@
 // maximum grows by more than 8 in the log2 domain, so O is seldom rescaled (the reference cancels).
 // 8-bit pages: scales stay outside the products, as in k_attn_stream.cu; q and the weights are fp16 there, bf16 otherwise.
 #include <algorithm>
-#include <cfloat>
 
 #include <cuda_fp16.h>
 
@@ -33,7 +32,6 @@ constexpr int kSpBlock = kSpTile * 128;   // 64 keys x 64 dims, 16 bits
 constexpr int kSpQBlock = 128 * 128;      // 128 rows x 64 dims
 constexpr int kSpRaw = 3;                 // stages of 8-bit rows
 constexpr int kSpMaxSlices = 32;
-constexpr float kSpLazy = 8.f;
 
 template <int D, bool I8, bool kPair>
 struct SpCfg {
@@ -311,7 +309,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
 
     const int count = steps(g);
     const uint32_t o_addr = o_base + lane_off + g * D;
-    float m = -FLT_MAX, l = 0.f;
+    float m = kPieceNone, l = 0.f;
     bool ok = true;
     for (int i = 0; i < count; i++) {
       const int t = tile_of(g, i), slot = t % NS;
@@ -365,7 +363,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
         for (int c = 0; c < 32; c++) mx4[c & 3] = sp_max3(mx4[c & 3], s[c].x, s[c].y);
         mx = sp_max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * kLog2;  // the factor is positive: it commutes with the maximum
       }
-      const bool grow = mx > m + kSpLazy;
+      const bool grow = mx > m + kPieceLazy;
       if (__any_sync(0xffffffffu, grow)) {
         const float m_new = grow ? mx : m, f = piece_ex2(m - m_new);
         if (i > 0) {  // O holds the products of every step before this one; none is under way behind it
@@ -417,15 +415,14 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
     float f0 = 1.f, f1 = 0.f;
     bool other = false;
     if (!kPair) {
-      if (count == 0) m = -INFINITY;
       meet[g * 128 + row] = make_float2(m, l);
       tc_fence_before();
       asm volatile("bar.sync 1, 256;" ::: "memory");
       tc_fence_after();
       const float2 x = meet[row], y = meet[128 + row];
       m = fmaxf(x.x, y.x);
-      f0 = piece_weight(x.x, m);
-      f1 = piece_weight(y.x, m);
+      f0 = piece_ex2(x.x - m);
+      f1 = piece_ex2(y.x - m);
       other = n > 1;
       l = x.y * f0 + (other ? y.y * f1 : 0.f);
     }
@@ -577,7 +574,7 @@ attn_join_kernel(const SpArgs a, const float *__restrict__ own_o, const float *_
 #pragma unroll
     for (int j = 0; j < kSjUnroll; j++)
       if (s0 + j < slices) {
-        const float m_new = fmaxf(M, y[j].x), f = piece_weight(M, m_new), g = piece_weight(y[j].x, m_new);
+        const float m_new = fmaxf(M, y[j].x), f = piece_ex2(M - m_new), g = piece_ex2(y[j].x - m_new);
         M = m_new;
         l = l * f + y[j].y * g;
         o0.x = o0.x * f + u[j].x * g; o0.y = o0.y * f + u[j].y * g; o0.z = o0.z * f + u[j].z * g; o0.w = o0.w * f + u[j].w * g;

@@ -174,7 +174,7 @@ attn_stream_kernel(const StArgs a) {
     }
     if (!a.out)
       for (int i = threadIdx.x; i < n_heads; i += kStWarps * 32) {
-        a.state_ml[((size_t)t * n_heads + i) * 2] = -INFINITY;
+        a.state_ml[((size_t)t * n_heads + i) * 2] = kPieceNone;
         a.state_ml[((size_t)t * n_heads + i) * 2 + 1] = 0.f;
       }
   }
@@ -213,48 +213,76 @@ attn_stream_kernel(const StArgs a) {
   const uint32_t ring = smem_u32(st_smem) + warp * Cfg::kStages * Cfg::kStage;
   Cursor ahead = cur;
   int fetch = lo + warp, into = 0;                      // next tile to fetch, and its stage
-  int a_t = -1, a_keys = 0, win_first = 0, win = 0;     // of token a_t: keys, and 32 page numbers, one in each lane
+  int a_t = -1, a_keys = 0, a_first = 0, a_base = 0, win_first = 0, win = 0;  // of token a_t; 32 page numbers, one in each lane
   const int *a_pt = nullptr;
+  // A tile inside a page is one run of bytes: copy i of a lane is 512 bytes behind copy i - 1, there and (but for V's turn) here
+  constexpr int kCopies = Cfg::kPart / 512, kLaneRows = 32 / Cfg::kChunks;
+  const int lr = lane / Cfg::kChunks, lc = lane % Cfg::kChunks;
+  const uint32_t k_to = st_k_chunk<D, I8>(lr, lc) * 16;
+  uint32_t v_to[4];  // V's rows turn in eights
+#pragma unroll
+  for (int i = 0; i < 4; i++) v_to[i] = Cfg::kPart + st_v_chunk<D, I8>(i * kLaneRows % 8 + lr, lc) * 16 - i * kLaneRows % 8 * Cfg::kRow;
+  const long long v_rows = (long long)a.n_kv << a.page_shift;
+  const uint32_t lane_scale = (lane & 15) * 4 + (lane < 16 ? 0 : Cfg::kTok * 4) + 2 * Cfg::kPart;
+  const long long lane_scale_row = (lane & 15) + (lane < 16 ? 0 : v_rows);
+  auto page_of = [&](int pi, int last) {
+    if (pi < win_first || pi - win_first >= 32) {
+      win_first = pi;
+      win = a_pt[min(pi + lane, last)];
+    }
+    return (long long)__shfl_sync(0xffffffffu, win, pi - win_first);
+  };
   auto fetch_next = [&] {
     if (fetch < hi) {
-      while (fetch >= ahead.u1) next_pair(ahead);
+      if (fetch >= ahead.u1) {
+        do next_pair(ahead);
+        while (fetch >= ahead.u1);
+      }
       if (ahead.t != a_t) {
         a_t = ahead.t;
         a_keys = keys_of(a_t);
+        a_first = first_of(a_keys);
+        a_base = base_of(a_keys);
         a_pt = a.page_table + (size_t)a.pt_row[a_t] * a.max_pages;
         win_first = 1 << 30;
       }
-      const int first = first_of(a_keys), pos0 = base_of(a_keys) + (fetch - ahead.u0) * Cfg::kTok, last_page = (a_keys - 1) >> a.page_shift;
+      const int pos0 = a_base + (fetch - ahead.u0) * Cfg::kTok, last_page = (a_keys - 1) >> a.page_shift;
       const uint32_t dst = ring + into * Cfg::kStage;
-      long long row8[Cfg::kTok / 8];  // first row of every eight tokens' part of a page (pages are eight tokens or more)
-#pragma unroll
-      for (int e = 0; e < Cfg::kTok / 8; e++) {
-        const int pos = pos0 + 8 * e, pi = min(pos >> a.page_shift, last_page);
-        if (pi < win_first || pi - win_first >= 32) {
-          win_first = pi;
-          win = a_pt[min(pi + lane, last_page)];
-        }
-        const long long page = __shfl_sync(0xffffffffu, win, pi - win_first);
-        row8[e] = ((page * 2) * a.n_kv + ahead.h) * page_size + (pos & (page_size - 1));
-      }
-      const long long v_rows = (long long)a.n_kv * page_size;
       const char *pool = reinterpret_cast<const char *>(a.pool);
+      if (pos0 >= a_first && pos0 + Cfg::kTok <= a_keys && page_size >= Cfg::kTok) {
+        const long long row = ((page_of(pos0 >> a.page_shift, last_page) * 2 * a.n_kv + ahead.h) << a.page_shift) + (pos0 & (page_size - 1));
+        const char *k_src = pool + row * Cfg::kRow + lane * 16, *v_src = k_src + v_rows * Cfg::kRow;
 #pragma unroll
-      for (int i = 0; i < Cfg::kTok * Cfg::kChunks / 32; i++) {
-        const int id = i * 32 + lane, r = id / Cfg::kChunks, c = id % Cfg::kChunks;
-        const int e = i * (32 / Cfg::kChunks) / 8;
-        const long long row = row8[e] + (r & 7);
-        const bool in = pos0 + r >= first && pos0 + r < a_keys;
-        st_copy_16(dst + st_k_chunk<D, I8>(r, c) * 16, pool + row * Cfg::kRow + c * 16, in);
-        st_copy_16(dst + Cfg::kPart + st_v_chunk<D, I8>(r, c) * 16, pool + (row + v_rows) * Cfg::kRow + c * 16, in);
-      }
-      if (I8) {
+        for (int i = 0; i < kCopies; i++) {
+          st_copy_16(dst + k_to + i * 512, k_src + i * 512, true);
+          st_copy_16(dst + v_to[i & 3] + i * 512, v_src + i * 512, true);
+        }
+        if (I8) {
 #pragma unroll
-        for (int i = 0; i < Cfg::kSub; i++) {  // lanes 0-15: K, 16-31: V
-          const int r = i * 16 + (lane & 15);
-          const long long row = ((lane & 15) < 8 ? row8[2 * i] : row8[2 * i + 1]) + (r & 7) + (lane < 16 ? 0 : v_rows);
-          const bool in = pos0 + r >= first && pos0 + r < a_keys;
-          st_copy_4(dst + 2 * Cfg::kPart + ((lane < 16 ? 0 : Cfg::kTok) + r) * 4, a.scale + row, in);
+          for (int i = 0; i < Cfg::kSub; i++) st_copy_4(dst + lane_scale + i * 64, a.scale + row + lane_scale_row + i * 16, true);
+        }
+      } else {  // a history's first and last tile, pages that end inside a tile: rows one by one, zeros where they are not visible
+        long long row8[Cfg::kTok / 8];  // first row of every eight tokens' part of a page (pages are eight tokens or more)
+#pragma unroll
+        for (int e = 0; e < Cfg::kTok / 8; e++) {
+          const int pos = pos0 + 8 * e;
+          row8[e] = ((page_of(min(pos >> a.page_shift, last_page), last_page) * 2 * a.n_kv + ahead.h) << a.page_shift) + (pos & (page_size - 1));
+        }
+#pragma unroll
+        for (int i = 0; i < kCopies; i++) {
+          const int r = i * kLaneRows + lr;
+          const long long row = row8[i * kLaneRows / 8] + (r & 7);
+          const bool in = pos0 + r >= a_first && pos0 + r < a_keys;
+          st_copy_16(dst + k_to + i * 512, pool + row * Cfg::kRow + lc * 16, in);
+          st_copy_16(dst + v_to[i & 3] + i * 512, pool + (row + v_rows) * Cfg::kRow + lc * 16, in);
+        }
+        if (I8) {
+#pragma unroll
+          for (int i = 0; i < Cfg::kSub; i++) {  // lanes 0-15: K, 16-31: V
+            const int r = i * 16 + (lane & 15);
+            const long long row = ((lane & 15) < 8 ? row8[2 * i] : row8[2 * i + 1]) + (r & 7) + (lane < 16 ? 0 : v_rows);
+            st_copy_4(dst + lane_scale + i * 64, a.scale + row, pos0 + r >= a_first && pos0 + r < a_keys);
+          }
         }
       }
       fetch += kStWarps;
@@ -323,7 +351,7 @@ attn_stream_kernel(const StArgs a) {
     float oacc[KS][4];  // O^T: dims g kPer + 2 m (+ 1) of columns 2 tq (+ 1): {dim, column}, {dim, column + 1}, {dim + 1, column}, ..
 #pragma unroll
     for (int m = 0; m < KS; m++) { oacc[m][0] = 0.f; oacc[m][1] = 0.f; oacc[m][2] = 0.f; oacc[m][3] = 0.f; }
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    float m_run[2] = {kPieceNone, kPieceNone}, l_run[2] = {0.f, 0.f};
 
     for (; tile < end; tile += kStWarps) {
       st_copy_wait<Cfg::kStages - 2>();
@@ -357,7 +385,7 @@ attn_stream_kernel(const StArgs a) {
             st_mma<I8>(sa[1], x[2], y[2], x[3], y[3], qb[2 * i + 1][0], qb[2 * i + 1][1]);
           }
         }
-        // ---- running maximum; the whole warp acts only where one of its maxima grows
+        // ---- the reference follows the maximum where that grows by more than kPieceLazy; the whole warp acts then
         float k_f[2] = {1.f, 1.f}, v_f[2] = {1.f, 1.f};
         if (I8) {
           const uint32_t sc = at + 2 * Cfg::kPart + r0 * 4;
@@ -374,7 +402,7 @@ attn_stream_kernel(const StArgs a) {
           p[2 + e] = in1 ? (sa[0][2 + e] + sa[1][2 + e]) * (k_f[1] * qf[e]) : -INFINITY;
           mx[e] = fmaxf(p[e] + up0, p[2 + e] + up1);
         }
-        if (__any_sync(0xffffffffu, mx[0] > m_run[0] || mx[1] > m_run[1])) {
+        if (__any_sync(0xffffffffu, mx[0] > m_run[0] + kPieceLazy || mx[1] > m_run[1] + kPieceLazy)) {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; e++) {
@@ -383,7 +411,7 @@ attn_stream_kernel(const StArgs a) {
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
             const float m_new = fmaxf(m_run[e], x);
-            f[e] = piece_weight(m_run[e], m_new);
+            f[e] = piece_ex2(m_run[e] - m_new);
             l_run[e] *= f[e];
             m_run[e] = m_new;
           }
@@ -392,8 +420,8 @@ attn_stream_kernel(const StArgs a) {
         }
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          p[e] = piece_weight(p[e], m_run[e]);
-          p[2 + e] = piece_weight(p[2 + e], m_run[e]);
+          p[e] = piece_ex2(p[e] - m_run[e]);
+          p[2 + e] = piece_ex2(p[2 + e] - m_run[e]);
           l_run[e] += p[e] + p[2 + e];
         }
         uint32_t pb0, pb1, pl0 = 0u, pl1 = 0u;
@@ -503,13 +531,13 @@ attn_stream_kernel(const StArgs a) {
       __syncthreads();
       for (int it = threadIdx.x; it < kMeet * (D / 2); it += kStWarps * 32) {
         const int hh = it / (D / 2), h = h0 + hh, i = it % (D / 2), off = (2 * i) / kPer * (kPer + 2) + (2 * i) % kPer;
-        float M = -INFINITY, l = 0.f;
+        float M = kPieceNone, l = 0.f;
 #pragma unroll
         for (int w = 0; w < kStWarps; w++) M = fmaxf(M, s_m[w][h]);
         float2 o = make_float2(0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kStWarps; w++) {
-          const float f = piece_weight(s_m[w][h], M);
+          const float f = piece_ex2(s_m[w][h] - M);
           const float2 x = *reinterpret_cast<const float2 *>(s_o + (w * kMeet + hh) * Cfg::kHead + off);
           o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y);
           l = fmaf(s_l[w][h], f, l);
@@ -533,33 +561,45 @@ attn_stream_kernel(const StArgs a) {
       }
       __syncthreads();
       if (s_last) {
-        for (int it = threadIdx.x; it < G * (D / 2); it += kStWarps * 32) {
-          const int h = it / (D / 2), i = it % (D / 2);
-          float M = -INFINITY, l = 0.f;
-          float2 o = make_float2(0.f, 0.f);
-          for (int c0 = c_first; c0 <= c_last; c0 += 8) {  // eight pieces on their way at a time
-            float2 ml[8], x[8];
+        // four dims of a head to a thread at a time, as many pieces on their way as registers hold
+        constexpr int kQuads = G * D / 4, kTurns = (kQuads + kStWarps * 32 - 1) / (kStWarps * 32), kAhead = 8;
+        float M[kTurns], l[kTurns];
+        float4 o[kTurns];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-              const int c = c0 + j;
-              if (c <= c_last) {
-                const size_t sl = ((size_t)2 * c + (c == c_first ? 1 : 0)) * G + h;
-                ml[j] = __ldcg(reinterpret_cast<const float2 *>(a.piece_ml + sl * 2));
-                x[j] = __ldcg(reinterpret_cast<const float2 *>(a.piece_o + sl * D + 2 * i));
-              }
-            }
+        for (int k = 0; k < kTurns; k++) { M[k] = kPieceNone; l[k] = 0.f; o[k] = make_float4(0.f, 0.f, 0.f, 0.f); }
+        for (int c0 = c_first; c0 <= c_last; c0 += kAhead / kTurns) {
+          float2 ml[kAhead];
+          float4 x[kAhead];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-              if (c0 + j <= c_last) {
-                const float m_new = fmaxf(M, ml[j].x), f = piece_weight(M, m_new), fn = piece_weight(ml[j].x, m_new);
-                M = m_new;
-                l = l * f + ml[j].y * fn;
-                o.x = o.x * f + x[j].x * fn;
-                o.y = o.y * f + x[j].y * fn;
-              }
+          for (int j = 0; j < kAhead; j++) {
+            const int c = c0 + j / kTurns, quad = threadIdx.x + j % kTurns * kStWarps * 32;
+            if (c <= c_last && quad < kQuads) {
+              const size_t sl = (size_t)2 * c + (c == c_first ? 1 : 0);
+              ml[j] = __ldcg(reinterpret_cast<const float2 *>(a.piece_ml) + sl * G + quad / (D / 4));
+              x[j] = __ldcg(reinterpret_cast<const float4 *>(a.piece_o) + sl * kQuads + quad);
             }
           }
-          put(h, i, o, M, l);
+#pragma unroll
+          for (int j = 0; j < kAhead; j++) {
+            const int k = j % kTurns;
+            if (c0 + j / kTurns <= c_last && threadIdx.x + k * kStWarps * 32 < kQuads) {
+              const float m_new = fmaxf(M[k], ml[j].x), f = piece_ex2(M[k] - m_new), fn = piece_ex2(ml[j].x - m_new);
+              M[k] = m_new;
+              l[k] = l[k] * f + ml[j].y * fn;
+              o[k].x = o[k].x * f + x[j].x * fn;
+              o[k].y = o[k].y * f + x[j].y * fn;
+              o[k].z = o[k].z * f + x[j].z * fn;
+              o[k].w = o[k].w * f + x[j].w * fn;
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kTurns; k++) {
+          const int quad = threadIdx.x + k * kStWarps * 32, h = quad / (D / 4), i = quad % (D / 4) * 2;
+          if (quad < kQuads) {
+            put(h, i, make_float2(o[k].x, o[k].y), M[k], l[k]);
+            put(h, i + 1, make_float2(o[k].z, o[k].w), M[k], l[k]);
+          }
         }
       }
     }
