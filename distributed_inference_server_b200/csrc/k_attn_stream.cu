@@ -27,8 +27,8 @@
 namespace dis {
 
 constexpr int kStWarps = 4;
-constexpr int kStMaxT = 1024;           // tokens of one launch
-constexpr int kStMaxUnits = 1 << 16;    // (token, kv head) pairs of one launch: one counter each
+constexpr int kStMaxT = 512;            // tokens of one launch
+constexpr int kStCounters = 1 << 16;    // words kept for counters, of which two for each of a CTA's two pieces are used
 constexpr int kStMinShare = 2 * kStWarps;  // tiles of a CTA, at least
 
 template <int D, bool I8>
@@ -43,7 +43,7 @@ struct StCfg {
   static constexpr int kHead = 16 * (D / 16 + 1) + 4;     // floats between two heads' O in the merge: no bank twice in a half warp
   static constexpr int kCtas = I8 ? 3 : 2;                // per SM
   static constexpr int kRing = kStWarps * kStages * kStage;
-  static constexpr int meet(int G) { return G < 4 ? G : 4; }  // heads whose states meet in shared memory at a time
+  static constexpr int meet(int G) { return G * D <= 512 ? G : 512 / D; }  // heads whose states meet in shared memory at a time
   static constexpr int fixed(int G) { return kRing + kStWarps * meet(G) * kHead * 4; }
 };
 
@@ -102,6 +102,11 @@ __device__ __forceinline__ uint32_t st_transpose(uint32_t v) {  // an 8x8 matrix
   return r;
 }
 
+// floats of a piece's (m, l): whole 16 bytes
+__host__ __device__ constexpr int st_ml(int G) { return G < 2 ? 4 : 2 * G; }
+
+__host__ __device__ constexpr size_t stream_slots(int per_sm) { return 2 * (size_t)kNumSMs * per_sm; }
+
 struct StArgs {
   const uint16_t *q;
   const void *pool;
@@ -112,8 +117,9 @@ struct StArgs {
   int first;               // keys in front of this position are somebody else's, for the tokens that reach it
   uint16_t *out;           // the result, or nullptr: the states go to state_o, state_ml
   float *state_o, *state_ml;
-  int *counters;           // [T * n_kv], zero between calls
-  float *piece_o, *piece_ml;  // [2 per CTA][G][D], [2 per CTA][G][2]
+  int *counters;           // [2][2 per CTA], zero between calls
+  float *piece_o, *piece_ml;  // [2 per CTA][G][D], [2 per CTA][st_ml(G)]
+  float *group_o, *group_ml;  // of pieces joined, likewise
   int T, n_kv, page_shift;
   int late_wait;           // the kernel in front was told to let this one start once its own inputs were complete: wait for it at the end
 };
@@ -129,14 +135,14 @@ attn_stream_kernel(const StArgs a) {
   extern __shared__ __align__(16) uint8_t st_smem[];
   float *s_o = reinterpret_cast<float *>(st_smem + Cfg::kRing);  // [warp][kMeet heads][kHead]
   int *s_tiles = reinterpret_cast<int *>(s_o + kStWarps * kMeet * Cfg::kHead);  // [T + 1]: tiles of a kv head in front of token t
+  int *s_keys = s_tiles + a.T + 1, *s_row = s_keys + a.T;                          // [T] keys, page-table rows
   __shared__ float s_m[kStWarps][8], s_l[kStWarps][8];
-  __shared__ int s_scan[kStWarps], s_last;
+  __shared__ int s_scan[kStWarps], s_last[2];
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   pdl_launch_dependents();
   if (!a.late_wait) pdl_wait();
   const int n_heads = a.n_kv * G, page_size = 1 << a.page_shift, base0 = a.first / Cfg::kTok * Cfg::kTok;
-  auto keys_of = [&](int t) { return min(a.ctx[t], a.max_pages << a.page_shift); };
   auto first_of = [&](int keys) { return keys < a.first ? 0 : a.first; };  // a history that ends in front of it is all this kernel's
   auto base_of = [&](int keys) { return keys < a.first ? 0 : base0; };
 
@@ -145,7 +151,9 @@ attn_stream_kernel(const StArgs a) {
     const int t = t0 + threadIdx.x;
     int n = 0;
     if (t < a.T) {
-      const int keys = keys_of(t);
+      const int keys = min(a.ctx[t], a.max_pages << a.page_shift);
+      s_row[t] = a.pt_row[t];
+      s_keys[t] = keys;
       n = keys > first_of(keys) ? (keys - base_of(keys) + Cfg::kTok - 1) / Cfg::kTok : 0;
     }
     int x = n;
@@ -237,13 +245,15 @@ attn_stream_kernel(const StArgs a) {
       if (fetch >= ahead.u1) {
         do next_pair(ahead);
         while (fetch >= ahead.u1);
+        // its queries, on their way to L1 while the tiles in front of its first are taken
+        if (lane < G * D / 64) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.q + ((size_t)ahead.t * n_heads + ahead.h * G) * D + lane * 64));
       }
       if (ahead.t != a_t) {
         a_t = ahead.t;
-        a_keys = keys_of(a_t);
+        a_keys = s_keys[a_t];
         a_first = first_of(a_keys);
         a_base = base_of(a_keys);
-        a_pt = a.page_table + (size_t)a.pt_row[a_t] * a.max_pages;
+        a_pt = a.page_table + (size_t)s_row[a_t] * a.max_pages;
         win_first = 1 << 30;
       }
       const int pos0 = a_base + (fetch - ahead.u0) * Cfg::kTok, last_page = (a_keys - 1) >> a.page_shift;
@@ -262,26 +272,17 @@ attn_stream_kernel(const StArgs a) {
           for (int i = 0; i < Cfg::kSub; i++) st_copy_4(dst + lane_scale + i * 64, a.scale + row + lane_scale_row + i * 16, true);
         }
       } else {  // a history's first and last tile, pages that end inside a tile: rows one by one, zeros where they are not visible
-        long long row8[Cfg::kTok / 8];  // first row of every eight tokens' part of a page (pages are eight tokens or more)
-#pragma unroll
-        for (int e = 0; e < Cfg::kTok / 8; e++) {
-          const int pos = pos0 + 8 * e;
-          row8[e] = ((page_of(min(pos >> a.page_shift, last_page), last_page) * 2 * a.n_kv + ahead.h) << a.page_shift) + (pos & (page_size - 1));
-        }
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < kCopies; i++) {
-          const int r = i * kLaneRows + lr;
-          const long long row = row8[i * kLaneRows / 8] + (r & 7);
+          const int r = i * kLaneRows + lr, pos = pos0 + i * kLaneRows / 8 * 8;  // (pages are eight tokens or more)
+          const long long page = page_of(min(pos >> a.page_shift, last_page), last_page);
+          const long long row = ((page * 2 * a.n_kv + ahead.h) << a.page_shift) + (pos & (page_size - 1)) + (r & 7);
           const bool in = pos0 + r >= a_first && pos0 + r < a_keys;
           st_copy_16(dst + k_to + i * 512, pool + row * Cfg::kRow + lc * 16, in);
-          st_copy_16(dst + v_to[i & 3] + i * 512, pool + (row + v_rows) * Cfg::kRow + lc * 16, in);
-        }
-        if (I8) {
-#pragma unroll
-          for (int i = 0; i < Cfg::kSub; i++) {  // lanes 0-15: K, 16-31: V
-            const int r = i * 16 + (lane & 15);
-            const long long row = ((lane & 15) < 8 ? row8[2 * i] : row8[2 * i + 1]) + (r & 7) + (lane < 16 ? 0 : v_rows);
-            st_copy_4(dst + lane_scale + i * 64, a.scale + row, pos0 + r >= a_first && pos0 + r < a_keys);
+          st_copy_16(dst + Cfg::kPart + st_v_chunk<D, I8>(r, lc) * 16, pool + (row + v_rows) * Cfg::kRow + lc * 16, in);
+          if (I8 && lc == 0) {
+            st_copy_4(dst + 2 * Cfg::kPart + r * 4, a.scale + row, in);
+            st_copy_4(dst + 2 * Cfg::kPart + (Cfg::kTok + r) * 4, a.scale + row + v_rows, in);
           }
         }
       }
@@ -290,16 +291,32 @@ attn_stream_kernel(const StArgs a) {
     into = into + 1 == Cfg::kStages ? 0 : into + 1;
     st_copy_end();
   };
-  if (lo < hi) {
-#pragma unroll
-    for (int i = 0; i < Cfg::kStages - 1; i++) fetch_next();
-  }
 
   constexpr float kScale = (D == 128 ? 0.08838834764831845f : 0.125f) * 1.4426950408889634f;  // scores are kept in the log2 domain
   int tile = lo + warp, stage = 0;
-  while (cur.u0 < hi && lo < hi) {
+  if (lo < hi) {
+#pragma unroll 1
+    for (int i = 0; i < Cfg::kStages - 1; i++) fetch_next();
+  }
+  auto put = [&](size_t head, int i, float4 o, float m, float l) {  // four dims of a token's head
+    if (a.out) {
+      uint32_t *to = reinterpret_cast<uint32_t *>(a.out + head * D + i);
+      to[0] = float2_to_bf16x2(o.x / l, o.y / l);
+      to[1] = float2_to_bf16x2(o.z / l, o.w / l);
+    } else {
+      *reinterpret_cast<float4 *>(a.state_o + head * D + i) = o;
+      if (i == 0) *reinterpret_cast<float2 *>(a.state_ml + head * 2) = make_float2(m, l);
+    }
+  };
+  size_t part_row[2] = {0, 0};
+  int part_first[2] = {0, 0}, part_last[2] = {0, 0};
+  while (lo < hi) {
     // ================= one piece: tiles [max(u0, lo), min(u1, hi)) of a pair
-    const int end = min(cur.u1, hi), keys = keys_of(cur.t), first = first_of(keys), base = base_of(keys);
+    float oacc[KS][4];  // O^T: dims g kPer + 2 m (+ 1) of columns 2 tq (+ 1): {dim, column}, {dim, column + 1}, {dim + 1, column}, ..
+#pragma unroll
+    for (int m = 0; m < KS; m++) { oacc[m][0] = 0.f; oacc[m][1] = 0.f; oacc[m][2] = 0.f; oacc[m][3] = 0.f; }
+    float m_run[2] = {kPieceNone, kPieceNone}, l_run[2] = {0.f, 0.f};
+    const int end = min(cur.u1, hi), keys = s_keys[cur.t], first = first_of(keys), base = base_of(keys);
     // Q as the B operand: column g is head g (kTwice: the next G columns repeat it)
     uint32_t qb[KS][2];
     float qf[2] = {kScale, kScale};  // factor of the scores of columns 2 tq, 2 tq + 1
@@ -348,11 +365,6 @@ attn_stream_kernel(const StArgs a) {
         }
       }
     }
-    float oacc[KS][4];  // O^T: dims g kPer + 2 m (+ 1) of columns 2 tq (+ 1): {dim, column}, {dim, column + 1}, {dim + 1, column}, ..
-#pragma unroll
-    for (int m = 0; m < KS; m++) { oacc[m][0] = 0.f; oacc[m][1] = 0.f; oacc[m][2] = 0.f; oacc[m][3] = 0.f; }
-    float m_run[2] = {kPieceNone, kPieceNone}, l_run[2] = {0.f, 0.f};
-
     for (; tile < end; tile += kStWarps) {
       st_copy_wait<Cfg::kStages - 2>();
       __syncwarp();
@@ -392,16 +404,20 @@ attn_stream_kernel(const StArgs a) {
           k_f[0] = st_lds_f(sc); k_f[1] = st_lds_f(sc + 32);
           v_f[0] = st_lds_f(sc + Cfg::kTok * 4); v_f[1] = st_lds_f(sc + Cfg::kTok * 4 + 32);
         }
-        const int p0 = pos0 + r0, p1 = p0 + 8;
-        const bool in0 = p0 < keys && p0 >= first, in1 = p1 < keys && p1 >= first;
         const float up0 = I8 ? piece_log2_scale(v_f[0]) : 0.f, up1 = I8 ? piece_log2_scale(v_f[1]) : 0.f;
-        float p[4], mx[2];
+        float p[4], mx[2];  // p: scores without the head's factor
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          p[e] = in0 ? (sa[0][e] + sa[1][e]) * (k_f[0] * qf[e]) : -INFINITY;
-          p[2 + e] = in1 ? (sa[0][2 + e] + sa[1][2 + e]) * (k_f[1] * qf[e]) : -INFINITY;
-          mx[e] = fmaxf(p[e] + up0, p[2 + e] + up1);
+          p[e] = (sa[0][e] + sa[1][e]) * k_f[0];
+          p[2 + e] = (sa[0][2 + e] + sa[1][2 + e]) * k_f[1];
         }
+        if (pos0 < first || pos0 + Cfg::kTok > keys) {  // (uniform)
+          const int p0 = pos0 + r0, p1 = p0 + 8;
+          if (p0 < first || p0 >= keys) p[0] = p[1] = -INFINITY;
+          if (p1 < first || p1 >= keys) p[2] = p[3] = -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) mx[e] = fmaxf(fmaf(p[e], qf[e], up0), fmaf(p[2 + e], qf[e], up1));
         if (__any_sync(0xffffffffu, mx[0] > m_run[0] + kPieceLazy || mx[1] > m_run[1] + kPieceLazy)) {
           float f[2];
 #pragma unroll
@@ -420,8 +436,8 @@ attn_stream_kernel(const StArgs a) {
         }
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          p[e] = piece_ex2(p[e] - m_run[e]);
-          p[2 + e] = piece_ex2(p[2 + e] - m_run[e]);
+          p[e] = piece_ex2(fmaf(p[e], qf[e], -m_run[e]));
+          p[2 + e] = piece_ex2(fmaf(p[2 + e], qf[e], -m_run[e]));
           l_run[e] += p[e] + p[2 + e];
         }
         uint32_t pb0, pb1, pl0 = 0u, pl1 = 0u;
@@ -505,17 +521,10 @@ attn_stream_kernel(const StArgs a) {
 #pragma unroll
       for (int e = 0; e < 2; e++) { s_m[warp][2 * tq + e] = m_run[e]; s_l[warp][2 * tq + e] = l_run[e]; }
     }
+    const size_t row = (size_t)cur.t * n_heads + cur.h * G;             // of the pair's first head in the result
     const int c_first = cur.u0 / share, c_last = (cur.u1 - 1) / share;  // the CTAs that have a piece of this history
-    const int slot = 2 * blockIdx.x + (cur.u0 >= lo ? 1 : 0);
-    const size_t row = (size_t)cur.t * n_heads + cur.h * G;
-    auto put = [&](int h, int i, float2 o, float m, float l) {  // dims 2 i, 2 i + 1 of head h
-      if (a.out) {
-        *reinterpret_cast<uint32_t *>(a.out + (row + h) * D + 2 * i) = float2_to_bf16x2(o.x / l, o.y / l);
-      } else {
-        *reinterpret_cast<float2 *>(a.state_o + (row + h) * D + 2 * i) = o;
-        if (i == 0) *reinterpret_cast<float2 *>(a.state_ml + (row + h) * 2) = make_float2(m, l);
-      }
-    };
+    const int side = cur.u0 >= lo ? 1 : 0;  // (of the histories that others have pieces of too, one was begun before, one goes on)
+    const size_t slot = 2 * (size_t)blockIdx.x + side;
 #pragma unroll
     for (int h0 = 0; h0 < G; h0 += kMeet) {
       if (h0) __syncthreads();
@@ -529,93 +538,131 @@ attn_stream_kernel(const StArgs a) {
         }
       }
       __syncthreads();
-      for (int it = threadIdx.x; it < kMeet * (D / 2); it += kStWarps * 32) {
-        const int hh = it / (D / 2), h = h0 + hh, i = it % (D / 2), off = (2 * i) / kPer * (kPer + 2) + (2 * i) % kPer;
+      const int hh = threadIdx.x / (D / 4), h = h0 + hh, i = threadIdx.x % (D / 4) * 4;  // four dims of a head
+      if (hh < kMeet) {
+        const int off = i / kPer * (kPer + 2) + i % kPer;
         float M = kPieceNone, l = 0.f;
 #pragma unroll
         for (int w = 0; w < kStWarps; w++) M = fmaxf(M, s_m[w][h]);
-        float2 o = make_float2(0.f, 0.f);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kStWarps; w++) {
           const float f = piece_ex2(s_m[w][h] - M);
-          const float2 x = *reinterpret_cast<const float2 *>(s_o + (w * kMeet + hh) * Cfg::kHead + off);
-          o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y);
+          const float2 *x = reinterpret_cast<const float2 *>(s_o + (w * kMeet + hh) * Cfg::kHead + off), y = x[0], z = x[1];
+          o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(z.x, f, o.z); o.w = fmaf(z.y, f, o.w);
           l = fmaf(s_l[w][h], f, l);
         }
         if (c_first == c_last) {
-          put(h, i, o, M, l);
+          put(row + h, i, o, M, l);
         } else {
-          __stcg(reinterpret_cast<float2 *>(a.piece_o + ((size_t)slot * G + h) * D + 2 * i), o);
-          if (i == 0) __stcg(reinterpret_cast<float2 *>(a.piece_ml + ((size_t)slot * G + h) * 2), make_float2(M, l));
+          __stcg(reinterpret_cast<float4 *>(a.piece_o + (slot * G + h) * D + i), o);
+          if (i == 0) __stcg(reinterpret_cast<float2 *>(a.piece_ml + slot * st_ml(G) + 2 * h), make_float2(M, l));
         }
       }
     }
     if (c_first != c_last) {
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        int *count = a.counters + cur.t * a.n_kv + cur.h;
-        s_last = atomicAdd(count, 1) == c_last - c_first;
-        if (s_last) *count = 0;  // as the next call wants it
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_last) {
-        // four dims of a head to a thread at a time, as many pieces on their way as registers hold
-        constexpr int kQuads = G * D / 4, kTurns = (kQuads + kStWarps * 32 - 1) / (kStWarps * 32), kAhead = 8;
-        float M[kTurns], l[kTurns];
-        float4 o[kTurns];
-#pragma unroll
-        for (int k = 0; k < kTurns; k++) { M[k] = kPieceNone; l[k] = 0.f; o[k] = make_float4(0.f, 0.f, 0.f, 0.f); }
-        for (int c0 = c_first; c0 <= c_last; c0 += kAhead / kTurns) {
-          float2 ml[kAhead];
-          float4 x[kAhead];
-#pragma unroll
-          for (int j = 0; j < kAhead; j++) {
-            const int c = c0 + j / kTurns, quad = threadIdx.x + j % kTurns * kStWarps * 32;
-            if (c <= c_last && quad < kQuads) {
-              const size_t sl = (size_t)2 * c + (c == c_first ? 1 : 0);
-              ml[j] = __ldcg(reinterpret_cast<const float2 *>(a.piece_ml) + sl * G + quad / (D / 4));
-              x[j] = __ldcg(reinterpret_cast<const float4 *>(a.piece_o) + sl * kQuads + quad);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < kAhead; j++) {
-            const int k = j % kTurns;
-            if (c0 + j / kTurns <= c_last && threadIdx.x + k * kStWarps * 32 < kQuads) {
-              const float m_new = fmaxf(M[k], ml[j].x), f = piece_ex2(M[k] - m_new), fn = piece_ex2(ml[j].x - m_new);
-              M[k] = m_new;
-              l[k] = l[k] * f + ml[j].y * fn;
-              o[k].x = o[k].x * f + x[j].x * fn;
-              o[k].y = o[k].y * f + x[j].y * fn;
-              o[k].z = o[k].z * f + x[j].z * fn;
-              o[k].w = o[k].w * f + x[j].w * fn;
-            }
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < kTurns; k++) {
-          const int quad = threadIdx.x + k * kStWarps * 32, h = quad / (D / 4), i = quad % (D / 4) * 2;
-          if (quad < kQuads) {
-            put(h, i, make_float2(o[k].x, o[k].y), M[k], l[k]);
-            put(h, i + 1, make_float2(o[k].z, o[k].w), M[k], l[k]);
-          }
-        }
-      }
+      if (side) { part_row[1] = row; part_first[1] = c_first; part_last[1] = c_last; }
+      else { part_row[0] = row; part_first[0] = c_first; part_last[0] = c_last; }
     }
-    __syncthreads();  // the next piece's states may come
     if (cur.u1 >= hi) break;
     next_pair(cur);
+    __syncthreads();  // the next piece's states may come
   }
   st_copy_wait<0>();
+  st_copy_wait<0>();
+
+  // ================= histories in several CTAs: the one that ends last joins the pieces, in the order of the history.  More than eight are joined in
+  // about as many groups as a group has pieces, and then the groups: what one CTA reads at the end stays short however long the history is.  The
+  // barriers and one thread's fences on both sides order all threads' writes and reads; both histories' first counts share them
+  if (part_first[0] != part_last[0] || part_first[1] != part_last[1]) {
+    auto fan_of = [&](int parts) { return parts <= 8 ? parts : (int)ceilf(sqrtf((float)parts)); };
+    auto arrive = [&](int level, size_t slot, int n) {
+      int *count = a.counters + level * stream_slots(3) + slot;
+      __threadfence();
+      const bool last = atomicAdd(count, 1) == n - 1;
+      if (last) *count = 0;  // as the next call wants it
+      __threadfence();
+      return last;
+    };
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      const int c_first = threadIdx.x ? part_first[1] : part_first[0], c_last = threadIdx.x ? part_last[1] : part_last[0];
+      bool last = false;
+      if (c_first != c_last) {
+        const int fan = fan_of(c_last - c_first + 1), lead = c_first + ((int)blockIdx.x - c_first) / fan * fan;  // the group's first CTA
+        last = arrive(0, 2 * (size_t)lead + (lead == c_first ? 1 : 0), min(fan, c_last + 1 - lead));
+      }
+      s_last[threadIdx.x] = last;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int side = 0; side < 2; side++) {
+      if (!s_last[side]) continue;
+      const size_t row = side ? part_row[1] : part_row[0];
+      const int c_first = side ? part_first[1] : part_first[0], c_last = side ? part_last[1] : part_last[0];
+      const int parts = c_last - c_first + 1, fan = fan_of(parts), groups = (parts + fan - 1) / fan;
+      const int lead = c_first + ((int)blockIdx.x - c_first) / fan * fan;
+      auto slot_of = [&](int c) { return 2 * (size_t)c + (c == c_first ? 1 : 0); };
+      int n = min(fan, c_last + 1 - lead);
+#pragma unroll 1
+      for (int level = 0;; level++) {
+        if (level) {
+          __syncthreads();
+          if (threadIdx.x == 0) s_last[side] = arrive(1, slot_of(c_first), n);
+          __syncthreads();
+          if (!s_last[side]) break;
+        }
+        const bool whole = level || groups == 1;
+        const float *src_o = level ? a.group_o : a.piece_o, *src_ml = level ? a.group_ml : a.piece_ml;
+        // four dims of a head to a thread at a time, kAhead pieces' on their way
+        constexpr int kQuads = G * D / 4, kAhead = 8;
+#pragma unroll 1
+        for (int quad = threadIdx.x; quad < kQuads; quad += kStWarps * 32) {
+          const int h = quad / (D / 4), i = quad % (D / 4) * 4;
+          float M = kPieceNone, l = 0.f;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+          for (int k = 0; k < n; k += kAhead) {
+            float2 ml[kAhead];
+            float4 x[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; j++)
+              if (k + j < n) {
+                const size_t sl = slot_of(level ? c_first + (k + j) * fan : lead + k + j);
+                ml[j] = __ldcg(reinterpret_cast<const float2 *>(src_ml + sl * st_ml(G)) + h);
+                x[j] = __ldcg(reinterpret_cast<const float4 *>(src_o) + sl * kQuads + quad);
+              }
+#pragma unroll
+            for (int j = 0; j < kAhead; j++)
+              if (k + j < n) {
+                const float m_new = fmaxf(M, ml[j].x), f = piece_ex2(M - m_new), fn = piece_ex2(ml[j].x - m_new);
+                M = m_new;
+                l = l * f + ml[j].y * fn;
+                o.x = o.x * f + x[j].x * fn;
+                o.y = o.y * f + x[j].y * fn;
+                o.z = o.z * f + x[j].z * fn;
+                o.w = o.w * f + x[j].w * fn;
+              }
+          }
+          if (whole) {
+            put(row + h, i, o, M, l);
+          } else {
+            __stcg(reinterpret_cast<float4 *>(a.group_o) + slot_of(lead) * kQuads + quad, o);
+            if (i == 0) __stcg(reinterpret_cast<float2 *>(a.group_ml + slot_of(lead) * st_ml(G)) + h, make_float2(M, l));
+          }
+        }
+        if (whole) break;
+        n = groups;
+      }
+    }
+  }
   if (a.late_wait) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------------------- host
-static size_t stream_slots(int per_sm) { return 2 * (size_t)kNumSMs * per_sm; }
 size_t attn_stream_scratch_elems(int n_heads, int n_kv, int d) {  // counters, then the pieces of every resident CTA
   if (n_kv <= 0 || n_heads <= 0 || d <= 0) return 0;
-  return kStMaxUnits + stream_slots(3) * (size_t)(n_heads / n_kv) * (2 + (size_t)d);
+  return kStCounters + 2 * stream_slots(3) * ((size_t)(n_heads / n_kv) * d + st_ml(n_heads / n_kv));
 }
 
 template <int D, int G, bool I8>
@@ -624,8 +671,8 @@ static cudaError_t stream_launch(const StArgs &a, cudaStream_t st) {
   auto kern = attn_stream_kernel<D, G, I8>;
   constexpr int kFixed = Cfg::fixed(G);
   static DeviceOnce once;
-  DIS_CUDA_TRY(once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + (kStMaxT + 1) * 4); }));
-  return launch_k(kern, dim3(kNumSMs * Cfg::kCtas), dim3(kStWarps * 32), (size_t)kFixed + (a.T + 1) * 4, st, a);
+  DIS_CUDA_TRY(once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + (3 * kStMaxT + 1) * 4); }));
+  return launch_k(kern, dim3(kNumSMs * Cfg::kCtas), dim3(kStWarps * 32), (size_t)kFixed + (3 * a.T + 1) * 4, st, a);
 }
 
 template <bool I8>
@@ -642,15 +689,16 @@ static cudaError_t stream_dispatch(const StArgs &a, int G, int d, cudaStream_t s
 cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float *scale, const int *page_table, int max_pages, const int *pt_row,
                                const int *ctx, int first, uint16_t *out, float *state_o, float *state_ml, float *scratch, bool late_wait, int T,
                                int n_heads, int n_kv, int d, int page_size, cudaStream_t st) {
-  if (n_kv > kStMaxUnits) { set_last_error("attention over pieces: more than 65536 kv heads"); return cudaErrorInvalidValue; }
   // a launch's tiles are counted in 32 bits
   const long long most = ((long long)max_pages * page_size / 16 + 2) * n_kv;
-  const int G = n_heads / n_kv, step = (int)std::max(1ll, std::min({(long long)kStMaxT, (long long)kStMaxUnits / n_kv, 0x7fffffffll / most}));
+  const int G = n_heads / n_kv, step = (int)std::max(1ll, std::min({(long long)kStMaxT, 0x7fffffffll / most}));
   StArgs a{};
   a.pool = pool; a.scale = scale; a.page_table = page_table; a.max_pages = max_pages; a.first = first;
   a.counters = reinterpret_cast<int *>(scratch);
-  a.piece_o = scratch + kStMaxUnits;
-  a.piece_ml = a.piece_o + stream_slots(3) * (size_t)G * d;
+  a.piece_o = scratch + kStCounters;
+  a.group_o = a.piece_o + stream_slots(3) * (size_t)G * d;
+  a.piece_ml = a.group_o + stream_slots(3) * (size_t)G * d;
+  a.group_ml = a.piece_ml + stream_slots(3) * (size_t)st_ml(G);
   a.n_kv = n_kv;
   while ((1 << a.page_shift) < page_size) a.page_shift++;
   for (int t = 0; t < T; t += step) {
