@@ -308,6 +308,7 @@ static int cache_shape(const char *who, int T, int n_heads, int n_kv, int d, int
   else if (d != 64 && d != 128) what = "head_dim must be 64 or 128";
   else if (page_size < 8 || (page_size & (page_size - 1))) what = "page_size must be a power of two >= 8";
   else if (max_pages < 1 || (long long)max_pages * page_size > 0x7fffffffll) what = "max_pages must be positive and a table's row end below position 2^31";
+  else if (2ll * n_kv * page_size * d > 0x7fffffffll) what = "page_size: a page of 2^31 entries or more";
   if (!what) return DIS_OK;
   dis::set_last_error(std::string(who) + ": " + what);
   return DIS_ERR_INVALID_ARGUMENT;
