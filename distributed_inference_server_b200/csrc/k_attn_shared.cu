@@ -45,7 +45,8 @@ struct SpCfg {
   static constexpr int kRawScale = kRaw + (I8 ? kSpRaw * kRawBytes : 0);
   static constexpr int kScale = kRawScale + (I8 ? kSpRaw * 2 * kSpTile * 4 : 0);
   static constexpr int kMeet = kScale + (I8 ? kRing * kScaleFloats * 4 : 0);  // [group][row] (m, l)
-  static constexpr int kBars = kMeet + 2 * 128 * 8;
+  static constexpr int kUp = kMeet + 2 * 128 * 8;  // the rows' powers of two
+  static constexpr int kBars = kUp + 256 * 4;
   static constexpr int kSmem = kBars + 512;
   static constexpr int kThreads = I8 ? 512 : 384;
 };
@@ -264,49 +265,48 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
     const int g = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     constexpr float kLog2 = (D == 128 ? 0.08838834764831845f : 0.125f) * 1.4426950408889634f;
-    float q_up = 1.f;
-    {  // the query rows: K-major, 128B swizzle; rows behind the last are zeros.  One tile: each group brings half of every row
-      const int rt = rt0 + (kPair ? g : 0), rho = rt * 128 + row, t = rho >> a.g_shift;
-      const bool in = t < a.T;
-      const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (((size_t)t * a.n_kv + kvh) * (1 << a.g_shift) + (rho & ((1 << a.g_shift) - 1))) * D);
-      float down = 1.f;
-      if (I8) {  // fp16 after a power of two that brings the row's largest entry to [2^13, 2^14)
-        uint32_t big = 0;
-        if (in)
-          for (int c = 0; c < D / 8; c++) {
-            const uint4 v = src[c];
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    {  // The query rows: K-major, 128B swizzle, rows behind the last zeros; D / 8 lanes take a row.  The eight warps have 16 rows each of the one tile,
+       // or a group's four 32 each of the group's
+      constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kMine = kPair ? 32 : 16;
+      const int c = lane % kLanes, first_row = (kPair ? (warp & 3) : warp - 4) * kMine + lane / kLanes, rho0 = (rt0 + (kPair ? g : 0)) * 128;
+      uint4 v[kMine / kAtOnce];
 #pragma unroll
-            for (int k = 0; k < 4; k++) big = max(big, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-          }
-        const int ex = min(max((int)(big >> 7) - 127 - 13, -100), 100);
-        down = __int_as_float((127 - ex) << 23);
-        q_up = __int_as_float((127 + ex) << 23);
+      for (int k = 0; k < kMine / kAtOnce; k++) {
+        const int rho = rho0 + first_row + k * kAtOnce, t = rho >> a.g_shift;
+        v[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (t < a.T) v[k] = reinterpret_cast<const uint4 *>(a.q + (((size_t)t * a.n_kv + kvh) * (1 << a.g_shift) + (rho & ((1 << a.g_shift) - 1))) * D)[c];
       }
-      constexpr int kMine = kPair ? D / 8 : D / 16;
 #pragma unroll
-      for (int cc = 0; cc < kMine; cc++) {
-        const int c = (kPair ? 0 : g * kMine) + cc;
-        uint4 v = in ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-        if (I8) {
-          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      for (int k = 0; k < kMine / kAtOnce; k++) {
+        const int row = first_row + k * kAtOnce;
+        if (I8) {  // fp16 after a power of two that brings the row's largest entry to [2^13, 2^14)
+          uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w}, big = 0;
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const float2 f = bf16x2_to_float2(w[k]);
+          for (int j = 0; j < 4; j++) big = max(big, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
+#pragma unroll
+          for (int o = kLanes >> 1; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+          const int ex = min(max((int)(big >> 7) - 127 - 13, -100), 100);
+          const float down = __int_as_float((127 - ex) << 23);
+          if (c == 0) reinterpret_cast<float *>(sp_smem + Cfg::kUp)[(kPair ? g * 128 : 0) + row] = __int_as_float((127 + ex) << 23);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float2 f = bf16x2_to_float2(w[j]);
             const __half2 h = __floats2half2_rn(f.x * down, f.y * down);
-            w[k] = *reinterpret_cast<const uint32_t *>(&h);
+            w[j] = *reinterpret_cast<const uint32_t *>(&h);
           }
-          v = make_uint4(w[0], w[1], w[2], w[3]);
+          v[k] = make_uint4(w[0], w[1], w[2], w[3]);
         }
         const uint32_t off = (uint32_t)Cfg::kQ + (kPair ? g * kHalves * kSpQBlock : 0) + (uint32_t)(c >> 3) * kSpQBlock + (uint32_t)(row >> 3) * 1024 +
                              (uint32_t)(row & 7) * 128 + (uint32_t)(((c & 7) ^ (row & 7)) << 4);
-        *reinterpret_cast<uint4 *>(sp_smem + off) = v;
+        *reinterpret_cast<uint4 *>(sp_smem + off) = v[k];
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
 
+    float q_up = 1.f;
+    if (I8 && sp_wait(q_full, 0, fail)) q_up = reinterpret_cast<const float *>(sp_smem + Cfg::kUp)[(kPair ? g * 128 : 0) + row];
     const int count = steps(g);
     const uint32_t o_addr = o_base + lane_off + g * D;
     float m = kPieceNone, l = 0.f;
