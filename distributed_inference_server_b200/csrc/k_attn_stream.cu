@@ -13,7 +13,7 @@
 // which k index of K Q^T is free as long as Q agrees, so a lane's 16 bytes of a K row are its operand of four k-steps; and a lane's 16 dims of two
 // V rows, bytes interleaved, are its operand of eight m-tiles, the transposition being part of the conversion.
 //
-// Work: the histories of all (token, kv head) pairs laid end to end in tiles of 16 tokens (32 for 8-bit heads of 64), cut into equal shares, one per
+// Work: the histories of all (token, kv head) pairs laid end to end in tiles of 16 tokens, cut into equal shares, one per
 // resident CTA, whatever the lengths are: lengths are read on the device, nothing depends on their maximum.  The CTA's four warps take its
 // tiles in turn, each with a ring of its own filled by cp.async (no barrier of the block per tile, nothing to spin on), and merge their states at
 // the end of a history's piece.  A history in several CTAs is finished by whichever of them ends last, which adds the pieces in the
@@ -29,19 +29,20 @@ namespace dis {
 constexpr int kStWarps = 4;
 constexpr int kStMaxT = 512;            // tokens of one launch
 constexpr int kStCounters = 1 << 16;    // words kept for counters, of which two for each of a CTA's two pieces are used
-constexpr int kStMinShare = 2 * kStWarps;  // tiles of a CTA, at least
+constexpr int kStMinShare = kStWarps;   // tiles of a CTA, at least
 
 template <int D, bool I8>
 struct StCfg {
-  static constexpr int kSub = I8 && D == 64 ? 2 : 1;      // groups of 16 tokens in a tile
-  static constexpr int kTok = 16 * kSub;
+  static constexpr int kTok = 16;                         // tokens of a tile
   static constexpr int kRow = D * (I8 ? 1 : 2);           // bytes of a row
   static constexpr int kChunks = kRow / 16;
   static constexpr int kPart = kTok * kRow;               // K or V of a tile
   static constexpr int kStage = 2 * kPart + (I8 ? 2 * kTok * 4 : 0);
-  static constexpr int kStages = 3;
   static constexpr int kHead = 16 * (D / 16 + 1) + 4;     // floats between two heads' O in the merge: no bank twice in a half warp
-  static constexpr int kCtas = I8 ? 3 : 2;                // per SM
+  // Stages of a warp and CTAs of an SM, us of (8 bits) 32 histories to 6000, two of 60000, 64 of heads of 64; (bf16) 32 requests behind 6000 tokens: heads of
+  // 128 in 8 bits 3, 3: 30.4, 39.4; 2, 4: 31.0, 39.0; 4, 2: 32.1, 38.2; heads of 64 4, 4: 16.4; 3, 3 (tiles of 32 tokens): 18.3; bf16 2, 3: 26.2; 3, 2: 27.4
+  static constexpr int kStages = I8 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2);
+  static constexpr int kCtas = I8 && D == 64 ? 4 : 3;
   static constexpr int kRing = kStWarps * kStages * kStage;
   static constexpr int meet(int G) { return G * D <= 512 ? G : 512 / D; }  // heads whose states meet in shared memory at a time
   static constexpr int fixed(int G) { return kRing + kStWarps * meet(G) * kHead * 4; }
@@ -105,7 +106,7 @@ __device__ __forceinline__ uint32_t st_transpose(uint32_t v) {  // an 8x8 matrix
 // floats of a piece's (m, l): whole 16 bytes
 __host__ __device__ constexpr int st_ml(int G) { return G < 2 ? 4 : 2 * G; }
 
-__host__ __device__ constexpr size_t stream_slots(int per_sm) { return 2 * (size_t)kNumSMs * per_sm; }
+__host__ __device__ constexpr size_t stream_slots() { return 2 * 4 * (size_t)kNumSMs; }  // two of each resident CTA
 
 struct StArgs {
   const uint16_t *q;
@@ -123,6 +124,30 @@ struct StArgs {
   int T, n_kv, page_shift;
   int late_wait;           // the kernel in front was told to let this one start once its own inputs were complete: wait for it at the end
 };
+
+// A tile at a history's start or end, or over pages that end inside it, row by row: zeros where they are not visible.  (Not inlined: the kernel runs
+// this seldom, and how long its code is counts in every launch.)
+template <int D, bool I8>
+__device__ __noinline__ void st_fetch_rows(uint32_t dst, const char *pool, const float *scale, const int *pt, int pos0, int first, int keys, int page_shift,
+                                           int n_kv, int h) {
+  using Cfg = StCfg<D, I8>;
+  constexpr int kLaneRows = 32 / Cfg::kChunks;
+  const int lane = threadIdx.x & 31, lc = lane % Cfg::kChunks;
+  const long long v_rows = (long long)n_kv << page_shift;
+#pragma unroll 1
+  for (int r = lane / Cfg::kChunks; r < Cfg::kTok; r += kLaneRows) {
+    const int pos = pos0 + r;
+    const bool in = pos >= first && pos < keys;
+    const int at = min(max(pos, first), keys - 1);
+    const long long row = (((long long)pt[at >> page_shift] * 2 * n_kv + h) << page_shift) + (at & ((1 << page_shift) - 1));
+    st_copy_16(dst + st_k_chunk<D, I8>(r, lc) * 16, pool + row * Cfg::kRow + lc * 16, in);
+    st_copy_16(dst + Cfg::kPart + st_v_chunk<D, I8>(r, lc) * 16, pool + (row + v_rows) * Cfg::kRow + lc * 16, in);
+    if (I8 && lc == 0) {
+      st_copy_4(dst + 2 * Cfg::kPart + r * 4, scale + row, in);
+      st_copy_4(dst + 2 * Cfg::kPart + (Cfg::kTok + r) * 4, scale + row + v_rows, in);
+    }
+  }
+}
 
 template <int D, int G, bool I8>
 __global__ void __launch_bounds__(kStWarps * 32, StCfg<D, I8>::kCtas)
@@ -268,23 +293,10 @@ attn_stream_kernel(const StArgs a) {
           st_copy_16(dst + v_to[i & 3] + i * 512, v_src + i * 512, true);
         }
         if (I8) {
-#pragma unroll
-          for (int i = 0; i < Cfg::kSub; i++) st_copy_4(dst + lane_scale + i * 64, a.scale + row + lane_scale_row + i * 16, true);
+          st_copy_4(dst + lane_scale, a.scale + row + lane_scale_row, true);
         }
-      } else {  // a history's first and last tile, pages that end inside a tile: rows one by one, zeros where they are not visible
-#pragma unroll 1
-        for (int i = 0; i < kCopies; i++) {
-          const int r = i * kLaneRows + lr, pos = pos0 + i * kLaneRows / 8 * 8;  // (pages are eight tokens or more)
-          const long long page = page_of(min(pos >> a.page_shift, last_page), last_page);
-          const long long row = ((page * 2 * a.n_kv + ahead.h) << a.page_shift) + (pos & (page_size - 1)) + (r & 7);
-          const bool in = pos0 + r >= a_first && pos0 + r < a_keys;
-          st_copy_16(dst + k_to + i * 512, pool + row * Cfg::kRow + lc * 16, in);
-          st_copy_16(dst + Cfg::kPart + st_v_chunk<D, I8>(r, lc) * 16, pool + (row + v_rows) * Cfg::kRow + lc * 16, in);
-          if (I8 && lc == 0) {
-            st_copy_4(dst + 2 * Cfg::kPart + r * 4, a.scale + row, in);
-            st_copy_4(dst + 2 * Cfg::kPart + (Cfg::kTok + r) * 4, a.scale + row + v_rows, in);
-          }
-        }
+      } else {
+        st_fetch_rows<D, I8>(dst, pool, a.scale, a_pt, pos0, a_first, a_keys, a.page_shift, a.n_kv, ahead.h);
       }
       fetch += kStWarps;
     }
@@ -372,130 +384,125 @@ attn_stream_kernel(const StArgs a) {
       const uint32_t at = ring + stage * Cfg::kStage;
       stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
       const int pos0 = base + (tile - cur.u0) * Cfg::kTok;
+      // ---- S^T = K Q^T: tokens g, g + 8, columns 2 tq (+ 1); two accumulators halve the chain
+      float sa[2][4];
 #pragma unroll
-      for (int sub = 0; sub < Cfg::kSub; sub++) {
-        const int r0 = sub * 16 + g;
-        if (Cfg::kSub > 1 && sub > 0 && pos0 + sub * 16 >= keys) break;  // (uniform)
-        // ---- S^T = K Q^T: tokens r0, r0 + 8, columns 2 tq (+ 1); two accumulators halve the chain
-        float sa[2][4];
+      for (int e = 0; e < 2; e++) { sa[e][0] = 0.f; sa[e][1] = 0.f; sa[e][2] = 0.f; sa[e][3] = 0.f; }
 #pragma unroll
-        for (int e = 0; e < 2; e++) { sa[e][0] = 0.f; sa[e][1] = 0.f; sa[e][2] = 0.f; sa[e][3] = 0.f; }
+      for (int i = 0; i < Cfg::kChunks / 4; i++) {
+        const uint4 x4 = st_lds_16(at + st_k_chunk<D, I8>(g, tq + 4 * i) * 16), y4 = st_lds_16(at + st_k_chunk<D, I8>(g + 8, tq + 4 * i) * 16);
+        const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
+        if constexpr (I8) {
 #pragma unroll
-        for (int i = 0; i < Cfg::kChunks / 4; i++) {
-          const uint4 x4 = st_lds_16(at + st_k_chunk<D, I8>(r0, tq + 4 * i) * 16), y4 = st_lds_16(at + st_k_chunk<D, I8>(r0 + 8, tq + 4 * i) * 16);
-          const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
-          if constexpr (I8) {
+          for (int j = 0; j < 4; j++) {
+            uint32_t a0, a1, a2, a3;
+            bytes_to_half2(x[j] ^ 0x80808080u, a0, a2);
+            bytes_to_half2(y[j] ^ 0x80808080u, a1, a3);
+            st_mma<I8>(sa[j & 1], a0, a1, a2, a3, qb[i * 4 + j][0], qb[i * 4 + j][1]);
+          }
+        } else {
+          st_mma<I8>(sa[0], x[0], y[0], x[1], y[1], qb[2 * i][0], qb[2 * i][1]);
+          st_mma<I8>(sa[1], x[2], y[2], x[3], y[3], qb[2 * i + 1][0], qb[2 * i + 1][1]);
+        }
+      }
+      // ---- the reference follows the maximum where that grows by more than kPieceLazy; the whole warp acts then
+      float k_f[2] = {1.f, 1.f}, v_f[2] = {1.f, 1.f};
+      if (I8) {
+        const uint32_t sc = at + 2 * Cfg::kPart + g * 4;
+        k_f[0] = st_lds_f(sc); k_f[1] = st_lds_f(sc + 32);
+        v_f[0] = st_lds_f(sc + Cfg::kTok * 4); v_f[1] = st_lds_f(sc + Cfg::kTok * 4 + 32);
+      }
+      const float up0 = I8 ? piece_log2_scale(v_f[0]) : 0.f, up1 = I8 ? piece_log2_scale(v_f[1]) : 0.f;
+      float p[4], mx[2];  // p: scores without the head's factor
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              uint32_t a0, a1, a2, a3;
-              bytes_to_half2(x[j] ^ 0x80808080u, a0, a2);
-              bytes_to_half2(y[j] ^ 0x80808080u, a1, a3);
-              st_mma<I8>(sa[j & 1], a0, a1, a2, a3, qb[i * 4 + j][0], qb[i * 4 + j][1]);
-            }
+      for (int e = 0; e < 2; e++) {
+        p[e] = (sa[0][e] + sa[1][e]) * k_f[0];
+        p[2 + e] = (sa[0][2 + e] + sa[1][2 + e]) * k_f[1];
+      }
+      if (pos0 < first || pos0 + Cfg::kTok > keys) {  // (uniform)
+        const int p0 = pos0 + g, p1 = p0 + 8;
+        if (p0 < first || p0 >= keys) p[0] = p[1] = -INFINITY;
+        if (p1 < first || p1 >= keys) p[2] = p[3] = -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; e++) mx[e] = fmaxf(fmaf(p[e], qf[e], up0), fmaf(p[2 + e], qf[e], up1));
+      if (__any_sync(0xffffffffu, mx[0] > m_run[0] + kPieceLazy || mx[1] > m_run[1] + kPieceLazy)) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float x = mx[e];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          const float m_new = fmaxf(m_run[e], x);
+          f[e] = piece_ex2(m_run[e] - m_new);
+          l_run[e] *= f[e];
+          m_run[e] = m_new;
+        }
+#pragma unroll
+        for (int m = 0; m < KS; m++) { oacc[m][0] *= f[0]; oacc[m][1] *= f[1]; oacc[m][2] *= f[0]; oacc[m][3] *= f[1]; }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        p[e] = piece_ex2(fmaf(p[e], qf[e], -m_run[e]));
+        p[2 + e] = piece_ex2(fmaf(p[2 + e], qf[e], -m_run[e]));
+        l_run[e] += p[e] + p[2 + e];
+      }
+      uint32_t pb0, pb1, pl0 = 0u, pl1 = 0u;
+      if constexpr (I8) {
+        const __half2 h0 = __floats2half2_rn(p[0] * v_f[0], p[1] * v_f[0]), h1 = __floats2half2_rn(p[2] * v_f[1], p[3] * v_f[1]);
+        pb0 = st_transpose(*reinterpret_cast<const uint32_t *>(&h0));
+        pb1 = st_transpose(*reinterpret_cast<const uint32_t *>(&h1));
+      } else {
+        const uint32_t p01 = float2_to_bf16x2(p[0], p[1]), p23 = float2_to_bf16x2(p[2], p[3]);
+        const float2 r01 = bf16x2_to_float2(p01), r23 = bf16x2_to_float2(p23);
+        const uint32_t q01 = float2_to_bf16x2(p[0] - r01.x, p[1] - r01.y), q23 = float2_to_bf16x2(p[2] - r23.x, p[3] - r23.y);
+        const bool rest = kTwice && tq * 2 >= G;
+        pb0 = st_transpose(G == 1 ? (p01 & 0xffffu) | (q01 & 0xffff0000u) : rest ? q01 : p01);
+        pb1 = st_transpose(G == 1 ? (p23 & 0xffffu) | (q23 & 0xffff0000u) : rest ? q23 : p23);
+        if (!kTwice) { pl0 = st_transpose(q01); pl1 = st_transpose(q23); }
+      }
+      // ---- O^T += V^T P^T: tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9, dims g kPer ..
+      const uint32_t va = at + Cfg::kPart;
+      const int t0 = 2 * tq;
+      if constexpr (I8) {
+        uint32_t v[4][kPer / 4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int r = t0 + (k & 1) + (k >> 1) * 8;
+          if constexpr (D == 128) {
+            const uint4 w = st_lds_16(va + st_v_chunk<D, I8>(r, g) * 16);
+            v[k][0] = w.x; v[k][1] = w.y; v[k][2] = w.z; v[k][3] = w.w;
           } else {
-            st_mma<I8>(sa[0], x[0], y[0], x[1], y[1], qb[2 * i][0], qb[2 * i][1]);
-            st_mma<I8>(sa[1], x[2], y[2], x[3], y[3], qb[2 * i + 1][0], qb[2 * i + 1][1]);
-          }
-        }
-        // ---- the reference follows the maximum where that grows by more than kPieceLazy; the whole warp acts then
-        float k_f[2] = {1.f, 1.f}, v_f[2] = {1.f, 1.f};
-        if (I8) {
-          const uint32_t sc = at + 2 * Cfg::kPart + r0 * 4;
-          k_f[0] = st_lds_f(sc); k_f[1] = st_lds_f(sc + 32);
-          v_f[0] = st_lds_f(sc + Cfg::kTok * 4); v_f[1] = st_lds_f(sc + Cfg::kTok * 4 + 32);
-        }
-        const float up0 = I8 ? piece_log2_scale(v_f[0]) : 0.f, up1 = I8 ? piece_log2_scale(v_f[1]) : 0.f;
-        float p[4], mx[2];  // p: scores without the head's factor
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          p[e] = (sa[0][e] + sa[1][e]) * k_f[0];
-          p[2 + e] = (sa[0][2 + e] + sa[1][2 + e]) * k_f[1];
-        }
-        if (pos0 < first || pos0 + Cfg::kTok > keys) {  // (uniform)
-          const int p0 = pos0 + r0, p1 = p0 + 8;
-          if (p0 < first || p0 >= keys) p[0] = p[1] = -INFINITY;
-          if (p1 < first || p1 >= keys) p[2] = p[3] = -INFINITY;
-        }
-#pragma unroll
-        for (int e = 0; e < 2; e++) mx[e] = fmaxf(fmaf(p[e], qf[e], up0), fmaf(p[2 + e], qf[e], up1));
-        if (__any_sync(0xffffffffu, mx[0] > m_run[0] + kPieceLazy || mx[1] > m_run[1] + kPieceLazy)) {
-          float f[2];
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float x = mx[e];
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            const float m_new = fmaxf(m_run[e], x);
-            f[e] = piece_ex2(m_run[e] - m_new);
-            l_run[e] *= f[e];
-            m_run[e] = m_new;
+            const uint2 w = st_lds_8(va + st_v_chunk<D, I8>(r, g >> 1) * 16 + (g & 1) * 8);
+            v[k][0] = w.x; v[k][1] = w.y;
           }
 #pragma unroll
-          for (int m = 0; m < KS; m++) { oacc[m][0] *= f[0]; oacc[m][1] *= f[1]; oacc[m][2] *= f[0]; oacc[m][3] *= f[1]; }
+          for (int j = 0; j < kPer / 4; j++) v[k][j] ^= 0x80808080u;
         }
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          p[e] = piece_ex2(fmaf(p[e], qf[e], -m_run[e]));
-          p[2 + e] = piece_ex2(fmaf(p[2 + e], qf[e], -m_run[e]));
-          l_run[e] += p[e] + p[2 + e];
-        }
-        uint32_t pb0, pb1, pl0 = 0u, pl1 = 0u;
-        if constexpr (I8) {
-          const __half2 h0 = __floats2half2_rn(p[0] * v_f[0], p[1] * v_f[0]), h1 = __floats2half2_rn(p[2] * v_f[1], p[3] * v_f[1]);
-          pb0 = st_transpose(*reinterpret_cast<const uint32_t *>(&h0));
-          pb1 = st_transpose(*reinterpret_cast<const uint32_t *>(&h1));
-        } else {
-          const uint32_t p01 = float2_to_bf16x2(p[0], p[1]), p23 = float2_to_bf16x2(p[2], p[3]);
-          const float2 r01 = bf16x2_to_float2(p01), r23 = bf16x2_to_float2(p23);
-          const uint32_t q01 = float2_to_bf16x2(p[0] - r01.x, p[1] - r01.y), q23 = float2_to_bf16x2(p[2] - r23.x, p[3] - r23.y);
-          const bool rest = kTwice && tq * 2 >= G;
-          pb0 = st_transpose(G == 1 ? (p01 & 0xffffu) | (q01 & 0xffff0000u) : rest ? q01 : p01);
-          pb1 = st_transpose(G == 1 ? (p23 & 0xffffu) | (q23 & 0xffff0000u) : rest ? q23 : p23);
-          if (!kTwice) { pl0 = st_transpose(q01); pl1 = st_transpose(q23); }
-        }
-        // ---- O^T += V^T P^T: tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9, dims g kPer ..
-        const uint32_t va = at + Cfg::kPart;
-        const int t0 = sub * 16 + 2 * tq;
-        if constexpr (I8) {
-          uint32_t v[4][kPer / 4];
+        for (int j = 0; j < kPer / 4; j++) {
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const int r = t0 + (k & 1) + (k >> 1) * 8;
-            if constexpr (D == 128) {
-              const uint4 w = st_lds_16(va + st_v_chunk<D, I8>(r, g) * 16);
-              v[k][0] = w.x; v[k][1] = w.y; v[k][2] = w.z; v[k][3] = w.w;
-            } else {
-              const uint2 w = st_lds_8(va + st_v_chunk<D, I8>(r, g >> 1) * 16 + (g & 1) * 8);
-              v[k][0] = w.x; v[k][1] = w.y;
-            }
-#pragma unroll
-            for (int j = 0; j < kPer / 4; j++) v[k][j] ^= 0x80808080u;
+          for (int hf = 0; hf < 2; hf++) {
+            uint32_t a0, a1, a2, a3;
+            bytes_to_half2(__byte_perm(v[0][j], v[1][j], hf ? 0x7362 : 0x5140), a0, a1);
+            bytes_to_half2(__byte_perm(v[2][j], v[3][j], hf ? 0x7362 : 0x5140), a2, a3);
+            st_mma<I8>(oacc[2 * j + hf], a0, a1, a2, a3, pb0, pb1);
           }
+        }
+      } else {
 #pragma unroll
-          for (int j = 0; j < kPer / 4; j++) {
+        for (int cc = 0; cc < kPer / 8; cc++) {
+          uint4 w[4];
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-              uint32_t a0, a1, a2, a3;
-              bytes_to_half2(__byte_perm(v[0][j], v[1][j], hf ? 0x7362 : 0x5140), a0, a1);
-              bytes_to_half2(__byte_perm(v[2][j], v[3][j], hf ? 0x7362 : 0x5140), a2, a3);
-              st_mma<I8>(oacc[2 * j + hf], a0, a1, a2, a3, pb0, pb1);
-            }
-          }
-        } else {
+          for (int k = 0; k < 4; k++) w[k] = st_lds_16(va + st_v_chunk<D, I8>(t0 + (k & 1) + (k >> 1) * 8, g * (kPer / 8) + cc) * 16);
 #pragma unroll
-          for (int cc = 0; cc < kPer / 8; cc++) {
-            uint4 w[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) w[k] = st_lds_16(va + st_v_chunk<D, I8>(t0 + (k & 1) + (k >> 1) * 8, g * (kPer / 8) + cc) * 16);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              auto el = [&](int k) { return j == 0 ? w[k].x : j == 1 ? w[k].y : j == 2 ? w[k].z : w[k].w; };
-              const uint32_t a0 = __byte_perm(el(0), el(1), 0x5410), a1 = __byte_perm(el(0), el(1), 0x7632);
-              const uint32_t a2 = __byte_perm(el(2), el(3), 0x5410), a3 = __byte_perm(el(2), el(3), 0x7632);
-              st_mma<I8>(oacc[4 * cc + j], a0, a1, a2, a3, pb0, pb1);
-              if (!kTwice) st_mma<I8>(oacc[4 * cc + j], a0, a1, a2, a3, pl0, pl1);
-            }
+          for (int j = 0; j < 4; j++) {
+            auto el = [&](int k) { return j == 0 ? w[k].x : j == 1 ? w[k].y : j == 2 ? w[k].z : w[k].w; };
+            const uint32_t a0 = __byte_perm(el(0), el(1), 0x5410), a1 = __byte_perm(el(0), el(1), 0x7632);
+            const uint32_t a2 = __byte_perm(el(2), el(3), 0x5410), a3 = __byte_perm(el(2), el(3), 0x7632);
+            st_mma<I8>(oacc[4 * cc + j], a0, a1, a2, a3, pb0, pb1);
+            if (!kTwice) st_mma<I8>(oacc[4 * cc + j], a0, a1, a2, a3, pl0, pl1);
           }
         }
       }
@@ -577,7 +584,7 @@ attn_stream_kernel(const StArgs a) {
   if (part_first[0] != part_last[0] || part_first[1] != part_last[1]) {
     auto fan_of = [&](int parts) { return parts <= 8 ? parts : (int)ceilf(sqrtf((float)parts)); };
     auto arrive = [&](int level, size_t slot, int n) {
-      int *count = a.counters + level * stream_slots(3) + slot;
+      int *count = a.counters + level * stream_slots() + slot;
       __threadfence();
       const bool last = atomicAdd(count, 1) == n - 1;
       if (last) *count = 0;  // as the next call wants it
@@ -615,7 +622,7 @@ attn_stream_kernel(const StArgs a) {
         const bool whole = level || groups == 1;
         const float *src_o = level ? a.group_o : a.piece_o, *src_ml = level ? a.group_ml : a.piece_ml;
         // four dims of a head to a thread at a time, kAhead pieces' on their way
-        constexpr int kQuads = G * D / 4, kAhead = 8;
+        constexpr int kQuads = G * D / 4, kAhead = 4;
 #pragma unroll 1
         for (int quad = threadIdx.x; quad < kQuads; quad += kStWarps * 32) {
           const int h = quad / (D / 4), i = quad % (D / 4) * 4;
@@ -662,7 +669,7 @@ attn_stream_kernel(const StArgs a) {
 // ---------------------------------------------------------------------------------------- host
 size_t attn_stream_scratch_elems(int n_heads, int n_kv, int d) {  // counters, then the pieces of every resident CTA
   if (n_kv <= 0 || n_heads <= 0 || d <= 0) return 0;
-  return kStCounters + 2 * stream_slots(3) * ((size_t)(n_heads / n_kv) * d + st_ml(n_heads / n_kv));
+  return kStCounters + 2 * stream_slots() * ((size_t)(n_heads / n_kv) * d + st_ml(n_heads / n_kv));
 }
 
 template <int D, int G, bool I8>
@@ -696,9 +703,9 @@ cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float 
   a.pool = pool; a.scale = scale; a.page_table = page_table; a.max_pages = max_pages; a.first = first;
   a.counters = reinterpret_cast<int *>(scratch);
   a.piece_o = scratch + kStCounters;
-  a.group_o = a.piece_o + stream_slots(3) * (size_t)G * d;
-  a.piece_ml = a.group_o + stream_slots(3) * (size_t)G * d;
-  a.group_ml = a.piece_ml + stream_slots(3) * (size_t)st_ml(G);
+  a.group_o = a.piece_o + stream_slots() * (size_t)G * d;
+  a.piece_ml = a.group_o + stream_slots() * (size_t)G * d;
+  a.group_ml = a.piece_ml + stream_slots() * (size_t)st_ml(G);
   a.n_kv = n_kv;
   while ((1 << a.page_shift) < page_size) a.page_shift++;
   for (int t = 0; t < T; t += step) {
