@@ -2,10 +2,10 @@
 //
 // Positions [0, prefix) hold the same keys and values for all T tokens, so the T G query rows of a kv head are the rows of one matrix product
 // against them: K and V of the prefix are read once (per 256 rows) instead of T times, at tcgen05 rate.  Three kernels:
-//   attn_prefix_kernel   states (m, l, O) of 128 or 256 query rows of a kv head over a slice of the prefix
-//   attn_stream_kernel   states of every token over its own positions [prefix, ctx) (k_attn_stream.cu); it starts as SMs come free
+//   attn_stream_kernel   states (m, l, O) of every token over its own positions [prefix, ctx) (k_attn_stream.cu)
+//   attn_prefix_kernel   states of 128 or 256 query rows of a kv head over a slice of the prefix; it starts as SMs come free
 //   attn_join_kernel     result = the joined states: O / l of their sum under one reference
-// A token whose history ends inside the prefix goes through the second alone.
+// A token whose history ends inside the prefix goes through the first alone.
 //
 // Bytes: nkv 2 d b (prefix + sum of own lengths); operations: 4 G d T prefix nkv on the tensor cores and T G prefix nkv exponentials (16 per
 // clock and SM: 512 clocks per 128 rows x 64 keys beside 256 + 256 of the products for d = 128).
@@ -131,7 +131,7 @@ struct SpArgs {
   int max_pages, page_shift;
   float *state_o;         // [slice][kv head][128-row tile][D / 4][128] x 4 floats
   float *state_ml;        // [slice][kv head][128-row tile][128] x (m, l)
-  int T, g_shift, n_kv, prefix, row_tiles, slices;
+  int T, g_shift, n_kv, prefix, row_tiles, slices, late_wait;
 };
 
 template <int D, bool I8, bool kPair>
@@ -175,9 +175,10 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // First the predecessors' results, then the kernel behind this one: that one starts without waiting for them itself
-  pdl_wait();
+  // (Behind the allocation: a CTA of the next kernel that took its columns first would wait for this grid, and this CTA for those columns.)  The
+  // kernel in front let this one start once its own inputs, which are this one's too, were complete: it is waited for at the end
   pdl_launch_dependents();
+  if (!a.late_wait) pdl_wait();
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
   const uint32_t o_base = tmem + 4 * kSpTile;
@@ -538,6 +539,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc<512>(tmem);
+  if (a.late_wait) pdl_wait();
 }
 
 // The states of a row joined: thread = (row of a kv head, eight dims), lanes over rows, as the prefix's states lie.
@@ -641,6 +643,10 @@ cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float 
   if (n_kv > 65535 || a.row_tiles > 65535) { set_last_error("attn_shared: more than 65535 kv heads or 128-row tiles"); return cudaErrorInvalidValue; }
   TmaMap map{};
   if (!scale) DIS_CUDA_TRY(make_kv_map(&map, static_cast<const uint16_t *>(pool), n_pages * 2 * n_kv * page_size, d, page_size));
+  // The own parts first: their CTAs end one after the other, and the prefix's start as SMs come free
+  DIS_CUDA_TRY(launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, prefix, nullptr, own_o, own_ml, scratch, true, T, n_heads, n_kv, d,
+                                  page_size, st));
+  a.late_wait = pdl_enabled();
   const bool pair = a.row_tiles > 1;
 #define DIS_SP(DD, II, PP) DIS_CUDA_TRY((prefix_launch<DD, II, PP>(map, a, st)))
   if (d == 128) {
@@ -651,8 +657,6 @@ cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float 
     else { if (pair) DIS_SP(64, false, true); else DIS_SP(64, false, false); }
   }
 #undef DIS_SP
-  DIS_CUDA_TRY(launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, prefix, nullptr, own_o, own_ml, scratch, pdl_enabled(), T, n_heads,
-                                  n_kv, d, page_size, st));
   const dim3 grid((unsigned)((T * G + kSjRows - 1) / kSjRows), d / 32, n_kv);
   if (d == 128) return launch_k(attn_join_kernel<128>, grid, dim3(128), 0, st, a, (const float *)own_o, (const float *)own_ml, ctx, out);
   return launch_k(attn_join_kernel<64>, grid, dim3(128), 0, st, a, (const float *)own_o, (const float *)own_ml, ctx, out);

@@ -122,7 +122,7 @@ struct StArgs {
   float *piece_o, *piece_ml;  // [2 per CTA][G][D], [2 per CTA][st_ml(G)]
   float *group_o, *group_ml;  // of pieces joined, likewise
   int T, n_kv, page_shift;
-  int late_wait;           // the kernel in front was told to let this one start once its own inputs were complete: wait for it at the end
+  int inputs_first;        // the kernel behind reads the same inputs and does not wait for them: it may start when they are complete
 };
 
 // A tile at a history's start or end, or over pages that end inside it, row by row: zeros where they are not visible.  (Not inlined: the kernel runs
@@ -165,8 +165,9 @@ attn_stream_kernel(const StArgs a) {
   __shared__ int s_scan[kStWarps], s_last[2];
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-  pdl_launch_dependents();
-  if (!a.late_wait) pdl_wait();
+  if (!a.inputs_first) pdl_launch_dependents();
+  pdl_wait();
+  if (a.inputs_first) pdl_launch_dependents();
   const int n_heads = a.n_kv * G, page_size = 1 << a.page_shift, base0 = a.first / Cfg::kTok * Cfg::kTok;
   auto first_of = [&](int keys) { return keys < a.first ? 0 : a.first; };  // a history that ends in front of it is all this kernel's
   auto base_of = [&](int keys) { return keys < a.first ? 0 : base0; };
@@ -663,7 +664,6 @@ attn_stream_kernel(const StArgs a) {
       }
     }
   }
-  if (a.late_wait) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------------------- host
@@ -694,7 +694,7 @@ static cudaError_t stream_dispatch(const StArgs &a, int G, int d, cudaStream_t s
 }
 
 cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float *scale, const int *page_table, int max_pages, const int *pt_row,
-                               const int *ctx, int first, uint16_t *out, float *state_o, float *state_ml, float *scratch, bool late_wait, int T,
+                               const int *ctx, int first, uint16_t *out, float *state_o, float *state_ml, float *scratch, bool inputs_first, int T,
                                int n_heads, int n_kv, int d, int page_size, cudaStream_t st) {
   // a launch's tiles are counted in 32 bits
   const long long most = ((long long)max_pages * page_size / 16 + 2) * n_kv;
@@ -710,7 +710,7 @@ cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float 
   while ((1 << a.page_shift) < page_size) a.page_shift++;
   for (int t = 0; t < T; t += step) {
     a.T = std::min(step, T - t);
-    a.late_wait = late_wait && t == 0;  // (the next launch uses the same scratch)
+    a.inputs_first = inputs_first;
     a.q = q + (size_t)t * n_heads * d;
     a.pt_row = pt_row + t;
     a.ctx = ctx + t;

@@ -126,7 +126,7 @@ cudaError_t launch_kv_read_i8(const int8_t *pool, const float *scale, uint16_t *
 // part is zero between calls.
 size_t attn_stream_scratch_elems(int n_heads, int n_kv, int d);
 cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float *scale, const int *page_table, int max_pages, const int *pt_row,
-                               const int *ctx, int first, uint16_t *out, float *state_o, float *state_ml, float *scratch, bool late_wait, int T,
+                               const int *ctx, int first, uint16_t *out, float *state_o, float *state_ml, float *scratch, bool inputs_first, int T,
                                int n_heads, int n_kv, int d, int page_size, cudaStream_t st);
 
 // k_attn_shared.cu : the same where positions [0, prefix) are the same rows for every token
