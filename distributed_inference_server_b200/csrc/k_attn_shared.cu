@@ -606,6 +606,12 @@ static int shared_slices(int blocks, int tiles) {
 }
 static int shared_blocks(int T, int G, int n_kv) { const int rt = shared_row_tiles(T, G); return (rt > 1 ? (rt + 1) / 2 : 1) * n_kv; }
 
+// Whether the prefix is read once, or every token goes alone (one kernel, to which the others' reads of the same pages are hits in L2): from about 2^25 entries
+// of T prefixes on the former is ahead.  From graphs, own parts of 100, together / alone, us: 32 / 8 heads of 128, bf16: 4 x 8192 22.2 / 22.1, 8 x 4096 19.6 / 19.9,
+// 16 x 1024 18.2 / 14.9, 16 x 2048 18.7 / 19.7, 32 x 512 18.3 / 15.3, 32 x 1024 19.1 / 19.9, 32 x 4096 21.1 / 48.6; 64 / 8 heads in 8 bits: 16 x 2048 21.7 / 22.3, 32 x 1024
+// 25.9 / 21.6, 32 x 2048 27.5 / 31.0; 32 / 4 heads of 64: 16 x 4096 18.2 / 15.0, 32 x 4096 19.9 / 20.4, 64 x 1024 18.4 / 15.1, 64 x 2048 19.2 / 20.4
+bool attn_shared_pays(int T, int n_kv, int d, int prefix) { return T > 1 && (long long)T * prefix * n_kv * d >= 1 << 25; }
+
 size_t attn_shared_scratch_elems(int T, int n_heads, int n_kv, int d) {  // the stream's, its states, the slices' states
   if (T <= 0 || n_kv <= 0 || n_heads < n_kv || d <= 0) return 0;
   const int G = n_heads / n_kv, rt = shared_row_tiles(T, G);
@@ -628,7 +634,7 @@ cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float 
                                const int *pt_row, const int *ctx, int prefix, uint16_t *out, float *scratch, int T, int n_heads, int n_kv, int d,
                                int page_size, cudaStream_t st) {
   const int G = n_heads / n_kv;
-  if (T < 2 || prefix < 1)  // nothing to share
+  if (!attn_shared_pays(T, n_kv, d, prefix))
     return launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, 0, out, nullptr, nullptr, scratch, false, T, n_heads, n_kv, d, page_size, st);
   SpArgs a{};
   a.q = q; a.pool = static_cast<const int8_t *>(pool); a.scale = scale; a.page_table = page_table; a.pt_row = pt_row; a.max_pages = max_pages;

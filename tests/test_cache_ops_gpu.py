@@ -472,6 +472,54 @@ def test_shared_prefix_many_steps_again(int8, T, group, d, prefix):
         assert torch.equal(shared(c, q, 8 * group, prefix, area=area), first), k
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("T,group,nkv,d,page,prefix", [(72, 1, 8, 128, 16, 577), (64, 2, 8, 128, 8, 641), (40, 4, 8, 128, 64, 1000), (57, 8, 8, 128, 32, 704), (33, 4, 8, 128, 128, 1500),
+                                                      (80, 8, 8, 64, 8, 1001), (130, 1, 8, 64, 64, 640), (12, 4, 8, 128, 64, 4095), (5, 8, 8, 128, 16, 7000), (9, 2, 16, 64, 64, 5000)])
+def test_shared_prefix_read_once(int8, T, group, nkv, d, page, prefix):
+    """Sizes at which the prefix is read once: prefixes that end inside a tile and inside a page, one tile of rows and several, rows behind the last, and
+    among the histories some that end at the prefix's end, inside it, or are empty."""
+    assert lib().dis_k_attn_shared_in_common(T, nkv, d, prefix) == 1
+    own = np.random.default_rng(T).integers(0, 90, T)
+    ctx = [prefix + int(n) for n in own]
+    ctx[1], ctx[2], ctx[3] = prefix, prefix - 1, 0
+    ctx[T - 1] = prefix // 2
+    c = Cache(ctx, nkv, d, page, T + prefix, int8, prefix)
+    q = queries(T, nkv * group, d, prefix)
+    area = scratch(T, nkv * group, nkv, d, True)
+    out = shared(c, q, nkv * group, prefix, area=area)
+    near(out, attention(c, q, nkv * group, 2.0 ** -8))
+    assert int((out[3] != 0).sum()) == 0
+    area[1 << 16:].fill_(7.0)
+    assert torch.equal(shared(c, q, nkv * group, prefix, area=area), out)
+
+
+def test_shared_prefix_read_once_rows_without_numbers_and_sizes():
+    """A NaN among the prefix's keys reaches every token that sees it, in its kv head; scales from 2^-60 to 2^40; large scores."""
+    T, prefix = 40, 1000
+    ctx = [prefix + 1 + t for t in range(T)]
+    ctx[7] = 90
+    spread = lambda x, g: torch.where(torch.arange(2, device=DEV).view(1, 2, 1, 1, 1) == 1, torch.exp2(  # noqa: E731
+        (torch.rand(x.shape[0], 1, 1, x.shape[3], 1, generator=g, device=DEV) * 100 - 60).round()), torch.ones((), device=DEV))
+    c = Cache(ctx, 8, 128, 64, 51, True, prefix, amp=spread)
+    for size in (1.5, 30.0, 1e-30):
+        q = queries(T, 32, 128, 52, size)
+        near(shared(c, q, 32, prefix), attention(c, q, 32, 2.0 ** -8))
+    for int8 in (False, True):
+        c = Cache(ctx, 8, 128, 64, 53, int8, prefix)
+        q = queries(T, 32, 128, 54)
+        page = int(c.table[0, 5])  # positions 320 ..
+        if int8:
+            c.scale[page, 0, 1, 5] = NAN
+        else:
+            c.pool[page, 0, 1, 5] = NAN
+        out = shared(c, q, 32, prefix).view(T, 32, 128)
+        seen = [t for t in range(T) if t != 7]
+        assert bool(out[seen][:, 4:8].isnan().all())
+        o, tol = attention(c, q, 32, 2.0 ** -8)
+        ok = (out.double() - o).abs() <= tol
+        assert bool(ok[:, :4].all()) and bool(ok[:, 8:].all()) and bool(ok[7].all())
+
+
 def test_shared_prefix_sizes():
     """Large scores (one key wins), and values' scales from 2^-60 to 2^40, in 8-bit pages."""
     ctx = [700 + t for t in range(20)]
