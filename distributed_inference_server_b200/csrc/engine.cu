@@ -175,6 +175,7 @@ int Engine::init(const dis_engine_config *c) {
     s.o_rowmap = sec((size_t)max_batch * 4); s.o_temp = sec((size_t)max_batch * 4); s.o_topp = sec((size_t)max_batch * 4);
     s.o_seed = sec((size_t)max_batch * 8); s.o_step = sec((size_t)max_batch * 8);
     s.o_qb_tok0 = sec(ct * 4); s.o_qb_len = sec(ct * 4); s.o_qb_pos0 = sec(ct * 4); s.o_qb_ptrow = sec(ct * 4);
+    s.o_rd_row = sec((size_t)max_batch * 4); s.o_rd_ctx = sec((size_t)max_batch * 4);
     s.o_arstep = sec(16);
     s.bytes = o;
     cudaError_t e1 = cudaMallocHost(reinterpret_cast<void **>(&s.host), s.bytes);
@@ -188,7 +189,19 @@ int Engine::init(const dis_engine_config *c) {
   // ---- KV pages: [layer][page][2][nkv_l][page_size][d]
   {
     const size_t page_elems = (size_t)2 * nkv_l * page_size * m.head_dim;
-    const size_t page_bytes_all_layers = page_elems * 2 * L;
+    const bool int8 = c->flags & DIS_FLAG_KV_INT8;
+    if (c->flags & (DIS_FLAG_KV_INT8 | DIS_FLAG_ATTN_SHARED)) {
+      const int G = nh_l / nkv_l;
+      if (G != 1 && G != 2 && G != 4 && G != 8)
+        return fail(DIS_ERR_INVALID_ARGUMENT, "DIS_FLAG_KV_INT8 and DIS_FLAG_ATTN_SHARED need 1, 2, 4 or 8 query heads per kv head");
+      size_t area = attn_stream_scratch_elems(nh_l, nkv_l, m.head_dim);
+      if (c->flags & DIS_FLAG_ATTN_SHARED)
+        for (int t = 2; t <= max_batch; t++) area = std::max(area, attn_shared_scratch_elems(t, nh_l, nkv_l, m.head_dim));
+      ENG_CUDA(dev_alloc(&piece_area, area, &bytes_allocated));
+      ENG_CUDA(cudaMemset(piece_area, 0, area * sizeof(float)));
+    }
+    const size_t page_rows = (size_t)2 * nkv_l * page_size;  // (8 bits: a page of every layer, and one of bf16)
+    const size_t page_bytes_all_layers = int8 ? (page_elems + page_rows * 4) * L + page_elems * 2 : page_elems * 2 * L;
     int64_t want = c->kv_pages;
     const int64_t useful = (int64_t)max_batch * max_pages;
     if (want <= 0) {
@@ -201,11 +214,18 @@ int Engine::init(const dis_engine_config *c) {
     if (want < 1) return fail(DIS_ERR_OUT_OF_MEMORY, "no device memory left for KV pages");
     n_pages = want;
     kv_layer_stride = (size_t)n_pages * page_elems;
-    ENG_CUDA(dev_alloc(&kv_pool, kv_layer_stride * L, &bytes_allocated));
-    // stale rows inside a TMA box get probability 0 in attention, so they must never be NaN
-    ENG_CUDA(cudaMemset(kv_pool, 0, kv_layer_stride * L * sizeof(uint16_t)));
     kv_rows_per_layer = (long long)n_pages * 2 * nkv_l * page_size;
-    ENG_CUDA(make_kv_map(&kv_map, kv_pool, kv_rows_per_layer * (long long)L, m.head_dim, page_size));
+    const size_t bf16_layers = int8 ? 1 : L;
+    if (int8) {
+      ENG_CUDA(dev_alloc(&kv8_pool, kv_layer_stride * L, &bytes_allocated));
+      ENG_CUDA(dev_alloc(&kv8_scale, (size_t)kv_rows_per_layer * L, &bytes_allocated));
+      ENG_CUDA(cudaMemset(kv8_pool, 0, kv_layer_stride * L));
+      ENG_CUDA(cudaMemset(kv8_scale, 0, (size_t)kv_rows_per_layer * L * sizeof(float)));
+    }
+    ENG_CUDA(dev_alloc(&kv_pool, kv_layer_stride * bf16_layers, &bytes_allocated));
+    // stale rows inside a TMA box get probability 0 in attention, so they must never be NaN
+    ENG_CUDA(cudaMemset(kv_pool, 0, kv_layer_stride * bf16_layers * sizeof(uint16_t)));
+    ENG_CUDA(make_kv_map(&kv_map, kv_pool, kv_rows_per_layer * (long long)bf16_layers, m.head_dim, page_size));
     pages_ix.init(page_size, n_pages, (c->flags & DIS_FLAG_PREFIX_CACHE) != 0);
     ENG_CUDA(dev_alloc(&d_page_table, (size_t)max_batch * max_pages, &bytes_allocated));
     ENG_CUDA(cudaMallocHost(reinterpret_cast<void **>(&h_page_table), (size_t)max_batch * max_pages * sizeof(int)));
@@ -347,7 +367,7 @@ Engine::~Engine() {
   for (int r = 0; r < kTpMaxRanks; r++) if (peer_base[r]) cudaIpcCloseMemHandle(peer_base[r]);
   void *ptrs[] = {embed, wqkv, wo, wgu, wdown, lm_head, attn_norm, mlp_norm, final_norm, x, partial, logits, ar_buf,
                   attn_scratch, full_logits, gather_buf, cand_val, cand_val_all, cand_tok, cand_tok_all, cand_sum, cand_sum_all, xn, q, attn,
-                  act, d_out_tokens == h_out_tokens ? nullptr : d_out_tokens, kv_pool, d_page_table, rope_cos, rope_sin, meta_dec.dev, meta_pre.dev, sym};
+                  act, d_out_tokens == h_out_tokens ? nullptr : d_out_tokens, kv_pool, kv8_pool, kv8_scale, piece_area, d_page_table, rope_cos, rope_sin, meta_dec.dev, meta_pre.dev, sym};
   for (void *p : ptrs) if (p) cudaFree(p);
   if (h_out_tokens) cudaFreeHost(h_out_tokens);
   if (h_page_table) cudaFreeHost(h_page_table);
@@ -695,6 +715,31 @@ cudaError_t Engine::consume_pending(const float *gain, const int *row_map, int r
   return r;
 }
 
+// The sequences of a pass that reads prompts, from its query blocks (a sequence's blocks are consecutive): what has to be read back of each
+void Engine::plan_read_back(int n_blocks) {
+  n_read = 0;
+  if (!kv8_pool) return;
+  int *row = cur_meta->h<int>(cur_meta->o_rd_row), *ctx = cur_meta->h<int>(cur_meta->o_rd_ctx);
+  for (int b = 0; b < n_blocks; b++) {
+    const int r = cur_meta->h<int>(cur_meta->o_qb_ptrow)[b];
+    if (n_read == 0 || row[n_read - 1] != r) row[n_read++] = r;
+    ctx[n_read - 1] = cur_meta->h<int>(cur_meta->o_qb_pos0)[b] + cur_meta->h<int>(cur_meta->o_qb_len)[b];
+  }
+}
+
+// Leading pages that all listed sequences have in common
+int Engine::common_pages(int n, const int *slots) const {
+  const std::vector<int> &a = seqs[(size_t)slots[0]].pages;
+  size_t same = a.size();
+  for (int i = 1; i < n; i++) {
+    const std::vector<int> &b = seqs[(size_t)slots[i]].pages;
+    same = std::min(same, b.size());
+    for (size_t k = 0; k < same; k++)
+      if (a[k] != b[k]) same = k;
+  }
+  return (int)same;
+}
+
 cudaError_t Engine::enqueue_layers(int T, int n_splits) {
   const int H = m.hidden, d = m.head_dim;
   const bool gemv = (cfg.flags & DIS_FLAG_FORCE_GEMV) || T <= gemv_max_t;
@@ -734,23 +779,50 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
     prof_mark(P_QKV);
     if (!skip(P_QKV)) RET_CUDA(linear_partial(xn_map, xn, wqkv_map, wqkv, l * nqkv_l, T, nqkv_l, H, &s_qkv));
     else s_qkv = gemm_pick_split_k(T, nqkv_l, H);
-    uint16_t *pool = kv_pool + (size_t)l * kv_layer_stride;
-    if (n_qblocks > 0) {
+    const int pool_layer = kv8_pool ? 0 : l;
+    uint16_t *pool = kv_pool + (size_t)pool_layer * kv_layer_stride;
+    const long long row0 = (long long)pool_layer * kv_rows_per_layer;
+    int8_t *pool8 = kv8_pool ? kv8_pool + (size_t)l * kv_layer_stride : nullptr;
+    float *scale8 = kv8_pool ? kv8_scale + (size_t)l * kv_rows_per_layer : nullptr;
+    auto write_rows = [&]() -> cudaError_t {
       prof_mark(P_ROPE);
-      RET_CUDA(launch_rope_kv_write(partial, s_qkv, (long long)T * nqkv_l, q, pool, d_page_table, max_pages, ptrow, pos,
-                                    rope_cos, rope_sin, T, nh_l, nkv_l, d, page_size, stream));
+      kernel_launches++;
+      if (pool8)
+        return launch_rope_kv_write_i8(partial, s_qkv, (long long)T * nqkv_l, q, pool8, scale8, d_page_table, max_pages, ptrow, pos, rope_cos, rope_sin, T,
+                                       nh_l, nkv_l, d, page_size, stream);
+      return launch_rope_kv_write(partial, s_qkv, (long long)T * nqkv_l, q, pool, d_page_table, max_pages, ptrow, pos, rope_cos, rope_sin, T, nh_l, nkv_l, d,
+                                  page_size, stream);
+    };
+    if (n_qblocks > 0) {
+      RET_CUDA(write_rows());
+      if (pool8) {
+        RET_CUDA(launch_kv_read_i8(pool8, scale8, kv_pool, d_page_table, d_page_table, max_pages, cur_meta->d<int>(cur_meta->o_rd_row), nullptr,
+                                   cur_meta->d<int>(cur_meta->o_rd_ctx), n_read, nkv_l, d, page_size, stream));
+        kernel_launches++;
+      }
       prof_mark(P_ATTN);
       const int *qb_tok0 = cur_meta->d<int>(cur_meta->o_qb_tok0), *qb_len = cur_meta->d<int>(cur_meta->o_qb_len);
       const int *qb_pos0 = cur_meta->d<int>(cur_meta->o_qb_pos0), *qb_row = cur_meta->d<int>(cur_meta->o_qb_ptrow);
-      if (pf_tc) RET_CUDA(launch_attn_prefill_tc(kv_map, (long long)l * kv_rows_per_layer, q, d_page_table, max_pages, qb_tok0, qb_len, qb_pos0, qb_row, attn,
+      if (pf_tc) RET_CUDA(launch_attn_prefill_tc(kv_map, row0, q, d_page_table, max_pages, qb_tok0, qb_len, qb_pos0, qb_row, attn,
                                                  n_qblocks, nh_l, nkv_l, d, page_size, block_keys / n_qblocks, stream));
-      else RET_CUDA(launch_attn_prefill(kv_map, (long long)l * kv_rows_per_layer, q, d_page_table, max_pages, qb_tok0, qb_len, qb_pos0, qb_row, attn,
+      else RET_CUDA(launch_attn_prefill(kv_map, row0, q, d_page_table, max_pages, qb_tok0, qb_len, qb_pos0, qb_row, attn,
                                         n_qblocks, nh_l, nkv_l, d, page_size, stream));
-      kernel_launches += 2;
+      kernel_launches++;
+    } else if (pool8 || common_prefix > 0) {
+      RET_CUDA(write_rows());
+      prof_mark(P_ATTN);
+      const void *kv = pool8 ? static_cast<const void *>(pool8) : pool;
+      if (common_prefix > 0)
+        RET_CUDA(launch_attn_shared(q, kv, scale8, n_pages, d_page_table, max_pages, ptrow, ctx, common_prefix, attn, piece_area, T, nh_l, nkv_l, d, page_size,
+                                    stream));
+      else
+        RET_CUDA(launch_attn_stream(q, kv, scale8, d_page_table, max_pages, ptrow, ctx, 0, attn, nullptr, nullptr, piece_area, false, T, nh_l, nkv_l, d,
+                                    page_size, stream));
+      kernel_launches += common_prefix > 0 ? 3 : 1;
     } else {
       // decode: RoPE + KV write live inside the attention kernel (one kernel boundary less per layer)
       prof_mark(P_ATTN);
-      if (!skip(P_ATTN)) RET_CUDA(launch_attn_decode_fused(kv_map, (long long)l * kv_rows_per_layer, pool, partial, s_qkv, (long long)T * nqkv_l,
+      if (!skip(P_ATTN)) RET_CUDA(launch_attn_decode_fused(kv_map, row0, pool, partial, s_qkv, (long long)T * nqkv_l,
                                         pos, rope_cos, rope_sin, d_page_table, max_pages, ptrow, ctx, attn, attn_scratch,
                                         n_splits, T, nh_l, nkv_l, d, page_size, attn_share, stream));
       kernel_launches += n_splits > 1 ? 2 : 1;
@@ -939,6 +1011,7 @@ int Engine::prefill(int n, const int *slots, uint32_t *out_tokens, int *out_fini
       }
     }
     n_qblocks = QB;
+    plan_read_back(QB);
     last_T = T;
     rowmap_identity = false;
     ENG_CUDA(upload_step(T, R));
@@ -1076,6 +1149,7 @@ int Engine::step_mixed(int n, const int *slots, int max_prefill_tokens, uint32_t
   }
   if (T == 0) { last_rows = 0; return DIS_OK; }
   n_qblocks = QB;
+  plan_read_back(QB);
   last_T = T;
   rowmap_identity = false;
   ENG_CUDA(upload_step(T, R));
@@ -1186,6 +1260,13 @@ int Engine::decode(int n, const int *slots, uint32_t *out_tokens, int *out_finis
   const int n_splits = pick_attn_splits(T, max_ctx_b);
   // the attention's launch depends on how unlike the histories are, and so does the graph
   attn_share = attn_may_share(n_splits, T, nkv_l) && attn_sharing_pays(cur_meta->h<int>(cur_meta->o_ctx), T, nkv_l, m.head_dim);
+  common_prefix = 0;
+  if (cfg.flags & DIS_FLAG_ATTN_SHARED) {
+    std::vector<int> at;
+    for (int i : live) at.push_back(slots[i]);
+    const int keys = common_pages(T_live, at.data()) * page_size;
+    if (attn_shared_pays(T, nkv_l, m.head_dim, keys)) common_prefix = keys;
+  }
   last_T = T;
   rowmap_identity = true;
   ENG_CUDA(cudaEventRecord(ev0, stream));
@@ -1195,7 +1276,7 @@ int Engine::decode(int n, const int *slots, uint32_t *out_tokens, int *out_finis
     ENG_CUDA(enqueue_head(T, all_greedy));
     prof_mark(P_COUNT);
   } else {
-    const uint64_t key = ((uint64_t)T << 10) | ((uint64_t)n_splits << 2) | (attn_share ? 2u : 0u) | (all_greedy ? 1u : 0u);
+    const uint64_t key = ((uint64_t)(common_prefix / page_size) << 32) | ((uint64_t)T << 10) | ((uint64_t)n_splits << 2) | (attn_share ? 2u : 0u) | (all_greedy ? 1u : 0u);
     auto it = graphs.find(key);
     if (it == graphs.end()) {
       const uint64_t before = kernel_launches;

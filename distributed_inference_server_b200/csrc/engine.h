@@ -59,6 +59,7 @@ struct StepMeta {
   // sections (offsets in bytes)
   size_t o_tokens, o_pos, o_ptrow, o_ctx, o_rowmap, o_temp, o_topp, o_seed, o_step;
   size_t o_qb_tok0, o_qb_len, o_qb_pos0, o_qb_ptrow;  // prefill query blocks
+  size_t o_rd_row, o_rd_ctx;                           // sequences read back (DIS_FLAG_KV_INT8): page-table row, keys
   size_t o_arstep;                                     // forward-pass counter (epoch of the peer-memory exchange)
   size_t o_lb_tok0 = 0, o_lb_len = 0, o_ls = 0, o_lin = 0;  // latent attention of prompt portions: query blocks, spans, per (latent layer, slot) row of position 0
   size_t o_span = 0, o_ab_tok0 = 0, o_ab_len = 0, o_kb_tok0 = 0, o_kb_len = 0;       // layer-list family: span of each token; attention query blocks
@@ -103,6 +104,14 @@ struct Engine {
   size_t kv_layer_stride = 0;  // elements between layers in the pool
   long long kv_rows_per_layer = 0;
   TmaMap kv_map;  // the whole pool as [rows][head_dim]
+  // DIS_FLAG_KV_INT8: all layers' pages in 8 bits with their scales; kv_pool then holds one layer, read back for the prompts of a pass
+  int8_t *kv8_pool = nullptr;
+  float *kv8_scale = nullptr;
+  float *piece_area = nullptr;  // scratch of the attention over pieces (zero between calls)
+  int n_read = 0;               // sequences of the pass being enqueued whose histories are read back
+  int common_prefix = 0;        // positions that all sequences of this decode step have in common and that are read once (0: each by itself)
+  void plan_read_back(int n_blocks);
+  int common_pages(int n, const int *slots) const;
   bool use_pdl = true;  // programmatic dependent launch between the kernels of a step
   bool use_persist = true;  // prefill-sized projections through the persistent GEMM (DIS_GEMM_PERSIST=0: A/B runs)
   bool attn_share = false;  // decode attention of this step: a cluster's CTAs share its histories

@@ -82,6 +82,12 @@ typedef struct dis_model_config {
 #define DIS_FLAG_NO_PDL 4u     /* launch the kernels of a step without programmatic dependent launch */
 #define DIS_FLAG_PREFIX_CACHE 8u /* keep the full KV pages of finished prompts and map them into later requests that start
                                    with the same tokens (KVCacheManager::get_prefix, design.md:396; Property 9) */
+#define DIS_FLAG_KV_INT8 16u     /* keep keys and values in 8 bits (see dis_k_rope_kv_write_i8): about twice the pages in the same memory.  Decode steps
+                                   attend over them as they are; passes that read prompts turn the listed sequences' histories back into bf16, layer
+                                   by layer, in one layer's worth of extra pages */
+#define DIS_FLAG_ATTN_SHARED 32u /* decode steps read the pages that all of their sequences have in common once (dis_k_attn_shared), where that pays;
+                                   such pages come from DIS_FLAG_PREFIX_CACHE.  Both flags need 1, 2, 4 or 8 query heads per kv head and are refused
+                                   for layer-list decoders */
 typedef struct dis_engine_config {
   dis_model_config model;
   int32_t device;              /* CUDA ordinal (WorkerConfig.gpu_layers has no meaning here) */

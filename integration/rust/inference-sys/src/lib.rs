@@ -5,6 +5,8 @@ use std::os::raw::{c_char, c_int, c_void};
 
 pub const DIS_OK: c_int = 0;
 pub const DIS_FLAG_PREFIX_CACHE: u32 = 8;
+pub const DIS_FLAG_KV_INT8: u32 = 16;
+pub const DIS_FLAG_ATTN_SHARED: u32 = 32;
 
 #[repr(C)]
 #[derive(Clone, Copy, Default)]
