@@ -38,7 +38,10 @@ struct SpCfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kHalves * kSpBlock;
   static constexpr int kQBytes = (kPair ? 2 : 1) * kHalves * kSpQBlock;
-  static constexpr int kRing = D == 64 ? 6 : I8 ? (kPair ? 3 : 4) : (kPair ? 4 : 5);
+  // One tile of rows: an even number, so that a slot's tiles are all of one group, whose warps then wait for every phase of its barriers in turn.  (A
+  // warp that skips a phase takes the one before it for the one it waits for.)
+  static constexpr int kRing = D == 64 ? 6 : I8 && kPair ? 3 : 4;
+  static_assert(kPair || kRing % 2 == 0, "");
   static constexpr int kRawBytes = 2 * kSpTile * D;  // K and V rows of a tile in 8 bits
   static constexpr int kScaleFloats = 3 * kSpTile;   // of a tile: K factor, V scale, its log2
   static constexpr int kQ = 0, kK = kQBytes, kV = kK + kRing * kTileBytes, kRaw = kV + kRing * kTileBytes;
