@@ -151,6 +151,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
   auto s_full = [&](int g, int b) { return bars + 256u + 16u * g + 8u * b; };
   auto p_full = [&](int g, int b) { return bars + 288u + 16u * g + 8u * b; };
   auto pv_done = [&](int g) { return bars + 320u + 8u * g; };
+  auto o_done = [&](int g) { return bars + 352u + 8u * g; };
   const uint32_t q_full = bars + 336, tmem_slot = bars + 344, fail = bars + 348;
 
   const int slice = blockIdx.x, kvh = blockIdx.z, rt0 = blockIdx.y * (kPair ? 2 : 1);
@@ -167,7 +168,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
     }
     for (int g = 0; g < 2; g++) {
       for (int b = 0; b < 2; b++) { mbar_init(s_full(g, b), 1); mbar_init(p_full(g, b), 4); }
-      mbar_init(pv_done(g), 1);
+      mbar_init(pv_done(g), 1); mbar_init(o_done(g), 1);
     }
     mbar_init(q_full, 8);
     asm volatile("st.shared.u32 [%0], %1;" ::"r"(fail), "r"(0) : "memory");
@@ -260,6 +261,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
         for (uint32_t k = 0; k < kSpTile / 16; k++) umma_ts(o_base + g * D, p + 8 * k, b + k * 128, idesc_o, k > 0 ? 1u : (uint32_t)(i > 0));
         umma_commit(pv_done(g));
         umma_commit(v_empty(s));
+        if (i + 1 == count) umma_commit(o_done(g));
       }
       __syncwarp();
       if (i + 2 < count) ok = issue_s(i + 2);
@@ -410,9 +412,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
       if (lane == 0) mbar_arrive(p_full(g, i & 1));
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
-    // The last two products may both be under way: a wait for the last phase alone would take the one two before it for it
-    if (ok && count > 1) ok = sp_wait(pv_done(g), (uint32_t)count & 1u, fail);
-    if (ok && count > 0) ok = sp_wait(pv_done(g), (uint32_t)(count - 1) & 1u, fail);
+    // Of the last two products none, one or both may be complete, and pv_done's parity is the same before both and after both: the last has a barrier
+    // of its own
+    if (ok && count > 0) ok = sp_wait(o_done(g), 0, fail);
     tc_fence_after();
     // ---- the state: of this group's rows (kPair), or of both groups' keys joined, half of the columns each
     float2 *meet = reinterpret_cast<float2 *>(sp_smem + Cfg::kMeet);
