@@ -17,7 +17,13 @@
 // resident CTA, whatever the lengths are: lengths are read on the device, nothing depends on their maximum.  The CTA's four warps take its
 // tiles in turn, each with a ring of its own filled by cp.async (no barrier of the block per tile, nothing to spin on), and merge their states at
 // the end of a history's piece.  A history in several CTAs is finished by whichever of them ends last, which adds the pieces in the
-// order of the history: the result does not depend on who that is.
+// order of the history (more than eight of them in about sqrt(n) groups first, each added by the last CTA of the group): the result does not
+// depend on who that is.
+//
+// Measured (B200, 8 bits, from graphs; time at 6.54 TB/s, a plain copy's rate, beside it): 32 histories to 6000 tokens, 32 / 8 heads of 128, 30.2 us
+// (19.4); two to 60000, 64 / 8 heads, 39.4 (21.7); 64 to 3000, 32 / 4 heads of 64, 16.3 (5.3); four to 500 8.1 (0.3).  In the middle of a long
+// launch rows come in at 6 to 6.9 TB/s.  The rest: 2.5 to 5 us until every ring has been filled once, 2 to 3 us from the last row to the
+// result (states met in shared memory 0.5 to 1, fence and count 1.3, join 1), and CTAs of equal shares that end up to 15 % apart.
 #include <algorithm>
 
 #include <cuda_fp16.h>
