@@ -21,9 +21,10 @@
 // depend on who that is.
 //
 // Measured (B200, 8 bits, from graphs; time at 6.54 TB/s, a plain copy's rate, beside it): 32 histories to 6000 tokens, 32 / 8 heads of 128, 30.2 us
-// (19.4); two to 60000, 64 / 8 heads, 39.4 (21.7); 64 to 3000, 32 / 4 heads of 64, 16.3 (5.3); four to 500 8.1 (0.3).  In the middle of a long
+// (19.4); two to 60000, 64 / 8 heads, 37.7 (21.7); 64 to 3000, 32 / 4 heads of 64, 16.3 (5.3); four to 500 8.1 (0.3).  In the middle of a long
 // launch rows come in at 6 to 6.9 TB/s.  The rest: 2.5 to 5 us until every ring has been filled once, 2 to 3 us from the last row to the
-// result (states met in shared memory 0.5 to 1, fence and count 1.3, join 1), and CTAs of equal shares that end up to 15 % apart.
+// result (states met in shared memory 0.5 to 1, fence and count 1.3, join 1), and CTAs of equal shares that end up to 15 % apart.  (Tiles taken
+// as warps come free would even that out, and make the sums' order, so the result's last bits, differ from call to call.)
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -628,41 +629,54 @@ attn_stream_kernel(const StArgs a) {
         }
         const bool whole = level || groups == 1;
         const float *src_o = level ? a.group_o : a.piece_o, *src_ml = level ? a.group_ml : a.piece_ml;
-        // four dims of a head to a thread at a time, kAhead pieces' on their way
+        // four dims of a head to a thread (groups of eight: of two heads), kAhead pieces' on their way.  (Both heads at once: two histories of 60000 in 28
+        // pieces 40.1 -> 37.7 us; eight pieces at once are no faster and cost a short call 0.5 us: code is fetched anew at every launch)
         constexpr int kQuads = G * D / 4, kAhead = 4;
-#pragma unroll 1
-        for (int quad = threadIdx.x; quad < kQuads; quad += kStWarps * 32) {
-          const int h = quad / (D / 4), i = quad % (D / 4) * 4;
-          float M = kPieceNone, l = 0.f;
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int kMine = (kQuads + kStWarps * 32 - 1) / (kStWarps * 32);
+        if (threadIdx.x < kQuads) {
+          float M[kMine], l[kMine];
+          float4 o[kMine];
+#pragma unroll
+          for (int q = 0; q < kMine; q++) { M[q] = kPieceNone; l[q] = 0.f; o[q] = make_float4(0.f, 0.f, 0.f, 0.f); }
 #pragma unroll 1
           for (int k = 0; k < n; k += kAhead) {
-            float2 ml[kAhead];
-            float4 x[kAhead];
+            float2 ml[kAhead][kMine];
+            float4 x[kAhead][kMine];
 #pragma unroll
             for (int j = 0; j < kAhead; j++)
               if (k + j < n) {
                 const size_t sl = slot_of(level ? c_first + (k + j) * fan : lead + k + j);
-                ml[j] = __ldcg(reinterpret_cast<const float2 *>(src_ml + sl * st_ml(G)) + h);
-                x[j] = __ldcg(reinterpret_cast<const float4 *>(src_o) + sl * kQuads + quad);
+#pragma unroll
+                for (int q = 0; q < kMine; q++) {
+                  const int quad = threadIdx.x + q * kStWarps * 32;
+                  ml[j][q] = __ldcg(reinterpret_cast<const float2 *>(src_ml + sl * st_ml(G)) + quad / (D / 4));
+                  x[j][q] = __ldcg(reinterpret_cast<const float4 *>(src_o) + sl * kQuads + quad);
+                }
               }
 #pragma unroll
             for (int j = 0; j < kAhead; j++)
               if (k + j < n) {
-                const float m_new = fmaxf(M, ml[j].x), f = piece_ex2(M - m_new), fn = piece_ex2(ml[j].x - m_new);
-                M = m_new;
-                l = l * f + ml[j].y * fn;
-                o.x = o.x * f + x[j].x * fn;
-                o.y = o.y * f + x[j].y * fn;
-                o.z = o.z * f + x[j].z * fn;
-                o.w = o.w * f + x[j].w * fn;
+#pragma unroll
+                for (int q = 0; q < kMine; q++) {
+                  const float m_new = fmaxf(M[q], ml[j][q].x), f = piece_ex2(M[q] - m_new), fn = piece_ex2(ml[j][q].x - m_new);
+                  M[q] = m_new;
+                  l[q] = l[q] * f + ml[j][q].y * fn;
+                  o[q].x = o[q].x * f + x[j][q].x * fn;
+                  o[q].y = o[q].y * f + x[j][q].y * fn;
+                  o[q].z = o[q].z * f + x[j][q].z * fn;
+                  o[q].w = o[q].w * f + x[j][q].w * fn;
+                }
               }
           }
-          if (whole) {
-            put(row + h, i, o, M, l);
-          } else {
-            __stcg(reinterpret_cast<float4 *>(a.group_o) + slot_of(lead) * kQuads + quad, o);
-            if (i == 0) __stcg(reinterpret_cast<float2 *>(a.group_ml + slot_of(lead) * st_ml(G)) + h, make_float2(M, l));
+#pragma unroll
+          for (int q = 0; q < kMine; q++) {
+            const int quad = threadIdx.x + q * kStWarps * 32, h = quad / (D / 4), i = quad % (D / 4) * 4;
+            if (whole) {
+              put(row + h, i, o[q], M[q], l[q]);
+            } else {
+              __stcg(reinterpret_cast<float4 *>(a.group_o) + slot_of(lead) * kQuads + quad, o[q]);
+              if (i == 0) __stcg(reinterpret_cast<float2 *>(a.group_ml + slot_of(lead) * st_ml(G)) + h, make_float2(M[q], l[q]));
+            }
           }
         }
         if (whole) break;
