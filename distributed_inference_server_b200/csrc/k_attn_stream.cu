@@ -20,10 +20,10 @@
 // order of the history (more than eight of them in about sqrt(n) groups first, each added by the last CTA of the group): the result does not
 // depend on who that is.
 //
-// Measured (B200, 8 bits, from graphs; time at 6.54 TB/s, a plain copy's rate, beside it): 32 histories to 6000 tokens, 32 / 8 heads of 128, 30.2 us
-// (19.4); two to 60000, 64 / 8 heads, 37.7 (21.7); 64 to 3000, 32 / 4 heads of 64, 16.3 (5.3); four to 500 8.1 (0.3).  In the middle of a long
+// Measured (B200, 8 bits, from graphs; time at 6.54 TB/s, a plain copy's rate, beside it): 32 histories to 6000 tokens, 32 / 8 heads of 128, 29.9 us
+// (19.4); two to 60000, 64 / 8 heads, 36.9 (21.7); 64 to 3000, 32 / 4 heads of 64, 15.9 (5.3); four to 500 7.8 (0.3).  In the middle of a long
 // launch rows come in at 6 to 6.9 TB/s.  The rest: 2.5 to 5 us until every ring has been filled once, 2 to 3 us from the last row to the
-// result (states met in shared memory 0.5 to 1, fence and count 1.3, join 1), and CTAs of equal shares that end up to 15 % apart.  (Tiles taken
+// result (states met in shared memory 0.5 to 1, count 0.9, join 1 a level), and CTAs of equal shares that end up to 15 % apart.  (Tiles taken
 // as warps come free would even that out, and make the sums' order, so the result's last bits, differ from call to call.)
 #include <algorithm>
 
@@ -588,15 +588,16 @@ attn_stream_kernel(const StArgs a) {
 
   // ================= histories in several CTAs: the one that ends last joins the pieces, in the order of the history.  More than eight are joined in
   // about as many groups as a group has pieces, and then the groups: what one CTA reads at the end stays short however long the history is.  The
-  // barriers and one thread's fences on both sides order all threads' writes and reads; both histories' first counts share them
+  // barriers and one thread's atomic, a release and an acquire, order all threads' writes and reads (with fences on both sides of a relaxed one
+  // 0.4 us more a level); both histories' first counts share them
   if (part_first[0] != part_last[0] || part_first[1] != part_last[1]) {
     auto fan_of = [&](int parts) { return parts <= 8 ? parts : (int)ceilf(sqrtf((float)parts)); };
     auto arrive = [&](int level, size_t slot, int n) {
       int *count = a.counters + level * stream_slots() + slot;
-      __threadfence();
-      const bool last = atomicAdd(count, 1) == n - 1;
+      int before;
+      asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+      const bool last = before == n - 1;
       if (last) *count = 0;  // as the next call wants it
-      __threadfence();
       return last;
     };
     __syncthreads();
