@@ -20,8 +20,8 @@
 // maximum grows by more than 8 in the log2 domain, so O is seldom rescaled (the reference cancels).
 // 8-bit pages: scales stay outside the products, as in k_attn_stream.cu; q and the weights are fp16 there, bf16 otherwise.
 //
-// Measured (B200, from graphs, all three kernels): 32 requests behind 6000 tokens, 32 / 8 heads of 128, own parts to 500, bf16: 26.6 us;
-// 64 behind 8000, 64 / 8 heads, own parts to 700, 8 bits: 54.8 (10.6 at a library product's rate, 7.6 for its bytes).  A step of 256 rows x 64 keys takes 1.0 us
+// Measured (B200, from graphs, all three kernels): 32 requests behind 6000 tokens, 32 / 8 heads of 128, own parts to 500, bf16: 26.2 us;
+// 64 behind 8000, 64 / 8 heads, own parts to 700, 8 bits: 53.7 (10.6 at a library product's rate, 7.6 for its bytes).  A step of 256 rows x 64 keys takes 1.0 us
 // in bf16 and 1.4 in 8 bits.  In clocks, bf16 / 8 bits: exponentials and P 1290 / 1264 (two warps to a scheduler, 1024 of them the exponentials alone),
 // maximum 200 / 619 (scales of K and V from shared memory), waits for scores 190 / 500.  The products take 1280 of the tensor pipe (S with N = 64
 // reads 6 KB of operands each, at shared memory's rate); 8 bits add the fp16 tiles and the scales to shared memory's load.  The score buffers are two per
@@ -620,9 +620,11 @@ static int shared_slices(int blocks, int tiles) {
 static int shared_blocks(int T, int G, int n_kv) { const int rt = shared_row_tiles(T, G); return (rt > 1 ? (rt + 1) / 2 : 1) * n_kv; }
 
 // Whether the prefix is read once, or every token goes alone (one kernel, to which the others' reads of the same pages are hits in L2): from about 2^25 entries
-// of T prefixes on the former is ahead.  From graphs, own parts of 100, together / alone, us: 32 / 8 heads of 128, bf16: 4 x 8192 22.2 / 22.1, 8 x 4096 19.6 / 19.9,
-// 16 x 1024 18.2 / 14.9, 16 x 2048 18.7 / 19.7, 32 x 512 18.3 / 15.3, 32 x 1024 19.1 / 19.9, 32 x 4096 21.1 / 48.6; 64 / 8 heads in 8 bits: 16 x 2048 21.7 / 22.3, 32 x 1024
-// 25.9 / 21.6, 32 x 2048 27.5 / 31.0; 32 / 4 heads of 64: 16 x 4096 18.2 / 15.0, 32 x 4096 19.9 / 20.4, 64 x 1024 18.4 / 15.1, 64 x 2048 19.2 / 20.4
+// of T prefixes on the former is ahead.  From graphs, own parts of 100, together / alone, us: 32 / 8 heads of 128, bf16: 4 x 8192 21.9 / 21.2, 8 x 4096 19.5 / 19.6,
+// 16 x 1024 18.2 / 14.6, 16 x 2048 18.4 / 19.4, 32 x 512 18.3 / 14.9, 32 x 1024 18.8 / 19.6, 32 x 4096 20.7 / 48.3; 32 / 4 heads of 64: 16 x 4096 18.2 / 14.8,
+// 32 x 4096 19.5 / 20.1, 64 x 1024 18.4 / 14.4, 64 x 2048 18.7 / 20.2.  More than 128 rows, and 8 bits, cross a little later, and at the rule's own
+// edge are behind: 64 x 512, bf16, 23.7 / 21.4 but 64 x 1024 25.1 / 31.7; 64 / 8 heads in 8 bits: 32 x 1024 25.1 / 20.7, 64 x 512 28.6 / 22.9, but 32 x 2048 26.7 / 29.7,
+// 64 x 1024 30.2 / 33.0
 bool attn_shared_pays(int T, int n_kv, int d, int prefix) { return T > 1 && (long long)T * prefix * n_kv * d >= 1 << 25; }
 
 size_t attn_shared_scratch_elems(int T, int n_heads, int n_kv, int d) {  // the stream's, its states, the slices' states
