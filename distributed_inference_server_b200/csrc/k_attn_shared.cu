@@ -11,11 +11,12 @@
 // clock and SM: 512 clocks per 128 rows x 64 keys beside 256 + 256 of the products for d = 128).
 //
 // attn_prefix_kernel, one CTA per SM:
-//   warp 0          bf16 pages: K and V tiles of 64 keys by TMA into a ring
+//   warp 0          bf16 pages: K and V tiles of 64 keys by TMA into a ring; 8-bit pages: their rows into a ring of their own
 //   warps 1, 2      the MMAs of softmax group 0 and 1: S = Q K^T (M128 N64), two tiles ahead of O += P V (M128 N = d)
 //   warps 4-7, 8-11 softmax groups, one thread per row.  Up to 128 rows: both groups have the same rows, group 0 the even key tiles, group 1
 //                   the odd ones, and their states are joined at the end; more: 128 rows each, and both read every tile (kPair)
-//   warps 12-15     8-bit pages: rows by cp.async into a ring of their own, turned to fp16 (exact) into the tiles' ring
+//   warps 12-15     8-bit pages: rows turned to fp16 (exact) into the tiles' ring.  They are near to being the bound, so they do nothing else: with the
+//                   rows' addresses and copies (cp.async) theirs too, a third of their time, 64 requests behind 64000 tokens took 179 us, now 168
 // TMEM: four score buffers of 64 columns, P over its scores, an O of d columns per group.  A group raises a row's reference only when its
 // maximum grows by more than 8 in the log2 domain, so O is seldom rescaled (the reference cancels).
 // 8-bit pages: scales stay outside the products, as in k_attn_stream.cu; q and the weights are fp16 there, bf16 otherwise.
@@ -38,7 +39,7 @@ namespace dis {
 constexpr int kSpTile = 64;               // keys of a tile
 constexpr int kSpBlock = kSpTile * 128;   // 64 keys x 64 dims, 16 bits
 constexpr int kSpQBlock = 128 * 128;      // 128 rows x 64 dims
-constexpr int kSpRaw = 3;                 // stages of 8-bit rows
+constexpr int kSpRaw = 3;                 // stages of 8-bit rows (and of their scales)
 constexpr int kSpMaxSlices = 32;
 
 template <int D, bool I8, bool kPair>
@@ -134,6 +135,11 @@ __device__ __forceinline__ void sp_rescale_16(uint32_t addr, float f) {
   sp_tmem_st_16(addr, v);
 }
 
+// size bytes (a multiple of 16, as both addresses are) to shared memory, counted by the barrier
+__device__ __forceinline__ void sp_bulk(uint32_t dst, const void *src, uint32_t size, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(size), "r"(bar) : "memory");
+}
+
 struct SpArgs {
   const uint16_t *q;
   const int8_t *pool;     // I8
@@ -160,6 +166,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
   auto p_full = [&](int g, int b) { return bars + 288u + 16u * g + 8u * b; };
   auto pv_done = [&](int g) { return bars + 320u + 8u * g; };
   auto o_done = [&](int g) { return bars + 352u + 8u * g; };
+  auto raw_full = [&](int s) { return bars + 368u + 8u * s; };
+  auto raw_empty = [&](int s) { return bars + 400u + 8u * s; };
   const uint32_t q_full = bars + 336, tmem_slot = bars + 344, fail = bars + 348;
 
   const int slice = blockIdx.x, kvh = blockIdx.z, rt0 = blockIdx.y * (kPair ? 2 : 1);
@@ -178,6 +186,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
       for (int b = 0; b < 2; b++) { mbar_init(s_full(g, b), 1); mbar_init(p_full(g, b), 4); }
       mbar_init(pv_done(g), 1); mbar_init(o_done(g), 1);
     }
+    for (int s = 0; s < kSpRaw; s++) { mbar_init(raw_full(s), 1); mbar_init(raw_empty(s), 4); }
     mbar_init(q_full, 8);
     asm volatile("st.shared.u32 [%0], %1;" ::"r"(fail), "r"(0) : "memory");
     fence_barrier_init();
@@ -233,6 +242,34 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
       for (int u = max(0, t - NS); u < t; u++)
         for (int v = 0; v < 2; v++)
           while (!sp_poll(v ? v_full(u % NS) : k_full(u % NS), (uint32_t)(u / NS) & 1u) && __all_sync(0xffffffffu, clock64() - began < kSpPatience)) {}
+    }
+  } else if (I8 && warp == 0) {
+    // ===== 8-bit rows: those of a page that a tile meets are one run of bytes, for K and for V; a lane to a run.  Behind the prefix nothing is
+    // copied: what lies there are whole numbers from before, under weights of zero
+    const int run = min(page_size, kSpTile);
+    int win_first = 1 << 30, win = 0, t = 0;
+    for (; t < n; t++) {
+      const int st = t % kSpRaw, first = (tile0 + t) * kSpTile, rows = min(kSpTile, a.prefix - first), p0 = first >> a.page_shift;
+      if (t >= kSpRaw && !sp_wait(raw_empty(st), (uint32_t)(t / kSpRaw - 1) & 1u, fail)) break;
+      if (p0 < win_first || p0 + 8 - win_first > 32) {  // a tile has at most eight pages
+        win_first = p0;
+        win = pt[min(p0 + lane, last_page)];
+      }
+      if (lane == 0) mbar_expect_tx(raw_full(st), 2 * rows * D);
+      const int at = lane * run, pos = first + at;
+      const long long page = __shfl_sync(0xffffffffu, win, (min(pos >> a.page_shift, last_page) - win_first) & 31);
+      if (at < rows) {
+        const int8_t *src = a.pool + (((page * 2) * a.n_kv + kvh) * page_size + (pos & (page_size - 1))) * D;
+        const uint32_t dst = base + Cfg::kRaw + st * Cfg::kRawBytes + at * D, bytes = min(run, rows - at) * D;
+        sp_bulk(dst, src, bytes, raw_full(st));
+        sp_bulk(dst + kSpTile * D, src + (long long)a.n_kv * page_size * D, bytes, raw_full(st));
+      }
+      __syncwarp();
+    }
+    if (sp_failed(fail)) {  // as above
+      const long long began = clock64();
+      for (int u = max(0, t - kSpRaw); u < t; u++)
+        while (!sp_poll(raw_full(u % kSpRaw), (uint32_t)(u / kSpRaw) & 1u) && __all_sync(0xffffffffu, clock64() - began < kSpPatience)) {}
     }
   } else if (warp == 1 || warp == 2) {
     // ===== MMA issuer of group g: the warp converged, one elected lane issues
@@ -470,37 +507,22 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
       if (kPair || g == 0) reinterpret_cast<float2 *>(a.state_ml)[tile * 128 + row] = make_float2(m, l);
     }
   } else if (I8 && warp >= 12) {
-    // ===== 8-bit rows to fp16 tiles.  A thread fetches what it turns itself: no barrier between the two rings
+    // ===== 8-bit rows to fp16 tiles.  A thread fetches the scale that it turns itself
     const int th = threadIdx.x - 384;
     constexpr int kPer = D / 16, kMine = kSpTile * kPer / 128;  // 16-byte chunks of a row; of K (and of V) for a thread
-    const uint32_t raw = base + Cfg::kRaw, raw_s = base + Cfg::kRawScale;
+    const uint32_t raw_s = base + Cfg::kRawScale;
     int win_first = 1 << 30, win = 0;
-    auto fetch = [&](int t) {  // every lane of a warp looks at rows in order: the page numbers are kept 32 at a time, one in each lane
+    auto fetch = [&](int t) {  // scales: threads 0-63 of K, 64-127 of V.  Every lane of a warp looks at rows in order: the page numbers are kept 32 at a time
       if (t < n) {
-        const int st = t % kSpRaw;
-#pragma unroll
-        for (int i = 0; i < kMine; i++) {
-          const int id = i * 128 + th, r = id / kPer, c = id % kPer;
-          const int pos = (tile0 + t) * kSpTile + r, p0 = (tile0 + t) * kSpTile >> a.page_shift;
-          const int pi = min(pos >> a.page_shift, last_page);
-          if (p0 < win_first || p0 + 8 - win_first > 32) {  // a tile has at most eight pages
-            win_first = p0;
-            win = pt[min(p0 + lane, last_page)];
-          }
-          const long long page = __shfl_sync(0xffffffffu, win, pi - win_first);
-          const long long row = ((page * 2) * a.n_kv + kvh) * page_size + (pos & (page_size - 1));
-          const uint32_t in = pos < a.prefix ? 16 : 0;
-          const int8_t *src = a.pool + row * D + c * 16;
-          const uint32_t dst = raw + st * Cfg::kRawBytes + id * 16;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in) : "memory");
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + kSpTile * D), "l"(src + (long long)a.n_kv * page_size * D), "r"(in) : "memory");
+        const int st = t % kSpRaw, p0 = (tile0 + t) * kSpTile >> a.page_shift;
+        if (p0 < win_first || p0 + 8 - win_first > 32) {
+          win_first = p0;
+          win = pt[min(p0 + lane, last_page)];
         }
-        {  // scales: threads 0-63 of K, 64-127 of V
-          const int r = th & 63, pos = (tile0 + t) * kSpTile + r, pi = min(pos >> a.page_shift, last_page);
-          const long long page = __shfl_sync(0xffffffffu, win, pi - win_first);
-          const long long row = ((page * 2 + (th >> 6)) * a.n_kv + kvh) * page_size + (pos & (page_size - 1));
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(raw_s + (st * 128 + th) * 4), "l"(a.scale + row), "r"(pos < a.prefix ? 4 : 0) : "memory");
-        }
+        const int r = th & 63, pos = (tile0 + t) * kSpTile + r, pi = min(pos >> a.page_shift, last_page);
+        const long long page = __shfl_sync(0xffffffffu, win, pi - win_first);
+        const long long row = ((page * 2 + (th >> 6)) * a.n_kv + kvh) * page_size + (pos & (page_size - 1));
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(raw_s + (st * 128 + th) * 4), "l"(a.scale + row), "r"(pos < a.prefix ? 4 : 0) : "memory");
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -510,6 +532,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
       const int s = t % NS, st = t % kSpRaw;
       fetch(t + kSpRaw - 1);  // into the stage that this thread read last
       asm volatile("cp.async.wait_group %0;" ::"n"(kSpRaw - 1) : "memory");
+      ok = sp_wait(raw_full(st), (uint32_t)(t / kSpRaw) & 1u, fail);
+      if (!ok) break;
 #pragma unroll
       for (int v = 0; v < 2; v++) {
         if (t >= NS) ok = sp_wait(v ? v_empty(s) : k_empty(s), (uint32_t)(t / NS - 1) & 1u, fail);
@@ -546,6 +570,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
         if (lane == 0) mbar_arrive(v ? v_full(s) : k_full(s));
       }
       if (!ok) break;
+      if (lane == 0) mbar_arrive(raw_empty(st));
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
