@@ -168,6 +168,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
   auto o_done = [&](int g) { return bars + 352u + 8u * g; };
   auto raw_full = [&](int s) { return bars + 368u + 8u * s; };
   auto raw_empty = [&](int s) { return bars + 400u + 8u * s; };
+  auto turn = [&](int g, int quarter) { return bars + 424u + 32u * g + 8u * quarter; };
   const uint32_t q_full = bars + 336, tmem_slot = bars + 344, fail = bars + 348;
 
   const int slice = blockIdx.x, kvh = blockIdx.z, rt0 = blockIdx.y * (kPair ? 2 : 1);
@@ -185,6 +186,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
     for (int g = 0; g < 2; g++) {
       for (int b = 0; b < 2; b++) { mbar_init(s_full(g, b), 1); mbar_init(p_full(g, b), 4); }
       mbar_init(pv_done(g), 1); mbar_init(o_done(g), 1);
+      for (int k = 0; k < 4; k++) mbar_init(turn(g, k), 1);
     }
     for (int s = 0; s < kSpRaw; s++) { mbar_init(raw_full(s), 1); mbar_init(raw_empty(s), 4); }
     mbar_init(q_full, 8);
@@ -362,6 +364,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
     const uint32_t o_addr = o_base + lane_off + g * D;
     float m = kPieceNone, l = 0.f;
     bool ok = true;
+    // 8 bits: the two warps of a scheduler take their exponentials in turn, group 0 first, so that one's maximum (scales from shared memory) runs under the
+    // other's exponentials: 53.8 -> 52.4 us (64 behind 8000; bf16, whose maximum is short: none)
+    if (I8 && g == 1 && lane == 0) mbar_arrive(turn(0, quarter));
     for (int i = 0; i < count; i++) {
       const int t = tile_of(g, i), slot = t % NS;
       ok = sp_wait(s_full(g, i & 1), (uint32_t)(i >> 1) & 1u, fail);
@@ -428,6 +433,10 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
         l *= f;
         m = m_new;
       }
+      if (I8) {
+        ok = sp_wait(turn(g, quarter), (uint32_t)i & 1u, fail);
+        if (!ok) break;
+      }
       const float2 neg = make_float2(-m, -m);
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -450,6 +459,10 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
           }
         }
         sp_tmem_st_16(s_addr + 16 * h, w);
+      }
+      if (I8) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(turn(g ^ 1, quarter));
       }
       sp_tmem_st_wait();
       tc_fence_before();
