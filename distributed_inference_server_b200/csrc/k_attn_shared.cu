@@ -22,12 +22,14 @@
 // 8-bit pages: scales stay outside the products, as in k_attn_stream.cu; q and the weights are fp16 there, bf16 otherwise.
 //
 // Measured (B200, from graphs, all three kernels): 32 requests behind 6000 tokens, 32 / 8 heads of 128, own parts to 500, bf16: 26.2 us;
-// 64 behind 8000, 64 / 8 heads, own parts to 700, 8 bits: 53.7 (10.6 at a library product's rate, 7.6 for its bytes).  A step of 256 rows x 64 keys takes 1.0 us
-// in bf16 and 1.4 in 8 bits.  In clocks, bf16 / 8 bits: exponentials and P 1290 / 1264 (two warps to a scheduler, 1024 of them the exponentials alone),
-// maximum 200 / 619 (scales of K and V from shared memory), waits for scores 190 / 500.  The products take 1280 of the tensor pipe (S with N = 64
-// reads 6 KB of operands each, at shared memory's rate); 8 bits add the fp16 tiles and the scales to shared memory's load.  The score buffers are two per
-// group so that a group's next product runs under its softmax: one of twice the keys, which needs 1024 clocks instead, was slower (54.9 -> 59.9 us),
-// the two groups being in phase.  A CTA's start (queries, barriers, TMEM) and end (128 KB of state) are six steps' worth.
+// 64 behind 8000, 64 / 8 heads, own parts to 700, 8 bits: 51.7 (10.6 at a library product's rate, 7.6 for its bytes).  A step of 256 rows x 64 keys takes 1.0 us
+// in bf16 and 1.27 in 8 bits.  In clocks, bf16: exponentials and P 1290 (two warps to a scheduler, 1024 of them the exponentials alone), maximum 200,
+// waits for scores 190, of 1760; the products take 1280 of the tensor pipe (S with N = 64 reads 6 KB of operands each, at shared memory's rate).  8 bits: a group's
+// exponentials 970 (in turn), maximum 560 (scales of K and V from shared memory), its turn 190, P's hand-over 125, the tile's fp16 rows 330, of 2210: shared memory
+// and issue slots are shared with the warps that turn rows to fp16.  Eight of those instead of four (96 registers), rows through registers, or tiles of half
+// the size were slower (161 us of 64 behind 64000 -> 182, 230, 210).  The score buffers are two per group so that a group's next product runs under its
+// softmax: one of twice the keys, which needs 1024 clocks of tensor pipe instead, was slower (bf16 131 -> 154 us at 64000), the two groups being in phase.  A
+// CTA's start (queries, barriers, TMEM) and end (128 KB of state) are six steps' worth.
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -661,8 +663,8 @@ static int shared_blocks(int T, int G, int n_kv) { const int rt = shared_row_til
 // of T prefixes on the former is ahead.  From graphs, own parts of 100, together / alone, us: 32 / 8 heads of 128, bf16: 4 x 8192 21.9 / 21.2, 8 x 4096 19.5 / 19.6,
 // 16 x 1024 18.2 / 14.6, 16 x 2048 18.4 / 19.4, 32 x 512 18.3 / 14.9, 32 x 1024 18.8 / 19.6, 32 x 4096 20.7 / 48.3; 32 / 4 heads of 64: 16 x 4096 18.2 / 14.8,
 // 32 x 4096 19.5 / 20.1, 64 x 1024 18.4 / 14.4, 64 x 2048 18.7 / 20.2.  More than 128 rows, and 8 bits, cross a little later, and at the rule's own
-// edge are behind: 64 x 512, bf16, 23.7 / 21.4 but 64 x 1024 25.1 / 31.7; 64 / 8 heads in 8 bits: 32 x 1024 25.1 / 20.7, 64 x 512 28.6 / 22.9, but 32 x 2048 26.7 / 29.7,
-// 64 x 1024 30.2 / 33.0
+// edge are behind: 64 x 512, bf16, 23.7 / 21.4 but 64 x 1024 25.1 / 31.7; 64 / 8 heads in 8 bits: 32 x 1024 24.8 / 20.8, 64 x 512 28.6 / 23.1, but 32 x 2048 26.1 / 29.9,
+// 64 x 1024 30.0 / 32.7
 bool attn_shared_pays(int T, int n_kv, int d, int prefix) { return T > 1 && (long long)T * prefix * n_kv * d >= 1 << 25; }
 
 size_t attn_shared_scratch_elems(int T, int n_heads, int n_kv, int d) {  // the stream's, its states, the slices' states
