@@ -26,8 +26,8 @@
 // in bf16 and 1.27 in 8 bits.  In clocks, bf16: exponentials and P 1290 (two warps to a scheduler, 1024 of them the exponentials alone), maximum 200,
 // waits for scores 190, of 1760; the products take 1280 of the tensor pipe (S with N = 64 reads 6 KB of operands each, at shared memory's rate).  8 bits: a group's
 // exponentials 970 (in turn), maximum 560 (scales of K and V from shared memory), its turn 190, P's hand-over 125, the tile's fp16 rows 330, of 2210: shared memory
-// and issue slots are shared with the warps that turn rows to fp16.  Eight of those instead of four (96 registers), rows through registers, or tiles of half
-// the size were slower (161 us of 64 behind 64000 -> 182, 230, 210).  The score buffers are two per group so that a group's next product runs under its
+// and issue slots are shared with the warps that turn rows to fp16.  Eight of those instead of four (96 registers) were slower (64 behind 64000
+// 161 -> 182 us), as were rows through registers (179 -> 230 before warp 0 copied them) or turned in units of half a tile (-> 210).  The score buffers are two per group so that a group's next product runs under its
 // softmax: one of twice the keys, which needs 1024 clocks of tensor pipe instead, was slower (bf16 131 -> 154 us at 64000), the two groups being in phase.  A
 // CTA's start (queries, barriers, TMEM) and end (128 KB of state) are six steps' worth.
 #include <algorithm>
