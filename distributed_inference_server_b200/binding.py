@@ -189,7 +189,7 @@ PROTOTYPES = {
     "dis_k_kv_read_i8": (C.c_int, [vp, vp, vp, vp, vp, C.c_int32, vp, vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, vp]),
     "dis_k_attn_paged_i8_scratch_elems": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "dis_k_attn_paged_i8": (C.c_int, [vp, vp, vp, vp, C.c_int32, vp, vp, vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, vp]),
-    "dis_k_attn_shared_in_common": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "dis_k_attn_shared_in_common": (C.c_int, [C.c_int32] * 6),
     "dis_k_attn_shared_scratch_elems": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "dis_k_attn_shared": (C.c_int, [vp, vp, vp, C.c_int64, vp, C.c_int32, vp, vp, C.c_int32, vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                     C.c_int32, vp]),

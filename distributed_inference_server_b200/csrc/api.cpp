@@ -365,7 +365,9 @@ int dis_k_attn_paged_i8(const uint16_t *q, const int8_t *pool, const float *scal
   return k_ret(dis::launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, 0, out, nullptr, nullptr, scratch, false, T, n_heads, n_kv, d,
                                        page_size, (cudaStream_t)stream));
 }
-int dis_k_attn_shared_in_common(int32_t T, int32_t n_kv, int32_t d, int32_t prefix) { return dis::attn_shared_pays(T, n_kv, d, prefix) ? 1 : 0; }
+int dis_k_attn_shared_in_common(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d, int32_t prefix, int32_t int8) {
+  return dis::attn_shared_pays(T, n_heads, n_kv, d, prefix, int8 != 0) ? 1 : 0;
+}
 size_t dis_k_attn_shared_scratch_elems(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d) {
   return T > 0 ? dis::attn_shared_scratch_elems(T, n_heads, n_kv, d) : 0;
 }

@@ -1265,7 +1265,7 @@ int Engine::decode(int n, const int *slots, uint32_t *out_tokens, int *out_finis
     std::vector<int> at;
     for (int i : live) at.push_back(slots[i]);
     const int keys = common_pages(T_live, at.data()) * page_size;
-    if (attn_shared_pays(T, nkv_l, m.head_dim, keys)) common_prefix = keys;
+    if (attn_shared_pays(T, nh_l, nkv_l, m.head_dim, keys, kv8_pool != nullptr)) common_prefix = keys;
   }
   last_T = T;
   rowmap_identity = true;

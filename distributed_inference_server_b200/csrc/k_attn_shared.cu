@@ -659,13 +659,19 @@ static int shared_slices(int blocks, int tiles) {
 }
 static int shared_blocks(int T, int G, int n_kv) { const int rt = shared_row_tiles(T, G); return (rt > 1 ? (rt + 1) / 2 : 1) * n_kv; }
 
-// Whether the prefix is read once, or every token goes alone (one kernel, to which the others' reads of the same pages are hits in L2): from about 2^25 entries
-// of T prefixes on the former is ahead.  From graphs, own parts of 100, together / alone, us: 32 / 8 heads of 128, bf16: 4 x 8192 21.9 / 21.2, 8 x 4096 19.5 / 19.6,
-// 16 x 1024 18.2 / 14.6, 16 x 2048 18.4 / 19.4, 32 x 512 18.3 / 14.9, 32 x 1024 18.8 / 19.6, 32 x 4096 20.7 / 48.3; 32 / 4 heads of 64: 16 x 4096 18.2 / 14.8,
-// 32 x 4096 19.5 / 20.1, 64 x 1024 18.4 / 14.4, 64 x 2048 18.7 / 20.2.  More than 128 rows, and 8 bits, cross a little later, and at the rule's own
-// edge are behind: 64 x 512, bf16, 23.7 / 21.4 but 64 x 1024 25.1 / 31.7; 64 / 8 heads in 8 bits: 32 x 1024 24.8 / 20.8, 64 x 512 28.6 / 23.1, but 32 x 2048 26.1 / 29.9,
-// 64 x 1024 30.0 / 32.7
-bool attn_shared_pays(int T, int n_kv, int d, int prefix) { return T > 1 && (long long)T * prefix * n_kv * d >= 1 << 25; }
+// Whether the prefix is read once, or every token goes alone (one kernel, to which the others' reads of the same pages are hits in L2): from 2^25 entries of T
+// prefixes on the former is ahead; heads of 128 in two tiles of rows or more, and in 8 bits, each cross a quarter later.  From graphs, own parts of 100,
+// together / alone, us, at 1, 1.25 and 1.5 times 2^25 entries:
+//   32 / 8 heads of 128, bf16   16 tokens 18.6 / 19.4, 19.1 / 21.8, 19.3 / 24.3;  32: 19.2 / 19.5, 19.0 / 22.1, 19.4 / 24.4;  64 (two tiles): 24.2 / 21.5, 24.3 / 24.6, 24.9 / 27.0
+//   the same in 8 bits          8: 21.3 / 19.0, 22.5 / 21.5, 23.5 / 23.6;  32: 20.4 / 19.1, 20.1 / 21.4, 20.6 / 23.7;  64: 26.2 / 21.1, 26.1 / 23.8, 26.9 / 26.1
+//   64 / 8 heads, 8 bits        16: 20.7 / 20.9, 21.2 / 22.9, 21.6 / 24.9;  32 (two tiles): 25.5 / 20.8, 25.5 / 23.2, 26.0 / 25.2;  64: 29.7 / 23.1, 29.7 / 25.9, 30.2 / 28.2
+//   32 / 4 heads of 64, 8 bits  16: 20.7 / 22.2, 21.4 / 25.9, 22.3 / 28.5;  64 (four tiles): 20.9 / 21.3, 21.7 / 24.2, 22.0 / 26.9
+// (four tokens in 8 bits cross later still: 28.0 / 24.3 at 1.5); at half of 2^25, bf16: 16 18.2 / 14.6, 32 18.3 / 14.9
+bool attn_shared_pays(int T, int n_heads, int n_kv, int d, int prefix, bool int8) {
+  if (T < 2 || n_kv < 1) return false;
+  const int quarters = 4 + (d == 128 ? (T > 128 / std::max(n_heads / n_kv, 1)) + int8 : 0);
+  return (long long)T * prefix * n_kv * d >= (long long)quarters << 23;
+}
 
 size_t attn_shared_scratch_elems(int T, int n_heads, int n_kv, int d) {  // the stream's, its states, the slices' states
   if (T <= 0 || n_kv <= 0 || n_heads < n_kv || d <= 0) return 0;
@@ -689,7 +695,7 @@ cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float 
                                const int *pt_row, const int *ctx, int prefix, uint16_t *out, float *scratch, int T, int n_heads, int n_kv, int d,
                                int page_size, cudaStream_t st) {
   const int G = n_heads / n_kv;
-  if (!attn_shared_pays(T, n_kv, d, prefix))
+  if (!attn_shared_pays(T, n_heads, n_kv, d, prefix, scale != nullptr))
     return launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, 0, out, nullptr, nullptr, scratch, false, T, n_heads, n_kv, d, page_size, st);
   SpArgs a{};
   a.q = q; a.pool = static_cast<const int8_t *>(pool); a.scale = scale; a.page_table = page_table; a.pt_row = pt_row; a.max_pages = max_pages;

@@ -130,7 +130,7 @@ cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float 
                                int n_heads, int n_kv, int d, int page_size, cudaStream_t st);
 
 // k_attn_shared.cu : the same where positions [0, prefix) are the same rows for every token
-bool attn_shared_pays(int T, int n_kv, int d, int prefix);
+bool attn_shared_pays(int T, int n_heads, int n_kv, int d, int prefix, bool int8);
 size_t attn_shared_scratch_elems(int T, int n_heads, int n_kv, int d);
 cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float *scale, long long n_pages, const int *page_table, int max_pages,
                                const int *pt_row, const int *ctx, int prefix, uint16_t *out, float *scratch, int T, int n_heads, int n_kv, int d,

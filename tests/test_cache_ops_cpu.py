@@ -16,10 +16,12 @@ def test_scratch_grows_with_nothing_but_its_arguments():
     assert lib.dis_k_attn_shared_scratch_elems(0, 32, 8, 128) == lib.dis_k_attn_shared_scratch_elems(4, 32, 0, 128) == 0
 
 
-@pytest.mark.parametrize("T,nkv,d,prefix,want", [(1, 8, 128, 1 << 20, 0), (2, 8, 128, 0, 0), (32, 8, 128, 1024, 1), (32, 8, 128, 1023, 0), (64, 4, 64, 2048, 1),
-                                                 (8, 4, 64, 1000, 0), (1000, 64, 128, 1 << 21, 1)])
-def test_when_a_prefix_is_read_once(T, nkv, d, prefix, want):
-    assert B.load().dis_k_attn_shared_in_common(T, nkv, d, prefix) == want
+@pytest.mark.parametrize("T,nh,nkv,d,prefix,int8,want", [
+    (1, 32, 8, 128, 1 << 20, 0, 0), (2, 32, 8, 128, 0, 0, 0), (32, 32, 8, 128, 1024, 0, 1), (32, 32, 8, 128, 1023, 0, 0), (64, 32, 4, 64, 2048, 1, 1),
+    (8, 32, 4, 64, 1000, 0, 0), (1000, 64, 64, 128, 1 << 21, 1, 1), (32, 32, 8, 128, 1279, 1, 0), (32, 32, 8, 128, 1280, 1, 1), (33, 32, 8, 128, 1241, 0, 0),
+    (33, 32, 8, 128, 1242, 0, 1), (64, 64, 8, 128, 767, 1, 0), (64, 64, 8, 128, 768, 1, 1), (4, 0, 0, 128, 1 << 20, 0, 0)])
+def test_when_a_prefix_is_read_once(T, nh, nkv, d, prefix, int8, want):
+    assert B.load().dis_k_attn_shared_in_common(T, nh, nkv, d, prefix, int8) == want
 
 
 def test_no_cpu_fallback():

@@ -473,12 +473,12 @@ def test_shared_prefix_many_steps_again(int8, T, group, d, prefix):
 
 
 @pytest.mark.parametrize("int8", [False, True])
-@pytest.mark.parametrize("T,group,nkv,d,page,prefix", [(72, 1, 8, 128, 16, 577), (64, 2, 8, 128, 8, 641), (40, 4, 8, 128, 64, 1000), (57, 8, 8, 128, 32, 704), (33, 4, 8, 128, 128, 1500),
-                                                      (80, 8, 8, 64, 8, 1001), (130, 1, 8, 64, 64, 640), (12, 4, 8, 128, 64, 4095), (5, 8, 8, 128, 16, 7000), (9, 2, 16, 64, 64, 5000)])
+@pytest.mark.parametrize("T,group,nkv,d,page,prefix", [(72, 1, 8, 128, 16, 577), (64, 2, 8, 128, 8, 641), (40, 4, 8, 128, 64, 1250), (57, 8, 8, 128, 32, 896), (33, 4, 8, 128, 128, 1500),
+                                                      (80, 8, 8, 64, 8, 1001), (130, 1, 8, 64, 64, 640), (12, 4, 8, 128, 64, 4095), (5, 8, 8, 128, 16, 8300), (9, 2, 16, 64, 64, 5000)])
 def test_shared_prefix_read_once(int8, T, group, nkv, d, page, prefix):
     """Sizes at which the prefix is read once: prefixes that end inside a tile and inside a page, one tile of rows and several, rows behind the last, and
     among the histories some that end at the prefix's end, inside it, or are empty."""
-    assert lib().dis_k_attn_shared_in_common(T, nkv, d, prefix) == 1
+    assert lib().dis_k_attn_shared_in_common(T, nkv * group, nkv, d, prefix, int8) == 1
     own = np.random.default_rng(T).integers(0, 90, T)
     ctx = [prefix + int(n) for n in own]
     ctx[1], ctx[2], ctx[3] = prefix, prefix - 1, 0
@@ -495,7 +495,7 @@ def test_shared_prefix_read_once(int8, T, group, nkv, d, page, prefix):
 
 def test_shared_prefix_read_once_rows_without_numbers_and_sizes():
     """A NaN among the prefix's keys reaches every token that sees it, in its kv head; scales from 2^-60 to 2^40; large scores."""
-    T, prefix = 40, 1000
+    T, prefix = 40, 1250
     ctx = [prefix + 1 + t for t in range(T)]
     ctx[7] = 90
     spread = lambda x, g: torch.where(torch.arange(2, device=DEV).view(1, 2, 1, 1, 1) == 1, torch.exp2(  # noqa: E731

@@ -130,7 +130,7 @@ def test_common_pages_are_read_once(int8):
     rng = np.random.default_rng(3)
     base = rng.integers(0, shape.vocab, 1300).tolist()
     prompts = [base + rng.integers(0, shape.vocab, 3 + 5 * i).tolist() for i in range(32)]
-    assert B.load().dis_k_attn_shared_in_common(32, 8, 128, 1296) == 1
+    assert B.load().dis_k_attn_shared_in_common(32, 32, 8, 128, 1296, int8) == 1
     runs = []
     for shared in (0, B.FLAG_ATTN_SHARED):
         e = make_engine(shape, seed=5, max_batch=32, kv_pages=500, page_size=16, max_step_tokens=4096, flags=B.FLAG_PREFIX_CACHE | shared | (B.FLAG_KV_INT8 if int8 else 0))
