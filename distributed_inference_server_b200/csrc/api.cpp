@@ -383,7 +383,7 @@ int dis_k_attn_shared(const uint16_t *q, const void *kv_pool, const float *scale
   if (!q || !kv_pool || !page_table || !pt_row || !ctx || !out || !scratch) return cache_refuse(me, "null pointer");
   if (off(q, 16) || off(kv_pool, 16) || off(scratch, 16) || off(out, 4)) return cache_refuse(me, "q, the pool and scratch start on 16 bytes, out on 4");
   CallOverlap overlap(stream);
-  return k_ret(dis::launch_attn_shared(q, kv_pool, scale, n_pages, page_table, max_pages, pt_row, ctx, prefix, out, scratch, T, n_heads, n_kv, d, page_size,
+  return k_ret(dis::launch_attn_shared(q, kv_pool, scale, n_pages, page_table, max_pages, pt_row, ctx, prefix, out, scratch, T, n_heads, n_kv, d, page_size, true,
                                        (cudaStream_t)stream));
 }
 int dis_k_sample(const float *logits, int64_t ld, int32_t T, int32_t V, const float *temperature, const float *top_p,

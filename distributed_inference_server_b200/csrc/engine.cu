@@ -814,7 +814,7 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
       const void *kv = pool8 ? static_cast<const void *>(pool8) : pool;
       if (common_prefix > 0)
         RET_CUDA(launch_attn_shared(q, kv, scale8, n_pages, d_page_table, max_pages, ptrow, ctx, common_prefix, attn, piece_area, T, nh_l, nkv_l, d, page_size,
-                                    stream));
+                                    false, stream));
       else
         RET_CUDA(launch_attn_stream(q, kv, scale8, d_page_table, max_pages, ptrow, ctx, 0, attn, nullptr, nullptr, piece_area, false, T, nh_l, nkv_l, d,
                                     page_size, stream));

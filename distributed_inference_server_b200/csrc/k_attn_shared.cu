@@ -693,7 +693,7 @@ static cudaError_t prefix_launch(const TmaMap &map, const SpArgs &a, cudaStream_
 
 cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float *scale, long long n_pages, const int *page_table, int max_pages,
                                const int *pt_row, const int *ctx, int prefix, uint16_t *out, float *scratch, int T, int n_heads, int n_kv, int d,
-                               int page_size, cudaStream_t st) {
+                               int page_size, bool chain, cudaStream_t st) {
   const int G = n_heads / n_kv;
   if (!attn_shared_pays(T, n_heads, n_kv, d, prefix, scale != nullptr))
     return launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, 0, out, nullptr, nullptr, scratch, false, T, n_heads, n_kv, d, page_size, st);
@@ -713,6 +713,9 @@ cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float 
   // The own parts first: their CTAs end one after the other, and the prefix's start as SMs come free
   DIS_CUDA_TRY(launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, prefix, nullptr, own_o, own_ml, scratch, true, T, n_heads, n_kv, d,
                                   page_size, st));
+  // (chain: the kernels behind the first overlap with the one in front of them even where the first may not with what is in front of it)
+  struct Pdl { const bool was = pdl_enabled(); ~Pdl() { pdl_enabled() = was; } } pdl;
+  pdl_enabled() |= chain;
   a.late_wait = pdl_enabled();
   const bool pair = a.row_tiles > 1;
 #define DIS_SP(DD, II, PP) DIS_CUDA_TRY((prefix_launch<DD, II, PP>(map, a, st)))

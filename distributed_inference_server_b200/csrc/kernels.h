@@ -134,7 +134,7 @@ bool attn_shared_pays(int T, int n_heads, int n_kv, int d, int prefix, bool int8
 size_t attn_shared_scratch_elems(int T, int n_heads, int n_kv, int d);
 cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float *scale, long long n_pages, const int *page_table, int max_pages,
                                const int *pt_row, const int *ctx, int prefix, uint16_t *out, float *scratch, int T, int n_heads, int n_kv, int d,
-                               int page_size, cudaStream_t st);
+                               int page_size, bool chain, cudaStream_t st);
 
 // k_gemm_tcgen05.cu
 cudaError_t make_tma_map_2d(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows);
