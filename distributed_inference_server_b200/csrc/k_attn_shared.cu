@@ -662,14 +662,18 @@ static int shared_blocks(int T, int G, int n_kv) { const int rt = shared_row_til
 // Whether the prefix is read once, or every token goes alone (one kernel, to which the others' reads of the same pages are hits in L2): from 2^25 entries of T
 // prefixes on the former is ahead; heads of 128 in two tiles of rows or more, and in 8 bits, each cross a quarter later.  From graphs, own parts of 100,
 // together / alone, us, at 1, 1.25 and 1.5 times 2^25 entries:
-//   32 / 8 heads of 128, bf16   16 tokens 18.6 / 19.4, 19.1 / 21.8, 19.3 / 24.3;  32: 19.2 / 19.5, 19.0 / 22.1, 19.4 / 24.4;  64 (two tiles): 24.2 / 21.5, 24.3 / 24.6, 24.9 / 27.0
-//   the same in 8 bits          8: 21.3 / 19.0, 22.5 / 21.5, 23.5 / 23.6;  32: 20.4 / 19.1, 20.1 / 21.4, 20.6 / 23.7;  64: 26.2 / 21.1, 26.1 / 23.8, 26.9 / 26.1
-//   64 / 8 heads, 8 bits        16: 20.7 / 20.9, 21.2 / 22.9, 21.6 / 24.9;  32 (two tiles): 25.5 / 20.8, 25.5 / 23.2, 26.0 / 25.2;  64: 29.7 / 23.1, 29.7 / 25.9, 30.2 / 28.2
-//   32 / 4 heads of 64, 8 bits  16: 20.7 / 22.2, 21.4 / 25.9, 22.3 / 28.5;  64 (four tiles): 20.9 / 21.3, 21.7 / 24.2, 22.0 / 26.9
-// (four tokens in 8 bits cross later still: 28.0 / 24.3 at 1.5); at half of 2^25, bf16: 16 18.2 / 14.6, 32 18.3 / 14.9
+//   32 / 8 heads of 128, bf16   16 tokens 18.6 / 19.3, 18.1 / 21.8, 19.4 / 24.0;  32: 19.2 / 19.6, 17.6 / 22.1, 18.5 / 24.4;  64 (two tiles): 24.2 / 21.5, 22.9 / 24.6, 23.6 / 26.9
+//   the same in 8 bits          8: 21.3 / 19.0, 22.7 / 21.6, 23.7 / 23.6;  32: 20.4 / 19.1, 18.8 / 21.4, 19.9 / 23.7;  64: 26.2 / 21.1, 26.1 / 23.8, 26.6 / 26.0
+//   64 / 8 heads, 8 bits        16: 20.7 / 20.9, 21.8 / 23.0, 24.3 / 24.7;  32 (two tiles): 25.5 / 20.8, 25.5 / 23.2, 25.8 / 25.2;  64: 29.7 / 23.1, 29.7 / 25.9, 28.2 / 28.2
+//   32 / 4 heads of 64, 8 bits  16: 18.1 / 22.2, 19.1 / 25.7, 20.3 / 28.6;  64 (four tiles): 20.7 / 21.1, 21.1 / 24.2, 21.8 / 26.7
+// at half of 2^25, bf16: 16 18.2 / 14.6, 32 18.3 / 14.9.
+// A few tokens make little of a product's 128 rows, and the prefix has to be turned to fp16 all the same.  At 1.5, 2 and 4 times 2^25: 32 / 8 heads of 128, 8 bits
+// 2: 38.2 / 25.6, 45.1 / 30.1, 73.4 / 48.9;  4: 28.3 / 24.4, 32.4 / 28.9, 46.2 / 46.9;  6: 25.2 / 25.0, 26.3 / 28.7, 37.2 / 46.3;  heads of 64 in 8 bits
+// 4: 30.6 / 30.5, 36.5 / 36.2, 59.3 / 59.3;  6: 26.2 / 30.1, 29.5 / 36.8, 44.7 / 57.9;  bf16, heads of 128, 2: 33.7 / 34.2, 39.5 / 38.8, 61.4 / 78.2 (at 1: 26.7 / 22.3);
+// 4: 24.0 / 25.3, 26.8 / 31.1, 40.0 / 61.3
 bool attn_shared_pays(int T, int n_heads, int n_kv, int d, int prefix, bool int8) {
-  if (T < 2 || n_kv < 1) return false;
-  const int quarters = 4 + (d == 128 ? (T > 128 / std::max(n_heads / n_kv, 1)) + int8 : 0);
+  if (T < (int8 ? 6 : 2) || n_kv < 1) return false;
+  const int quarters = (T < 4 ? 8 : 4) + (d == 128 ? (T > 128 / std::max(n_heads / n_kv, 1)) + int8 : 0);
   return (long long)T * prefix * n_kv * d >= (long long)quarters << 23;
 }
 

@@ -437,8 +437,8 @@ DIS_API int dis_k_attn_paged_i8(const uint16_t *q, const int8_t *pool, const flo
  * the first ctx[t] positions of the prefix.  kv_pool: bf16 pages (scale NULL) or 8-bit pages with their scales; n_pages pages.
  * Rows of a bf16 prefix page past `prefix` must hold finite values, as for dis_k_attn_paged.  scratch: dis_k_attn_shared_scratch_elems()
  * floats under the terms of dis_k_attn_paged_i8, whose scratch it may be too. */
-/* Whether dis_k_attn_shared reads the prefix once for these sizes (int8: 8-bit pages): below about 2^25 entries of T prefixes every token by itself, in
- * one kernel, is ahead.  The result is the same to rounding.  Needs no GPU. */
+/* Whether dis_k_attn_shared reads the prefix once for these sizes (int8: 8-bit pages): below about 2^25 entries of T prefixes, and for a few tokens
+ * over 8-bit pages, every token by itself, in one kernel, is ahead.  The result is the same to rounding.  Needs no GPU. */
 DIS_API int dis_k_attn_shared_in_common(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d, int32_t prefix, int32_t int8);
 DIS_API size_t dis_k_attn_shared_scratch_elems(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d);
 DIS_API int dis_k_attn_shared(const uint16_t *q, const void *kv_pool, const float *scale, int64_t n_pages, const int32_t *page_table,

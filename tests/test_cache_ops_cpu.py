@@ -19,7 +19,8 @@ def test_scratch_grows_with_nothing_but_its_arguments():
 @pytest.mark.parametrize("T,nh,nkv,d,prefix,int8,want", [
     (1, 32, 8, 128, 1 << 20, 0, 0), (2, 32, 8, 128, 0, 0, 0), (32, 32, 8, 128, 1024, 0, 1), (32, 32, 8, 128, 1023, 0, 0), (64, 32, 4, 64, 2048, 1, 1),
     (8, 32, 4, 64, 1000, 0, 0), (1000, 64, 64, 128, 1 << 21, 1, 1), (32, 32, 8, 128, 1279, 1, 0), (32, 32, 8, 128, 1280, 1, 1), (33, 32, 8, 128, 1241, 0, 0),
-    (33, 32, 8, 128, 1242, 0, 1), (64, 64, 8, 128, 767, 1, 0), (64, 64, 8, 128, 768, 1, 1), (4, 0, 0, 128, 1 << 20, 0, 0)])
+    (33, 32, 8, 128, 1242, 0, 1), (64, 64, 8, 128, 767, 1, 0), (64, 64, 8, 128, 768, 1, 1), (4, 0, 0, 128, 1 << 20, 0, 0), (5, 32, 8, 128, 1 << 20, 1, 0),
+    (6, 32, 8, 128, 6827, 1, 1), (2, 32, 8, 128, 32767, 0, 0), (2, 32, 8, 128, 32768, 0, 1), (4, 32, 8, 128, 8192, 0, 1)])
 def test_when_a_prefix_is_read_once(T, nh, nkv, d, prefix, int8, want):
     assert B.load().dis_k_attn_shared_in_common(T, nh, nkv, d, prefix, int8) == want
 

@@ -474,7 +474,7 @@ def test_shared_prefix_many_steps_again(int8, T, group, d, prefix):
 
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("T,group,nkv,d,page,prefix", [(72, 1, 8, 128, 16, 577), (64, 2, 8, 128, 8, 641), (40, 4, 8, 128, 64, 1250), (57, 8, 8, 128, 32, 896), (33, 4, 8, 128, 128, 1500),
-                                                      (80, 8, 8, 64, 8, 1001), (130, 1, 8, 64, 64, 640), (12, 4, 8, 128, 64, 4095), (5, 8, 8, 128, 16, 8300), (9, 2, 16, 64, 64, 5000)])
+                                                      (80, 8, 8, 64, 8, 1001), (130, 1, 8, 64, 64, 640), (12, 4, 8, 128, 64, 4095), (6, 8, 8, 128, 16, 7000), (9, 2, 16, 64, 64, 5000)])
 def test_shared_prefix_read_once(int8, T, group, nkv, d, page, prefix):
     """Sizes at which the prefix is read once: prefixes that end inside a tile and inside a page, one tile of rows and several, rows behind the last, and
     among the histories some that end at the prefix's end, inside it, or are empty."""
