@@ -21,8 +21,8 @@
 // maximum grows by more than 8 in the log2 domain, so O is seldom rescaled (the reference cancels).
 // 8-bit pages: scales stay outside the products, as in k_attn_stream.cu; q and the weights are fp16 there, bf16 otherwise.
 //
-// Measured (B200, from graphs, all three kernels): 32 requests behind 6000 tokens, 32 / 8 heads of 128, own parts to 500, bf16: 26.2 us;
-// 64 behind 8000, 64 / 8 heads, own parts to 700, 8 bits: 51.7 (10.6 at a library product's rate, 7.6 for its bytes).  A step of 256 rows x 64 keys takes 1.0 us
+// Measured (B200, from graphs, all three kernels): 32 requests behind 6000 tokens, 32 / 8 heads of 128, own parts to 500, bf16: 24.9 us;
+// 64 behind 8000, 64 / 8 heads, own parts to 700, 8 bits: 50.1 (10.6 at a library product's rate, 7.6 for its bytes).  A step of 256 rows x 64 keys takes 1.0 us
 // in bf16 and 1.27 in 8 bits.  In clocks, bf16: exponentials and P 1290 (two warps to a scheduler, 1024 of them the exponentials alone), maximum 200,
 // waits for scores 190, of 1760; the products take 1280 of the tensor pipe (S with N = 64 reads 6 KB of operands each, at shared memory's rate).  8 bits: a group's
 // exponentials 970 (in turn), maximum 560 (scales of K and V from shared memory), its turn 190, P's hand-over 125, the tile's fp16 rows 330, of 2210: shared memory
