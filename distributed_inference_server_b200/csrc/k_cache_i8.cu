@@ -148,6 +148,7 @@ kv_read_i8_kernel(const int8_t *__restrict__ pool, const float *__restrict__ sca
   const int planes = 2 * n_kv << page_shift;  // rows of a page
   const int per_page = (int)((((long long)planes << d_shift) + kCrBytes - 1) / kCrBytes), per = d_shift - 4;  // units of a page; log2 of a row's 16-byte chunks
   const long long units = (long long)s_pages[n_rows] * per_page;
+  const bool wide = (reinterpret_cast<uintptr_t>(out) & 31u) == 0;  // (every offset into the pool is a multiple of 32 bytes)
   for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const int pg = (int)(unit / per_page), part = (int)(unit % per_page);
     int b = 0, e = n_rows;  // the row with s_pages[r] <= pg < s_pages[r + 1]
@@ -181,9 +182,15 @@ kv_read_i8_kernel(const int8_t *__restrict__ pool, const float *__restrict__ sca
           y[2 * j] = float2_to_bf16x2(q4.x * s[k], q4.y * s[k]);
           y[2 * j + 1] = float2_to_bf16x2(q4.z * s[k], q4.w * s[k]);
         }
-        // a whole 32-byte sector at a time: as two halves, stored by two instructions, L2 takes every sector twice
-        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + (dst << d_shift) + (long long)c * 16), "r"(y[0]), "r"(y[1]), "r"(y[2]),
-                     "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
+        uint16_t *to = out + (dst << d_shift) + (long long)c * 16;
+        // a whole 32-byte sector at a time (where the pool starts on one): as two halves, stored by two instructions, L2 takes every sector twice
+        if (wide) {
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]),
+                       "r"(y[6]), "r"(y[7]) : "memory");
+        } else {
+          reinterpret_cast<uint4 *>(to)[0] = make_uint4(y[0], y[1], y[2], y[3]);
+          reinterpret_cast<uint4 *>(to)[1] = make_uint4(y[4], y[5], y[6], y[7]);
+        }
       }
     }
   }
