@@ -138,6 +138,7 @@ PROTOTYPES = {
     "dis_engine_last_logprobs": (C.c_int, [vp, C.c_int32, vp, vp]),
     "dis_engine_profile_decode": (C.c_int, [vp, C.c_int32, vp, vp, vp, vp, vp]),
     "dis_engine_replay_last_step": (C.c_int, [vp, C.c_int32, f32p]),
+    "dis_engine_graph_stats": (C.c_int, [vp, C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
     "dis_engine_status": (C.c_int, [vp, C.POINTER(WorkerStatus)]),
     "dis_engine_model_info": (C.c_int, [vp, C.POINTER(ModelConfig)]),
     "dis_tp_unique_id": (C.c_int, [vp]),

@@ -135,6 +135,15 @@ int dis_engine_replay_last_step(dis_engine *e, int32_t n, float *avg_ms) {
   LOCKED(e);
   return e->eng.replay_last_step(n, avg_ms);
 }
+int dis_engine_graph_stats(dis_engine *e, int64_t *kept, int64_t *captured) {
+  if (int rc = guard_null(e)) return rc;
+  LOCKED(e);
+  if (!kept || !captured) return e->eng.fail(DIS_ERR_INVALID_ARGUMENT, "graph_stats: null pointer");
+  *kept = 0;
+  for (auto &g : e->eng.graphs) *kept += g.second != nullptr;
+  *captured = (int64_t)e->eng.graphs_captured;
+  return DIS_OK;
+}
 int dis_engine_last_logits(dis_engine *e, float *host, int32_t n_rows) {
   if (int rc = guard_null(e)) return rc;
   LOCKED(e);
@@ -362,7 +371,7 @@ int dis_k_attn_paged_i8(const uint16_t *q, const int8_t *pool, const float *scal
   if (!q || !pool || !scale || !page_table || !pt_row || !ctx || !out || !scratch) return cache_refuse(me, "null pointer");
   if (off(q, 16) || off(pool, 16) || off(scratch, 16) || off(out, 4)) return cache_refuse(me, "q, the pool and scratch start on 16 bytes, out on 4");
   CallOverlap overlap(stream);
-  return k_ret(dis::launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, 0, out, nullptr, nullptr, scratch, false, T, n_heads, n_kv, d,
+  return k_ret(dis::launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, 0, nullptr, out, nullptr, nullptr, scratch, false, T, n_heads, n_kv, d,
                                        page_size, (cudaStream_t)stream));
 }
 int dis_k_attn_shared_in_common(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d, int32_t prefix, int32_t int8) {
@@ -383,8 +392,8 @@ int dis_k_attn_shared(const uint16_t *q, const void *kv_pool, const float *scale
   if (!q || !kv_pool || !page_table || !pt_row || !ctx || !out || !scratch) return cache_refuse(me, "null pointer");
   if (off(q, 16) || off(kv_pool, 16) || off(scratch, 16) || off(out, 4)) return cache_refuse(me, "q, the pool and scratch start on 16 bytes, out on 4");
   CallOverlap overlap(stream);
-  return k_ret(dis::launch_attn_shared(q, kv_pool, scale, n_pages, page_table, max_pages, pt_row, ctx, prefix, out, scratch, T, n_heads, n_kv, d, page_size, true,
-                                       (cudaStream_t)stream));
+  return k_ret(dis::launch_attn_shared(q, kv_pool, scale, n_pages, page_table, max_pages, pt_row, ctx, prefix, nullptr, out, scratch, T, n_heads, n_kv, d, page_size,
+                                       true, (cudaStream_t)stream));
 }
 int dis_k_sample(const float *logits, int64_t ld, int32_t T, int32_t V, const float *temperature, const float *top_p,
                  const uint64_t *seeds, const uint64_t *steps, uint32_t *out_tokens, float *out_logprob, void *stream) {

@@ -176,6 +176,7 @@ int Engine::init(const dis_engine_config *c) {
     s.o_seed = sec((size_t)max_batch * 8); s.o_step = sec((size_t)max_batch * 8);
     s.o_qb_tok0 = sec(ct * 4); s.o_qb_len = sec(ct * 4); s.o_qb_pos0 = sec(ct * 4); s.o_qb_ptrow = sec(ct * 4);
     s.o_rd_row = sec((size_t)max_batch * 4); s.o_rd_ctx = sec((size_t)max_batch * 4);
+    s.o_prefix = sec(16);
     s.o_arstep = sec(16);
     s.bytes = o;
     cudaError_t e1 = cudaMallocHost(reinterpret_cast<void **>(&s.host), s.bytes);
@@ -239,6 +240,7 @@ int Engine::init(const dis_engine_config *c) {
   if (const char *g = getenv("DIS_GEMM_PERSIST")) use_persist = atoi(g) != 0;
   if (const char *g = getenv("DIS_GEMV_MAX_T")) gemv_max_t = std::max(0, std::min(kGemvMaxT, atoi(g)));
   if (const char *g = getenv("DIS_ATTN_MAX_SPLITS")) max_attn_splits = atoi(g);
+  if (const char *g = getenv("DIS_MAX_GRAPHS")) max_graphs = (size_t)std::max(1, atoi(g));
   // Measurement aid, never set in production: DIS_DEBUG_SKIP=norm,attn,... leaves those kernel classes out of the
   // decode step (its results are then garbage) so that step time with and without a class gives the class's marginal
   // cost INSIDE the graph, where programmatic dependent launch overlaps neighbours and ncu's isolated times mislead.
@@ -813,11 +815,11 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
       prof_mark(P_ATTN);
       const void *kv = pool8 ? static_cast<const void *>(pool8) : pool;
       if (common_prefix > 0)
-        RET_CUDA(launch_attn_shared(q, kv, scale8, n_pages, d_page_table, max_pages, ptrow, ctx, common_prefix, attn, piece_area, T, nh_l, nkv_l, d, page_size,
-                                    false, stream));
+        RET_CUDA(launch_attn_shared(q, kv, scale8, n_pages, d_page_table, max_pages, ptrow, ctx, common_prefix, cur_meta->d<int>(cur_meta->o_prefix), attn, piece_area, T, nh_l,
+                                    nkv_l, d, page_size, false, stream));
       else
-        RET_CUDA(launch_attn_stream(q, kv, scale8, d_page_table, max_pages, ptrow, ctx, 0, attn, nullptr, nullptr, piece_area, false, T, nh_l, nkv_l, d,
-                                    page_size, stream));
+        RET_CUDA(launch_attn_stream(q, kv, scale8, d_page_table, max_pages, ptrow, ctx, 0, nullptr, attn, nullptr, nullptr, piece_area, false, T, nh_l, nkv_l,
+                                    d, page_size, stream));
       kernel_launches += common_prefix > 0 ? 3 : 1;
     } else {
       // decode: RoPE + KV write live inside the attention kernel (one kernel boundary less per layer)
@@ -1239,7 +1241,7 @@ int Engine::decode(int n, const int *slots, uint32_t *out_tokens, int *out_finis
   }
   const int T_live = (int)live.size();
   if (T_live == 0) { last_rows = 0; return DIS_OK; }
-  // One CUDA graph exists per (rows, attention splits): a batch that drains one sequence at a time would capture a new
+  // One CUDA graph exists per rows and launch of the attention (splits, or slices of a common prefix): a batch that drains one sequence at a time would capture a new
   // graph at every size.  Above 8 rows the step is padded to the next multiple of 8 with copies of the last live row
   // (same slot, token and position: the copies recompute and rewrite exactly the same K/V row and their tokens are
   // ignored), so at most max_batch / 8 + 8 sizes are ever captured.
@@ -1260,13 +1262,15 @@ int Engine::decode(int n, const int *slots, uint32_t *out_tokens, int *out_finis
   const int n_splits = pick_attn_splits(T, max_ctx_b);
   // the attention's launch depends on how unlike the histories are, and so does the graph
   attn_share = attn_may_share(n_splits, T, nkv_l) && attn_sharing_pays(cur_meta->h<int>(cur_meta->o_ctx), T, nkv_l, m.head_dim);
-  common_prefix = 0;
+  common_prefix = prefix_slices = 0;
   if (cfg.flags & DIS_FLAG_ATTN_SHARED) {
     std::vector<int> at;
     for (int i : live) at.push_back(slots[i]);
     const int keys = common_pages(T_live, at.data()) * page_size;
-    if (attn_shared_pays(T, nh_l, nkv_l, m.head_dim, keys, kv8_pool != nullptr)) common_prefix = keys;
+    prefix_slices = attn_shared_slices(T, nh_l, nkv_l, m.head_dim, keys, kv8_pool != nullptr);
+    if (prefix_slices > 0) common_prefix = keys;
   }
+  cur_meta->h<int>(cur_meta->o_prefix)[0] = common_prefix;
   last_T = T;
   rowmap_identity = true;
   ENG_CUDA(cudaEventRecord(ev0, stream));
@@ -1276,9 +1280,19 @@ int Engine::decode(int n, const int *slots, uint32_t *out_tokens, int *out_finis
     ENG_CUDA(enqueue_head(T, all_greedy));
     prof_mark(P_COUNT);
   } else {
-    const uint64_t key = ((uint64_t)(common_prefix / page_size) << 32) | ((uint64_t)T << 10) | ((uint64_t)n_splits << 2) | (attn_share ? 2u : 0u) | (all_greedy ? 1u : 0u);
+    // Attention over pieces has one launch per T, or per T and slices of a common prefix, whose length its kernels read from the step's metadata; the
+    // other is launched by splits and sharing
+    const bool pieces = kv8_pool || common_prefix > 0;
+    const uint64_t launch = pieces ? (uint64_t)prefix_slices << 32 : ((uint64_t)n_splits << 2) | (attn_share ? 2u : 0u);
+    const uint64_t key = launch | ((uint64_t)T << 10) | (all_greedy ? 1u : 0u);
     auto it = graphs.find(key);
     if (it == graphs.end()) {
+      if (graphs.size() >= max_graphs) {  // more shapes than a server meets in a while: start over (no graph runs between steps)
+        for (auto &g : graphs) cudaGraphExecDestroy(g.second);
+        graphs.clear();
+        graph_launches.clear();
+        last_graph = nullptr;
+      }
       const uint64_t before = kernel_launches;
       cudaGraph_t g = nullptr;
       ENG_CUDA(cudaStreamBeginCapture(stream, cudaStreamCaptureModeThreadLocal));
@@ -1296,6 +1310,7 @@ int Engine::decode(int n, const int *slots, uint32_t *out_tokens, int *out_finis
       cudaGraphDestroy(g);
       graph_launches[key] = kernel_launches - before;
       kernel_launches = before;
+      graphs_captured++;
       it = graphs.emplace(key, ex).first;
     }
     ENG_CUDA(cudaGraphLaunch(it->second, stream));

@@ -60,6 +60,7 @@ struct StepMeta {
   size_t o_tokens, o_pos, o_ptrow, o_ctx, o_rowmap, o_temp, o_topp, o_seed, o_step;
   size_t o_qb_tok0, o_qb_len, o_qb_pos0, o_qb_ptrow;  // prefill query blocks
   size_t o_rd_row, o_rd_ctx;                           // sequences read back (DIS_FLAG_KV_INT8): page-table row, keys
+  size_t o_prefix = 0;                                 // positions that the step's sequences have in common (Engine::common_prefix)
   size_t o_arstep;                                     // forward-pass counter (epoch of the peer-memory exchange)
   size_t o_lb_tok0 = 0, o_lb_len = 0, o_ls = 0, o_lin = 0;  // latent attention of prompt portions: query blocks, spans, per (latent layer, slot) row of position 0
   size_t o_span = 0, o_ab_tok0 = 0, o_ab_len = 0, o_kb_tok0 = 0, o_kb_len = 0;       // layer-list family: span of each token; attention query blocks
@@ -110,6 +111,7 @@ struct Engine {
   float *piece_area = nullptr;  // scratch of the attention over pieces (zero between calls)
   int n_read = 0;               // sequences of the pass being enqueued whose histories are read back
   int common_prefix = 0;        // positions that all sequences of this decode step have in common and that are read once (0: each by itself)
+  int prefix_slices = 0;        // slices of them (attn_shared_slices)
   void plan_read_back(int n_blocks);
   int common_pages(int n, const int *slots) const;
   bool use_pdl = true;  // programmatic dependent launch between the kernels of a step
@@ -131,8 +133,10 @@ struct Engine {
   std::vector<uint64_t> slot_stamp;  // duplicate-slot detection in O(n): stamp of the last call that listed the slot
   uint64_t call_stamp = 0;
   int last_rows = 0;  // logits rows of the last call
-  // decode graphs keyed by (T, n_splits, all_greedy)
+  // decode graphs keyed by what their launches depend on (see decode); all are dropped when there would be more than max_graphs
+  size_t max_graphs = 512;  // DIS_MAX_GRAPHS
   std::map<uint64_t, cudaGraphExec_t> graphs;
+  uint64_t graphs_captured = 0;
   std::map<uint64_t, uint64_t> graph_launches;  // kernels per replay of each graph
   // projection output still to be added to the residual when enqueue_layers returns
   const float *pend_ptr = nullptr;

@@ -151,6 +151,7 @@ struct SpArgs {
   float *state_o;         // [slice][kv head][128-row tile][D / 4][128] x 4 floats
   float *state_ml;        // [slice][kv head][128-row tile][128] x (m, l)
   int T, g_shift, n_kv, prefix, row_tiles, slices, late_wait, let_next;
+  const int *prefix_at;   // where the prefix is instead of in `prefix` (a captured launch serves every prefix of as many slices), or nullptr
 };
 
 template <int D, bool I8, bool kPair>
@@ -175,7 +176,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
 
   const int slice = blockIdx.x, kvh = blockIdx.z, rt0 = blockIdx.y * (kPair ? 2 : 1);
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const int n_all = (a.prefix + kSpTile - 1) / kSpTile;
+  const int prefix = a.prefix_at ? *a.prefix_at : a.prefix;
+  const int n_all = (prefix + kSpTile - 1) / kSpTile;
   const int tile0 = (int)((long long)n_all * slice / a.slices), n = (int)((long long)n_all * (slice + 1) / a.slices) - tile0;  // n >= 1
   auto steps = [&](int g) { return kPair ? n : (n + 1 - g) >> 1; };
   auto tile_of = [&](int g, int i) { return kPair ? i : 2 * i + g; };
@@ -207,12 +209,12 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
   const uint32_t o_base = tmem + 4 * kSpTile;
-  const int page_size = 1 << a.page_shift, last_page = (a.prefix - 1) >> a.page_shift;
+  const int page_size = 1 << a.page_shift, last_page = (prefix - 1) >> a.page_shift;
   const int *pt = a.page_table + (size_t)a.pt_row[0] * a.max_pages;
 
   if (!I8 && warp == 0) {
     // ===== K and V tiles by TMA; one lane acts, all hold page numbers
-    const int box_rows = min(page_size, kSpTile), last_box = (a.prefix - 1) / box_rows * box_rows;
+    const int box_rows = min(page_size, kSpTile), last_box = (prefix - 1) / box_rows * box_rows;
     int win_first = 1 << 30, win = 0;
     tma_prefetch_desc(&kv_map);
     int t = 0;
@@ -253,7 +255,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
     const int run = min(page_size, kSpTile);
     int win_first = 1 << 30, win = 0, t = 0;
     for (; t < n; t++) {
-      const int st = t % kSpRaw, first = (tile0 + t) * kSpTile, rows = min(kSpTile, a.prefix - first), p0 = first >> a.page_shift;
+      const int st = t % kSpRaw, first = (tile0 + t) * kSpTile, rows = min(kSpTile, prefix - first), p0 = first >> a.page_shift;
       if (t >= kSpRaw && !sp_wait(raw_empty(st), (uint32_t)(t / kSpRaw - 1) & 1u, fail)) break;
       if (p0 < win_first || p0 + 8 - win_first > 32) {  // a tile has at most eight pages
         win_first = p0;
@@ -386,7 +388,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
         for (int c = 0; c < 32; c++) s[c] = make_float2(__uint_as_float(raw[c >> 4][2 * (c & 15)]), __uint_as_float(raw[c >> 4][2 * (c & 15) + 1]));
       }
       const float4 *k_f = reinterpret_cast<const float4 *>(sp_smem + Cfg::kScale + slot * Cfg::kScaleFloats * 4);
-      const int rest = a.prefix - (tile0 + t) * kSpTile;  // keys of the tile that exist
+      const int rest = prefix - (tile0 + t) * kSpTile;  // keys of the tile that exist
       float2 f2;
       if (I8) {
 #pragma unroll
@@ -537,7 +539,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
         const int r = th & 63, pos = (tile0 + t) * kSpTile + r, pi = min(pos >> a.page_shift, last_page);
         const long long page = __shfl_sync(0xffffffffu, win, pi - win_first);
         const long long row = ((page * 2 + (th >> 6)) * a.n_kv + kvh) * page_size + (pos & (page_size - 1));
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(raw_s + (st * 128 + th) * 4), "l"(a.scale + row), "r"(pos < a.prefix ? 4 : 0) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(raw_s + (st * 128 + th) * 4), "l"(a.scale + row), "r"(pos < prefix ? 4 : 0) : "memory");
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -613,7 +615,7 @@ attn_join_kernel(const SpArgs a, const float *__restrict__ own_o, const float *_
   const float4 *x = reinterpret_cast<const float4 *>(own_o + head * D + chunk * 8);
   float M = ml.x, l = ml.y;
   float4 o0 = x[0], o1 = x[1];
-  const int slices = ctx[t] < a.prefix ? 0 : a.slices;
+  const int slices = ctx[t] < (a.prefix_at ? *a.prefix_at : a.prefix) ? 0 : a.slices;
   const size_t step = (size_t)a.n_kv * a.row_tiles;
   const size_t tile = (size_t)kvh * a.row_tiles + (rho >> 7);
   for (int s0 = 0; s0 < slices; s0 += kSjUnroll) {
@@ -679,6 +681,11 @@ bool attn_shared_pays(int T, int n_heads, int n_kv, int d, int prefix, bool int8
   return (long long)T * prefix * n_kv * d >= (long long)quarters << 23;
 }
 
+int attn_shared_slices(int T, int n_heads, int n_kv, int d, int prefix, bool int8) {
+  if (!attn_shared_pays(T, n_heads, n_kv, d, prefix, int8)) return 0;
+  return shared_slices(shared_blocks(T, n_heads / n_kv, n_kv), (prefix + kSpTile - 1) / kSpTile);
+}
+
 size_t attn_shared_scratch_elems(int T, int n_heads, int n_kv, int d) {  // the stream's, its states, the slices' states
   if (T <= 0 || n_kv <= 0 || n_heads < n_kv || d <= 0) return 0;
   const int G = n_heads / n_kv, rt = shared_row_tiles(T, G);
@@ -698,18 +705,19 @@ static cudaError_t prefix_launch(const TmaMap &map, const SpArgs &a, cudaStream_
 }
 
 cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float *scale, long long n_pages, const int *page_table, int max_pages,
-                               const int *pt_row, const int *ctx, int prefix, uint16_t *out, float *scratch, int T, int n_heads, int n_kv, int d,
-                               int page_size, bool chain, cudaStream_t st) {
+                               const int *pt_row, const int *ctx, int prefix, const int *prefix_at, uint16_t *out, float *scratch, int T, int n_heads, int n_kv,
+                               int d, int page_size, bool chain, cudaStream_t st) {
   const int G = n_heads / n_kv;
-  if (!attn_shared_pays(T, n_heads, n_kv, d, prefix, scale != nullptr))
-    return launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, 0, out, nullptr, nullptr, scratch, false, T, n_heads, n_kv, d, page_size, st);
+  const int slices = attn_shared_slices(T, n_heads, n_kv, d, prefix, scale != nullptr);
+  if (slices == 0)
+    return launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, 0, nullptr, out, nullptr, nullptr, scratch, false, T, n_heads, n_kv, d, page_size, st);
   SpArgs a{};
   a.q = q; a.pool = static_cast<const int8_t *>(pool); a.scale = scale; a.page_table = page_table; a.pt_row = pt_row; a.max_pages = max_pages;
   while ((1 << a.page_shift) < page_size) a.page_shift++;
   while ((1 << a.g_shift) < G) a.g_shift++;
-  a.T = T; a.n_kv = n_kv; a.prefix = prefix;
+  a.T = T; a.n_kv = n_kv; a.prefix = prefix; a.prefix_at = prefix_at;
   a.row_tiles = shared_row_tiles(T, G);
-  a.slices = shared_slices(shared_blocks(T, G, n_kv), (prefix + kSpTile - 1) / kSpTile);
+  a.slices = slices;
   float *own_o = scratch + (attn_stream_scratch_elems(n_heads, n_kv, d) + 3) / 4 * 4, *own_ml = own_o + (size_t)T * n_heads * d;
   a.state_o = own_o + ((size_t)T * n_heads * (2 + (size_t)d) + 3) / 4 * 4;
   a.state_ml = a.state_o + (size_t)a.slices * n_kv * a.row_tiles * 128 * d;
@@ -717,8 +725,8 @@ cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float 
   TmaMap map{};
   if (!scale) DIS_CUDA_TRY(make_kv_map(&map, static_cast<const uint16_t *>(pool), n_pages * 2 * n_kv * page_size, d, page_size));
   // The own parts first: their CTAs end one after the other, and the prefix's start as SMs come free
-  DIS_CUDA_TRY(launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, prefix, nullptr, own_o, own_ml, scratch, true, T, n_heads, n_kv, d,
-                                  page_size, st));
+  DIS_CUDA_TRY(launch_attn_stream(q, pool, scale, page_table, max_pages, pt_row, ctx, prefix, prefix_at, nullptr, own_o, own_ml, scratch, true, T, n_heads, n_kv,
+                                  d, page_size, st));
   // (chain, a call of the C ABI: the kernels behind the first overlap with the one in front of them even under capture, where the first may not with what is in
   // front of it)
   struct Pdl { const bool was = pdl_enabled(); ~Pdl() { pdl_enabled() = was; } } pdl;

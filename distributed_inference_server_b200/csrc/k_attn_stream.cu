@@ -123,6 +123,7 @@ struct StArgs {
   int max_pages;
   const int *pt_row, *ctx;
   int first;               // keys in front of this position are somebody else's, for the tokens that reach it
+  const int *first_at;     // where that position is instead, or nullptr
   uint16_t *out;           // the result, or nullptr: the states go to state_o, state_ml
   float *state_o, *state_ml;
   int *counters;           // [2][2 per CTA], zero between calls
@@ -174,9 +175,9 @@ attn_stream_kernel(const StArgs a) {
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   pdl_wait();
   if (a.inputs_first) pdl_launch_dependents();
-  const int n_heads = a.n_kv * G, page_size = 1 << a.page_shift, base0 = a.first / Cfg::kTok * Cfg::kTok;
-  auto first_of = [&](int keys) { return keys < a.first ? 0 : a.first; };  // a history that ends in front of it is all this kernel's
-  auto base_of = [&](int keys) { return keys < a.first ? 0 : base0; };
+  const int n_heads = a.n_kv * G, page_size = 1 << a.page_shift, first_own = a.first_at ? *a.first_at : a.first, base0 = first_own / Cfg::kTok * Cfg::kTok;
+  auto first_of = [&](int keys) { return keys < first_own ? 0 : first_own; };  // a history that ends in front of it is all this kernel's
+  auto base_of = [&](int keys) { return keys < first_own ? 0 : base0; };
 
   // ---- tiles in front of each token; tokens without keys of their own get their result here
   for (int t0 = 0, sum = 0; t0 < a.T; t0 += kStWarps * 32) {
@@ -716,13 +717,13 @@ static cudaError_t stream_dispatch(const StArgs &a, int G, int d, cudaStream_t s
 }
 
 cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float *scale, const int *page_table, int max_pages, const int *pt_row,
-                               const int *ctx, int first, uint16_t *out, float *state_o, float *state_ml, float *scratch, bool inputs_first, int T,
-                               int n_heads, int n_kv, int d, int page_size, cudaStream_t st) {
+                               const int *ctx, int first, const int *first_at, uint16_t *out, float *state_o, float *state_ml, float *scratch,
+                               bool inputs_first, int T, int n_heads, int n_kv, int d, int page_size, cudaStream_t st) {
   // a launch's tiles are counted in 32 bits
   const long long most = ((long long)max_pages * page_size / 16 + 2) * n_kv;
   const int G = n_heads / n_kv, step = (int)std::max(1ll, std::min({(long long)kStMaxT, 0x7fffffffll / most}));
   StArgs a{};
-  a.pool = pool; a.scale = scale; a.page_table = page_table; a.max_pages = max_pages; a.first = first;
+  a.pool = pool; a.scale = scale; a.page_table = page_table; a.max_pages = max_pages; a.first = first; a.first_at = first_at;
   a.counters = reinterpret_cast<int *>(scratch);
   a.piece_o = scratch + kStCounters;
   a.group_o = a.piece_o + stream_slots() * (size_t)G * d;

@@ -123,18 +123,20 @@ cudaError_t launch_kv_read_i8(const int8_t *pool, const float *scale, uint16_t *
 
 // k_attn_stream.cu : attention of single tokens over the keys from position `first` on, in equal shares whatever the lengths are.  scale: of the
 // 8-bit pool (nullptr: a bf16 pool).  out, or the states (m, l, O) in state_ml [T][n_heads][2] and state_o [T][n_heads][d].  scratch: its first
-// part is zero between calls.
+// part is zero between calls.  first_at: where `first` is read from when the kernel runs (nullptr: as given).
 size_t attn_stream_scratch_elems(int n_heads, int n_kv, int d);
 cudaError_t launch_attn_stream(const uint16_t *q, const void *pool, const float *scale, const int *page_table, int max_pages, const int *pt_row,
-                               const int *ctx, int first, uint16_t *out, float *state_o, float *state_ml, float *scratch, bool inputs_first, int T,
-                               int n_heads, int n_kv, int d, int page_size, cudaStream_t st);
+                               const int *ctx, int first, const int *first_at, uint16_t *out, float *state_o, float *state_ml, float *scratch,
+                               bool inputs_first, int T, int n_heads, int n_kv, int d, int page_size, cudaStream_t st);
 
-// k_attn_shared.cu : the same where positions [0, prefix) are the same rows for every token
+// k_attn_shared.cu : the same where positions [0, prefix) are the same rows for every token.  prefix_at: where the prefix is read from when the kernels run
+// (nullptr: as given); `prefix` then only settles the launches, which are those of every prefix with as many slices.  No slices: every token goes alone.
 bool attn_shared_pays(int T, int n_heads, int n_kv, int d, int prefix, bool int8);
+int attn_shared_slices(int T, int n_heads, int n_kv, int d, int prefix, bool int8);
 size_t attn_shared_scratch_elems(int T, int n_heads, int n_kv, int d);
 cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float *scale, long long n_pages, const int *page_table, int max_pages,
-                               const int *pt_row, const int *ctx, int prefix, uint16_t *out, float *scratch, int T, int n_heads, int n_kv, int d,
-                               int page_size, bool chain, cudaStream_t st);
+                               const int *pt_row, const int *ctx, int prefix, const int *prefix_at, uint16_t *out, float *scratch, int T, int n_heads, int n_kv,
+                               int d, int page_size, bool chain, cudaStream_t st);
 
 // k_gemm_tcgen05.cu
 cudaError_t make_tma_map_2d(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows);

@@ -1314,6 +1314,7 @@ int Engine::stack_step(int n, const int *slots, int max_prefill_tokens, uint32_t
       cudaGraphDestroy(g);
       kernel_launches = before + graph_launches[key];
       it->second = ex;
+      graphs_captured++;
       ENG_CUDA(cudaGraphLaunch(ex, stream));
     }
   }

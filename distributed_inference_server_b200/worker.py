@@ -308,6 +308,12 @@ class Engine:
         self._check(self.lib.dis_engine_replay_last_step(self.h, int(n), C.byref(ms)))
         return float(ms.value)
 
+    def graph_stats(self) -> "tuple[int, int]":
+        """CUDA graphs of decode steps: kept now, and captured so far."""
+        kept, captured = C.c_int64(), C.c_int64()
+        self._check(self.lib.dis_engine_graph_stats(self.h, C.byref(kept), C.byref(captured)))
+        return int(kept.value), int(captured.value)
+
     def last_logprobs(self, slots) -> np.ndarray:
         """TokenEvent.logprob of the token each listed sequence got from its latest prefill/decode call."""
         s = np.ascontiguousarray(slots, dtype=np.int32)

@@ -188,6 +188,9 @@ DIS_API int dis_engine_profile_decode(dis_engine *e, int32_t n, const int32_t *s
  * one replay.  The difference to the time of a real step is what the host adds between steps (metadata upload,
  * launch, token read-back, the caller's own work). */
 DIS_API int dis_engine_replay_last_step(dis_engine *e, int32_t n, float *avg_ms);
+/* CUDA graphs of decode steps: kept now (a bounded number), and captured in the engine's life.  A step whose launches no kept graph has
+ * captures one, which takes some milliseconds. */
+DIS_API int dis_engine_graph_stats(dis_engine *e, int64_t *kept, int64_t *captured);
 /* Logits of the last prefill/decode call, row i = i-th listed sequence, [n][vocab] fp32 (gathered
  * across tensor-parallel ranks). For parity tests. */
 DIS_API int dis_engine_last_logits(dis_engine *e, float *host, int32_t n_rows);
