@@ -20,11 +20,16 @@ __device__ __forceinline__ float piece_ex2(float x) {
 // makes the sums NaN.
 constexpr float kPieceNone = -1e30f;
 constexpr float kPieceLazy = 8.f;
+// 8-bit pages: weights times value scales are fp16 in the products, which ends at 2^16 and has no numbers between multiples of 2^-24.  The reference stays
+// this far below the largest, so that they are at most 2^(kPieceLazy + kPieceDown) and lose 2^-32 of the largest, not 2^-25: the sum of weights counts what
+// they lose, and many small ones behind a large one would all be lost to the same side.
+constexpr float kPieceDown = 7.f;
 
-// log2 of a value row's scale, of 2^-87 for one below it (a row of zeros; the smallest scale otherwise) and for NaN
+// log2 of a value row's scale, of 2^-80 for one below it (a row of zeros, or one whose largest entry is below 2^-73: 2^7 less room under the largest product,
+// the room that kPieceDown makes) and for NaN.  Weights are then at most 2^95, and sums of 2^31 of them numbers
 __device__ __forceinline__ float piece_log2_scale(float s) {
   float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(s, 6.462348536e-27f)));
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(s, 8.271806126e-25f)));
   return y;
 }
 

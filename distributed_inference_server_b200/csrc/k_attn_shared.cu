@@ -18,7 +18,7 @@
 //   warps 12-15     8-bit pages: rows turned to fp16 (exact) into the tiles' ring.  They are near to being the bound, so they do nothing else: with the
 //                   rows' addresses and copies (cp.async) theirs too, a third of their time, 64 requests behind 64000 tokens took 179 us, now 168
 // TMEM: four score buffers of 64 columns, P over its scores, an O of d columns per group.  A group raises a row's reference only when its
-// maximum grows by more than 8 in the log2 domain, so O is seldom rescaled (the reference cancels).
+// maximum has grown by more than 8 in the log2 domain, so O is seldom rescaled (the reference cancels).
 // 8-bit pages: scales stay outside the products, as in k_attn_stream.cu; q and the weights are fp16 there, bf16 otherwise.
 //
 // Measured (B200, from graphs, all three kernels): 32 requests behind 6000 tokens, 32 / 8 heads of 128, own parts to 500, bf16: 24.9 us;
@@ -423,9 +423,10 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
         for (int c = 0; c < 32; c++) mx4[c & 3] = sp_max3(mx4[c & 3], s[c].x, s[c].y);
         mx = sp_max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * kLog2;  // the factor is positive: it commutes with the maximum
       }
-      const bool grow = mx > m + kPieceLazy;
+      constexpr float kDown = I8 ? kPieceDown : 0.f;
+      const bool grow = mx > m + (kPieceLazy + kDown);
       if (__any_sync(0xffffffffu, grow)) {
-        const float m_new = grow ? mx : m, f = piece_ex2(m - m_new);
+        const float m_new = grow ? mx - kDown : m, f = piece_ex2(m - m_new);
         if (i > 0) {  // O holds the products of every step before this one; none is under way behind it
           ok = sp_wait(pv_done(g), (uint32_t)(i - 1) & 1u, fail);
           if (!ok) break;

@@ -4,9 +4,9 @@
 // 8-bit rows: k = ks k8, v = vs v8 with whole numbers k8, v8 and one fp32 factor per token and kv head.  The factors stay outside the products:
 //   s_j = (q . k8_j) ks_j / sqrt d,   o = sum_j (p_j vs_j) v8_j / sum_j p_j,   p_j = 2^(s_j - m)
 // so the operands are exact in fp16 or nearly: k8 and v8 by themselves, q after a power of two per head that brings its largest entry to
-// [2^13, 2^14) (entries below 2^-28 of it lose bits), and p_j vs_j because m is the largest s_j + log2 vs_j instead of the largest s_j: no product
-// is above 1, the largest is 1, and each loses 2^-11 of itself at most (bf16: 2^-8) or, below 2^-14, 2^-25.  Which m a softmax is taken under
-// cancels; vs is at least 2^-87 or counted as that, so that sum p_j stays within fp32.  m, l, O and the scores are fp32.
+// [2^13, 2^14) (entries below 2^-28 of it lose bits), and p_j vs_j because m follows the largest s_j + log2 vs_j instead of the largest s_j, 2^7 below
+// it: no product is above 2^15, and each loses 2^-11 of itself at most (bf16: 2^-8) or, below 2^-14, 2^-25, which is 2^-32 of the largest.  Which m a softmax
+// is taken under cancels; vs below 2^-80 counts as that in m, so that sum p_j stays within fp32.  m, l, O and the scores are fp32.
 //
 // HBM-bound: 2 (d + 4) bytes (i8) or 4 d (bf16) per token and kv head, 4 G d operations on mma.sync m16n8k16 (tokens are its rows, the up to eight
 // heads its columns: S^T = K Q^T, O^T = V^T P^T).  Operands go from shared memory to registers by 16-byte loads without ldmatrix: which dim is
@@ -434,7 +434,8 @@ attn_stream_kernel(const StArgs a) {
       }
 #pragma unroll
       for (int e = 0; e < 2; e++) mx[e] = fmaxf(fmaf(p[e], qf[e], up0), fmaf(p[2 + e], qf[e], up1));
-      if (__any_sync(0xffffffffu, mx[0] > m_run[0] + kPieceLazy || mx[1] > m_run[1] + kPieceLazy)) {
+      constexpr float kDown = I8 ? kPieceDown : 0.f, kRaise = kPieceLazy + kDown;
+      if (__any_sync(0xffffffffu, mx[0] > m_run[0] + kRaise || mx[1] > m_run[1] + kRaise)) {
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -442,7 +443,7 @@ attn_stream_kernel(const StArgs a) {
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          const float m_new = fmaxf(m_run[e], x);
+          const float m_new = fmaxf(m_run[e], x - kDown);
           f[e] = piece_ex2(m_run[e] - m_new);
           l_run[e] *= f[e];
           m_run[e] = m_new;

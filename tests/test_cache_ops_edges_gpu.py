@@ -6,7 +6,7 @@ import torch
 
 from tests import _gpu_util as G
 from tests._gpu_util import DEV, check, dev_i32, lib, ptr, sync
-from tests.test_cache_ops_gpu import Cache
+from tests.test_cache_ops_gpu import Cache, attention, decode, near, shared
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,58 @@ def test_read_into_a_pool_that_starts_on_16_bytes(d, page, off):
     want = torch.where(used, c.value.float().to(torch.bfloat16), torch.zeros((), dtype=torch.bfloat16, device=DEV))
     assert torch.equal(back, want)
     assert int((area[:off] != 0).sum()) == 0 and int((area[off + back.numel():] != 0).sum()) == 0
+
+
+# ------------------------------------------------------------------------------------------------ a leading key and a long flat history
+class Flat(Cache):
+    """Histories whose first key leads for a query along dimension 0; all others score 0 there.  Its value is 1 in dimension 0 and 0 elsewhere, theirs are
+    random with a largest entry of 1: every other dimension of the result is the sum of many weights, each a tiny part of the first."""
+
+    def __init__(self, ctx, nkv, d, page, seed, common=0):
+        super().__init__(ctx, nkv, d, page, seed, True, common, spread=False, amp=self.rows_of)
+
+    def rows_of(self, x, g):
+        v = torch.rand(x.shape, generator=g, device=DEV) * 0.5 + 0.5
+        v[:, 0, ..., 0] = 0.0
+        v[:, 1, ..., 1] = 1.0
+        for b in range(self.table.shape[0]):
+            if self.ctx[b] > 0:
+                first = int(self.table[b, 0])
+                v[first, :, :, 0] = 0.0
+                v[first, :, :, 0, 0] = 1.0
+        return v / torch.where(x == 0, 1.0, x)  # (the base multiplies its normal numbers by this)
+
+
+def along_0(T, nh, d, size):
+    q = torch.zeros(T, nh, d, device=DEV)
+    q[:, :, 0] = size
+    return G._guarded_copy(q.view(T, nh * d).to(torch.bfloat16))
+
+
+def flat_bound(c, q, nh):
+    """As `attention` bounds 8-bit pages, with the products' smallest step at 2^-32 of the largest."""
+    c.int8 = False  # (its own term is 2^-25)
+    o, tol = attention(c, q, nh, 2.0 ** -11)
+    c.int8 = True
+    for t in range(q.shape[0]):
+        k, v = c.rows(t)
+        p = torch.softmax(q[t].double().view(c.nkv, nh // c.nkv, c.d) @ k.transpose(1, 2) / c.d ** 0.5, -1)
+        vs = (v.abs().amax(-1) / 127)[:, None]
+        whole = (v / vs[..., 0, :, None]).abs().sum(1)[:, None]
+        tol[t] += (2.0 ** -32 * (p * vs).amax(-1, keepdim=True) * whole).reshape(nh, c.d)
+    return o, tol
+
+
+def test_decode_many_small_weights_behind_a_large_one():
+    """The others' weights are 2^-25.2 of the first's (140 / sqrt(64) / ln 2).  32 tiles of a history lie in one or two CTAs."""
+    c = Flat([512] * 512, 1, 64, 64, 3)
+    q = along_0(512, 1, 64, 140.0)
+    near(decode(c, q, 1), flat_bound(c, q, 1))
+
+
+def test_shared_prefix_many_small_weights_behind_a_large_one():
+    T, nkv, prefix = 40, 32, 512
+    assert lib().dis_k_attn_shared_in_common(T, nkv, nkv, 64, prefix, 1) == 1
+    c = Flat([prefix + 1 + t % 5 for t in range(T)], nkv, 64, 64, 4, prefix)
+    q = along_0(T, nkv, 64, 140.0)
+    near(shared(c, q, nkv, prefix), flat_bound(c, q, nkv))
