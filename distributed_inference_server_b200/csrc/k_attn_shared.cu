@@ -12,14 +12,17 @@
 //
 // attn_prefix_kernel, one CTA per SM:
 //   warp 0          bf16 pages: K and V tiles of 64 keys by TMA into a ring; 8-bit pages: their rows into a ring of their own
-//   warps 1, 2      the MMAs of softmax group 0 and 1: S = Q K^T (M128 N64), two tiles ahead of O += P V (M128 N = d)
+//   warps 1, 2      the MMAs of softmax group 0 and 1: S = Q K^T (M128 N64), two tiles ahead of O += P V (M128 N = d; bf16: twice)
 //   warps 4-7, 8-11 softmax groups, one thread per row.  Up to 128 rows: both groups have the same rows, group 0 the even key tiles, group 1
 //                   the odd ones, and their states are joined at the end; more: 128 rows each, and both read every tile (kPair)
 //   warps 12-15     8-bit pages: rows turned to fp16 (exact) into the tiles' ring.  They are near to being the bound, so they do nothing else: with the
 //                   rows' addresses and copies (cp.async) theirs too, a third of their time, 64 requests behind 64000 tokens took 179 us, now 168
 // TMEM: four score buffers of 64 columns, P over its scores, an O of d columns per group.  A group raises a row's reference only when its
 // maximum has grown by more than 8 in the log2 domain, so O is seldom rescaled (the reference cancels).
-// 8-bit pages: scales stay outside the products, as in k_attn_stream.cu; q and the weights are fp16 there, bf16 otherwise.
+// 8-bit pages: scales stay outside the products, as in k_attn_stream.cu; q and the weights are fp16 there.  bf16 pages: V is bf16, so the weights have to be,
+// and enter O += P V as two bf16 halves, one product behind the other: with the upper half alone (2^-9 of a weight) results were 2.0e-3 from 64 bits where
+// every token by itself gives 1.7e-3, and what a step's results are worth would have depended on its batch.  P and its rest fill the 64 columns of the scores.
+// 32 requests behind 6000 24.2 -> 24.8 us, 64 behind 64000 128 -> 156.
 //
 // Measured (B200, from graphs, all three kernels): 32 requests behind 6000 tokens, 32 / 8 heads of 128, own parts to 500, bf16: 24.9 us;
 // 64 behind 8000, 64 / 8 heads, own parts to 700, 8 bits: 50.1 (10.6 at a library product's rate, 7.6 for its bytes).  A step of 256 rows x 64 keys takes 1.0 us
@@ -310,6 +313,10 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
         const uint32_t b = v_lo + s * (Cfg::kTileBytes >> 4), p = tmem + (2 * g + (i & 1)) * kSpTile;
 #pragma unroll
         for (uint32_t k = 0; k < kSpTile / 16; k++) umma_ts(o_base + g * D, p + 8 * k, b + k * 128, idesc_o, k > 0 ? 1u : (uint32_t)(i > 0));
+        if (!I8) {  // the weights' rests
+#pragma unroll
+          for (uint32_t k = 0; k < kSpTile / 16; k++) umma_ts(o_base + g * D, p + kSpTile / 2 + 8 * k, b + k * 128, idesc_o, 1u);
+        }
         umma_commit(pv_done(g));
         umma_commit(v_empty(s));
         if (i + 1 == count) umma_commit(o_done(g));
@@ -446,24 +453,27 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap kv_map, const SpArgs a) {
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        uint32_t w[16];
+        uint32_t w[16], low[16];
 #pragma unroll
         for (int c = 0; c < 16; c++) {
           float2 p = sp_fma2(s[16 * h + c], f2, neg);
           p.x = piece_ex2(p.x);
           p.y = piece_ex2(p.y);
+          sum[c & 1] = sp_add2(sum[c & 1], p);
           if (I8) {
-            sum[c & 1] = sp_add2(sum[c & 1], p);
             const float2 vs = reinterpret_cast<const float2 *>(k_f + kSpTile / 4)[16 * h + c];
             p = sp_mul2(p, vs);
             const __half2 hp = __floats2half2_rn(p.x, p.y);
             w[c] = *reinterpret_cast<const uint32_t *>(&hp);
           } else {
+            // two halves, 16 bits of the weight, as decode attention over bf16 pages has them elsewhere
             w[c] = float2_to_bf16x2(p.x, p.y);
-            sum[c & 1] = sp_add2(sum[c & 1], bf16x2_to_float2(w[c]));  // as P V takes them, rounded: a row that one key dominates keeps its weight at 1
+            const float2 top = bf16x2_to_float2(w[c]);
+            low[c] = float2_to_bf16x2(p.x - top.x, p.y - top.y);
           }
         }
         sp_tmem_st_16(s_addr + 16 * h, w);
+        if (!I8) sp_tmem_st_16(s_addr + kSpTile / 2 + 16 * h, low);
       }
       if (I8) {
         __syncwarp();

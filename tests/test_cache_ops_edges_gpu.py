@@ -6,7 +6,7 @@ import torch
 
 from tests import _gpu_util as G
 from tests._gpu_util import DEV, check, dev_i32, lib, ptr, sync
-from tests.test_cache_ops_gpu import Cache, attention, decode, near, shared
+from tests.test_cache_ops_gpu import Cache, attention, decode, near, queries, shared
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,16 @@ def test_shared_prefix_many_small_weights_behind_a_large_one():
     c = Flat([prefix + 1 + t % 5 for t in range(T)], nkv, 64, 64, 4, prefix)
     q = along_0(T, nkv, 64, 140.0)
     near(shared(c, q, nkv, prefix), flat_bound(c, q, nkv))
+
+
+# ------------------------------------------------------------------------------------------------ weights of a shared prefix
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("T,group,nkv,d,page,prefix", [(32, 4, 8, 128, 64, 2000), (70, 4, 8, 128, 16, 1501), (130, 1, 8, 64, 64, 1400), (80, 8, 8, 64, 32, 1001)])
+def test_shared_prefix_weights(int8, T, group, nkv, d, page, prefix):
+    """Weights enter the product as two bf16 halves (2^-16 of a weight) over bf16 pages, in fp16 (2^-11) over 8-bit ones, read once or not."""
+    assert lib().dis_k_attn_shared_in_common(T, nkv * group, nkv, d, prefix, int8) == 1
+    ctx = [prefix + 1 + 3 * t % 60 for t in range(T)]
+    c = Cache(ctx, nkv, d, page, T + d, int8, prefix)
+    q = queries(T, nkv * group, d, 61)
+    out = shared(c, q, nkv * group, prefix)
+    near(out, attention(c, q, nkv * group, 2.0 ** -11 if int8 else 2.0 ** -16))
