@@ -688,6 +688,7 @@ static int shared_blocks(int T, int G, int n_kv) { const int rt = shared_row_til
 // 4: 24.0 / 25.3, 26.8 / 31.1, 40.0 / 61.3
 bool attn_shared_pays(int T, int n_heads, int n_kv, int d, int prefix, bool int8) {
   if (T < (int8 ? 6 : 2) || n_kv < 1) return false;
+  if (n_kv > 65535 || shared_row_tiles(T, std::max(n_heads / n_kv, 1)) > 65535) return false;  // (a grid's sides)
   const int quarters = (T < 4 ? 8 : 4) + (d == 128 ? (T > 128 / std::max(n_heads / n_kv, 1)) + int8 : 0);
   return (long long)T * prefix * n_kv * d >= (long long)quarters << 23;
 }
@@ -732,7 +733,6 @@ cudaError_t launch_attn_shared(const uint16_t *q, const void *pool, const float 
   float *own_o = scratch + (attn_stream_scratch_elems(n_heads, n_kv, d) + 3) / 4 * 4, *own_ml = own_o + (size_t)T * n_heads * d;
   a.state_o = own_o + ((size_t)T * n_heads * (2 + (size_t)d) + 3) / 4 * 4;
   a.state_ml = a.state_o + (size_t)a.slices * n_kv * a.row_tiles * 128 * d;
-  if (n_kv > 65535 || a.row_tiles > 65535) { set_last_error("attn_shared: more than 65535 kv heads or 128-row tiles"); return cudaErrorInvalidValue; }
   TmaMap map{};
   if (!scale) DIS_CUDA_TRY(make_kv_map(&map, static_cast<const uint16_t *>(pool), n_pages * 2 * n_kv * page_size, d, page_size));
   // The own parts first: their CTAs end one after the other, and the prefix's start as SMs come free
