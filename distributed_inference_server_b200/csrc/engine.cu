@@ -811,15 +811,17 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
                                         n_qblocks, nh_l, nkv_l, d, page_size, stream));
       kernel_launches++;
     } else if (pool8 || common_prefix > 0) {
-      RET_CUDA(write_rows());
+      if (!skip(P_ROPE)) RET_CUDA(write_rows());
       prof_mark(P_ATTN);
       const void *kv = pool8 ? static_cast<const void *>(pool8) : pool;
-      if (common_prefix > 0)
-        RET_CUDA(launch_attn_shared(q, kv, scale8, n_pages, d_page_table, max_pages, ptrow, ctx, common_prefix, cur_meta->d<int>(cur_meta->o_prefix), attn, piece_area, T, nh_l,
-                                    nkv_l, d, page_size, false, stream));
-      else
+      if (skip(P_ATTN)) {
+      } else if (common_prefix > 0) {
+        RET_CUDA(launch_attn_shared(q, kv, scale8, n_pages, d_page_table, max_pages, ptrow, ctx, common_prefix, cur_meta->d<int>(cur_meta->o_prefix), attn,
+                                    piece_area, T, nh_l, nkv_l, d, page_size, false, stream));
+      } else {
         RET_CUDA(launch_attn_stream(q, kv, scale8, d_page_table, max_pages, ptrow, ctx, 0, nullptr, attn, nullptr, nullptr, piece_area, false, T, nh_l, nkv_l,
                                     d, page_size, stream));
+      }
       kernel_launches += common_prefix > 0 ? 3 : 1;
     } else {
       // decode: RoPE + KV write live inside the attention kernel (one kernel boundary less per layer)
