@@ -37,6 +37,8 @@ constexpr int kStWarps = 4;
 constexpr int kStMaxT = 512;            // tokens of one launch
 constexpr int kStCounters = 1 << 16;    // words kept for counters, of which two for each of a CTA's two pieces are used
 constexpr int kStMinShare = kStWarps;   // tiles of a CTA, at least
+constexpr int kSmSmem = 228 * 1024;     // shared memory of an SM, of which a CTA takes 1 KB besides its own, in units of 128 bytes
+constexpr int kStStatic = (2 * kStWarps * 8 + kStWarps + 2) * 4;  // static shared memory of the kernel
 
 template <int D, bool I8>
 struct StCfg {
@@ -703,7 +705,10 @@ static cudaError_t stream_launch(const StArgs &a, cudaStream_t st) {
   constexpr int kFixed = Cfg::fixed(G);
   static DeviceOnce once;
   DIS_CUDA_TRY(once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + (3 * kStMaxT + 1) * 4); }));
-  return launch_k(kern, dim3(kNumSMs * Cfg::kCtas), dim3(kStWarps * 32), (size_t)kFixed + (3 * a.T + 1) * 4, st, a);
+  // A share for each CTA that is resident, so that all of them run at once: the tokens' lengths take shared memory too, and from 126 tokens on bf16 heads of 128
+  // have room for two CTAs of an SM, not three.  (Shares for three: 126 tokens to 600 40.7 us, for two 31.9; 200 to 2100 127.8, 108.6; 500 to 900 160, 137)
+  const int smem = kFixed + (3 * a.T + 1) * 4, ctas = std::min(Cfg::kCtas, kSmSmem / ((smem + kStStatic + 127) / 128 * 128 + 1024));
+  return launch_k(kern, dim3(kNumSMs * ctas), dim3(kStWarps * 32), (size_t)smem, st, a);
 }
 
 template <bool I8>

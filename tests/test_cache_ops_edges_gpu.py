@@ -6,7 +6,7 @@ import torch
 
 from tests import _gpu_util as G
 from tests._gpu_util import DEV, check, dev_i32, lib, ptr, sync
-from tests.test_cache_ops_gpu import Cache, attention, decode, near, queries, shared
+from tests.test_cache_ops_gpu import Cache, attention, decode, near, queries, scratch, shared
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +96,52 @@ def test_shared_prefix_weights(int8, T, group, nkv, d, page, prefix):
     q = queries(T, nkv * group, d, 61)
     out = shared(c, q, nkv * group, prefix)
     near(out, attention(c, q, nkv * group, 2.0 ** -11 if int8 else 2.0 ** -16))
+
+
+# ------------------------------------------------------------------------------------------------ many tokens
+@pytest.mark.parametrize("T", [125, 126, 300, 600])
+@pytest.mark.parametrize("int8", [False, True])
+def test_many_tokens_alone(int8, T):
+    """Every token by itself, around the number of tokens from which fewer CTAs of heads of 128 over bf16 pages are resident, and past one launch's 512."""
+    prefix, nkv, group = 20, 2, 4
+    ctx = [prefix + int(v) for v in np.random.default_rng(T).integers(0, 150, T)]
+    ctx[0], ctx[5], ctx[T - 1] = prefix + 150, 0, 7
+    assert lib().dis_k_attn_shared_in_common(T, nkv * group, nkv, 128, prefix, int8) == 0
+    c = Cache(ctx, nkv, 128, 16, T, int8, prefix)
+    q = queries(T, nkv * group, 128, 62)
+    near(shared(c, q, nkv * group, prefix), attention(c, q, nkv * group, 2.0 ** -11 if int8 else 2.0 ** -16))
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("T,group,nkv,d", [(520, 1, 8, 64), (1030, 4, 4, 128)])
+def test_many_tokens_with_a_prefix_read_once(int8, T, group, nkv, d):
+    """More tokens than one launch of the own parts takes: the prefix's kernel starts behind the last of them."""
+    prefix = 333
+    assert lib().dis_k_attn_shared_in_common(T, nkv * group, nkv, d, prefix, int8) == 1
+    ctx = [prefix + int(v) for v in np.random.default_rng(T).integers(0, 40, T)]
+    ctx[3], ctx[513], ctx[T - 1] = 0, prefix - 1, prefix
+    c = Cache(ctx, nkv, d, 16, T, int8, prefix)
+    q = queries(T, nkv * group, d, 63)
+    area = scratch(T, nkv * group, nkv, d, True)
+    out = shared(c, q, nkv * group, prefix, area=area)
+    near(out, attention(c, q, nkv * group, 2.0 ** -11 if int8 else 2.0 ** -16))
+    area[1 << 16:].fill_(3.0)
+    assert torch.equal(shared(c, q, nkv * group, prefix, area=area), out)
+
+
+def test_read_back_of_more_rows_than_one_launch():
+    rows, nkv, d, page = 2100, 1, 64, 8
+    ctx = [int(v) for v in np.random.default_rng(5).integers(0, 20, rows)]
+    first = [int(v) for v in np.random.default_rng(6).integers(0, 12, rows)]
+    c = Cache(ctx, nkv, d, page, 8)
+    back = G.zeros((c.n_pages, 2, nkv, page, d), torch.bfloat16)
+    check(lib().dis_k_kv_read_i8(ptr(c.pool), ptr(c.scale), ptr(back), ptr(c.d_table), ptr(c.d_table), c.width, ptr(dev_i32(np.arange(rows))), ptr(dev_i32(first)),
+                                 ptr(dev_i32(ctx)), rows, nkv, d, page, None))
+    sync()
+    want = torch.zeros_like(back)
+    for b in range(rows):
+        pos = np.arange(first[b], ctx[b])
+        if len(pos):
+            at, slot = torch.from_numpy(c.table[b, pos // page].astype(np.int64)).to(DEV), torch.from_numpy(pos % page).to(DEV)
+            want[at, :, :, slot] = c.value[at, :, :, slot].float().to(torch.bfloat16)
+    assert torch.equal(back, want)
