@@ -13,8 +13,9 @@ namespace dis {
 // D / 8 lanes take a row of q, k or v: four entries and the four that rotate with them each, so that a row's maximum is three or four shuffles
 // away and nothing is kept in between.  Bound by HBM at prompt size: the fp32 projection is read once, 4 bytes an entry and K slice; by latency
 // (positions -> page -> row) for a decode step's tokens.
-// kMany: eight CTAs to an SM (32 registers) keep more loads on their way, 35.0 -> 30.8 us for 6900 tokens of 32 + 2 x 8 heads of 128; a decode step's
-// few tokens in four K slices keep a row's slices on their way instead (5.9 us with their read-back, 6.5 with 32 registers).
+// kMany: eight CTAs to an SM (32 registers) keep more loads on their way; few CTAs keep a row's K slices on their way instead.  They cross at about five
+// CTAs an SM.  us, many / few (CTAs): 32 + 2 x 8 heads of 128, one slice 384 2.6 / 2.6, 600 2.8 / 3.0, 1200 3.7 / 4.1, 4800 9.6 / 11.8, 14400 30.8 / 42.0; four slices
+// 96 3.1 / 2.9, 384 3.3 / 3.3, 900 4.6 / 5.1; 32 + 2 x 4 heads of 64, one slice 600 2.6 / 2.4, 800 2.8 / 3.0; four slices 800 3.7 / 3.6, 1200 4.3 / 5.0.
 // With the read-back of all histories: six prompts behind 2048 tokens each, 32 / 8 heads of 128, 45.8 us (37.6 at a plain copy's rate).
 constexpr int kCwThreads = 256;
 
@@ -88,7 +89,7 @@ static cudaError_t write_launch(const float *qkv, int n_partial, long long parti
                                 int shift, cudaStream_t st) {
   constexpr int kRows = kCwThreads / (D / 8);
   const long long ctas = (long long)T * ((n_heads + 2 * n_kv + kRows - 1) / kRows);
-  auto kern = ctas >= 4 * 8 * kNumSMs ? rope_kv_write_i8_kernel<D, true> : rope_kv_write_i8_kernel<D, false>;
+  auto kern = ctas >= 5 * kNumSMs ? rope_kv_write_i8_kernel<D, true> : rope_kv_write_i8_kernel<D, false>;
   return launch_k(kern, dim3((unsigned)ctas), dim3(kCwThreads), 0, st, qkv, n_partial, partial_stride, q, pool, scale, page_table, max_pages, pt_row, pos,
                   rope_cos, rope_sin, n_heads, n_kv, shift);
 }

@@ -7,6 +7,7 @@ import torch
 from tests import _gpu_util as G
 from tests._gpu_util import DEV, check, dev_i32, lib, ptr, sync
 from tests.test_cache_ops_gpu import Cache, attention, decode, near, queries, scratch, shared
+from tests.test_cache_ops_gpu import test_write_and_read as write_and_read
 
 pytestmark = pytest.mark.gpu
 
@@ -145,3 +146,12 @@ def test_read_back_of_more_rows_than_one_launch():
             at, slot = torch.from_numpy(c.table[b, pos // page].astype(np.int64)).to(DEV), torch.from_numpy(pos % page).to(DEV)
             want[at, :, :, slot] = c.value[at, :, :, slot].float().to(torch.bfloat16)
     assert torch.equal(back, want)
+
+
+# ------------------------------------------------------------------------------------------------ writing
+@pytest.mark.parametrize("nh,nkv,d,page,S,lens", [(32, 8, 128, 64, 1, [700, 300]), (32, 4, 64, 16, 3, [500, 1, 90]), (8, 8, 128, 16, 4, [800]), (64, 8, 128, 32, 2, [148])])
+def test_write_of_many_tokens(nh, nkv, d, page, S, lens):
+    """More CTAs than five an SM: the variant that keeps eight of them there."""
+    rows = 256 // (d // 8)
+    assert sum(lens) * -(-(nh + 2 * nkv) // rows) >= 5 * 148
+    write_and_read(nh, nkv, d, page, S, lens)
