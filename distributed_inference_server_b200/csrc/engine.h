@@ -105,7 +105,7 @@ struct Engine {
   size_t kv_layer_stride = 0;  // elements between layers in the pool
   long long kv_rows_per_layer = 0;
   TmaMap kv_map;  // the whole pool as [rows][head_dim]
-  // DIS_FLAG_KV_INT8: all layers' pages in 8 bits with their scales; kv_pool then holds one layer, read back for the prompts of a pass
+  // DIS_FLAG_KV_INT8: all layers' pages in 8 bits with their scales; kv_pool then holds one layer, read back for the sequences of a pass that reads prompts
   int8_t *kv8_pool = nullptr;
   float *kv8_scale = nullptr;
   float *piece_area = nullptr;  // scratch of the attention over pieces (zero between calls)

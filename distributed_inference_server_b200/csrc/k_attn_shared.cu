@@ -24,15 +24,16 @@
 // every token by itself gives 1.7e-3, and what a step's results are worth would have depended on its batch.  P and its rest fill the 64 columns of the scores.
 // 32 requests behind 6000 24.2 -> 24.8 us, 64 behind 64000 128 -> 156.
 //
-// Measured (B200, from graphs, all three kernels): 32 requests behind 6000 tokens, 32 / 8 heads of 128, own parts to 500, bf16: 24.9 us;
-// 64 behind 8000, 64 / 8 heads, own parts to 700, 8 bits: 50.1 (10.6 at a library product's rate, 7.6 for its bytes).  A step of 256 rows x 64 keys takes 1.0 us
-// in bf16 and 1.27 in 8 bits.  In clocks, bf16: exponentials and P 1290 (two warps to a scheduler, 1024 of them the exponentials alone), maximum 200,
-// waits for scores 190, of 1760; the products take 1280 of the tensor pipe (S with N = 64 reads 6 KB of operands each, at shared memory's rate).  8 bits: a group's
-// exponentials 970 (in turn), maximum 560 (scales of K and V from shared memory), its turn 190, P's hand-over 125, the tile's fp16 rows 330, of 2210: shared memory
-// and issue slots are shared with the warps that turn rows to fp16.  Eight of those instead of four (96 registers) were slower (64 behind 64000
-// 161 -> 182 us), as were rows through registers (179 -> 230 before warp 0 copied them) or turned in units of half a tile (-> 210).  The score buffers are two per group so that a group's next product runs under its
-// softmax: one of twice the keys, which needs 1024 clocks of tensor pipe instead, was slower (bf16 131 -> 154 us at 64000), the two groups being in phase.  A
-// CTA's start (queries, barriers, TMEM) and end (128 KB of state) are six steps' worth.
+// Measured (B200, from graphs, all three kernels): 32 requests behind 6000 tokens, 32 / 8 heads of 128, own parts to 500, bf16: 24.8 us (6.9 for its bytes);
+// 64 behind 8000, 64 / 8 heads, own parts to 700, 8 bits: 50.7 (10.6 at a library product's rate, 7.6 for its bytes).  A step of 256 rows x 64 keys takes
+// 1.2 to 1.3 us in both (slope from 16000 to 64000 tokens).  bf16: the products take 1792 clocks of the tensor pipe a step (S with N = 64 reads 6 KB of operands
+// each, at shared memory's rate, 768; P V twice 1024); exponentials and P, two warps to a scheduler, took 1290 before the weights' rests, 1024 of them the
+// exponentials alone.  8 bits: a group's exponentials 970 (in turn), maximum 560 (scales of K and V from shared memory), its turn 190, P's hand-over 125, the
+// tile's fp16 rows 330, of 2210: shared memory and issue slots are shared with the warps that turn rows to fp16.  Eight of those instead of four (96 registers) were
+// slower (64 behind 64000 161 -> 182 us), as were rows through registers (179 -> 230 before warp 0 copied them) or turned in units of half a tile (-> 210).  The score buffers
+// are two per group so that a group's next product runs under its softmax: one of twice the keys, which needs a third less of the tensor pipe for S, was
+// slower (bf16 with weights in one half, 131 -> 154 us at 64000), the two groups being in phase.  A CTA's start (queries, barriers, TMEM) and end (128 KB of state)
+// are six steps' worth: the 64 behind 8000 have 14 steps a CTA, some 18 us; the rest is that start and end, the own parts in front and the join behind.
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -676,16 +677,16 @@ static int shared_blocks(int T, int G, int n_kv) { const int rt = shared_row_til
 
 // Whether the prefix is read once, or every token goes alone (one kernel, to which the others' reads of the same pages are hits in L2): from 2^25 entries of T
 // prefixes on the former is ahead; heads of 128 in two tiles of rows or more, and in 8 bits, each cross a quarter later.  From graphs, own parts of 100,
-// together / alone, us, at 1, 1.25 and 1.5 times 2^25 entries:
-//   32 / 8 heads of 128, bf16   16 tokens 18.6 / 19.3, 18.1 / 21.8, 19.4 / 24.0;  32: 19.2 / 19.6, 17.6 / 22.1, 18.5 / 24.4;  64 (two tiles): 24.2 / 21.5, 22.9 / 24.6, 23.6 / 26.9
-//   the same in 8 bits          8: 21.3 / 19.0, 22.7 / 21.6, 23.7 / 23.6;  32: 20.4 / 19.1, 18.8 / 21.4, 19.9 / 23.7;  64: 26.2 / 21.1, 26.1 / 23.8, 26.6 / 26.0
-//   64 / 8 heads, 8 bits        16: 20.7 / 20.9, 21.8 / 23.0, 24.3 / 24.7;  32 (two tiles): 25.5 / 20.8, 25.5 / 23.2, 25.8 / 25.2;  64: 29.7 / 23.1, 29.7 / 25.9, 28.2 / 28.2
-//   32 / 4 heads of 64, 8 bits  16: 18.1 / 22.2, 19.1 / 25.7, 20.3 / 28.6;  64 (four tiles): 20.7 / 21.1, 21.1 / 24.2, 21.8 / 26.7
-// at half of 2^25, bf16: 16 18.2 / 14.6, 32 18.3 / 14.9.
-// A few tokens make little of a product's 128 rows, and the prefix has to be turned to fp16 all the same.  At 1.5, 2 and 4 times 2^25: 32 / 8 heads of 128, 8 bits
-// 2: 38.2 / 25.6, 45.1 / 30.1, 73.4 / 48.9;  4: 28.3 / 24.4, 32.4 / 28.9, 46.2 / 46.9;  6: 25.2 / 25.0, 26.3 / 28.7, 37.2 / 46.3;  heads of 64 in 8 bits
-// 4: 30.6 / 30.5, 36.5 / 36.2, 59.3 / 59.3;  6: 26.2 / 30.1, 29.5 / 36.8, 44.7 / 57.9;  bf16, heads of 128, 2: 33.7 / 34.2, 39.5 / 38.8, 61.4 / 78.2 (at 1: 26.7 / 22.3);
-// 4: 24.0 / 25.3, 26.8 / 31.1, 40.0 / 61.3
+// together / alone, us, at 1 and 1.25 times 2^25 entries:
+//   32 / 8 heads of 128, bf16   16 tokens 17.3 / 19.5, 16.8 / 22.2;  32: 18.5 / 19.6, 15.9 / 21.9;  64 (two tiles): 19.7 / 21.5, 20.2 / 23.8
+//   the same in 8 bits          16: 18.8 / 19.2, 17.6 / 22.0;  32: 20.7 / 19.5, 17.1 / 21.7;  64: 21.3 / 21.3, 21.9 / 23.4
+//   64 / 8 heads, 8 bits        16: 20.3 / 21.0, 18.8 / 23.8;  32 (two tiles): 25.2 / 21.2, 21.8 / 23.5;  64: 25.1 / 23.3, 24.0 / 25.5
+//   32 / 4 heads of 64, 8 bits  16: 18.0 / 23.2, 18.6 / 25.9;  64 (four tiles): 19.8 / 21.5, 20.5 / 24.4
+// A few tokens make little of a product's 128 rows: two or three over bf16 pages cross at 2 times 2^25 (2 tokens at 1, 1.5, 2, 4: 28.5 / 24.2, 35.0 / 32.3,
+// 40.8 / 39.3, 63.5 / 87.1; 4 tokens at 1: 19.5 / 21.5).  Over 8-bit pages, which have to be turned to fp16 as well, fewer than six go alone at every length.  For two
+// that is ahead to 131072 tokens of 8 heads of 128 at least (128.4 / 100.2).  A prefix read once passes three somewhere between 32768 and 131072 (45.9 / 42.0, 129 / 145), four
+// near 25000 (8192 21.7 / 21.1, 32768 46.1 / 49.7), five before 8192 (21.7 / 23.9; 131072 130 / 211); of 4 heads of 64 four are level at 131072 (59.9 / 59.4): what so few
+// could gain there the rule leaves aside.
 bool attn_shared_pays(int T, int n_heads, int n_kv, int d, int prefix, bool int8) {
   if (T < (int8 ? 6 : 2) || n_kv < 1) return false;
   if (n_kv > 65535 || shared_row_tiles(T, std::max(n_heads / n_kv, 1)) > 65535) return false;  // (a grid's sides)

@@ -21,7 +21,7 @@
 // depend on who that is.
 //
 // Measured (B200, 8 bits, from graphs; time at 6.54 TB/s, a plain copy's rate, beside it): 32 histories to 6000 tokens, 32 / 8 heads of 128, 29.7 us
-// (19.4); two to 60000, 64 / 8 heads, 36.2 (21.7); 64 to 3000, 32 / 4 heads of 64, 16.0 (5.3); four to 500 7.7 (0.3).  In the middle of a long
+// (19.4); two to 60000, 64 / 8 heads, 37 (21.7); 64 to 3000, 32 / 4 heads of 64, 15.5 (5.3); four to 500 7.9 (0.3).  In the middle of a long
 // launch rows come in at 6 to 6.9 TB/s.  The rest: 2.5 to 5 us until every ring has been filled once, 2 to 3 us from the last row to the
 // result (states met in shared memory 0.5 to 1, count 0.9, join 1 a level), and CTAs of equal shares that end up to 15 % apart.  (Tiles taken
 // as warps come free would even that out, and make the sums' order, so the result's last bits, differ from call to call.)

@@ -16,7 +16,7 @@ namespace dis {
 // kMany: eight CTAs to an SM (32 registers) keep more loads on their way; few CTAs keep a row's K slices on their way instead.  They cross at about five
 // CTAs an SM.  us, many / few (CTAs): 32 + 2 x 8 heads of 128, one slice 384 2.6 / 2.6, 600 2.8 / 3.0, 1200 3.7 / 4.1, 4800 9.6 / 11.8, 14400 30.8 / 42.0; four slices
 // 96 3.1 / 2.9, 384 3.3 / 3.3, 900 4.6 / 5.1; 32 + 2 x 4 heads of 64, one slice 600 2.6 / 2.4, 800 2.8 / 3.0; four slices 800 3.7 / 3.6, 1200 4.3 / 5.0.
-// With the read-back of all histories: six prompts behind 2048 tokens each, 32 / 8 heads of 128, 45.8 us (37.6 at a plain copy's rate).
+// With the read-back of all histories: six prompts to 2500 tokens (5404 in all) behind 5318, 32 / 8 heads of 128, 45.5 us (37.6 at a plain copy's rate).
 constexpr int kCwThreads = 256;
 
 template <int D, bool kMany>
@@ -107,7 +107,7 @@ cudaError_t launch_rope_kv_write_i8(const float *qkv, int n_partial, long long p
 // HBM-bound: d + 4 bytes in, 2 d out per row.  The pages that the histories' positions lie in are laid end to end, a unit being 16 KB of one of
 // them, and dealt to the resident CTAs in turn, whatever the lengths are; a thread turns 16 entries at a time.
 constexpr int kCrThreads = 256, kCrUnroll = 4, kCrBytes = kCrThreads * kCrUnroll * 16, kCrMaxRows = 1024;
-// CTAs per SM of the grid, twice what is resident: 16 histories to 6000, heads of 8 x 128, 31.0 -> 29.0 us; 24 per SM 28.6, but a row's 2 us for a call that
+// CTAs per SM of the grid, twice what is resident: 16 histories to 6000, 8 heads of 128, 31.0 -> 29.0 us; 24 per SM 28.6, but a row's 2 us for a call that
 // reads one token back of each of 32
 constexpr int kCrCtas = 12;
 

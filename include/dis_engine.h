@@ -82,9 +82,9 @@ typedef struct dis_model_config {
 #define DIS_FLAG_NO_PDL 4u     /* launch the kernels of a step without programmatic dependent launch */
 #define DIS_FLAG_PREFIX_CACHE 8u /* keep the full KV pages of finished prompts and map them into later requests that start
                                    with the same tokens (KVCacheManager::get_prefix, design.md:396; Property 9) */
-#define DIS_FLAG_KV_INT8 16u     /* keep keys and values in 8 bits (see dis_k_rope_kv_write_i8): about twice the pages in the same memory.  Decode steps
-                                   attend over them as they are; passes that read prompts turn the listed sequences' histories back into bf16, layer
-                                   by layer, in one layer's worth of extra pages */
+#define DIS_FLAG_KV_INT8 16u     /* keep keys and values in 8 bits (see dis_k_rope_kv_write_i8): 1.7 to 1.9 times the pages in the same memory.
+                                   Decode steps attend over them as they are; passes that read prompts turn the histories of all listed sequences,
+                                   running ones among them, back into bf16, layer by layer, in one layer's worth of extra pages */
 #define DIS_FLAG_ATTN_SHARED 32u /* decode steps read the pages that all of their sequences have in common once (dis_k_attn_shared), where that pays;
                                    such pages come from DIS_FLAG_PREFIX_CACHE.  Both flags need 1, 2, 4 or 8 query heads per kv head and are refused
                                    for layer-list decoders */
@@ -436,17 +436,19 @@ DIS_API int dis_k_attn_paged_i8(const uint16_t *q, const int8_t *pool, const flo
                                 const int32_t *pt_row, const int32_t *ctx, uint16_t *out, float *scratch, int32_t T, int32_t n_heads,
                                 int32_t n_kv, int32_t d, int32_t page_size, void *stream);
 /* The same for a batch whose requests share a prefix: positions [0, prefix) hold the same keys and values for every token and are read once for
- * all of them, through the pages of the first token's row; positions [prefix, ctx[t]) are each token's own.  A token with ctx[t] <= prefix sees
- * the first ctx[t] positions of the prefix.  kv_pool: bf16 pages (scale NULL) or 8-bit pages with their scales; n_pages pages.
+ * all of them, through the pages of the first token's row, which has to list all of the prefix's even where that token's own history ends before;
+ * positions [prefix, ctx[t]) are each token's own.  A token with ctx[t] <= prefix sees the first ctx[t] positions of the prefix.
+ * Weights enter the products as two bf16 halves over bf16 pages, in fp16 over 8-bit ones, whichever way a call goes.  kv_pool: bf16 pages (scale NULL) or 8-bit pages with their scales; n_pages pages.
  * Rows of a bf16 prefix page past `prefix` must hold finite values, as for dis_k_attn_paged.  scratch: dis_k_attn_shared_scratch_elems()
  * floats under the terms of dis_k_attn_paged_i8, whose scratch it may be too. */
-/* Whether dis_k_attn_shared reads the prefix once for these sizes (int8: 8-bit pages): below about 2^25 entries of T prefixes, and for a few tokens
- * over 8-bit pages, every token by itself, in one kernel, is ahead.  The result is the same to rounding.  Needs no GPU. */
-DIS_API int dis_k_attn_shared_in_common(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d, int32_t prefix, int32_t int8);
 DIS_API size_t dis_k_attn_shared_scratch_elems(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d);
 DIS_API int dis_k_attn_shared(const uint16_t *q, const void *kv_pool, const float *scale, int64_t n_pages, const int32_t *page_table,
                               int32_t max_pages, const int32_t *pt_row, const int32_t *ctx, int32_t prefix, uint16_t *out, float *scratch,
                               int32_t T, int32_t n_heads, int32_t n_kv, int32_t d, int32_t page_size, void *stream);
+/* Whether dis_k_attn_shared reads the prefix once for these sizes (int8: 8-bit pages): below about 2^25 entries of T prefixes, for fewer than six tokens
+ * over 8-bit pages, and where there are more than 65535 kv heads or tiles of 128 query rows, every token goes by itself, in one kernel.  The result is the same
+ * to rounding.  Needs no GPU. */
+DIS_API int dis_k_attn_shared_in_common(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d, int32_t prefix, int32_t int8);
 /* Sampler over fp32 logits [T][V] (row stride ld): temperature 0 -> argmax, lowest index wins ties;
  * else nucleus sampling as oracle/llama_oracle.c states it.  out_tokens[T]; out_logprob[T] (may be NULL) receives
  * the chosen token's log-probability (see dis_engine_last_logprobs). */
