@@ -194,6 +194,12 @@ PROTOTYPES = {
     "dis_k_attn_shared_scratch_elems": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "dis_k_attn_shared": (C.c_int, [vp, vp, vp, C.c_int64, vp, C.c_int32, vp, vp, C.c_int32, vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                     C.c_int32, vp]),
+    "dis_k_quant_f8": (C.c_int, [vp, vp, vp, C.c_int32, C.c_int32, vp]),
+    "dis_k_quant_weight_f8": (C.c_int, [vp, vp, vp, C.c_int32, C.c_int32, vp]),
+    "dis_k_add_rmsnorm_f8": (C.c_int, [vp, vp, vp, vp, C.c_int32, C.c_int64, vp, vp, vp, vp, C.c_int32, C.c_int32, C.c_float, vp]),
+    "dis_k_gemm_f8": (C.c_int, [vp, vp, vp, vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, vp]),
+    "dis_k_gemm_silu_f8": (C.c_int, [vp, vp, vp, vp, vp, vp, C.c_int32, C.c_int32, C.c_int32, vp]),
+    "dis_k_ffn_f8": (C.c_int, [vp] * 10 + [C.c_int32] * 4 + [vp]),
     "dis_k_sample_vocab_parallel_area_bytes": (C.c_size_t, [C.c_int32, C.c_int32]),
     "dis_k_sample_vocab_parallel": (C.c_int, [vp, C.c_int32, C.c_int32, C.c_int32, vp, vp, vp, vp, C.c_uint32, vp, C.c_int32, vp, vp, vp]),
     "dis_k_sample": (C.c_int, [vp, C.c_int64, C.c_int32, C.c_int32, vp, vp, vp, vp, vp, vp, vp]),

@@ -395,6 +395,119 @@ int dis_k_attn_shared(const uint16_t *q, const void *kv_pool, const float *scale
   return k_ret(dis::launch_attn_shared(q, kv_pool, scale, n_pages, page_table, max_pages, pt_row, ctx, prefix, nullptr, out, scratch, T, n_heads, n_kv, d, page_size,
                                        true, (cudaStream_t)stream));
 }
+// What the calls on 8-bit floating point ask of their sizes; 0 or the refusal's code.  rows: of the activations, n: of the weight (0: none),
+// k: entries of a row
+static int f8_shape(const char *who, int rows, long long n, int k) {
+  const char *what = nullptr;
+  if (rows < 0) what = "a negative number of rows";
+  else if (rows > 65535 * 32) what = "more than 65535 * 32 rows";
+  else if (k < 16 || k % 16) what = "rows must hold a positive multiple of 16 entries";
+  else if (n < 0 || n > 65535ll * 128) what = "a weight has 1 to 65535 * 128 rows";
+  if (!what) return DIS_OK;
+  dis::set_last_error(std::string(who) + ": " + what);
+  return DIS_ERR_INVALID_ARGUMENT;
+}
+
+int dis_k_quant_f8(const uint16_t *x, uint8_t *x8, float *scale, int32_t T, int32_t K, void *stream) {
+  static const char *me = "quant_f8";
+  if (int rc = need_gpu()) return rc;
+  if (int rc = f8_shape(me, T, 0, K)) return rc;
+  if (T == 0) return DIS_OK;
+  if (!x || !x8 || !scale) return cache_refuse(me, "null pointer");
+  if (off(x, 16) || off(x8, 16) || off(scale, 4)) return cache_refuse(me, "x and x8 start on 16 bytes, the scales on 4");
+  CallOverlap overlap(stream);
+  return k_ret(dis::launch_quant_f8(x, x8, scale, T, K, (cudaStream_t)stream));
+}
+int dis_k_quant_weight_f8(const uint16_t *w, uint8_t *w8, float *scale, int32_t N, int32_t K, void *stream) {
+  static const char *me = "quant_weight_f8";
+  if (int rc = need_gpu()) return rc;
+  if (int rc = f8_shape(me, 0, N, K)) return rc;
+  if (N == 0) return DIS_OK;
+  if (!w || !w8 || !scale) return cache_refuse(me, "null pointer");
+  if (off(w, 16) || off(w8, 16) || off(scale, 4)) return cache_refuse(me, "w and w8 start on 16 bytes, the scales on 4");
+  CallOverlap overlap(stream);
+  return k_ret(dis::launch_quant_weight_f8(w, w8, scale, N, K, (cudaStream_t)stream));
+}
+int dis_k_add_rmsnorm_f8(float *x, const uint32_t *tokens, const uint16_t *embed, const float *partial, int32_t n_partial, int64_t partial_stride,
+                         const float *gain, uint8_t *x8, float *scale, const int32_t *row_map, int32_t T, int32_t H, float eps, void *stream) {
+  static const char *me = "add_rmsnorm_f8";
+  if (int rc = need_gpu()) return rc;
+  if (int rc = f8_shape(me, T, 0, H)) return rc;
+  if (H > 51200) return cache_refuse(me, "rows of more than 51200 entries");
+  if (n_partial < 0) return cache_refuse(me, "a negative number of partial sums");
+  if (T == 0) return DIS_OK;
+  if (!x || !gain || !x8 || !scale || (tokens && !embed) || (!tokens && n_partial > 0 && !partial)) return cache_refuse(me, "null pointer");
+  if (off(x, 16) || off(gain, 16) || off(x8, 16) || off(scale, 4) || (tokens && off(embed, 16)) || (!tokens && n_partial > 0 && (off(partial, 16) || (n_partial > 1 && partial_stride % 4))))
+    return cache_refuse(me, "x, embed, the partial sums and their slices, gain and x8 start on 16 bytes, the scales on 4");
+  CallOverlap overlap(stream);
+  return k_ret(dis::launch_add_rmsnorm_f8(x, tokens, embed, partial, tokens ? 0 : n_partial, partial_stride, gain, x8, scale, row_map, T, H, eps, (cudaStream_t)stream));
+}
+
+static int gemm_f8_checks(const char *me, const uint8_t *x8, const float *xs, const uint8_t *w8, const float *ws, const void *out) {
+  if (!x8 || !xs || !w8 || !ws || !out) return cache_refuse(me, "null pointer");
+  if (off(x8, 16) || off(w8, 16) || off(xs, 4) || off(ws, 4)) return cache_refuse(me, "the 8-bit rows start on 16 bytes, their scales on 4");
+  return DIS_OK;
+}
+static int gemm_f8_out(const char *me, const void *out, int out_dtype) {
+  if (out_dtype != DIS_F32 && out_dtype != DIS_BF16) return cache_refuse(me, "out_dtype must be DIS_F32 or DIS_BF16");
+  if (off(out, out_dtype == DIS_F32 ? 4 : 2)) return cache_refuse(me, "out starts on a whole element");
+  return DIS_OK;
+}
+static cudaError_t gemm_f8_call(const uint8_t *x8, const float *xs, const uint8_t *w8, const float *ws, void *out, int out_dtype, int T, int N, int K, cudaStream_t st) {
+  dis::TmaMap wm, xm;
+  cudaError_t e = dis::make_f8_map(&wm, w8, (uint64_t)N, (uint64_t)K, 128);
+  if (e == cudaSuccess) e = dis::make_f8_map(&xm, x8, (uint64_t)T, (uint64_t)K, dis::gemm_f8_token_box(T, N, K, false));
+  if (e != cudaSuccess) return e;
+  return dis::launch_gemm_f8(wm, xm, xs, ws, out, out_dtype == DIS_BF16, T, N, K, 0, st);
+}
+static cudaError_t gemm_silu_f8_call(const uint8_t *x8, const float *xs, const uint8_t *wgu8, const float *wgus, uint8_t *h8, float *hs, int T, int I, int K, cudaStream_t st) {
+  dis::TmaMap wm, xm;
+  cudaError_t e = dis::make_f8_map(&wm, wgu8, 2ull * I, (uint64_t)K, 128);
+  if (e == cudaSuccess) e = dis::make_f8_map(&xm, x8, (uint64_t)T, (uint64_t)K, dis::gemm_f8_token_box(T, I, K, true));
+  if (e != cudaSuccess) return e;
+  return dis::launch_gemm_silu_f8(wm, xm, xs, wgus, h8, hs, T, I, K, 0, st);
+}
+
+int dis_k_gemm_f8(const uint8_t *x8, const float *xs, const uint8_t *w8, const float *ws, void *out, int32_t out_dtype, int32_t T, int32_t N, int32_t K,
+                  void *stream) {
+  static const char *me = "gemm_f8";
+  if (int rc = need_gpu()) return rc;
+  if (int rc = f8_shape(me, T, N, K)) return rc;
+  if (T == 0 || N == 0) return DIS_OK;
+  if (int rc = gemm_f8_checks(me, x8, xs, w8, ws, out)) return rc;
+  if (int rc = gemm_f8_out(me, out, out_dtype)) return rc;
+  CallOverlap overlap(stream);
+  return k_ret(gemm_f8_call(x8, xs, w8, ws, out, out_dtype, T, N, K, (cudaStream_t)stream));
+}
+int dis_k_gemm_silu_f8(const uint8_t *x8, const float *xs, const uint8_t *wgu8, const float *wgus, uint8_t *h8, float *hs, int32_t T, int32_t I, int32_t K,
+                       void *stream) {
+  static const char *me = "gemm_silu_f8";
+  if (int rc = need_gpu()) return rc;
+  if (int rc = f8_shape(me, T, I, K)) return rc;
+  if (I % 16) return cache_refuse(me, "the inner size must be a multiple of 16");
+  if (T == 0 || I == 0) return DIS_OK;
+  if (int rc = gemm_f8_checks(me, x8, xs, wgu8, wgus, h8)) return rc;
+  if (!hs || off(h8, 16) || off(hs, 4)) return cache_refuse(me, "h8 starts on 16 bytes, its scales on 4");
+  CallOverlap overlap(stream);
+  return k_ret(gemm_silu_f8_call(x8, xs, wgu8, wgus, h8, hs, T, I, K, (cudaStream_t)stream));
+}
+int dis_k_ffn_f8(const uint16_t *x, const uint8_t *wgu8, const float *wgus, const uint8_t *wd8, const float *wds, uint8_t *x8, float *xs, uint8_t *h8,
+                 float *hs, void *out, int32_t out_dtype, int32_t T, int32_t H, int32_t I, void *stream) {
+  static const char *me = "ffn_f8";
+  if (int rc = need_gpu()) return rc;
+  if (int rc = f8_shape(me, T, I, H)) return rc;
+  if (int rc = f8_shape(me, T, H, I)) return rc;
+  if (T == 0) return DIS_OK;
+  if (!x || off(x, 16)) return cache_refuse(me, "x must be there and start on 16 bytes");
+  if (int rc = gemm_f8_checks(me, x8, xs, wgu8, wgus, h8)) return rc;
+  if (int rc = gemm_f8_checks(me, h8, hs, wd8, wds, out)) return rc;
+  if (int rc = gemm_f8_out(me, out, out_dtype)) return rc;
+  CallOverlap overlap(stream);
+  cudaError_t e = dis::launch_quant_f8(x, x8, xs, T, H, (cudaStream_t)stream);
+  if (e == cudaSuccess) e = gemm_silu_f8_call(x8, xs, wgu8, wgus, h8, hs, T, I, H, (cudaStream_t)stream);
+  if (e == cudaSuccess) e = gemm_f8_call(h8, hs, wd8, wds, out, out_dtype, T, H, I, (cudaStream_t)stream);
+  return k_ret(e);
+}
 int dis_k_sample(const float *logits, int64_t ld, int32_t T, int32_t V, const float *temperature, const float *top_p,
                  const uint64_t *seeds, const uint64_t *steps, uint32_t *out_tokens, float *out_logprob, void *stream) {
   if (int rc = need_gpu()) return rc;

@@ -1,0 +1,606 @@
+// k_gemm_f8.cu -- products in 8-bit floating point with a scale for each block of 128, on tcgen05 (kind::f8f6f4, e4m3 x e4m3 -> fp32):
+//
+//   y[t][n] = sum_b xs[b][t] ws[n / 128][b] sum_{k in block b} x8[t][k] w8[n][k]      x8 [T][K], w8 [N][K], b = k / 128
+//
+// plain (fp32 or bf16 rows) or as the gate-up product of a feed-forward block: h = silu(g) u of the fused [2][I][K] weight, itself turned
+// into 8 bits (f8.cuh).  A block's 128 entries are one 128-byte swizzle row, so a stage of the TMA ring is a block: its four MMAs make
+// a fresh accumulator in tensor memory, and the epilogue warps add it, times both scales, to sums that they keep in registers.  Scales
+// that are not powers of two and differ from block to block cannot be left to the MMA.
+//
+// Tokens are the MMA's rows (TMEM lanes) and features its columns at every size: a thread owns one token, so a block's two scales are one
+// factor per thread.  With few tokens most lanes compute on what happens to lie in shared memory; nothing waits for them: what bounds
+// such a product is the weight coming from HBM.
+//
+// Two kernels:
+//   tile  a CTA per 128 x 128 (gate-up: 128 x 128 + 128) tile and, where the tiles are few, a cluster of up to eight CTAs that share its K:
+//         each leaves its sums in its own shared memory, and after a cluster barrier every CTA finishes a share of the tokens.
+//   pair  two CTAs per 256 x 256 tile (cta_group::2), persistent, for many tokens: an SM brings 32 KB per block for 512 clocks of the
+//         tensor pipe, and reads its 128 x 256 sums from TMEM in the meantime.
+#include <cuda.h>
+
+#include "f8.cuh"
+#include "kernels.h"
+
+namespace dis {
+
+namespace {
+
+constexpr int kF8Threads = 320;  // warp 0 TMA, warp 1 MMA + TMEM, warps 2-9 sums: warp % 4 picks 32 tokens, (warp - 2) / 4 half of the columns
+constexpr int kF8Box = 128 * kF8Block;  // bytes of 128 rows of a block
+
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kUmmaDescHi)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kUmmaDescHi)
+      : "memory");
+}
+// Instruction descriptor: D = f32, A = B = e4m3, both K-major
+__host__ __device__ constexpr uint32_t f8_idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+// sums += factor * (32 columns of tensor memory)
+__device__ __forceinline__ void add_scaled(const uint32_t (&v)[32], float factor, uint64_t *sums) {
+  uint64_t f;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "f"(factor));
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(v[2 * i]), "r"(v[2 * i + 1]));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sums[i]) : "l"(p), "l"(f));
+  }
+}
+__device__ __forceinline__ float2 pair_of(uint64_t s) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(s));
+  return r;
+}
+
+// The scales of a thread's token and of its columns' weight rows, fetched ahead: the token's four blocks at a time, the weight's 32, one
+// per lane (they are the same for the whole warp).  Blocks are asked for in order from begin()'s first on.
+template <int kW>
+struct Scales {
+  const float *xs, *ws[kW];
+  int T, t, end;          // blocks from `end` on are not read
+  float x[4], x_next[4], w[kW], w_next[kW];
+  __device__ __forceinline__ void fetch_x(int b) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x_next[i] = t < T && b + i < end ? xs[(size_t)(b + i) * T + t] : 0.f;
+  }
+  __device__ __forceinline__ void fetch_w(int b) {
+    const int l = b + (int)(threadIdx.x & 31);
+#pragma unroll
+    for (int j = 0; j < kW; j++) w_next[j] = l < end && ws[j] ? ws[j][l] : 0.f;
+  }
+  // i: blocks since begin(); returns the factors of block first + i
+  __device__ __forceinline__ void get(int first, int i, float (&f)[kW]) {
+    if ((i & 3) == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[j] = x_next[j];
+      fetch_x(first + i + 4);
+    }
+    if ((i & 31) == 0) {
+#pragma unroll
+      for (int j = 0; j < kW; j++) w[j] = w_next[j];
+      fetch_w(first + i + 32);
+    }
+    const float a = (i & 2) ? ((i & 1) ? x[3] : x[2]) : ((i & 1) ? x[1] : x[0]);
+#pragma unroll
+    for (int j = 0; j < kW; j++) f[j] = a * __shfl_sync(0xffffffffu, w[j], i & 31);
+  }
+};
+
+__device__ __forceinline__ float silu(float g) { return gate_act_fast(0, g); }
+
+// ------------------------------------------------------------------------------------------------ tile kernel
+// The ring's stages, then the barriers.  kGated: 128 gate rows and 128 up rows per stage, 256 accumulator columns; else 128 of each.
+template <bool kGated>
+struct TileCfg {
+  static constexpr int kCols = kGated ? 256 : 128;
+  static constexpr int kTmem = 2 * kCols;  // two accumulators: a block's sums are taken while the next block's MMAs run
+  static constexpr int kLd = kCols + 4;    // floats of a token's row of sums in shared memory: rows of 32 lanes start on different banks
+  static int stage_bytes(int tile_t) { return tile_t * kF8Block + (kGated ? 2 : 1) * kF8Box; }
+  // The sums take the ring's place.  (The MMA reads 128 token rows whatever tile_t is: past a shorter tile lie the stage's weight rows.)
+  static int body_bytes(int stages, int tile_t, int rows) {
+    const int ring = stages * stage_bytes(tile_t), sums = rows * kLd * 4;
+    return ring > sums ? ring : sums;
+  }
+};
+
+template <bool kGated>
+__global__ void __launch_bounds__(kF8Threads, kGated ? 1 : 2)
+gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const float *__restrict__ xs,
+                    const float *__restrict__ ws, void *__restrict__ out, float *__restrict__ out_scale, int out_bf16, int T, int N, int K,
+                    int w_row0, int split, int tile_t, int stages, uint32_t bar_off, int weights_first, int wide) {
+  using Cfg = TileCfg<kGated>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t a_bytes = (uint32_t)tile_t * kF8Block, stage_bytes = a_bytes + (kGated ? 2u : 1u) * kF8Box;
+  const uint32_t bar_base = smem_base + bar_off;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (stages + s); };
+  auto acc_full = [&](uint32_t b) { return bar_base + 8u * (2 * stages + b); };
+  auto acc_empty = [&](uint32_t b) { return bar_base + 8u * (2 * stages + 2 + b); };
+  const uint32_t tmem_slot = bar_base + 8u * (2 * stages + 4);
+
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  const int tile = blockIdx.x / split, slice = blockIdx.x - tile * split;  // a cluster is one tile's slices, in order
+  const int n0 = tile * 128, t0 = blockIdx.y * tile_t, rows = min(tile_t, T - t0);
+  const int num_kb = (K + kF8Block - 1) / kF8Block;
+  const int kb0 = (int)((long long)num_kb * slice / split), kb1 = (int)((long long)num_kb * (slice + 1) / split);
+  const int quarters = (rows + 31) >> 5;  // of the lanes that hold tokens
+
+  const int pre = min(kb1 - kb0, stages);
+  auto load_w = [&](int kb, int s) {
+    const uint32_t dst = smem_base + s * stage_bytes + a_bytes;
+    tma_load_2d(dst, &w_map, kb * kF8Block, w_row0 + n0, full_bar(s), kEvictFirst);
+    if (kGated) tma_load_2d(dst + kF8Box, &w_map, kb * kF8Block, w_row0 + N + n0, full_bar(s), kEvictFirst);
+  };
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&w_map);
+    tma_prefetch_desc(&x_map);
+    for (int s = 0; s < stages; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+    for (uint32_t b = 0; b < 2; b++) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 2 * quarters); }
+    fence_barrier_init();
+    fence_proxy_async();
+    if (weights_first)
+      for (int i = 0; i < pre; i++) { mbar_expect_tx(full_bar(i), stage_bytes); load_w(kb0 + i, i); }
+    else
+      for (int i = 0; i < pre; i++) {  // a weight that the kernel ahead may be writing: as far as L2
+        tma_prefetch_2d(&w_map, (kb0 + i) * kF8Block, w_row0 + n0);
+        if (kGated) tma_prefetch_2d(&w_map, (kb0 + i) * kF8Block, w_row0 + N + n0);
+      }
+  }
+  if (warp == 1) tmem_alloc<Cfg::kTmem>(tmem_slot);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem_base;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      pdl_wait();
+      for (int i = 0; i < pre; i++) {
+        if (!weights_first) { mbar_expect_tx(full_bar(i), stage_bytes); load_w(kb0 + i, i); }
+        tma_load_2d(smem_base + i * stage_bytes, &x_map, (kb0 + i) * kF8Block, t0, full_bar(i), kEvictLast);
+      }
+      int s = pre == stages ? 0 : pre;
+      uint32_t phase = pre == stages ? 1u : 0u;
+      for (int kb = kb0 + pre; kb < kb1; kb++) {
+        mbar_wait(empty_bar(s), phase ^ 1u);
+        mbar_expect_tx(full_bar(s), stage_bytes);
+        load_w(kb, s);
+        tma_load_2d(smem_base + s * stage_bytes, &x_map, kb * kF8Block, t0, full_bar(s), kEvictLast);
+        if (++s == stages) { s = 0; phase ^= 1u; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = f8_idesc(128, Cfg::kCols);
+    const uint32_t lo0 = umma_lo(smem_base);
+    uint32_t lo = lo0, phase = 0, buf = 0, aphase = 0;
+    int s = 0;
+    for (int kb = kb0; kb < kb1; kb++) {
+      mbar_wait(acc_empty(buf), aphase ^ 1u);  // (passes on first use)
+      mbar_wait(full_bar(s), phase);
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) umma_f8(tmem_base + buf * Cfg::kCols, lo + 2 * k, lo + (a_bytes >> 4) + 2 * k, idesc, k > 0 ? 1u : 0u);
+        umma_commit(empty_bar(s));
+        umma_commit(acc_full(buf));
+      }
+      __syncwarp();
+      lo += stage_bytes >> 4;
+      if (++s == stages) { s = 0; phase ^= 1u; lo = lo0; }
+      aphase ^= buf;
+      buf ^= 1u;
+    }
+  } else if ((warp & 3) < quarters) {
+    // Columns of a warp: its half of the features; gate-up: 64 gate columns and the 64 up columns of the same features
+    const int quarter = warp & 3, half = (warp - 2) >> 2, r = quarter * 32 + lane;
+    pdl_wait();
+    Scales<kGated ? 2 : 1> sc;
+    sc.xs = xs; sc.T = T; sc.t = r < rows ? t0 + r : T; sc.end = kb1;
+    sc.ws[0] = ws + (size_t)tile * num_kb;
+    if (kGated) sc.ws[kGated ? 1 : 0] = ws + ((size_t)((N + 127) / 128) + tile) * num_kb;
+    sc.fetch_x(kb0);
+    sc.fetch_w(kb0);
+    uint64_t sums[Cfg::kCols / 4];
+#pragma unroll
+    for (int i = 0; i < Cfg::kCols / 4; i++) sums[i] = 0;
+    const uint32_t cols = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 64;
+    uint32_t buf = 0, aphase = 0;
+    for (int kb = kb0; kb < kb1; kb++) {
+      float f[kGated ? 2 : 1];
+      sc.get(kb0, kb - kb0, f);
+      mbar_wait(acc_full(buf), aphase);
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < (kGated ? 4 : 2); c++) {
+        uint32_t v[32];
+        tmem_ld_32x32(cols + buf * Cfg::kCols + (c >> 1) * 128 + (c & 1) * 32, v);
+        tmem_ld_wait();
+        if (c == (kGated ? 3 : 1)) {  // everything of this buffer is in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty(buf));
+        }
+        add_scaled(v, f[kGated ? c >> 1 : 0], sums + 16 * c);
+      }
+      aphase ^= buf;
+      buf ^= 1u;
+    }
+    // The last MMAs have read the ring: the tokens' sums take its place
+    if (r < rows) {
+#pragma unroll
+      for (int c = 0; c < (kGated ? 2 : 1); c++) {
+        const uint32_t at = smem_base + (uint32_t)(r * Cfg::kLd + c * 128 + half * 64) * 4;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float2 a = pair_of(sums[32 * c + 2 * i]), b = pair_of(sums[32 * c + 2 * i + 1]);
+          asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + 16 * i), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y) : "memory");
+        }
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  if (split > 1) cluster_sync(); else __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc<Cfg::kTmem>(tmem_base);
+  pdl_wait();  // (not all warps have been there, and all write)
+
+  // ===== every CTA of the cluster finishes a share of the tokens: a warp a token, four columns a lane, all slices' sums in order
+  for (int r = slice + split * warp; r < rows; r += split * (kF8Threads / 32)) {
+    float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t at = smem_base + (uint32_t)(r * Cfg::kLd + lane * 4) * 4;
+#pragma unroll 4
+    for (int p = 0; p < split; p++) {
+      uint32_t from = at;
+      if (split > 1) from = cluster_bar(at, (uint32_t)p);  // (a plain shared address is this CTA's own)
+      float a[4];
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]) : "r"(from) : "memory");
+#pragma unroll
+      for (int i = 0; i < 4; i++) g[i] += a[i];
+      if (kGated) {
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]) : "r"(from + 512u) : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; i++) u[i] += a[i];
+      }
+    }
+    const int n = n0 + lane * 4, t = t0 + r;
+    if (kGated) {  // N features are a multiple of 16: a lane's four are all there or none
+#pragma unroll
+      for (int i = 0; i < 4; i++) g[i] = n < N ? silu(g[i]) * u[i] : 0.f;
+      const float s = f8_scale(__reduce_max_sync(0xffffffffu, f8_top4(g[0], g[1], g[2], g[3]))), q = f8_inverse(s);
+      if (n < N) *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(out) + (size_t)t * N + n) = f8_pack4(g[0] * q, g[1] * q, g[2] * q, g[3] * q);
+      if (lane == 0) out_scale[(size_t)tile * T + t] = s;
+    } else if (out_bf16) {
+      uint16_t *o = static_cast<uint16_t *>(out) + (size_t)t * N + n;
+      if (wide && n < N) *reinterpret_cast<uint2 *>(o) = make_uint2(float2_to_bf16x2(g[0], g[1]), float2_to_bf16x2(g[2], g[3]));
+      else
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (n + i < N) o[i] = float_to_bf16_bits(g[i]);
+    } else {
+      float *o = static_cast<float *>(out) + (size_t)t * N + n;
+      if (wide && n < N) *reinterpret_cast<float4 *>(o) = make_float4(g[0], g[1], g[2], g[3]);
+      else
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (n + i < N) o[i] = g[i];
+    }
+  }
+  if (split > 1) cluster_sync();  // no CTA leaves while another reads its sums
+}
+
+// ------------------------------------------------------------------------------------------------ pair kernel
+constexpr int kF8PairStages = 6;
+constexpr int kF8PairStage = 2 * kF8Box;  // one CTA's 128 token rows and 128 feature rows of a block
+constexpr int kF8PairSmem = kF8PairStages * kF8PairStage + 1024 + 256 + 1024;
+constexpr int kF8PairCols = 256;
+
+enum { kF8OutF32 = 0, kF8OutBf16 = 1, kF8OutGated = 2 };
+
+template <int kOut>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8Threads, 1)
+gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const float *__restrict__ xs,
+                    const float *__restrict__ ws, void *__restrict__ out, float *__restrict__ out_scale, int T, int N, int K, int w_row0,
+                    int w_row_step, int tiles_n, int tiles_t, int t_fast, int wide) {
+  constexpr bool kGated = kOut == kF8OutGated;
+  constexpr int kTileN = kGated ? 128 : 256;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bar_base = smem_base + kF8PairStages * kF8PairStage;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };                                  // (first CTA's are used)
+  auto empty_bar = [&](int s) { return bar_base + 8u * (kF8PairStages + s); };
+  auto acc_full = [&](uint32_t b) { return bar_base + 8u * (2 * kF8PairStages + b); };
+  auto acc_empty = [&](uint32_t b) { return bar_base + 8u * (2 * kF8PairStages + 2 + b); };  // (first CTA's are used)
+  const uint32_t tmem_slot = bar_base + 8u * (2 * kF8PairStages + 4);
+  const uint32_t tops = bar_base + 256u;  // [128 tokens][2 halves] largest magnitudes of a gated tile
+
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+  const int num_kb = (K + kF8Block - 1) / kF8Block, n_tiles = tiles_n * tiles_t;
+  auto tile_n = [&](int tile) { return t_fast ? tile / tiles_t : tile % tiles_n; };
+  auto tile_t0 = [&](int tile) { return (t_fast ? tile % tiles_t : tile / tiles_n) * 256 + (int)rank * 128; };
+  const uint64_t w_hint = t_fast ? kEvictFirst : kEvictLast, x_hint = t_fast ? kEvictLast : kEvictFirst;
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&w_map);
+    tma_prefetch_desc(&x_map);
+    for (int s = 0; s < kF8PairStages; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+    for (uint32_t b = 0; b < 2; b++) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 16); }  // 8 warps of each CTA
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the other CTA's barriers and tensor memory are ready as well
+  tc_fence_after();
+  uint32_t tmem_base;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      pdl_wait();
+      int s = 0;
+      uint32_t phase = 0;
+      for (int tile = pair; tile < n_tiles; tile += pairs) {
+        const int t0 = tile_t0(tile), wr = w_row0 + tile_n(tile) * kTileN + (int)rank * w_row_step;  // (gated: gate rows | up rows)
+        for (int kb = 0; kb < num_kb; kb++) {
+          mbar_wait(empty_bar(s), phase ^ 1u);  // passes on the first lap
+          if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kF8PairStage);
+          const uint32_t bar = cluster_bar(full_bar(s), 0), a = smem_base + s * kF8PairStage;
+          tma_load_2d_pair(a, &x_map, kb * kF8Block, t0, bar, x_hint);
+          tma_load_2d_pair(a + kF8Box, &w_map, kb * kF8Block, wr, bar, w_hint);
+          if (++s == kF8PairStages) { s = 0; phase ^= 1u; }
+        }
+      }
+      // The first CTA's commits still arrive at this CTA's barriers: wait for the last of every stage before the CTA may end.
+      for (int i = 0; i < kF8PairStages; i++) {  // (a stage never filled passes at once)
+        mbar_wait(empty_bar(s), phase ^ 1u);
+        if (++s == kF8PairStages) { s = 0; phase ^= 1u; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      constexpr uint32_t idesc = f8_idesc(256, kF8PairCols);
+      const uint32_t lo0 = umma_lo(smem_base);
+      uint32_t lo = lo0, phase = 0, buf = 0, aphase = 0;
+      int s = 0;
+      for (int tile = pair; tile < n_tiles; tile += pairs)
+        for (int kb = 0; kb < num_kb; kb++) {
+          mbar_wait_cluster(acc_empty(buf), aphase ^ 1u);  // both CTAs have taken this buffer (passes on first use)
+          mbar_wait_cluster(full_bar(s), phase);
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++)
+              umma_f8_pair(tmem_base + buf * kF8PairCols, lo + 2 * k, lo + (kF8Box >> 4) + 2 * k, idesc, k > 0 ? 1u : 0u);
+            umma_commit_pair(empty_bar(s));
+            umma_commit_pair(acc_full(buf));
+          }
+          __syncwarp();
+          lo += kF8PairStage >> 4;
+          if (++s == kF8PairStages) { s = 0; phase ^= 1u; lo = lo0; }
+          aphase ^= buf;
+          buf ^= 1u;
+        }
+    }
+  } else {
+    // A warp's 128 columns: its half of the features; gated: 64 gate columns and the 64 up columns of the same features
+    const int quarter = warp & 3, half = (warp - 2) >> 2, r = quarter * 32 + lane;
+    const uint32_t empty0 = cluster_bar(acc_empty(0), 0), empty1 = cluster_bar(acc_empty(1), 0);
+    const uint32_t cols = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * (kGated ? 64 : 128);
+    const int blocks_n = (N + 127) / 128;
+    Scales<kGated ? 2 : 1> sc;
+    sc.xs = xs; sc.T = T; sc.end = num_kb;
+    auto aim = [&](int tile) {  // the scales of a tile, its first ones on their way
+      const int b = kGated ? tile_n(tile) : tile_n(tile) * 2 + half;
+      sc.t = tile < n_tiles ? tile_t0(tile) + r : T;
+      sc.ws[0] = tile < n_tiles && b < blocks_n ? ws + (size_t)b * num_kb : nullptr;
+      if (kGated) sc.ws[kGated ? 1 : 0] = tile < n_tiles ? ws + ((size_t)blocks_n + b) * num_kb : nullptr;
+      sc.fetch_x(0);
+      sc.fetch_w(0);
+    };
+    pdl_wait();
+    aim(pair);
+    uint32_t buf = 0, aphase = 0;
+    for (int tile = pair; tile < n_tiles; tile += pairs) {
+      uint64_t sums[64];
+#pragma unroll
+      for (int i = 0; i < 64; i++) sums[i] = 0;
+      for (int kb = 0; kb < num_kb; kb++) {
+        float f[kGated ? 2 : 1];
+        sc.get(0, kb, f);
+        mbar_wait_cluster(acc_full(buf), aphase);
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          uint32_t v[32];
+          tmem_ld_32x32(cols + buf * kF8PairCols + (kGated ? (c >> 1) * 128 + (c & 1) * 32 : c * 32), v);
+          tmem_ld_wait();
+          if (c == 3) {  // everything of this buffer is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(buf ? empty1 : empty0);
+          }
+          add_scaled(v, f[kGated ? c >> 1 : 0], sums + 16 * c);
+        }
+        aphase ^= buf;
+        buf ^= 1u;
+      }
+      aim(tile + pairs);
+      const int t = tile_t0(tile) + r, n0 = tile_n(tile) * kTileN + half * (kGated ? 64 : 128);
+      if (kGated) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+          const float2 g = pair_of(sums[i]), u = pair_of(sums[32 + i]);
+          const float a = n0 + 2 * i < N ? silu(g.x) * u.x : 0.f, b = n0 + 2 * i < N ? silu(g.y) * u.y : 0.f;  // (N is even)
+          top = max(top, max(f8_bits(a), f8_bits(b)));
+          asm("mov.b64 %0, {%1, %2};" : "=l"(sums[i]) : "f"(a), "f"(b));
+        }
+        // the token's other 64 features are a thread of the other half's: 64 threads of two warps meet
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(tops + (uint32_t)(r * 2 + half) * 4), "r"(top) : "memory");
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        uint32_t other;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(other) : "r"(tops + (uint32_t)(r * 2 + (half ^ 1)) * 4) : "memory");
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        const float s = f8_scale(max(top, other)), q = f8_inverse(s);
+        if (t < T) {
+          uint8_t *o = static_cast<uint8_t *>(out) + (size_t)t * N + n0;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {  // 16 features at a time: N is a multiple of 16
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const float2 a = pair_of(sums[8 * i + 2 * j]), b = pair_of(sums[8 * i + 2 * j + 1]);
+              w[j] = f8_pack4(a.x * q, a.y * q, b.x * q, b.y * q);
+            }
+            if (n0 + 16 * i < N) *reinterpret_cast<uint4 *>(o + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          if (half == 0) out_scale[(size_t)tile_n(tile) * T + t] = s;
+        }
+      } else if (t < T) {
+#pragma unroll
+        for (int c = 0; c < 8; c++) {  // 16 features at a time
+          const int n = n0 + 16 * c;
+          uint32_t v[16];
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float2 a = pair_of(sums[8 * c + i]);
+            v[2 * i] = __float_as_uint(a.x);
+            v[2 * i + 1] = __float_as_uint(a.y);
+          }
+          if (kOut == kF8OutF32) {
+            float *o = static_cast<float *>(out) + (size_t)t * N + n;
+            if (wide && n + 16 <= N) { st_32(o, v); st_32(o + 8, v + 8); }
+            else
+#pragma unroll
+              for (int i = 0; i < 16; i++)
+                if (n + i < N) o[i] = __uint_as_float(v[i]);
+          } else {
+            uint16_t *o = static_cast<uint16_t *>(out) + (size_t)t * N + n;
+            if (wide && n + 16 <= N) {
+              uint32_t p[8];
+#pragma unroll
+              for (int i = 0; i < 8; i++) p[i] = float2_to_bf16x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+              st_32(o, p);
+            } else
+#pragma unroll
+              for (int i = 0; i < 16; i++)
+                if (n + i < N) o[i] = float_to_bf16_bits(__uint_as_float(v[i]));
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other's MMAs, commits or arrivals may still reach it
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
+}
+
+constexpr int kF8MaxSmem = 227 * 1024;
+constexpr int kTileRest = 1024 + 256;  // alignment, barriers
+
+// How a tile kernel's work is laid out: tokens of a tile and CTAs of a cluster
+int tile_tokens(int T) { return T <= 32 ? 32 : T <= 64 ? 64 : 128; }
+int tile_split(int T, int N, int K, bool gated) {
+  const long long tiles = (long long)((N + 127) / 128) * ((T + tile_tokens(T) - 1) / tile_tokens(T));
+  const int num_kb = (K + kF8Block - 1) / kF8Block;
+  const long long room = (gated ? 1 : 2) * kNumSMs;  // resident CTAs
+  int s = (int)(room / tiles);
+  s = s > 8 ? 8 : s;
+  s = s > num_kb / 2 ? num_kb / 2 : s;
+  return s < 1 ? 1 : s;
+}
+
+template <bool kGated>
+cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int out_bf16, int T, int N,
+                        int K, int w_row0, int wide, cudaStream_t st) {
+  using Cfg = TileCfg<kGated>;
+  static DeviceOnce once;
+  DIS_CUDA_TRY(once.run([&] { return cudaFuncSetAttribute(gemm_f8_tile_kernel<kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8MaxSmem); }));
+  const int tile_t = tile_tokens(T), split = tile_split(T, N, K, kGated);
+  const int tiles_n = (N + 127) / 128, tiles_t = (T + tile_t - 1) / tile_t, rows = tile_t;
+  if (tiles_t > 65535) { set_last_error("gemm_f8: too many tokens"); return cudaErrorInvalidValue; }
+  const int per = ((K + kF8Block - 1) / kF8Block + split - 1) / split;  // blocks of a slice, at most
+  const bool two = !kGated && (long long)tiles_n * tiles_t * split > kNumSMs;
+  const int budget = two ? 112 * 1024 : 220 * 1024;
+  int stages = 2;
+  while (stages < per && stages < 12 && Cfg::body_bytes(stages + 1, tile_t, rows) + kTileRest <= budget) stages++;
+  const uint32_t bar_off = (uint32_t)Cfg::body_bytes(stages, tile_t, rows);
+  const int smem = (int)bar_off + kTileRest;
+  const int weights_first = !(pdl_enabled() && !pdl_weights_settled());
+  return launch_k_cluster(gemm_f8_tile_kernel<kGated>, dim3(tiles_n * split, tiles_t), dim3(kF8Threads), (size_t)smem, st, split,
+                          *reinterpret_cast<const CUtensorMap *>(&w_map), *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, out_bf16, T, N, K,
+                          w_row0, split, tile_t, stages, bar_off, weights_first, wide);
+}
+
+template <int kOut>
+cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int T, int N, int K,
+                           int w_row0, int wide, cudaStream_t st) {
+  static DeviceOnce once;
+  DIS_CUDA_TRY(once.run([&] { return cudaFuncSetAttribute(gemm_f8_pair_kernel<kOut>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8PairSmem); }));
+  const int feats = kOut == kF8OutGated ? 128 : 256;
+  const int tiles_n = (N + feats - 1) / feats, tiles_t = (T + 255) / 256;
+  const long long n_tiles = (long long)tiles_n * tiles_t;
+  if (n_tiles > (1 << 30)) { set_last_error("gemm_f8: too many tiles"); return cudaErrorInvalidValue; }
+  const int pairs = n_tiles < kNumSMs / 2 ? (int)n_tiles : kNumSMs / 2;
+  const int t_fast = (long long)(kOut == kF8OutGated ? 2 : 1) * N > (long long)T ? 1 : 0;  // as gemm_pair_kernel: the smaller operand stays in L2
+  return launch_k(gemm_f8_pair_kernel<kOut>, dim3(2 * pairs), dim3(kF8Threads), (size_t)kF8PairSmem, st, *reinterpret_cast<const CUtensorMap *>(&w_map),
+                  *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, T, N, K, w_row0, kOut == kF8OutGated ? N : 128, tiles_n, tiles_t, t_fast, wide);
+}
+
+}  // namespace
+
+bool gemm_f8_in_pairs(int T, int N, int K, bool gated) { return T > 256; }
+uint32_t gemm_f8_token_box(int T, int N, int K, bool gated) { return gemm_f8_in_pairs(T, N, K, gated) ? 128u : (uint32_t)tile_tokens(T); }
+
+// w_map: 128-row boxes over [..][K] e4m3, x_map: boxes of gemm_f8_token_box() rows
+cudaError_t launch_gemm_f8(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, bool bf16, int T, int N, int K, int w_row0,
+                           cudaStream_t st) {
+  if (T <= 0 || N <= 0) return cudaSuccess;
+  const uintptr_t at = (uintptr_t)out;
+  if (gemm_f8_in_pairs(T, N, K, false)) {
+    const int wide = (at & 31u) == 0 && N % (bf16 ? 16 : 8) == 0;  // every piece of a row starts on 32 bytes
+    return bf16 ? pair_f8_launch<kF8OutBf16>(w_map, x_map, xs, ws, out, nullptr, T, N, K, w_row0, wide, st)
+                : pair_f8_launch<kF8OutF32>(w_map, x_map, xs, ws, out, nullptr, T, N, K, w_row0, wide, st);
+  }
+  const int wide = N % 4 == 0 && (at & (bf16 ? 7u : 15u)) == 0;
+  return tile_launch<false>(w_map, x_map, xs, ws, out, nullptr, bf16 ? 1 : 0, T, N, K, w_row0, wide, st);
+}
+
+// h = silu(gate) * up in 8 bits; gate rows at w_row0, up rows at w_row0 + I; ws: the gate's blocks, then the up's
+cudaError_t launch_gemm_silu_f8(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, uint8_t *h8, float *hs, int T, int I, int K,
+                                int w_row0, cudaStream_t st) {
+  if (T <= 0 || I <= 0) return cudaSuccess;
+  if (gemm_f8_in_pairs(T, I, K, true)) return pair_f8_launch<kF8OutGated>(w_map, x_map, xs, ws, h8, hs, T, I, K, w_row0, 0, st);
+  return tile_launch<true>(w_map, x_map, xs, ws, h8, hs, 0, T, I, K, w_row0, 0, st);
+}
+
+}  // namespace dis

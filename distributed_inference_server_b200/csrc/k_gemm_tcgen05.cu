@@ -230,20 +230,27 @@ static EncodeTiledFn get_encode_fn() {
 
 static_assert(sizeof(TmaMap) == sizeof(CUtensorMap), "TmaMap must mirror CUtensorMap");
 
-cudaError_t make_tma_map_2d(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+// Rows of `cols` elements of `elem` bytes, boxes of box_rows rows of 128 bytes
+static cudaError_t make_map(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows, CUtensorMapDataType type, uint32_t elem) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) { set_last_error("cuTensorMapEncodeTiled is not available from this driver"); return cudaErrorNotSupported; }
-  if (cols % 8 != 0 || ((uintptr_t)base & 15u)) { set_last_error("TMA map: row length must be a multiple of 8 bf16 and base 16-byte aligned"); return cudaErrorInvalidValue; }
+  if (cols * elem % 16 != 0 || ((uintptr_t)base & 15u)) { set_last_error(elem == 2 ? "TMA map: row length must be a multiple of 8 bf16 and base 16-byte aligned" : "TMA map: row length must be a multiple of 16 bytes and base 16-byte aligned"); return cudaErrorInvalidValue; }
   if (box_rows == 0 || box_rows > 256) { set_last_error("TMA map: box rows must be 1..256"); return cudaErrorInvalidValue; }
   const cuuint64_t dims[2] = {cols, rows};
-  const cuuint64_t strides[1] = {cols * 2};
-  const cuuint32_t box[2] = {(cuuint32_t)kBK, box_rows};
+  const cuuint64_t strides[1] = {cols * elem};
+  const cuuint32_t box[2] = {128 / elem, box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = fn(reinterpret_cast<CUtensorMap *>(out), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base),
+  const CUresult r = fn(reinterpret_cast<CUtensorMap *>(out), type, 2, const_cast<void *>(base),
                         dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { set_last_error("cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r)); return cudaErrorInvalidValue; }
   return cudaSuccess;
+}
+cudaError_t make_tma_map_2d(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+  return make_map(out, base, rows, cols, box_rows, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2);
+}
+cudaError_t make_f8_map(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+  return make_map(out, base, rows, cols, box_rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
 }
 
 // UMMA N (token tile): 32 / 64 for decode batches (HBM-bound), 128 and 256 for prefill (the wider the token tile,

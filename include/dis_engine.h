@@ -449,6 +449,36 @@ DIS_API int dis_k_attn_shared(const uint16_t *q, const void *kv_pool, const floa
  * over 8-bit pages, and where there are more than 65535 kv heads or tiles of 128 query rows, every token goes by itself, in one kernel.  The result is the same
  * to rounding.  Needs no GPU. */
 DIS_API int dis_k_attn_shared_in_common(int32_t T, int32_t n_heads, int32_t n_kv, int32_t d, int32_t prefix, int32_t int8);
+/* ---- products in 8-bit floating point ------------------------------------------------------------- *
+ * Rows of activations [T][K] in 8 bits: e4m3 values x8 and one fp32 scale for each 128 entries, scale [ceil(K / 128)][T]; an entry stands for x8 s.
+ * What is written here has s = 2^ceil(log2(max|x| / 448)), not below 2^-126, and x8 = x / s rounded to the nearest value, ties to even; a block
+ * with an infinity or NaN has the scale NaN, and whatever takes it is NaN.  Weights [N][K] have one scale for each block of 128 x 128, scale
+ * [ceil(N / 128)][ceil(K / 128)], any fp32 number (as checkpoints hold them, or from dis_k_quant_weight_f8); a fused gate-up weight [2][I][K]
+ * has the gate's blocks, then the up's: 2 ceil(I / 128) rows of scales.  Sums are fp32: a block's 128 products by the tensor cores, their sums times both
+ * scales added by fp32 FMAs; results do not change from call to call.  K is a positive multiple of 16 (its last block may be shorter), I too; N and T
+ * are any.  Sizes that do not fit, null pointers and starts off the boundaries given are refused with DIS_ERR_INVALID_ARGUMENT before anything is
+ * launched.  8-bit rows and bf16 inputs start on 16 bytes.  T = 0 or N = 0 is a call without work. */
+
+/* bf16 rows [T][K] into 8 bits */
+DIS_API int dis_k_quant_f8(const uint16_t *x, uint8_t *x8, float *scale, int32_t T, int32_t K, void *stream);
+/* A bf16 weight [N][K] into 8 bits, blocks of 128 x 128 */
+DIS_API int dis_k_quant_weight_f8(const uint16_t *w, uint8_t *w8, float *scale, int32_t N, int32_t K, void *stream);
+/* dis_k_add_rmsnorm whose normed rows leave in 8 bits (from fp32, without a rounding to bf16 between).  H a multiple of 16, at most 51200; x, embed, the
+ * partial sums and their slices and gain start on 16 bytes.  With row_map, row t is made from row row_map[t] and x stays as it is. */
+DIS_API int dis_k_add_rmsnorm_f8(float *x, const uint32_t *tokens, const uint16_t *embed, const float *partial, int32_t n_partial,
+                                 int64_t partial_stride, const float *gain, uint8_t *x8, float *scale, const int32_t *row_map, int32_t T, int32_t H,
+                                 float eps, void *stream);
+/* out[t][n] = sum_k x[t][k] w[n][k]; out_dtype DIS_F32 or DIS_BF16 */
+DIS_API int dis_k_gemm_f8(const uint8_t *x8, const float *xs, const uint8_t *w8, const float *ws, void *out, int32_t out_dtype, int32_t T, int32_t N,
+                          int32_t K, void *stream);
+/* The gate-up product of a feed-forward block, h = silu(x Wgate^T) (x Wup^T), itself turned into 8 bits: h8 [T][I], hs [ceil(I / 128)][T] */
+DIS_API int dis_k_gemm_silu_f8(const uint8_t *x8, const float *xs, const uint8_t *wgu8, const float *wgus, uint8_t *h8, float *hs, int32_t T, int32_t I,
+                               int32_t K, void *stream);
+/* A whole feed-forward block in one call: x bf16 [T][H] into x8, xs; the gate-up product into h8, hs; out [T][H] = h Wdown^T, wd8 [H][I].  x8 [T][H], xs
+ * [ceil(H / 128)][T], h8 [T][I] and hs [ceil(I / 128)][T] are the caller's and hold what their names say afterwards. */
+DIS_API int dis_k_ffn_f8(const uint16_t *x, const uint8_t *wgu8, const float *wgus, const uint8_t *wd8, const float *wds, uint8_t *x8, float *xs,
+                         uint8_t *h8, float *hs, void *out, int32_t out_dtype, int32_t T, int32_t H, int32_t I, void *stream);
+
 /* Sampler over fp32 logits [T][V] (row stride ld): temperature 0 -> argmax, lowest index wins ties;
  * else nucleus sampling as oracle/llama_oracle.c states it.  out_tokens[T]; out_logprob[T] (may be NULL) receives
  * the chosen token's log-probability (see dis_engine_last_logprobs). */
