@@ -46,6 +46,10 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint32_t a_lo, uin
       ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kUmmaDescHi)
       : "memory");
 }
+// An arrival at a barrier of either CTA of the pair that publishes no memory: what it says, that tensor memory has been read, is ordered by the
+// fences of tcgen05.  (With release at cluster scope, and the waits with acquire, every block waited for the scales still on their way: the
+// pair kernel took 2.9 thousand clocks a block.)
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // Instruction descriptor: D = f32, A = B = e4m3, both K-major
 __host__ __device__ constexpr uint32_t f8_idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 
@@ -308,15 +312,23 @@ gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
 }
 
 // ------------------------------------------------------------------------------------------------ pair kernel
+// What bounds a block is the way of an accumulator: MMAs, commit, the sums' warps reading it, their arrival at the first CTA.  With two
+// buffers of 256 columns that way is longer than two blocks' MMAs; so a block's 256 columns are two products of 128, each with buffers and
+// warps of its own, and the way is that much shorter.  Half h takes rows [64 h, 64 h + 64) of each CTA's 128 feature rows: its columns
+// are 64 features of the first CTA's and 64 of the second's (gated: the gate and the up of the same 64 features).
+// Three warpgroups: warp 0 TMA, warp 1 MMA; warpgroups 1 and 2 a half's sums each, 128 columns a thread in registers, which the first
+// warpgroup leaves them (setmaxnreg).
+constexpr int kF8PairThreads = 384;
+constexpr int kF8PairRegs = 168, kF8PairRegsLow = 40, kF8PairRegsHigh = 232;  // at launch, of the first warpgroup, of the others
+static_assert(128 * kF8PairRegsLow + 256 * kF8PairRegsHigh <= kF8PairThreads * kF8PairRegs, "more registers than the block is launched with");
 constexpr int kF8PairStages = 6;
 constexpr int kF8PairStage = 2 * kF8Box;  // one CTA's 128 token rows and 128 feature rows of a block
 constexpr int kF8PairSmem = kF8PairStages * kF8PairStage + 1024 + 256 + 1024;
-constexpr int kF8PairCols = 256;
 
 enum { kF8OutF32 = 0, kF8OutBf16 = 1, kF8OutGated = 2 };
 
 template <int kOut>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8Threads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8PairThreads, 1)
 gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const float *__restrict__ xs,
                     const float *__restrict__ ws, void *__restrict__ out, float *__restrict__ out_scale, int T, int N, int K, int w_row0,
                     int w_row_step, int tiles_n, int tiles_t, int t_fast, int wide) {
@@ -325,11 +337,11 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bar_base = smem_base + kF8PairStages * kF8PairStage;
-  auto full_bar = [&](int s) { return bar_base + 8u * s; };                                  // (first CTA's are used)
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };                                        // (first CTA's are used)
   auto empty_bar = [&](int s) { return bar_base + 8u * (kF8PairStages + s); };
-  auto acc_full = [&](uint32_t b) { return bar_base + 8u * (2 * kF8PairStages + b); };
-  auto acc_empty = [&](uint32_t b) { return bar_base + 8u * (2 * kF8PairStages + 2 + b); };  // (first CTA's are used)
-  const uint32_t tmem_slot = bar_base + 8u * (2 * kF8PairStages + 4);
+  auto acc_full = [&](uint32_t h, uint32_t b) { return bar_base + 8u * (2 * kF8PairStages + 2 * b + h); };
+  auto acc_empty = [&](uint32_t h, uint32_t b) { return bar_base + 8u * (2 * kF8PairStages + 4 + 2 * b + h); };  // (first CTA's are used)
+  const uint32_t tmem_slot = bar_base + 8u * (2 * kF8PairStages + 8);
   const uint32_t tops = bar_base + 256u;  // [128 tokens][2 halves] largest magnitudes of a gated tile
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
@@ -345,7 +357,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
     tma_prefetch_desc(&w_map);
     tma_prefetch_desc(&x_map);
     for (int s = 0; s < kF8PairStages; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-    for (uint32_t b = 0; b < 2; b++) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 16); }  // 8 warps of each CTA
+    for (uint32_t b = 0; b < 2; b++)
+      for (uint32_t h = 0; h < 2; h++) { mbar_init(acc_full(h, b), 1); mbar_init(acc_empty(h, b), 8); }  // 4 warps of each CTA
     fence_barrier_init();
     fence_proxy_async();
   }
@@ -361,48 +374,52 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
   pdl_launch_dependents();
 
-  if (warp == 0) {
-    if (lane == 0) {
-      pdl_wait();
-      int s = 0;
-      uint32_t phase = 0;
-      for (int tile = pair; tile < n_tiles; tile += pairs) {
-        const int t0 = tile_t0(tile), wr = w_row0 + tile_n(tile) * kTileN + (int)rank * w_row_step;  // (gated: gate rows | up rows)
-        for (int kb = 0; kb < num_kb; kb++) {
-          mbar_wait(empty_bar(s), phase ^ 1u);  // passes on the first lap
-          if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kF8PairStage);
-          const uint32_t bar = cluster_bar(full_bar(s), 0), a = smem_base + s * kF8PairStage;
-          tma_load_2d_pair(a, &x_map, kb * kF8Block, t0, bar, x_hint);
-          tma_load_2d_pair(a + kF8Box, &w_map, kb * kF8Block, wr, bar, w_hint);
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8PairRegsLow));
+    if (warp == 0) {
+      if (lane == 0) {
+        pdl_wait();
+        int s = 0;
+        uint32_t phase = 0;
+        for (int tile = pair; tile < n_tiles; tile += pairs) {
+          const int t0 = tile_t0(tile), wr = w_row0 + tile_n(tile) * kTileN + (int)rank * w_row_step;  // (gated: gate rows | up rows)
+          for (int kb = 0; kb < num_kb; kb++) {
+            mbar_wait(empty_bar(s), phase ^ 1u);  // passes on the first lap
+            if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kF8PairStage);
+            const uint32_t bar = cluster_bar(full_bar(s), 0), a = smem_base + s * kF8PairStage;
+            tma_load_2d_pair(a, &x_map, kb * kF8Block, t0, bar, x_hint);
+            tma_load_2d_pair(a + kF8Box, &w_map, kb * kF8Block, wr, bar, w_hint);
+            if (++s == kF8PairStages) { s = 0; phase ^= 1u; }
+          }
+        }
+        // The first CTA's commits still arrive at this CTA's barriers: wait for the last of every stage before the CTA may end.
+        for (int i = 0; i < kF8PairStages; i++) {  // (a stage never filled passes at once)
+          mbar_wait(empty_bar(s), phase ^ 1u);
           if (++s == kF8PairStages) { s = 0; phase ^= 1u; }
         }
       }
-      // The first CTA's commits still arrive at this CTA's barriers: wait for the last of every stage before the CTA may end.
-      for (int i = 0; i < kF8PairStages; i++) {  // (a stage never filled passes at once)
-        mbar_wait(empty_bar(s), phase ^ 1u);
-        if (++s == kF8PairStages) { s = 0; phase ^= 1u; }
-      }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    if (rank == 0) {
-      constexpr uint32_t idesc = f8_idesc(256, kF8PairCols);
+      __syncwarp();
+    } else if (warp == 1 && rank == 0) {
+      constexpr uint32_t idesc = f8_idesc(256, 128);
       const uint32_t lo0 = umma_lo(smem_base);
       uint32_t lo = lo0, phase = 0, buf = 0, aphase = 0;
       int s = 0;
       for (int tile = pair; tile < n_tiles; tile += pairs)
         for (int kb = 0; kb < num_kb; kb++) {
-          mbar_wait_cluster(acc_empty(buf), aphase ^ 1u);  // both CTAs have taken this buffer (passes on first use)
-          mbar_wait_cluster(full_bar(s), phase);
-          tc_fence_after();
-          if (elect_one()) {
+          mbar_wait(full_bar(s), phase);
 #pragma unroll
-            for (uint32_t k = 0; k < 4; k++)
-              umma_f8_pair(tmem_base + buf * kF8PairCols, lo + 2 * k, lo + (kF8Box >> 4) + 2 * k, idesc, k > 0 ? 1u : 0u);
-            umma_commit_pair(empty_bar(s));
-            umma_commit_pair(acc_full(buf));
+          for (uint32_t h = 0; h < 2; h++) {
+            mbar_wait(acc_empty(h, buf), aphase ^ 1u);  // both CTAs have taken this buffer (passes on first use)
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (uint32_t k = 0; k < 4; k++)
+                umma_f8_pair(tmem_base + buf * 256u + h * 128u, lo + 2 * k, lo + ((kF8Box + h * (kF8Box / 2)) >> 4) + 2 * k, idesc, k > 0 ? 1u : 0u);
+              umma_commit_pair(acc_full(h, buf));
+              if (h == 1) umma_commit_pair(empty_bar(s));
+            }
+            __syncwarp();
           }
-          __syncwarp();
           lo += kF8PairStage >> 4;
           if (++s == kF8PairStages) { s = 0; phase ^= 1u; lo = lo0; }
           aphase ^= buf;
@@ -410,18 +427,19 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
         }
     }
   } else {
-    // A warp's 128 columns: its half of the features; gated: 64 gate columns and the 64 up columns of the same features
-    const int quarter = warp & 3, half = (warp - 2) >> 2, r = quarter * 32 + lane;
-    const uint32_t empty0 = cluster_bar(acc_empty(0), 0), empty1 = cluster_bar(acc_empty(1), 0);
-    const uint32_t cols = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * (kGated ? 64 : 128);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8PairRegsHigh));
+    const int quarter = warp & 3, half = (warp >> 2) - 1, r = quarter * 32 + lane;
+    const uint32_t empty0 = cluster_bar(acc_empty(half, 0), 0), empty1 = cluster_bar(acc_empty(half, 1), 0);
+    const uint32_t cols = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128u;
     const int blocks_n = (N + 127) / 128;
-    Scales<kGated ? 2 : 1> sc;
+    Scales<2> sc;  // of the first CTA's features and of the second's
     sc.xs = xs; sc.T = T; sc.end = num_kb;
     auto aim = [&](int tile) {  // the scales of a tile, its first ones on their way
-      const int b = kGated ? tile_n(tile) : tile_n(tile) * 2 + half;
-      sc.t = tile < n_tiles ? tile_t0(tile) + r : T;
-      sc.ws[0] = tile < n_tiles && b < blocks_n ? ws + (size_t)b * num_kb : nullptr;
-      if (kGated) sc.ws[kGated ? 1 : 0] = tile < n_tiles ? ws + ((size_t)blocks_n + b) * num_kb : nullptr;
+      const bool any = tile < n_tiles;
+      const int b = tile_n(tile) * (kTileN / 128), b2 = kGated ? blocks_n + b : b + 1;
+      sc.t = any ? tile_t0(tile) + r : T;
+      sc.ws[0] = any ? ws + (size_t)b * num_kb : nullptr;
+      sc.ws[1] = any && (kGated || b2 < blocks_n) ? ws + (size_t)b2 * num_kb : nullptr;
       sc.fetch_x(0);
       sc.fetch_w(0);
     };
@@ -433,27 +451,28 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
 #pragma unroll
       for (int i = 0; i < 64; i++) sums[i] = 0;
       for (int kb = 0; kb < num_kb; kb++) {
-        float f[kGated ? 2 : 1];
+        float f[2];
         sc.get(0, kb, f);
-        mbar_wait_cluster(acc_full(buf), aphase);
+        mbar_wait(acc_full(half, buf), aphase);
         tc_fence_after();
+        uint32_t v[2][32];
+        tmem_ld_32x32(cols + buf * 256u, v[0]);
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-          uint32_t v[32];
-          tmem_ld_32x32(cols + buf * kF8PairCols + (kGated ? (c >> 1) * 128 + (c & 1) * 32 : c * 32), v);
           tmem_ld_wait();
-          if (c == 3) {  // everything of this buffer is in registers
+          if (c < 3) tmem_ld_32x32(cols + buf * 256u + 32 * (c + 1), v[(c + 1) & 1]);
+          else {  // everything of this buffer is in registers
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(buf ? empty1 : empty0);
+            if (lane == 0) mbar_arrive_at(buf ? empty1 : empty0);
           }
-          add_scaled(v, f[kGated ? c >> 1 : 0], sums + 16 * c);
+          add_scaled(v[c & 1], f[c >> 1], sums + 16 * c);
         }
         aphase ^= buf;
         buf ^= 1u;
       }
       aim(tile + pairs);
-      const int t = tile_t0(tile) + r, n0 = tile_n(tile) * kTileN + half * (kGated ? 64 : 128);
+      const int t = tile_t0(tile) + r, n0 = tile_n(tile) * kTileN + half * 64;
       if (kGated) {
         uint32_t top = 0;
 #pragma unroll
@@ -486,8 +505,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
         }
       } else if (t < T) {
 #pragma unroll
-        for (int c = 0; c < 8; c++) {  // 16 features at a time
-          const int n = n0 + 16 * c;
+        for (int c = 0; c < 8; c++) {  // 16 features at a time: four times of the first CTA's, four of the second's
+          const int n = n0 + 16 * c + (c >= 4 ? 64 : 0);
           uint32_t v[16];
 #pragma unroll
           for (int i = 0; i < 8; i++) {
@@ -565,14 +584,20 @@ template <int kOut>
 cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int T, int N, int K,
                            int w_row0, int wide, cudaStream_t st) {
   static DeviceOnce once;
-  DIS_CUDA_TRY(once.run([&] { return cudaFuncSetAttribute(gemm_f8_pair_kernel<kOut>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8PairSmem); }));
+  DIS_CUDA_TRY(once.run([&] {
+    // a block launched with fewer registers would wait for those that its warpgroups ask for
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, gemm_f8_pair_kernel<kOut>);
+    if (e == cudaSuccess && at.numRegs != kF8PairRegs) e = cudaErrorInvalidKernelImage;
+    return e == cudaSuccess ? cudaFuncSetAttribute(gemm_f8_pair_kernel<kOut>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8PairSmem) : e;
+  }));
   const int feats = kOut == kF8OutGated ? 128 : 256;
   const int tiles_n = (N + feats - 1) / feats, tiles_t = (T + 255) / 256;
   const long long n_tiles = (long long)tiles_n * tiles_t;
   if (n_tiles > (1 << 30)) { set_last_error("gemm_f8: too many tiles"); return cudaErrorInvalidValue; }
   const int pairs = n_tiles < kNumSMs / 2 ? (int)n_tiles : kNumSMs / 2;
   const int t_fast = (long long)(kOut == kF8OutGated ? 2 : 1) * N > (long long)T ? 1 : 0;  // as gemm_pair_kernel: the smaller operand stays in L2
-  return launch_k(gemm_f8_pair_kernel<kOut>, dim3(2 * pairs), dim3(kF8Threads), (size_t)kF8PairSmem, st, *reinterpret_cast<const CUtensorMap *>(&w_map),
+  return launch_k(gemm_f8_pair_kernel<kOut>, dim3(2 * pairs), dim3(kF8PairThreads), (size_t)kF8PairSmem, st, *reinterpret_cast<const CUtensorMap *>(&w_map),
                   *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, T, N, K, w_row0, kOut == kF8OutGated ? N : 128, tiles_n, tiles_t, t_fast, wide);
 }
 
