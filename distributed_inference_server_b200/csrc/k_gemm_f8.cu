@@ -53,12 +53,13 @@ __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) { asm volatile("mba
 // Instruction descriptor: D = f32, A = B = e4m3, both K-major
 __host__ __device__ constexpr uint32_t f8_idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 
-// sums += factor * (32 columns of tensor memory)
-__device__ __forceinline__ void add_scaled(const uint32_t (&v)[32], float factor, uint64_t *sums) {
+// sums += factor * (kCols columns of tensor memory)
+template <int kCols>
+__device__ __forceinline__ void add_scaled(const uint32_t (&v)[kCols], float factor, uint64_t *sums) {
   uint64_t f;
   asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "f"(factor));
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
+  for (int i = 0; i < kCols / 2; i++) {
     uint64_t p;
     asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(v[2 * i]), "r"(v[2 * i + 1]));
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sums[i]) : "l"(p), "l"(f));
@@ -105,6 +106,91 @@ struct Scales {
 };
 
 __device__ __forceinline__ float silu(float g) { return gate_act_fast(0, g); }
+
+// ------------------------------------------------------------------------------------------------ the end of a tile
+// What the CTAs of a cluster that share a tile's K have in common: sums of 128 or 256 columns per token, rows of kLd floats in each CTA's shared
+// memory.  Token rows first, first + step, ... are finished here: the slices' sums are added in order (the same result at every call), a
+// warp a token, four columns (and the four that lie 128 behind) a lane, four tokens at once: one token's way through loads, activation,
+// maximum and stores takes half a microsecond and they have to overlap.
+//   plain, 128 columns     features n0 + [0, 128)
+//   plain, 256 columns     features n0 + [0, 256)
+//   gated, 256 columns     gate and up of features n0 + [0, 128)
+struct TileOut {
+  void *out;
+  float *scale;   // gated: of the rows in 8 bits
+  int T, N, t0, n0, wide, bf16;
+};
+__device__ __forceinline__ void ld_peer4(float (&v)[4], uint32_t at) {
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void store4(const TileOut &o, int t, int n, const float (&v)[4]) {
+  if (o.bf16) {
+    uint16_t *p = static_cast<uint16_t *>(o.out) + (size_t)t * o.N + n;
+    if (o.wide && n < o.N) *reinterpret_cast<uint2 *>(p) = make_uint2(float2_to_bf16x2(v[0], v[1]), float2_to_bf16x2(v[2], v[3]));
+    else
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (n + i < o.N) p[i] = float_to_bf16_bits(v[i]);
+  } else {
+    float *p = static_cast<float *>(o.out) + (size_t)t * o.N + n;
+    if (o.wide && n < o.N) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (n + i < o.N) p[i] = v[i];
+  }
+}
+// peer0, peer_step: cluster ranks of the CTAs that hold the slices
+template <bool kGated, int kCols, int kLd>
+__device__ __forceinline__ void finish_tokens(uint32_t base, int rows, int first, int step, int split, int peer0, int peer_step, const TileOut &o) {
+  const int lane = threadIdx.x & 31;
+  for (int r0 = first; r0 < rows; r0 += 4 * step) {
+    float a[4][4], b[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) a[j][i] = b[j][i] = 0.f;
+    for (int p = 0; p < split; p++) {
+      const uint32_t from = (split > 1 ? cluster_bar(base, (uint32_t)(peer0 + p * peer_step)) : base) + (uint32_t)lane * 16u;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (r0 + j * step < rows) {
+          float v[4], u[4];
+          const uint32_t at = from + (uint32_t)((r0 + j * step) * kLd) * 4u;
+          ld_peer4(v, at);
+          if (kCols == 256) ld_peer4(u, at + 512u);
+#pragma unroll
+          for (int i = 0; i < 4; i++) { a[j][i] += v[i]; if (kCols == 256) b[j][i] += u[i]; }
+        }
+    }
+    const int n = o.n0 + lane * 4;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int t = o.t0 + r0 + j * step;
+      if (r0 + j * step >= rows) break;
+      if (kGated) {  // N features are a multiple of 16: a lane's four are all there or none
+#pragma unroll
+        for (int i = 0; i < 4; i++) a[j][i] = n < o.N ? silu(a[j][i]) * b[j][i] : 0.f;
+        const float s = f8_scale(__reduce_max_sync(0xffffffffu, f8_top4(a[j][0], a[j][1], a[j][2], a[j][3]))), q = f8_inverse(s);
+        if (n < o.N) *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(o.out) + (size_t)t * o.N + n) = f8_pack4(a[j][0] * q, a[j][1] * q, a[j][2] * q, a[j][3] * q);
+        if (lane == 0) o.scale[(size_t)(o.n0 / kF8Block) * o.T + t] = s;
+      } else {
+        store4(o, t, n, a[j]);
+        if (kCols == 256) store4(o, t, n + 128, b[j]);
+      }
+    }
+  }
+}
+// A thread's sums to its token's row: 64 columns from col on (sums: 32 pairs)
+__device__ __forceinline__ void put_sums(uint32_t row, int col, const uint64_t *sums) {
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const float2 a = pair_of(sums[2 * i]), b = pair_of(sums[2 * i + 1]);
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(row + (uint32_t)(col + 4 * i) * 4u), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y) : "memory");
+  }
+}
+// A cluster barrier that publishes nothing: reads of other CTAs' shared memory are over.  (With release it waits for the stores to global memory too, a microsecond.)
+__device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------------------ tile kernel
 // The ring's stages, then the barriers.  kGated: 128 gate rows and 128 up rows per stage, 256 accumulator columns; else 128 of each.
@@ -232,32 +318,27 @@ gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
       sc.get(kb0, kb - kb0, f);
       mbar_wait(acc_full(buf), aphase);
       tc_fence_after();
+      constexpr int CH = 16, kChunks = Cfg::kCols / 2 / CH;  // (32 columns at a time cost registers that two CTAs an SM do not have)
 #pragma unroll
-      for (int c = 0; c < (kGated ? 4 : 2); c++) {
-        uint32_t v[32];
-        tmem_ld_32x32(cols + buf * Cfg::kCols + (c >> 1) * 128 + (c & 1) * 32, v);
+      for (int c = 0; c < kChunks; c++) {
+        uint32_t v[CH];
+        tmem_ld_cols(cols + buf * Cfg::kCols + (c * CH / 64) * 128 + c * CH % 64, v);
         tmem_ld_wait();
-        if (c == (kGated ? 3 : 1)) {  // everything of this buffer is in registers
+        if (c == kChunks - 1) {  // everything of this buffer is in registers
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(acc_empty(buf));
         }
-        add_scaled(v, f[kGated ? c >> 1 : 0], sums + 16 * c);
+        add_scaled(v, f[kGated ? c * CH / 64 : 0], sums + CH / 2 * c);
       }
       aphase ^= buf;
       buf ^= 1u;
     }
     // The last MMAs have read the ring: the tokens' sums take its place
     if (r < rows) {
-#pragma unroll
-      for (int c = 0; c < (kGated ? 2 : 1); c++) {
-        const uint32_t at = smem_base + (uint32_t)(r * Cfg::kLd + c * 128 + half * 64) * 4;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const float2 a = pair_of(sums[32 * c + 2 * i]), b = pair_of(sums[32 * c + 2 * i + 1]);
-          asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + 16 * i), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y) : "memory");
-        }
-      }
+      const uint32_t row = smem_base + (uint32_t)(r * Cfg::kLd) * 4u;
+      put_sums(row, half * 64, sums);
+      if (kGated) put_sums(row, 128 + half * 64, sums + (kGated ? 32 : 0));
     }
     __syncwarp();
   }
@@ -267,48 +348,10 @@ gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   if (warp == 1) tmem_dealloc<Cfg::kTmem>(tmem_base);
   pdl_wait();  // (not all warps have been there, and all write)
 
-  // ===== every CTA of the cluster finishes a share of the tokens: a warp a token, four columns a lane, all slices' sums in order
-  for (int r = slice + split * warp; r < rows; r += split * (kF8Threads / 32)) {
-    float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-    const uint32_t at = smem_base + (uint32_t)(r * Cfg::kLd + lane * 4) * 4;
-#pragma unroll 4
-    for (int p = 0; p < split; p++) {
-      uint32_t from = at;
-      if (split > 1) from = cluster_bar(at, (uint32_t)p);  // (a plain shared address is this CTA's own)
-      float a[4];
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]) : "r"(from) : "memory");
-#pragma unroll
-      for (int i = 0; i < 4; i++) g[i] += a[i];
-      if (kGated) {
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]) : "r"(from + 512u) : "memory");
-#pragma unroll
-        for (int i = 0; i < 4; i++) u[i] += a[i];
-      }
-    }
-    const int n = n0 + lane * 4, t = t0 + r;
-    if (kGated) {  // N features are a multiple of 16: a lane's four are all there or none
-#pragma unroll
-      for (int i = 0; i < 4; i++) g[i] = n < N ? silu(g[i]) * u[i] : 0.f;
-      const float s = f8_scale(__reduce_max_sync(0xffffffffu, f8_top4(g[0], g[1], g[2], g[3]))), q = f8_inverse(s);
-      if (n < N) *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(out) + (size_t)t * N + n) = f8_pack4(g[0] * q, g[1] * q, g[2] * q, g[3] * q);
-      if (lane == 0) out_scale[(size_t)tile * T + t] = s;
-    } else if (out_bf16) {
-      uint16_t *o = static_cast<uint16_t *>(out) + (size_t)t * N + n;
-      if (wide && n < N) *reinterpret_cast<uint2 *>(o) = make_uint2(float2_to_bf16x2(g[0], g[1]), float2_to_bf16x2(g[2], g[3]));
-      else
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (n + i < N) o[i] = float_to_bf16_bits(g[i]);
-    } else {
-      float *o = static_cast<float *>(out) + (size_t)t * N + n;
-      if (wide && n < N) *reinterpret_cast<float4 *>(o) = make_float4(g[0], g[1], g[2], g[3]);
-      else
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (n + i < N) o[i] = g[i];
-    }
-  }
-  if (split > 1) cluster_sync();  // no CTA leaves while another reads its sums
+  // every CTA of the cluster finishes a share of the tokens
+  const TileOut o{out, out_scale, T, N, t0, n0, wide, out_bf16};
+  finish_tokens<kGated, Cfg::kCols, Cfg::kLd>(smem_base, rows, slice + split * warp, split * (kF8Threads / 32), split, 0, 1, o);
+  if (split > 1) cluster_meet();  // no CTA leaves while another reads its sums
 }
 
 // ------------------------------------------------------------------------------------------------ pair kernel
@@ -323,15 +366,19 @@ constexpr int kF8PairRegs = 168, kF8PairRegsLow = 40, kF8PairRegsHigh = 232;  //
 static_assert(128 * kF8PairRegsLow + 256 * kF8PairRegsHigh <= kF8PairThreads * kF8PairRegs, "more registers than the block is launched with");
 constexpr int kF8PairStages = 6;
 constexpr int kF8PairStage = 2 * kF8Box;  // one CTA's 128 token rows and 128 feature rows of a block
+constexpr int kF8PairLd = 260;              // floats of a token's row of sums in shared memory
+static_assert(128 * kF8PairLd * 4 <= kF8PairStages * kF8PairStage, "the sums take the ring's place");
 constexpr int kF8PairSmem = kF8PairStages * kF8PairStage + 1024 + 256 + 1024;
 
 enum { kF8OutF32 = 0, kF8OutBf16 = 1, kF8OutGated = 2 };
 
-template <int kOut>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8PairThreads, 1)
+// kSplit: a cluster of several pairs has one tile and shares its K; else the pairs walk the tiles
+template <int kOut, bool kSplit>
+__global__ void __launch_bounds__(kF8PairThreads, 1)
 gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const float *__restrict__ xs,
                     const float *__restrict__ ws, void *__restrict__ out, float *__restrict__ out_scale, int T, int N, int K, int w_row0,
-                    int w_row_step, int tiles_n, int tiles_t, int t_fast, int wide) {
+                    int w_row_step, int tiles_n, int tiles_t, int t_fast, int n_split, int wide) {
+  const int split = kSplit ? n_split : 1;
   constexpr bool kGated = kOut == kF8OutGated;
   constexpr int kTileN = kGated ? 128 : 256;
   extern __shared__ uint8_t smem_raw[];
@@ -345,10 +392,13 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   const uint32_t tops = bar_base + 256u;  // [128 tokens][2 halves] largest magnitudes of a gated tile
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  uint32_t rank;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
-  const int num_kb = (K + kF8Block - 1) / kF8Block, n_tiles = tiles_n * tiles_t;
+  uint32_t cta;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
+  const uint32_t rank = cta & 1u, leader = cta & ~1u, slice = cta >> 1;  // of the pair; its first CTA; the pair's share of K
+  const int n_tiles = tiles_n * tiles_t, num_kb = (K + kF8Block - 1) / kF8Block;
+  const int kb0 = (int)((long long)num_kb * slice / split), kb1 = (int)((long long)num_kb * (slice + 1) / split);
+  // one slice: the pairs walk the tiles; several: a cluster has one tile
+  const int pair = ((int)blockIdx.x >> 1) / split, pairs = kSplit ? n_tiles : (int)gridDim.x >> 1;
   auto tile_n = [&](int tile) { return t_fast ? tile / tiles_t : tile % tiles_n; };
   auto tile_t0 = [&](int tile) { return (t_fast ? tile % tiles_t : tile / tiles_n) * 256 + (int)rank * 128; };
   const uint64_t w_hint = t_fast ? kEvictFirst : kEvictLast, x_hint = t_fast ? kEvictLast : kEvictFirst;
@@ -383,10 +433,10 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
         uint32_t phase = 0;
         for (int tile = pair; tile < n_tiles; tile += pairs) {
           const int t0 = tile_t0(tile), wr = w_row0 + tile_n(tile) * kTileN + (int)rank * w_row_step;  // (gated: gate rows | up rows)
-          for (int kb = 0; kb < num_kb; kb++) {
+          for (int kb = kb0; kb < kb1; kb++) {
             mbar_wait(empty_bar(s), phase ^ 1u);  // passes on the first lap
             if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kF8PairStage);
-            const uint32_t bar = cluster_bar(full_bar(s), 0), a = smem_base + s * kF8PairStage;
+            const uint32_t bar = cluster_bar(full_bar(s), leader), a = smem_base + s * kF8PairStage;
             tma_load_2d_pair(a, &x_map, kb * kF8Block, t0, bar, x_hint);
             tma_load_2d_pair(a + kF8Box, &w_map, kb * kF8Block, wr, bar, w_hint);
             if (++s == kF8PairStages) { s = 0; phase ^= 1u; }
@@ -405,7 +455,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
       uint32_t lo = lo0, phase = 0, buf = 0, aphase = 0;
       int s = 0;
       for (int tile = pair; tile < n_tiles; tile += pairs)
-        for (int kb = 0; kb < num_kb; kb++) {
+        for (int kb = kb0; kb < kb1; kb++) {
           mbar_wait(full_bar(s), phase);
 #pragma unroll
           for (uint32_t h = 0; h < 2; h++) {
@@ -415,8 +465,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
 #pragma unroll
               for (uint32_t k = 0; k < 4; k++)
                 umma_f8_pair(tmem_base + buf * 256u + h * 128u, lo + 2 * k, lo + ((kF8Box + h * (kF8Box / 2)) >> 4) + 2 * k, idesc, k > 0 ? 1u : 0u);
-              umma_commit_pair(acc_full(h, buf));
-              if (h == 1) umma_commit_pair(empty_bar(s));
+              umma_commit_pair(acc_full(h, buf), leader);
+              if (h == 1) umma_commit_pair(empty_bar(s), leader);
             }
             __syncwarp();
           }
@@ -426,22 +476,23 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
           buf ^= 1u;
         }
     }
+    if (kSplit) { tc_fence_before(); __syncwarp(); cluster_sync(); }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8PairRegsHigh));
     const int quarter = warp & 3, half = (warp >> 2) - 1, r = quarter * 32 + lane;
-    const uint32_t empty0 = cluster_bar(acc_empty(half, 0), 0), empty1 = cluster_bar(acc_empty(half, 1), 0);
+    const uint32_t empty0 = cluster_bar(acc_empty(half, 0), leader), empty1 = cluster_bar(acc_empty(half, 1), leader);
     const uint32_t cols = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128u;
     const int blocks_n = (N + 127) / 128;
     Scales<2> sc;  // of the first CTA's features and of the second's
-    sc.xs = xs; sc.T = T; sc.end = num_kb;
+    sc.xs = xs; sc.T = T; sc.end = kb1;
     auto aim = [&](int tile) {  // the scales of a tile, its first ones on their way
       const bool any = tile < n_tiles;
       const int b = tile_n(tile) * (kTileN / 128), b2 = kGated ? blocks_n + b : b + 1;
       sc.t = any ? tile_t0(tile) + r : T;
       sc.ws[0] = any ? ws + (size_t)b * num_kb : nullptr;
       sc.ws[1] = any && (kGated || b2 < blocks_n) ? ws + (size_t)b2 * num_kb : nullptr;
-      sc.fetch_x(0);
-      sc.fetch_w(0);
+      sc.fetch_x(kb0);
+      sc.fetch_w(kb0);
     };
     pdl_wait();
     aim(pair);
@@ -450,26 +501,41 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
       uint64_t sums[64];
 #pragma unroll
       for (int i = 0; i < 64; i++) sums[i] = 0;
-      for (int kb = 0; kb < num_kb; kb++) {
+      for (int kb = kb0; kb < kb1; kb++) {
         float f[2];
-        sc.get(0, kb, f);
+        sc.get(kb0, kb - kb0, f);
         mbar_wait(acc_full(half, buf), aphase);
         tc_fence_after();
         uint32_t v[2][32];
-        tmem_ld_32x32(cols + buf * 256u, v[0]);
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          tmem_ld_wait();
-          if (c < 3) tmem_ld_32x32(cols + buf * 256u + 32 * (c + 1), v[(c + 1) & 1]);
-          else {  // everything of this buffer is in registers
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_at(buf ? empty1 : empty0);
-          }
-          add_scaled(v[c & 1], f[c >> 1], sums + 16 * c);
-        }
+        const uint32_t at = cols + buf * 256u;
+        tmem_ld_32x32(at, v[0]);
+        tmem_ld_32x32(at + 32u, v[1]);
+        tmem_ld_wait();
+        add_scaled(v[0], f[0], sums);
+        tmem_ld_32x32(at + 64u, v[0]);
+        add_scaled(v[1], f[0], sums + 16);
+        tmem_ld_32x32(at + 96u, v[1]);
+        tmem_ld_wait();
+        tc_fence_before();  // everything of this buffer is in registers
+        __syncwarp();
+        if (lane == 0) mbar_arrive_at(buf ? empty1 : empty0);
+        add_scaled(v[0], f[1], sums + 32);
+        add_scaled(v[1], f[1], sums + 48);
         aphase ^= buf;
         buf ^= 1u;
+      }
+      if (kSplit) {
+        // The ring is free once both halves' last MMAs have read it.  Every CTA finishes its share of its 128 tokens.
+        asm volatile("bar.sync 5, 256;" ::: "memory");
+        const uint32_t row = smem_base + (uint32_t)(r * kF8PairLd) * 4u;
+        put_sums(row, half * 64, sums);
+        put_sums(row, 128 + half * 64, sums + 32);
+        tc_fence_before();
+        cluster_sync();
+        const int t0 = tile_t0(tile);
+        const TileOut o{out, out_scale, T, N, t0, tile_n(tile) * kTileN, (wide >> 1) & 1, kOut == kF8OutBf16};
+        finish_tokens<kGated, 256, kF8PairLd>(smem_base, min(128, T - t0), (int)slice + split * (warp - 4), split * 8, split, (int)rank, 2, o);
+        break;
       }
       aim(tile + pairs);
       const int t = tile_t0(tile) + r, n0 = tile_n(tile) * kTileN + half * 64;
@@ -516,14 +582,14 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
           }
           if (kOut == kF8OutF32) {
             float *o = static_cast<float *>(out) + (size_t)t * N + n;
-            if (wide && n + 16 <= N) { st_32(o, v); st_32(o + 8, v + 8); }
+            if ((wide & 1) && n + 16 <= N) { st_32(o, v); st_32(o + 8, v + 8); }
             else
 #pragma unroll
               for (int i = 0; i < 16; i++)
                 if (n + i < N) o[i] = __uint_as_float(v[i]);
           } else {
             uint16_t *o = static_cast<uint16_t *>(out) + (size_t)t * N + n;
-            if (wide && n + 16 <= N) {
+            if ((wide & 1) && n + 16 <= N) {
               uint32_t p[8];
 #pragma unroll
               for (int i = 0; i < 8; i++) p[i] = float2_to_bf16x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
@@ -539,7 +605,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // neither CTA leaves while the other's MMAs, commits or arrivals may still reach it
+  cluster_meet();  // no CTA leaves while another's MMAs, commits or arrivals may still reach it, or another reads its sums
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
 }
 
@@ -569,7 +635,7 @@ cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *x
   if (tiles_t > 65535) { set_last_error("gemm_f8: too many tokens"); return cudaErrorInvalidValue; }
   const int per = ((K + kF8Block - 1) / kF8Block + split - 1) / split;  // blocks of a slice, at most
   const bool two = !kGated && (long long)tiles_n * tiles_t * split > kNumSMs;
-  const int budget = two ? 112 * 1024 : 220 * 1024;
+  const int budget = two ? 92 * 1024 : 220 * 1024;
   int stages = 2;
   while (stages < per && stages < 12 && Cfg::body_bytes(stages + 1, tile_t, rows) + kTileRest <= budget) stages++;
   const uint32_t bar_off = (uint32_t)Cfg::body_bytes(stages, tile_t, rows);
@@ -580,25 +646,42 @@ cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *x
                           w_row0, split, tile_t, stages, bar_off, weights_first, wide);
 }
 
-template <int kOut>
-cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int T, int N, int K,
-                           int w_row0, int wide, cudaStream_t st) {
+// Pairs that share a tile's K: where the tiles are few, as many as fit at once (clusters of up to 8 CTAs, an SM each)
+int pair_split(int T, int N, int K, bool gated) {
+  const int feats = gated ? 128 : 256, num_kb = (K + kF8Block - 1) / kF8Block;
+  const long long tiles = (long long)((N + feats - 1) / feats) * ((T + 255) / 256);
+  int s = 1;
+  while (s < 4 && tiles * s * 2 <= (s == 1 ? 70 : 64) && num_kb >= 8 * s) s *= 2;
+  return s;
+}
+
+template <int kOut, bool kSplit>
+cudaError_t pair_f8_launch_as(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int T, int N, int K,
+                           int w_row0, int wide, int split, cudaStream_t st) {
   static DeviceOnce once;
   DIS_CUDA_TRY(once.run([&] {
     // a block launched with fewer registers would wait for those that its warpgroups ask for
     cudaFuncAttributes at;
-    cudaError_t e = cudaFuncGetAttributes(&at, gemm_f8_pair_kernel<kOut>);
+    cudaError_t e = cudaFuncGetAttributes(&at, gemm_f8_pair_kernel<kOut, kSplit>);
     if (e == cudaSuccess && at.numRegs != kF8PairRegs) e = cudaErrorInvalidKernelImage;
-    return e == cudaSuccess ? cudaFuncSetAttribute(gemm_f8_pair_kernel<kOut>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8PairSmem) : e;
+    return e == cudaSuccess ? cudaFuncSetAttribute(gemm_f8_pair_kernel<kOut, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8PairSmem) : e;
   }));
   const int feats = kOut == kF8OutGated ? 128 : 256;
   const int tiles_n = (N + feats - 1) / feats, tiles_t = (T + 255) / 256;
   const long long n_tiles = (long long)tiles_n * tiles_t;
   if (n_tiles > (1 << 30)) { set_last_error("gemm_f8: too many tiles"); return cudaErrorInvalidValue; }
-  const int pairs = n_tiles < kNumSMs / 2 ? (int)n_tiles : kNumSMs / 2;
+  const int pairs = kSplit ? (int)n_tiles * split : n_tiles < kNumSMs / 2 ? (int)n_tiles : kNumSMs / 2;
   const int t_fast = (long long)(kOut == kF8OutGated ? 2 : 1) * N > (long long)T ? 1 : 0;  // as gemm_pair_kernel: the smaller operand stays in L2
-  return launch_k(gemm_f8_pair_kernel<kOut>, dim3(2 * pairs), dim3(kF8PairThreads), (size_t)kF8PairSmem, st, *reinterpret_cast<const CUtensorMap *>(&w_map),
-                  *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, T, N, K, w_row0, kOut == kF8OutGated ? N : 128, tiles_n, tiles_t, t_fast, wide);
+  return launch_k_cluster(gemm_f8_pair_kernel<kOut, kSplit>, dim3(2 * pairs), dim3(kF8PairThreads), (size_t)kF8PairSmem, st, 2 * split, *reinterpret_cast<const CUtensorMap *>(&w_map),
+                  *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, T, N, K, w_row0, kOut == kF8OutGated ? N : 128, tiles_n, tiles_t, t_fast, split, wide);
+}
+
+template <int kOut>
+cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int T, int N, int K,
+                           int w_row0, int wide, cudaStream_t st) {
+  const int split = pair_split(T, N, K, kOut == kF8OutGated);
+  return split > 1 ? pair_f8_launch_as<kOut, true>(w_map, x_map, xs, ws, out, out_scale, T, N, K, w_row0, wide, split, st)
+                   : pair_f8_launch_as<kOut, false>(w_map, x_map, xs, ws, out, out_scale, T, N, K, w_row0, wide, 1, st);
 }
 
 }  // namespace
@@ -612,7 +695,8 @@ cudaError_t launch_gemm_f8(const TmaMap &w_map, const TmaMap &x_map, const float
   if (T <= 0 || N <= 0) return cudaSuccess;
   const uintptr_t at = (uintptr_t)out;
   if (gemm_f8_in_pairs(T, N, K, false)) {
-    const int wide = (at & 31u) == 0 && N % (bf16 ? 16 : 8) == 0;  // every piece of a row starts on 32 bytes
+    // every piece of a row starts on 32 bytes; on four elements
+    const int wide = ((at & 31u) == 0 && N % (bf16 ? 16 : 8) == 0 ? 1 : 0) | (N % 4 == 0 && (at & (bf16 ? 7u : 15u)) == 0 ? 2 : 0);
     return bf16 ? pair_f8_launch<kF8OutBf16>(w_map, x_map, xs, ws, out, nullptr, T, N, K, w_row0, wide, st)
                 : pair_f8_launch<kF8OutF32>(w_map, x_map, xs, ws, out, nullptr, T, N, K, w_row0, wide, st);
   }
