@@ -108,13 +108,12 @@ struct Scales {
 __device__ __forceinline__ float silu(float g) { return gate_act_fast(0, g); }
 
 // ------------------------------------------------------------------------------------------------ the end of a tile
-// What the CTAs of a cluster that share a tile's K have in common: sums of 128 or 256 columns per token, rows of kLd floats in each CTA's shared
+// What the CTAs of a cluster that share a tile's K have in common: sums of a tile's columns per token, rows of kLd floats in each CTA's shared
 // memory.  Token rows first, first + step, ... are finished here: the slices' sums are added in order (the same result at every call), a
-// warp a token, four columns (and the four that lie 128 behind) a lane, four tokens at once: one token's way through loads, activation,
+// warp a token, four columns (gated: and the four that lie 128 behind) a lane, four tokens at once: one token's way through loads, activation,
 // maximum and stores takes half a microsecond and they have to overlap.
-//   plain, 128 columns     features n0 + [0, 128)
-//   plain, 256 columns     features n0 + [0, 256)
-//   gated, 256 columns     gate and up of features n0 + [0, 128)
+//   plain     128 columns, features n0 + [0, 128)
+//   gated     256 columns, gate and up of features n0 + [0, 128)
 struct TileOut {
   void *out;
   float *scale;   // gated: of the rows in 8 bits
@@ -140,9 +139,8 @@ __device__ __forceinline__ void store4(const TileOut &o, int t, int n, const flo
         if (n + i < o.N) p[i] = v[i];
   }
 }
-// peer0, peer_step: cluster ranks of the CTAs that hold the slices
-template <bool kGated, int kCols, int kLd>
-__device__ __forceinline__ void finish_tokens(uint32_t base, int rows, int first, int step, int split, int peer0, int peer_step, const TileOut &o) {
+template <bool kGated, int kLd>
+__device__ __forceinline__ void finish_tokens(uint32_t base, int rows, int first, int step, int split, const TileOut &o) {
   const int lane = threadIdx.x & 31;
   for (int r0 = first; r0 < rows; r0 += 4 * step) {
     float a[4][4], b[4][4];
@@ -151,16 +149,16 @@ __device__ __forceinline__ void finish_tokens(uint32_t base, int rows, int first
 #pragma unroll
       for (int i = 0; i < 4; i++) a[j][i] = b[j][i] = 0.f;
     for (int p = 0; p < split; p++) {
-      const uint32_t from = (split > 1 ? cluster_bar(base, (uint32_t)(peer0 + p * peer_step)) : base) + (uint32_t)lane * 16u;
+      const uint32_t from = (split > 1 ? cluster_bar(base, (uint32_t)p) : base) + (uint32_t)lane * 16u;
 #pragma unroll
       for (int j = 0; j < 4; j++)
         if (r0 + j * step < rows) {
           float v[4], u[4];
           const uint32_t at = from + (uint32_t)((r0 + j * step) * kLd) * 4u;
           ld_peer4(v, at);
-          if (kCols == 256) ld_peer4(u, at + 512u);
+          if (kGated) ld_peer4(u, at + 512u);
 #pragma unroll
-          for (int i = 0; i < 4; i++) { a[j][i] += v[i]; if (kCols == 256) b[j][i] += u[i]; }
+          for (int i = 0; i < 4; i++) { a[j][i] += v[i]; if (kGated) b[j][i] += u[i]; }
         }
     }
     const int n = o.n0 + lane * 4;
@@ -176,7 +174,6 @@ __device__ __forceinline__ void finish_tokens(uint32_t base, int rows, int first
         if (lane == 0) o.scale[(size_t)(o.n0 / kF8Block) * o.T + t] = s;
       } else {
         store4(o, t, n, a[j]);
-        if (kCols == 256) store4(o, t, n + 128, b[j]);
       }
     }
   }
@@ -350,55 +347,58 @@ gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
 
   // every CTA of the cluster finishes a share of the tokens
   const TileOut o{out, out_scale, T, N, t0, n0, wide, out_bf16};
-  finish_tokens<kGated, Cfg::kCols, Cfg::kLd>(smem_base, rows, slice + split * warp, split * (kF8Threads / 32), split, 0, 1, o);
+  finish_tokens<kGated, Cfg::kLd>(smem_base, rows, slice + split * warp, split * (kF8Threads / 32), split, o);
   if (split > 1) cluster_meet();  // no CTA leaves while another reads its sums
 }
 
 // ------------------------------------------------------------------------------------------------ pair kernel
 // What bounds a block is the way of an accumulator: MMAs, commit, the sums' warps reading it, their arrival at the first CTA.  With two
-// buffers of 256 columns that way is longer than two blocks' MMAs; so a block's 256 columns are two products of 128, each with buffers and
-// warps of its own, and the way is that much shorter.  Half h takes rows [64 h, 64 h + 64) of each CTA's 128 feature rows: its columns
-// are 64 features of the first CTA's and 64 of the second's (gated: the gate and the up of the same 64 features).
-// Three warpgroups: warp 0 TMA, warp 1 MMA; warpgroups 1 and 2 a half's sums each, 128 columns a thread in registers, which the first
-// warpgroup leaves them (setmaxnreg).
+// buffers of 256 columns that way is longer than two blocks' MMAs; so products have 128 columns, four buffers and, of a tile of 256 columns,
+// warps of their own: product h takes rows [64 h, 64 h + 64) of each CTA's 128 feature rows, its columns are 64 features of the first CTA's
+// and 64 of the second's (gated: the gate and the up of the same 64 features).
+// A tile of 128 columns (64 feature rows a CTA, one product a block, half of its columns a warpgroup) is for few tiles: it brings 24 KB into an SM
+// for half the MMAs of 32.
+// Three warpgroups: warp 0 TMA, warp 1 MMA; warpgroups 1 and 2 the sums, BN / 2 columns a thread in registers, which the first warpgroup
+// leaves them (setmaxnreg).
 constexpr int kF8PairThreads = 384;
 constexpr int kF8PairRegs = 168, kF8PairRegsLow = 40, kF8PairRegsHigh = 232;  // at launch, of the first warpgroup, of the others
 static_assert(128 * kF8PairRegsLow + 256 * kF8PairRegsHigh <= kF8PairThreads * kF8PairRegs, "more registers than the block is launched with");
-constexpr int kF8PairStages = 6;
-constexpr int kF8PairStage = 2 * kF8Box;  // one CTA's 128 token rows and 128 feature rows of a block
-constexpr int kF8PairLd = 260;              // floats of a token's row of sums in shared memory
-static_assert(128 * kF8PairLd * 4 <= kF8PairStages * kF8PairStage, "the sums take the ring's place");
-constexpr int kF8PairSmem = kF8PairStages * kF8PairStage + 1024 + 256 + 1024;
+
+template <int BN>
+struct PairCfg {
+  static constexpr int kProducts = BN / 128, kBufs = 4 / kProducts;  // of a block; accumulators of each product
+  static constexpr int kFeatRows = BN / 2;                           // of one CTA
+  static constexpr int kStage = kF8Box + kFeatRows * kF8Block;       // one CTA's 128 token rows and its feature rows of a block
+  static constexpr int kStages = BN == 256 ? 6 : 8;
+  static constexpr int kSmem = kStages * kStage + 1024 + 256 + 1024;
+};
 
 enum { kF8OutF32 = 0, kF8OutBf16 = 1, kF8OutGated = 2 };
 
-// kSplit: a cluster of several pairs has one tile and shares its K; else the pairs walk the tiles
-template <int kOut, bool kSplit>
-__global__ void __launch_bounds__(kF8PairThreads, 1)
+template <int kOut, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8PairThreads, 1)
 gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const float *__restrict__ xs,
                     const float *__restrict__ ws, void *__restrict__ out, float *__restrict__ out_scale, int T, int N, int K, int w_row0,
-                    int w_row_step, int tiles_n, int tiles_t, int t_fast, int n_split, int wide) {
-  const int split = kSplit ? n_split : 1;
+                    int w_row_step, int tiles_n, int tiles_t, int t_fast, int wide) {
+  using Cfg = PairCfg<BN>;
   constexpr bool kGated = kOut == kF8OutGated;
-  constexpr int kTileN = kGated ? 128 : 256;
+  constexpr int kTileN = kGated ? BN / 2 : BN;
+  constexpr int kW = Cfg::kProducts;  // weight scales of a thread's columns
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t bar_base = smem_base + kF8PairStages * kF8PairStage;
-  auto full_bar = [&](int s) { return bar_base + 8u * s; };                                        // (first CTA's are used)
-  auto empty_bar = [&](int s) { return bar_base + 8u * (kF8PairStages + s); };
-  auto acc_full = [&](uint32_t h, uint32_t b) { return bar_base + 8u * (2 * kF8PairStages + 2 * b + h); };
-  auto acc_empty = [&](uint32_t h, uint32_t b) { return bar_base + 8u * (2 * kF8PairStages + 4 + 2 * b + h); };  // (first CTA's are used)
-  const uint32_t tmem_slot = bar_base + 8u * (2 * kF8PairStages + 8);
+  const uint32_t bar_base = smem_base + Cfg::kStages * Cfg::kStage;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };                                  // (first CTA's are used)
+  auto empty_bar = [&](int s) { return bar_base + 8u * (Cfg::kStages + s); };
+  auto acc_full = [&](uint32_t slot) { return bar_base + 8u * (2 * Cfg::kStages + slot); };
+  auto acc_empty = [&](uint32_t slot) { return bar_base + 8u * (2 * Cfg::kStages + 4 + slot); };  // (first CTA's are used)
+  const uint32_t tmem_slot = bar_base + 8u * (2 * Cfg::kStages + 8);
   const uint32_t tops = bar_base + 256u;  // [128 tokens][2 halves] largest magnitudes of a gated tile
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  uint32_t cta;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
-  const uint32_t rank = cta & 1u, leader = cta & ~1u, slice = cta >> 1;  // of the pair; its first CTA; the pair's share of K
-  const int n_tiles = tiles_n * tiles_t, num_kb = (K + kF8Block - 1) / kF8Block;
-  const int kb0 = (int)((long long)num_kb * slice / split), kb1 = (int)((long long)num_kb * (slice + 1) / split);
-  // one slice: the pairs walk the tiles; several: a cluster has one tile
-  const int pair = ((int)blockIdx.x >> 1) / split, pairs = kSplit ? n_tiles : (int)gridDim.x >> 1;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+  const int num_kb = (K + kF8Block - 1) / kF8Block, n_tiles = tiles_n * tiles_t;
   auto tile_n = [&](int tile) { return t_fast ? tile / tiles_t : tile % tiles_n; };
   auto tile_t0 = [&](int tile) { return (t_fast ? tile % tiles_t : tile / tiles_n) * 256 + (int)rank * 128; };
   const uint64_t w_hint = t_fast ? kEvictFirst : kEvictLast, x_hint = t_fast ? kEvictLast : kEvictFirst;
@@ -406,9 +406,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&w_map);
     tma_prefetch_desc(&x_map);
-    for (int s = 0; s < kF8PairStages; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-    for (uint32_t b = 0; b < 2; b++)
-      for (uint32_t h = 0; h < 2; h++) { mbar_init(acc_full(h, b), 1); mbar_init(acc_empty(h, b), 8); }  // 4 warps of each CTA
+    for (int s = 0; s < Cfg::kStages; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+    for (uint32_t i = 0; i < 4; i++) { mbar_init(acc_full(i), 1); mbar_init(acc_empty(i), 16 / Cfg::kProducts); }  // warps of both CTAs
     fence_barrier_init();
     fence_proxy_async();
   }
@@ -433,19 +432,19 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
         uint32_t phase = 0;
         for (int tile = pair; tile < n_tiles; tile += pairs) {
           const int t0 = tile_t0(tile), wr = w_row0 + tile_n(tile) * kTileN + (int)rank * w_row_step;  // (gated: gate rows | up rows)
-          for (int kb = kb0; kb < kb1; kb++) {
+          for (int kb = 0; kb < num_kb; kb++) {
             mbar_wait(empty_bar(s), phase ^ 1u);  // passes on the first lap
-            if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kF8PairStage);
-            const uint32_t bar = cluster_bar(full_bar(s), leader), a = smem_base + s * kF8PairStage;
+            if (rank == 0) mbar_expect_tx(full_bar(s), 2 * Cfg::kStage);
+            const uint32_t bar = cluster_bar(full_bar(s), 0), a = smem_base + s * Cfg::kStage;
             tma_load_2d_pair(a, &x_map, kb * kF8Block, t0, bar, x_hint);
             tma_load_2d_pair(a + kF8Box, &w_map, kb * kF8Block, wr, bar, w_hint);
-            if (++s == kF8PairStages) { s = 0; phase ^= 1u; }
+            if (++s == Cfg::kStages) { s = 0; phase ^= 1u; }
           }
         }
         // The first CTA's commits still arrive at this CTA's barriers: wait for the last of every stage before the CTA may end.
-        for (int i = 0; i < kF8PairStages; i++) {  // (a stage never filled passes at once)
+        for (int i = 0; i < Cfg::kStages; i++) {  // (a stage never filled passes at once)
           mbar_wait(empty_bar(s), phase ^ 1u);
-          if (++s == kF8PairStages) { s = 0; phase ^= 1u; }
+          if (++s == Cfg::kStages) { s = 0; phase ^= 1u; }
         }
       }
       __syncwarp();
@@ -455,91 +454,78 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
       uint32_t lo = lo0, phase = 0, buf = 0, aphase = 0;
       int s = 0;
       for (int tile = pair; tile < n_tiles; tile += pairs)
-        for (int kb = kb0; kb < kb1; kb++) {
+        for (int kb = 0; kb < num_kb; kb++) {
           mbar_wait(full_bar(s), phase);
 #pragma unroll
-          for (uint32_t h = 0; h < 2; h++) {
-            mbar_wait(acc_empty(h, buf), aphase ^ 1u);  // both CTAs have taken this buffer (passes on first use)
+          for (uint32_t h = 0; h < Cfg::kProducts; h++) {
+            const uint32_t slot = buf * Cfg::kProducts + h;
+            mbar_wait(acc_empty(slot), aphase ^ 1u);  // both CTAs have taken this buffer (passes on first use)
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
               for (uint32_t k = 0; k < 4; k++)
-                umma_f8_pair(tmem_base + buf * 256u + h * 128u, lo + 2 * k, lo + ((kF8Box + h * (kF8Box / 2)) >> 4) + 2 * k, idesc, k > 0 ? 1u : 0u);
-              umma_commit_pair(acc_full(h, buf), leader);
-              if (h == 1) umma_commit_pair(empty_bar(s), leader);
+                umma_f8_pair(tmem_base + slot * 128u, lo + 2 * k, lo + ((kF8Box + h * (kF8Box / 2)) >> 4) + 2 * k, idesc, k > 0 ? 1u : 0u);
+              umma_commit_pair(acc_full(slot));
+              if (h == Cfg::kProducts - 1) umma_commit_pair(empty_bar(s));
             }
             __syncwarp();
           }
-          lo += kF8PairStage >> 4;
-          if (++s == kF8PairStages) { s = 0; phase ^= 1u; lo = lo0; }
-          aphase ^= buf;
-          buf ^= 1u;
+          lo += Cfg::kStage >> 4;
+          if (++s == Cfg::kStages) { s = 0; phase ^= 1u; lo = lo0; }
+          if (++buf == Cfg::kBufs) { buf = 0; aphase ^= 1u; }
         }
     }
-    if (kSplit) { tc_fence_before(); __syncwarp(); cluster_sync(); }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8PairRegsHigh));
     const int quarter = warp & 3, half = (warp >> 2) - 1, r = quarter * 32 + lane;
-    const uint32_t empty0 = cluster_bar(acc_empty(half, 0), leader), empty1 = cluster_bar(acc_empty(half, 1), leader);
-    const uint32_t cols = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128u;
+    const uint32_t empty0 = cluster_bar(acc_empty(0), 0);
+    const uint32_t cols = tmem_base + ((uint32_t)(quarter * 32) << 16) + (BN == 256 ? 0u : half * 64u);
     const int blocks_n = (N + 127) / 128;
-    Scales<2> sc;  // of the first CTA's features and of the second's
-    sc.xs = xs; sc.T = T; sc.end = kb1;
+    Scales<kW> sc;  // of the first CTA's features and of the second's
+    sc.xs = xs; sc.T = T; sc.end = num_kb;
     auto aim = [&](int tile) {  // the scales of a tile, its first ones on their way
       const bool any = tile < n_tiles;
       const int b = tile_n(tile) * (kTileN / 128), b2 = kGated ? blocks_n + b : b + 1;
       sc.t = any ? tile_t0(tile) + r : T;
       sc.ws[0] = any ? ws + (size_t)b * num_kb : nullptr;
-      sc.ws[1] = any && (kGated || b2 < blocks_n) ? ws + (size_t)b2 * num_kb : nullptr;
-      sc.fetch_x(kb0);
-      sc.fetch_w(kb0);
+      if (kW == 2) sc.ws[kW - 1] = any && (kGated || b2 < blocks_n) ? ws + (size_t)b2 * num_kb : nullptr;
+      sc.fetch_x(0);
+      sc.fetch_w(0);
     };
     pdl_wait();
     aim(pair);
     uint32_t buf = 0, aphase = 0;
     for (int tile = pair; tile < n_tiles; tile += pairs) {
-      uint64_t sums[64];
+      uint64_t sums[BN / 4];
 #pragma unroll
-      for (int i = 0; i < 64; i++) sums[i] = 0;
-      for (int kb = kb0; kb < kb1; kb++) {
-        float f[2];
-        sc.get(kb0, kb - kb0, f);
-        mbar_wait(acc_full(half, buf), aphase);
+      for (int i = 0; i < BN / 4; i++) sums[i] = 0;
+      for (int kb = 0; kb < num_kb; kb++) {
+        float f[kW];
+        sc.get(0, kb, f);
+        const uint32_t slot = buf * Cfg::kProducts + (BN == 256 ? half : 0), at = cols + slot * 128u;
+        mbar_wait(acc_full(slot), aphase);
         tc_fence_after();
         uint32_t v[2][32];
-        const uint32_t at = cols + buf * 256u;
         tmem_ld_32x32(at, v[0]);
         tmem_ld_32x32(at + 32u, v[1]);
         tmem_ld_wait();
-        add_scaled(v[0], f[0], sums);
-        tmem_ld_32x32(at + 64u, v[0]);
-        add_scaled(v[1], f[0], sums + 16);
-        tmem_ld_32x32(at + 96u, v[1]);
-        tmem_ld_wait();
+        if (BN == 256) {
+          add_scaled(v[0], f[0], sums);
+          tmem_ld_32x32(at + 64u, v[0]);
+          add_scaled(v[1], f[0], sums + 16);
+          tmem_ld_32x32(at + 96u, v[1]);
+          tmem_ld_wait();
+        }
         tc_fence_before();  // everything of this buffer is in registers
         __syncwarp();
-        if (lane == 0) mbar_arrive_at(buf ? empty1 : empty0);
-        add_scaled(v[0], f[1], sums + 32);
-        add_scaled(v[1], f[1], sums + 48);
-        aphase ^= buf;
-        buf ^= 1u;
-      }
-      if (kSplit) {
-        // The ring is free once both halves' last MMAs have read it.  Every CTA finishes its share of its 128 tokens.
-        asm volatile("bar.sync 5, 256;" ::: "memory");
-        const uint32_t row = smem_base + (uint32_t)(r * kF8PairLd) * 4u;
-        put_sums(row, half * 64, sums);
-        put_sums(row, 128 + half * 64, sums + 32);
-        tc_fence_before();
-        cluster_sync();
-        const int t0 = tile_t0(tile);
-        const TileOut o{out, out_scale, T, N, t0, tile_n(tile) * kTileN, (wide >> 1) & 1, kOut == kF8OutBf16};
-        finish_tokens<kGated, 256, kF8PairLd>(smem_base, min(128, T - t0), (int)slice + split * (warp - 4), split * 8, split, (int)rank, 2, o);
-        break;
+        if (lane == 0) mbar_arrive_at(empty0 + 8u * slot);
+        add_scaled(v[0], f[kW - 1], sums + (BN / 4 - 32));
+        add_scaled(v[1], f[kW - 1], sums + (BN / 4 - 16));
+        if (++buf == Cfg::kBufs) { buf = 0; aphase ^= 1u; }
       }
       aim(tile + pairs);
       const int t = tile_t0(tile) + r, n0 = tile_n(tile) * kTileN + half * 64;
-      if (kGated) {
+      if constexpr (kGated) {
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 32; i++) {
@@ -548,7 +534,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
           top = max(top, max(f8_bits(a), f8_bits(b)));
           asm("mov.b64 %0, {%1, %2};" : "=l"(sums[i]) : "f"(a), "f"(b));
         }
-        // the token's other 64 features are a thread of the other half's: 64 threads of two warps meet
+        // the token's other 64 features are a thread of the other warpgroup's: 64 threads of two warps meet
         asm volatile("st.shared.u32 [%0], %1;" ::"r"(tops + (uint32_t)(r * 2 + half) * 4), "r"(top) : "memory");
         asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
         uint32_t other;
@@ -571,7 +557,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
         }
       } else if (t < T) {
 #pragma unroll
-        for (int c = 0; c < 8; c++) {  // 16 features at a time: four times of the first CTA's, four of the second's
+        for (int c = 0; c < BN / 32; c++) {  // 16 features at a time: four times of the first 128, four of the second
           const int n = n0 + 16 * c + (c >= 4 ? 64 : 0);
           uint32_t v[16];
 #pragma unroll
@@ -582,14 +568,14 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
           }
           if (kOut == kF8OutF32) {
             float *o = static_cast<float *>(out) + (size_t)t * N + n;
-            if ((wide & 1) && n + 16 <= N) { st_32(o, v); st_32(o + 8, v + 8); }
+            if (wide && n + 16 <= N) { st_32(o, v); st_32(o + 8, v + 8); }
             else
 #pragma unroll
               for (int i = 0; i < 16; i++)
                 if (n + i < N) o[i] = __uint_as_float(v[i]);
           } else {
             uint16_t *o = static_cast<uint16_t *>(out) + (size_t)t * N + n;
-            if ((wide & 1) && n + 16 <= N) {
+            if (wide && n + 16 <= N) {
               uint32_t p[8];
 #pragma unroll
               for (int i = 0; i < 8; i++) p[i] = float2_to_bf16x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
@@ -605,7 +591,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   }
   tc_fence_before();
   __syncthreads();
-  cluster_meet();  // no CTA leaves while another's MMAs, commits or arrivals may still reach it, or another reads its sums
+  cluster_meet();  // neither CTA leaves while the other's MMAs, commits or arrivals may still reach it
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
 }
 
@@ -646,59 +632,52 @@ cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *x
                           w_row0, split, tile_t, stages, bar_off, weights_first, wide);
 }
 
-// Pairs that share a tile's K: where the tiles are few, as many as fit at once (clusters of up to 8 CTAs, an SM each)
-int pair_split(int T, int N, int K, bool gated) {
-  const int feats = gated ? 128 : 256, num_kb = (K + kF8Block - 1) / kF8Block;
-  const long long tiles = (long long)((N + feats - 1) / feats) * ((T + 255) / 256);
-  int s = 1;
-  while (s < 4 && tiles * s * 2 <= (s == 1 ? 70 : 64) && num_kb >= 8 * s) s *= 2;
-  return s;
+// Columns of a pair's tile.  (Gated: 256, a tile is a block of 128 features under one scale.)
+int pair_f8_columns(int T, int N, int K, bool gated) {
+  return gated ? 256 : 256;
 }
 
-template <int kOut, bool kSplit>
-cudaError_t pair_f8_launch_as(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int T, int N, int K,
-                           int w_row0, int wide, int split, cudaStream_t st) {
+template <int kOut, int BN>
+cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int T, int N, int K,
+                           int w_row0, int wide, cudaStream_t st) {
+  using Cfg = PairCfg<BN>;
   static DeviceOnce once;
   DIS_CUDA_TRY(once.run([&] {
     // a block launched with fewer registers would wait for those that its warpgroups ask for
     cudaFuncAttributes at;
-    cudaError_t e = cudaFuncGetAttributes(&at, gemm_f8_pair_kernel<kOut, kSplit>);
+    cudaError_t e = cudaFuncGetAttributes(&at, gemm_f8_pair_kernel<kOut, BN>);
     if (e == cudaSuccess && at.numRegs != kF8PairRegs) e = cudaErrorInvalidKernelImage;
-    return e == cudaSuccess ? cudaFuncSetAttribute(gemm_f8_pair_kernel<kOut, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8PairSmem) : e;
+    return e == cudaSuccess ? cudaFuncSetAttribute(gemm_f8_pair_kernel<kOut, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem) : e;
   }));
-  const int feats = kOut == kF8OutGated ? 128 : 256;
+  const int feats = kOut == kF8OutGated ? BN / 2 : BN;
   const int tiles_n = (N + feats - 1) / feats, tiles_t = (T + 255) / 256;
   const long long n_tiles = (long long)tiles_n * tiles_t;
   if (n_tiles > (1 << 30)) { set_last_error("gemm_f8: too many tiles"); return cudaErrorInvalidValue; }
-  const int pairs = kSplit ? (int)n_tiles * split : n_tiles < kNumSMs / 2 ? (int)n_tiles : kNumSMs / 2;
+  const int pairs = n_tiles < kNumSMs / 2 ? (int)n_tiles : kNumSMs / 2;
   const int t_fast = (long long)(kOut == kF8OutGated ? 2 : 1) * N > (long long)T ? 1 : 0;  // as gemm_pair_kernel: the smaller operand stays in L2
-  return launch_k_cluster(gemm_f8_pair_kernel<kOut, kSplit>, dim3(2 * pairs), dim3(kF8PairThreads), (size_t)kF8PairSmem, st, 2 * split, *reinterpret_cast<const CUtensorMap *>(&w_map),
-                  *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, T, N, K, w_row0, kOut == kF8OutGated ? N : 128, tiles_n, tiles_t, t_fast, split, wide);
-}
-
-template <int kOut>
-cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int T, int N, int K,
-                           int w_row0, int wide, cudaStream_t st) {
-  const int split = pair_split(T, N, K, kOut == kF8OutGated);
-  return split > 1 ? pair_f8_launch_as<kOut, true>(w_map, x_map, xs, ws, out, out_scale, T, N, K, w_row0, wide, split, st)
-                   : pair_f8_launch_as<kOut, false>(w_map, x_map, xs, ws, out, out_scale, T, N, K, w_row0, wide, 1, st);
+  return launch_k(gemm_f8_pair_kernel<kOut, BN>, dim3(2 * pairs), dim3(kF8PairThreads), (size_t)Cfg::kSmem, st, *reinterpret_cast<const CUtensorMap *>(&w_map),
+                  *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, T, N, K, w_row0, kOut == kF8OutGated ? N : Cfg::kFeatRows, tiles_n, tiles_t,
+                  t_fast, wide);
 }
 
 }  // namespace
 
 bool gemm_f8_in_pairs(int T, int N, int K, bool gated) { return T > 256; }
 uint32_t gemm_f8_token_box(int T, int N, int K, bool gated) { return gemm_f8_in_pairs(T, N, K, gated) ? 128u : (uint32_t)tile_tokens(T); }
+uint32_t gemm_f8_feature_box(int T, int N, int K, bool gated) {
+  return gemm_f8_in_pairs(T, N, K, gated) && pair_f8_columns(T, N, K, gated) == 128 ? 64u : 128u;
+}
 
-// w_map: 128-row boxes over [..][K] e4m3, x_map: boxes of gemm_f8_token_box() rows
 cudaError_t launch_gemm_f8(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, bool bf16, int T, int N, int K, int w_row0,
                            cudaStream_t st) {
   if (T <= 0 || N <= 0) return cudaSuccess;
   const uintptr_t at = (uintptr_t)out;
   if (gemm_f8_in_pairs(T, N, K, false)) {
-    // every piece of a row starts on 32 bytes; on four elements
-    const int wide = ((at & 31u) == 0 && N % (bf16 ? 16 : 8) == 0 ? 1 : 0) | (N % 4 == 0 && (at & (bf16 ? 7u : 15u)) == 0 ? 2 : 0);
-    return bf16 ? pair_f8_launch<kF8OutBf16>(w_map, x_map, xs, ws, out, nullptr, T, N, K, w_row0, wide, st)
-                : pair_f8_launch<kF8OutF32>(w_map, x_map, xs, ws, out, nullptr, T, N, K, w_row0, wide, st);
+    const int wide = (at & 31u) == 0 && N % (bf16 ? 16 : 8) == 0;  // every piece of a row starts on 32 bytes
+    const bool narrow = pair_f8_columns(T, N, K, false) == 128;
+    auto f = bf16 ? (narrow ? pair_f8_launch<kF8OutBf16, 128> : pair_f8_launch<kF8OutBf16, 256>)
+                  : (narrow ? pair_f8_launch<kF8OutF32, 128> : pair_f8_launch<kF8OutF32, 256>);
+    return f(w_map, x_map, xs, ws, out, nullptr, T, N, K, w_row0, wide, st);
   }
   const int wide = N % 4 == 0 && (at & (bf16 ? 7u : 15u)) == 0;
   return tile_launch<false>(w_map, x_map, xs, ws, out, nullptr, bf16 ? 1 : 0, T, N, K, w_row0, wide, st);
@@ -708,7 +687,7 @@ cudaError_t launch_gemm_f8(const TmaMap &w_map, const TmaMap &x_map, const float
 cudaError_t launch_gemm_silu_f8(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, uint8_t *h8, float *hs, int T, int I, int K,
                                 int w_row0, cudaStream_t st) {
   if (T <= 0 || I <= 0) return cudaSuccess;
-  if (gemm_f8_in_pairs(T, I, K, true)) return pair_f8_launch<kF8OutGated>(w_map, x_map, xs, ws, h8, hs, T, I, K, w_row0, 0, st);
+  if (gemm_f8_in_pairs(T, I, K, true)) return pair_f8_launch<kF8OutGated, 256>(w_map, x_map, xs, ws, h8, hs, T, I, K, w_row0, 0, st);
   return tile_launch<true>(w_map, x_map, xs, ws, h8, hs, 0, T, I, K, w_row0, 0, st);
 }
 

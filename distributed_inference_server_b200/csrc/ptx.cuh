@@ -156,9 +156,8 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void *map, 
       : "memory");
 }
 // arrives at the same barrier of both CTAs once all MMAs issued so far have completed
-// (leader: the pair's first CTA in its cluster)
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar, uint32_t leader = 0) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)(3u << leader)) : "memory");
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
