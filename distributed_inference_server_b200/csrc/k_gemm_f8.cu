@@ -358,11 +358,17 @@ gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
 // and 64 of the second's (gated: the gate and the up of the same 64 features).
 // A tile of 128 columns (64 feature rows a CTA, one product a block, half of its columns a warpgroup) is for few tiles: it brings 24 KB into an SM
 // for half the MMAs of 32.
-// Three warpgroups: warp 0 TMA, warp 1 MMA; warpgroups 1 and 2 the sums, BN / 2 columns a thread in registers, which the first warpgroup
-// leaves them (setmaxnreg).
+// Three warpgroups.  Warp 0 TMA.  Warps 1 and 3 MMA: two waits, four MMAs and their commits take one warp as long as a block's MMAs take, so
+// each issues one of a block's two products (128 columns: every second block).  Warp 2 the products of both scales, [block][token][two] in
+// shared memory, four blocks at a time: fetched and multiplied by the sums' warps themselves they cost a fifth of the kernel's time (8192^3 of
+// one value: 392 us against 329 without any).  Warpgroups 1 and 2 the sums, BN / 2 columns a thread in registers, which the first
+// warpgroup leaves them (setmaxnreg).
 constexpr int kF8PairThreads = 384;
 constexpr int kF8PairRegs = 168, kF8PairRegsLow = 40, kF8PairRegsHigh = 232;  // at launch, of the first warpgroup, of the others
 static_assert(128 * kF8PairRegsLow + 256 * kF8PairRegsHigh <= kF8PairThreads * kF8PairRegs, "more registers than the block is launched with");
+
+constexpr int kF8Group = 4, kF8Groups = 4;                  // blocks whose factors are made together; such groups kept
+constexpr int kF8GroupBytes = kF8Group * 128 * 2 * 4;
 
 template <int BN>
 struct PairCfg {
@@ -370,10 +376,21 @@ struct PairCfg {
   static constexpr int kFeatRows = BN / 2;                           // of one CTA
   static constexpr int kStage = kF8Box + kFeatRows * kF8Block;       // one CTA's 128 token rows and its feature rows of a block
   static constexpr int kStages = BN == 256 ? 6 : 8;
-  static constexpr int kSmem = kStages * kStage + 1024 + 256 + 1024;
+  static constexpr int kSmem = kStages * kStage + kF8Groups * kF8GroupBytes + 1024 + 256 + 1024;
 };
 
 enum { kF8OutF32 = 0, kF8OutBf16 = 1, kF8OutGated = 2 };
+
+// mbar_wait where the barrier has mostly been passed already: one look first, which costs less than a wait
+__device__ __forceinline__ void mbar_wait_soon(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (!ok) mbar_wait(bar, parity);
+}
 
 template <int kOut, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8PairThreads, 1)
@@ -386,12 +403,14 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   constexpr int kW = Cfg::kProducts;  // weight scales of a thread's columns
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t bar_base = smem_base + Cfg::kStages * Cfg::kStage;
+  const uint32_t factors = smem_base + Cfg::kStages * Cfg::kStage, bar_base = factors + kF8Groups * kF8GroupBytes;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };                                  // (first CTA's are used)
   auto empty_bar = [&](int s) { return bar_base + 8u * (Cfg::kStages + s); };
   auto acc_full = [&](uint32_t slot) { return bar_base + 8u * (2 * Cfg::kStages + slot); };
   auto acc_empty = [&](uint32_t slot) { return bar_base + 8u * (2 * Cfg::kStages + 4 + slot); };  // (first CTA's are used)
-  const uint32_t tmem_slot = bar_base + 8u * (2 * Cfg::kStages + 8);
+  auto f_full = [&](uint32_t g) { return bar_base + 8u * (2 * Cfg::kStages + 8 + g); };
+  auto f_empty = [&](uint32_t g) { return bar_base + 8u * (2 * Cfg::kStages + 8 + kF8Groups + g); };
+  const uint32_t tmem_slot = bar_base + 8u * (2 * Cfg::kStages + 8 + 2 * kF8Groups);
   const uint32_t tops = bar_base + 256u;  // [128 tokens][2 halves] largest magnitudes of a gated tile
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
@@ -406,8 +425,9 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&w_map);
     tma_prefetch_desc(&x_map);
-    for (int s = 0; s < Cfg::kStages; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+    for (int s = 0; s < Cfg::kStages; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), Cfg::kProducts); }
     for (uint32_t i = 0; i < 4; i++) { mbar_init(acc_full(i), 1); mbar_init(acc_empty(i), 16 / Cfg::kProducts); }  // warps of both CTAs
+    for (uint32_t g = 0; g < kF8Groups; g++) { mbar_init(f_full(g), 1); mbar_init(f_empty(g), 8); }
     fence_barrier_init();
     fence_proxy_async();
   }
@@ -448,25 +468,58 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
         }
       }
       __syncwarp();
-    } else if (warp == 1 && rank == 0) {
+    } else if (warp == 2) {
+      // Factors of four tokens a lane, two blocks' scales on their way at a time
+      pdl_wait();
+      const int blocks_n = (N + 127) / 128;
+      uint32_t g = 0, phase = 0;
+      for (int tile = pair; tile < n_tiles; tile += pairs) {
+        const int t0 = tile_t0(tile) + lane, b = tile_n(tile) * (kTileN / 128), b2 = kGated ? blocks_n + b : b + 1;
+        const float *w0 = ws + (size_t)b * num_kb, *w1 = BN == 256 && (kGated || b2 < blocks_n) ? ws + (size_t)b2 * num_kb : w0;  // (columns past N: whatever)
+        for (int kb = 0; kb < num_kb; kb += kF8Group) {
+          const uint32_t at = factors + g * (uint32_t)kF8GroupBytes + (uint32_t)lane * 8u;
+#pragma unroll
+          for (int k = 0; k < kF8Group; k += 2) {
+            float x[2][4], a[2], c[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const int at_kb = min(kb + k + i, num_kb - 1);
+#pragma unroll
+              for (int j = 0; j < 4; j++) x[i][j] = t0 + 32 * j < T ? xs[(size_t)at_kb * T + t0 + 32 * j] : 0.f;
+              a[i] = w0[at_kb];
+              c[i] = w1[at_kb];
+            }
+            if (k == 0) mbar_wait(f_empty(g), phase ^ 1u);  // passes on the first lap
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+              for (int j = 0; j < 4; j++)
+                asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + (k + i) * 1024u + j * 256u), "f"(x[i][j] * a[i]), "f"(x[i][j] * c[i]) : "memory");
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(f_full(g));
+          if (++g == kF8Groups) { g = 0; phase ^= 1u; }
+        }
+      }
+    } else if (rank == 0) {
       constexpr uint32_t idesc = f8_idesc(256, 128);
+      const uint32_t mine = (uint32_t)warp >> 1;  // warp 1: 0, warp 3: 1
       const uint32_t lo0 = umma_lo(smem_base);
       uint32_t lo = lo0, phase = 0, buf = 0, aphase = 0;
       int s = 0;
       for (int tile = pair; tile < n_tiles; tile += pairs)
         for (int kb = 0; kb < num_kb; kb++) {
-          mbar_wait(full_bar(s), phase);
-#pragma unroll
-          for (uint32_t h = 0; h < Cfg::kProducts; h++) {
-            const uint32_t slot = buf * Cfg::kProducts + h;
-            mbar_wait(acc_empty(slot), aphase ^ 1u);  // both CTAs have taken this buffer (passes on first use)
+          if (BN == 256 || (buf & 1u) == mine) {
+            const uint32_t h = BN == 256 ? mine : 0u, slot = buf * Cfg::kProducts + h;
+            mbar_wait_soon(full_bar(s), phase);
+            mbar_wait_soon(acc_empty(slot), aphase ^ 1u);  // both CTAs have taken this buffer (passes on first use)
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
               for (uint32_t k = 0; k < 4; k++)
                 umma_f8_pair(tmem_base + slot * 128u, lo + 2 * k, lo + ((kF8Box + h * (kF8Box / 2)) >> 4) + 2 * k, idesc, k > 0 ? 1u : 0u);
               umma_commit_pair(acc_full(slot));
-              if (h == Cfg::kProducts - 1) umma_commit_pair(empty_bar(s));
+              umma_commit_pair(empty_bar(s));
             }
             __syncwarp();
           }
@@ -478,32 +531,21 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8PairRegsHigh));
     const int quarter = warp & 3, half = (warp >> 2) - 1, r = quarter * 32 + lane;
-    const uint32_t empty0 = cluster_bar(acc_empty(0), 0);
+    const uint32_t empty0 = cluster_bar(acc_empty(0), 0), my_factors = factors + (uint32_t)r * 8u;
     const uint32_t cols = tmem_base + ((uint32_t)(quarter * 32) << 16) + (BN == 256 ? 0u : half * 64u);
-    const int blocks_n = (N + 127) / 128;
-    Scales<kW> sc;  // of the first CTA's features and of the second's
-    sc.xs = xs; sc.T = T; sc.end = num_kb;
-    auto aim = [&](int tile) {  // the scales of a tile, its first ones on their way
-      const bool any = tile < n_tiles;
-      const int b = tile_n(tile) * (kTileN / 128), b2 = kGated ? blocks_n + b : b + 1;
-      sc.t = any ? tile_t0(tile) + r : T;
-      sc.ws[0] = any ? ws + (size_t)b * num_kb : nullptr;
-      if (kW == 2) sc.ws[kW - 1] = any && (kGated || b2 < blocks_n) ? ws + (size_t)b2 * num_kb : nullptr;
-      sc.fetch_x(0);
-      sc.fetch_w(0);
-    };
     pdl_wait();
-    aim(pair);
+    uint32_t g = 0, fphase = 0;
     uint32_t buf = 0, aphase = 0;
     for (int tile = pair; tile < n_tiles; tile += pairs) {
       uint64_t sums[BN / 4];
 #pragma unroll
       for (int i = 0; i < BN / 4; i++) sums[i] = 0;
       for (int kb = 0; kb < num_kb; kb++) {
-        float f[kW];
-        sc.get(0, kb, f);
+        if ((kb & (kF8Group - 1)) == 0) mbar_wait_soon(f_full(g), fphase);
+        float f[2];  // (of the first CTA's features and of the second's)
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f[0]), "=f"(f[1]) : "r"(my_factors + g * (uint32_t)kF8GroupBytes + (kb & (kF8Group - 1)) * 1024u) : "memory");
         const uint32_t slot = buf * Cfg::kProducts + (BN == 256 ? half : 0), at = cols + slot * 128u;
-        mbar_wait(acc_full(slot), aphase);
+        mbar_wait_soon(acc_full(slot), aphase);
         tc_fence_after();
         uint32_t v[2][32];
         tmem_ld_32x32(at, v[0]);
@@ -519,11 +561,14 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
         tc_fence_before();  // everything of this buffer is in registers
         __syncwarp();
         if (lane == 0) mbar_arrive_at(empty0 + 8u * slot);
+        if ((kb & (kF8Group - 1)) == kF8Group - 1 || kb == num_kb - 1) {
+          if (lane == 0) mbar_arrive(f_empty(g));
+          if (++g == kF8Groups) { g = 0; fphase ^= 1u; }
+        }
         add_scaled(v[0], f[kW - 1], sums + (BN / 4 - 32));
         add_scaled(v[1], f[kW - 1], sums + (BN / 4 - 16));
         if (++buf == Cfg::kBufs) { buf = 0; aphase ^= 1u; }
       }
-      aim(tile + pairs);
       const int t = tile_t0(tile) + r, n0 = tile_n(tile) * kTileN + half * 64;
       if constexpr (kGated) {
         uint32_t top = 0;
