@@ -645,14 +645,17 @@ constexpr int kTileRest = 1024 + 256;  // alignment, barriers
 
 // How a tile kernel's work is laid out: tokens of a tile and CTAs of a cluster
 int tile_tokens(int T) { return T <= 32 ? 32 : T <= 64 ? 64 : 128; }
+// CTAs that share a tile's K: about eight blocks each and four CTAs at least, as far as all are resident at once (two an SM, fewer in large clusters,
+// which have to fit a GPC; gated one) and leave each two blocks; more than four only with few tokens.  Measured with 1 to 8 for nine shapes
+// and 1, 32, 64 and 128 tokens, the rule's choice is within 6 % of the best at 34 of the 36 and within 13 % at the rest.  us with 2 / 4 / 8:
+// 4096 x 4096, 32 tokens 10.8 / 8.3 / 9.0; 4096 x 14336, 32 tokens 23 / 17.0 / 14.7 and 128 tokens 27 / 18.5 / 20.6.
 int tile_split(int T, int N, int K, bool gated) {
   const long long tiles = (long long)((N + 127) / 128) * ((T + tile_tokens(T) - 1) / tile_tokens(T));
   const int num_kb = (K + kF8Block - 1) / kF8Block;
-  const long long room = (gated ? 1 : 2) * kNumSMs;  // resident CTAs
-  int s = (int)(room / tiles);
-  s = s > 8 ? 8 : s;
-  s = s > num_kb / 2 ? num_kb / 2 : s;
-  return s < 1 ? 1 : s;
+  const int want = num_kb / 8 < 4 || T > 64 ? 4 : num_kb / 8 > 8 ? 8 : num_kb / 8;
+  int s = 1;
+  while (s < want && num_kb >= 2 * (s + 1) && tiles * (s + 1) <= (gated ? (s + 1 <= 2 ? 148 : 120) : (s + 1 <= 2 ? 296 : 264))) s++;
+  return s;
 }
 
 template <bool kGated>
@@ -666,7 +669,8 @@ cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *x
   if (tiles_t > 65535) { set_last_error("gemm_f8: too many tokens"); return cudaErrorInvalidValue; }
   const int per = ((K + kF8Block - 1) / kF8Block + split - 1) / split;  // blocks of a slice, at most
   const bool two = !kGated && (long long)tiles_n * tiles_t * split > kNumSMs;
-  const int budget = two ? 92 * 1024 : 220 * 1024;
+  // (two an SM: a ring of four stages with up to 64 tokens is faster than one of five: 8192 x 8192, 32 tokens 15.5 and 15.8 us)
+  const int budget = (two ? tile_t < 128 ? 92 : 106 : 220) * 1024;
   int stages = 2;
   while (stages < per && stages < 12 && Cfg::body_bytes(stages + 1, tile_t, rows) + kTileRest <= budget) stages++;
   const uint32_t bar_off = (uint32_t)Cfg::body_bytes(stages, tile_t, rows);
@@ -677,10 +681,25 @@ cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *x
                           w_row0, split, tile_t, stages, bar_off, weights_first, wide);
 }
 
-// Columns of a pair's tile.  (Gated: 256, a tile is a block of 128 features under one scale.)
-int pair_f8_columns(int T, int N, int K, bool gated) {
-  return gated ? 256 : 256;
+// What a product takes behind its launch, in hundredths of a microsecond, fitted to ten shapes from 1024 x 1024 to 10240 x 8192 and 8192 x 28672 at
+// 128 to 1024 tokens: in pairs 25 and 37 per block for every round of tiles of 128 and of 256 columns, in tiles 60 per block of a slice for every
+// round of CTAs.
+int pair_f8_cost(int T, int N, int K, int columns) {
+  const long long tiles = (long long)((N + columns - 1) / columns) * ((T + 255) / 256), num_kb = (K + kF8Block - 1) / kF8Block;
+  const long long rounds = (tiles + kNumSMs / 2 - 1) / (kNumSMs / 2);
+  const long long cost = columns == 128 ? 350 + 25 * num_kb * rounds : 400 + 37 * num_kb * rounds;
+  return cost > 0x7fffffff ? 0x7fffffff : (int)cost;
 }
+int tile_cost(int T, int N, int K) {
+  const int split = tile_split(T, N, K, false), tile_t = tile_tokens(T);
+  const long long ctas = (long long)((N + 127) / 128) * ((T + tile_t - 1) / tile_t) * split;
+  const long long per = ((K + kF8Block - 1) / kF8Block + split - 1) / split, rounds = (ctas + 2 * kNumSMs - 1) / (2 * kNumSMs);
+  const long long cost = 600 + (split > 1 ? 100 : 0) + 60 * per * rounds;
+  return cost > 0x7fffffff ? 0x7fffffff : (int)cost;
+}
+// Columns of a pair's tile.  (Gated: 256, a tile is a block of 128 features under one scale.)  us with 128 / 256: 4096 x 4096, 512 tokens 13.8 / 18.0, 1024
+// tokens 21.5 / 20.4.
+int pair_f8_columns(int T, int N, int K, bool gated) { return gated || pair_f8_cost(T, N, K, 256) <= pair_f8_cost(T, N, K, 128) ? 256 : 128; }
 
 template <int kOut, int BN>
 cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int T, int N, int K,
@@ -707,7 +726,14 @@ cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float
 
 }  // namespace
 
-bool gemm_f8_in_pairs(int T, int N, int K, bool gated) { return T > 256; }
+// Which products run in pairs.  Up to 128 tokens none: a pair's tile is half empty (4096 x 14336, 128 tokens: 18.9 us in tiles, 31.4 in pairs; gate-up
+// 14336 x 4096, 128 tokens 30.6 and 35.3).  Gate-up products from there on (129 tokens: 49.5 and 35.1; 1024 x 1024, 129 tokens 11.0 and 9.8), plain ones
+// where the estimates say so (8192 x 8192, 200 tokens 24.0 and 21.2; but 2048 x 5632, 192 tokens 11.4 and 15.6).
+bool gemm_f8_in_pairs(int T, int N, int K, bool gated) {
+  if (T <= 128 || gated) return T > 128;
+  const int narrow = pair_f8_cost(T, N, K, 128), wide = pair_f8_cost(T, N, K, 256);
+  return (narrow < wide ? narrow : wide) < tile_cost(T, N, K);
+}
 uint32_t gemm_f8_token_box(int T, int N, int K, bool gated) { return gemm_f8_in_pairs(T, N, K, gated) ? 128u : (uint32_t)tile_tokens(T); }
 uint32_t gemm_f8_feature_box(int T, int N, int K, bool gated) {
   return gemm_f8_in_pairs(T, N, K, gated) && pair_f8_columns(T, N, K, gated) == 128 ? 64u : 128u;
