@@ -16,7 +16,7 @@ FINISH_NONE, FINISH_STOP, FINISH_LENGTH, FINISH_STOP_SEQUENCE, FINISH_FAILED = r
 (T_EMBED, T_ATTN_NORM, T_WQ, T_WK, T_WV, T_WO, T_MLP_NORM, T_WGATE, T_WUP, T_WDOWN, T_FINAL_NORM,
  T_LM_HEAD) = range(12)
 F32, BF16 = 0, 1
-FLAG_NO_GRAPH, FLAG_FORCE_GEMV, FLAG_NO_PDL, FLAG_PREFIX_CACHE, FLAG_KV_INT8, FLAG_ATTN_SHARED = 1, 2, 4, 8, 16, 32
+FLAG_NO_GRAPH, FLAG_FORCE_GEMV, FLAG_NO_PDL, FLAG_PREFIX_CACHE, FLAG_KV_INT8, FLAG_ATTN_SHARED, FLAG_WEIGHTS_F8 = 1, 2, 4, 8, 16, 32, 64
 PROF_CLASSES = ("norm", "qkv", "rope", "attn", "oproj", "gateup", "down", "allreduce", "head_norm", "lm_head",
                 "sample")
 

@@ -74,6 +74,11 @@ int Engine::init(const dis_engine_config *c) {
   vocab_l = m.vocab / tp_size;
   vocab_off = tp_rank * vocab_l;
   if (m.hidden % 8 || inter_l % 8 || qd_l % 8) return fail(DIS_ERR_INVALID_ARGUMENT, "hidden, inter/tp and n_heads*head_dim/tp must be multiples of 8");
+  if (c->flags & DIS_FLAG_WEIGHTS_F8) {
+    if (m.hidden % 16 || inter_l % 16 || qd_l % 128 || kvd_l % 128)
+      return fail(DIS_ERR_INVALID_ARGUMENT, "DIS_FLAG_WEIGHTS_F8 needs hidden and inter/tp multiples of 16, n_heads*head_dim/tp and n_kv_heads*head_dim/tp multiples of 128");
+    if (c->flags & DIS_FLAG_FORCE_GEMV) return fail(DIS_ERR_INVALID_ARGUMENT, "DIS_FLAG_WEIGHTS_F8 and DIS_FLAG_FORCE_GEMV: the GEMV kernel reads bf16 weights");
+  }
   max_batch = c->max_batch > 0 ? c->max_batch : 32;
   cap_tokens = c->max_step_tokens > 0 ? c->max_step_tokens : 8192;
   cap_tokens = std::max(cap_tokens, max_batch);
@@ -99,19 +104,26 @@ int Engine::init(const dis_engine_config *c) {
   const size_t L = m.layers, H = m.hidden;
   // ---- weights
   ENG_CUDA(dev_alloc(&embed, (size_t)m.vocab * H, &bytes_allocated));
-  ENG_CUDA(dev_alloc(&wqkv, L * nqkv_l * H, &bytes_allocated));
-  ENG_CUDA(dev_alloc(&wo, L * H * qd_l, &bytes_allocated));
-  ENG_CUDA(dev_alloc(&wgu, L * 2 * inter_l * H, &bytes_allocated));
-  ENG_CUDA(dev_alloc(&wdown, L * H * inter_l, &bytes_allocated));
+  f8 = (c->flags & DIS_FLAG_WEIGHTS_F8) != 0;
+  if (!f8) {
+    ENG_CUDA(dev_alloc(&wqkv, L * nqkv_l * H, &bytes_allocated));
+    ENG_CUDA(dev_alloc(&wo, L * H * qd_l, &bytes_allocated));
+    ENG_CUDA(dev_alloc(&wgu, L * 2 * inter_l * H, &bytes_allocated));
+    ENG_CUDA(dev_alloc(&wdown, L * H * inter_l, &bytes_allocated));
+  }
   ENG_CUDA(dev_alloc(&lm_head, (size_t)vocab_l * H, &bytes_allocated));
   ENG_CUDA(dev_alloc(&attn_norm, L * H, &bytes_allocated));
   ENG_CUDA(dev_alloc(&mlp_norm, L * H, &bytes_allocated));
   ENG_CUDA(dev_alloc(&final_norm, H, &bytes_allocated));
-  ENG_CUDA(make_tma_map_2d(&wqkv_map, wqkv, L * nqkv_l, H, 128));
-  ENG_CUDA(make_tma_map_2d(&wo_map, wo, L * H, qd_l, 128));
-  ENG_CUDA(make_tma_map_2d(&wgu_map, wgu, L * 2 * inter_l, H, (uint32_t)gemm_pick_tile_rows(inter_l)));
-  ENG_CUDA(make_tma_map_2d(&wgu_map128, wgu, L * 2 * inter_l, H, 128));
-  ENG_CUDA(make_tma_map_2d(&wdown_map, wdown, L * H, inter_l, 128));
+  if (f8) {
+    ENG_CUDA(init_f8());
+  } else {
+    ENG_CUDA(make_tma_map_2d(&wqkv_map, wqkv, L * nqkv_l, H, 128));
+    ENG_CUDA(make_tma_map_2d(&wo_map, wo, L * H, qd_l, 128));
+    ENG_CUDA(make_tma_map_2d(&wgu_map, wgu, L * 2 * inter_l, H, (uint32_t)gemm_pick_tile_rows(inter_l)));
+    ENG_CUDA(make_tma_map_2d(&wgu_map128, wgu, L * 2 * inter_l, H, 128));
+    ENG_CUDA(make_tma_map_2d(&wdown_map, wdown, L * H, inter_l, 128));
+  }
   ENG_CUDA(make_tma_map_2d(&lm_map, lm_head, vocab_l, H, 128));
   // ---- activations
   const size_t cap = cap_tokens;
@@ -121,7 +133,7 @@ int Engine::init(const dis_engine_config *c) {
   ENG_CUDA(dev_alloc(&xn, cap * H, &bytes_allocated));
   ENG_CUDA(dev_alloc(&q, cap * qd_l, &bytes_allocated));
   ENG_CUDA(dev_alloc(&attn, cap * qd_l, &bytes_allocated));
-  ENG_CUDA(dev_alloc(&act, cap * inter_l, &bytes_allocated));
+  if (!f8) ENG_CUDA(dev_alloc(&act, cap * inter_l, &bytes_allocated));
   ENG_CUDA(dev_alloc(&partial, partial_elems, &bytes_allocated));
   ENG_CUDA(dev_alloc(&logits, (size_t)max_batch * vocab_l, &bytes_allocated));
   attn_scratch_elems = (size_t)(max_batch + 2 * kNumSMs + 64) * nh_l * (2 + m.head_dim);
@@ -146,7 +158,7 @@ int Engine::init(const dis_engine_config *c) {
   for (int i = 0; i < 4; i++) {
     ENG_CUDA(make_tma_map_2d(&xn_map[i], xn, cap, H, boxes[i]));
     ENG_CUDA(make_tma_map_2d(&attn_map[i], attn, cap, qd_l, boxes[i]));
-    ENG_CUDA(make_tma_map_2d(&act_map[i], act, cap, inter_l, boxes[i]));
+    if (!f8) ENG_CUDA(make_tma_map_2d(&act_map[i], act, cap, inter_l, boxes[i]));
   }
   // ---- RoPE tables (computed in double on the host, like the oracle; values only depend on the math)
   {
@@ -287,6 +299,34 @@ int Engine::init(const dis_engine_config *c) {
   return DIS_OK;
 }
 
+// Weights and activations of DIS_FLAG_WEIGHTS_F8
+cudaError_t Engine::init_f8() {
+  const size_t L = m.layers, H = m.hidden, cap = cap_tokens;
+  auto blocks = [](size_t n) { return (n + 127) / 128; };
+  auto weight = [&](F8Weight &f, size_t rows, size_t cols, size_t row_blocks) -> cudaError_t {
+    f.layer_rows = rows;
+    f.layer_scales = row_blocks * blocks(cols);
+    RET_CUDA(dev_alloc(&f.w, L * rows * cols, &bytes_allocated));
+    RET_CUDA(dev_alloc(&f.scale, L * f.layer_scales, &bytes_allocated));
+    RET_CUDA(make_f8_map(&f.map[0], f.w, L * rows, cols, 128));
+    return make_f8_map(&f.map[1], f.w, L * rows, cols, 64);
+  };
+  RET_CUDA(weight(f8_qkv, nqkv_l, H, blocks(nqkv_l)));
+  RET_CUDA(weight(f8_o, H, qd_l, blocks(H)));
+  RET_CUDA(weight(f8_gu, 2 * (size_t)inter_l, H, 2 * blocks(inter_l)));
+  RET_CUDA(weight(f8_down, H, inter_l, blocks(H)));
+  RET_CUDA(dev_alloc(&f8_stage, std::max((size_t)qd_l, (size_t)inter_l) * H, &bytes_allocated));
+  auto rows = [&](uint8_t **x8, float **scale, TmaMap *maps, size_t cols) -> cudaError_t {
+    RET_CUDA(dev_alloc(x8, cap * cols, &bytes_allocated));
+    RET_CUDA(dev_alloc(scale, cap * blocks(cols), &bytes_allocated));
+    for (int i = 0; i < 3; i++) RET_CUDA(make_f8_map(&maps[i], *x8, cap, cols, 32u << i));
+    return cudaSuccess;
+  };
+  RET_CUDA(rows(&xn8, &xn_scale, xn8_map, H));
+  RET_CUDA(rows(&attn8, &attn_scale, attn8_map, qd_l));
+  return rows(&act8, &act_scale, act8_map, inter_l);
+}
+
 // ---- peer-memory exchange set-up: export this rank's symmetric buffer, import everybody's
 int Engine::tp_export(uint8_t out[64]) {
   if (tp_size <= 1 || !sym) return fail(DIS_ERR_INVALID_ARGUMENT, "tp_export: engine is not tensor parallel");
@@ -369,7 +409,8 @@ Engine::~Engine() {
   for (int r = 0; r < kTpMaxRanks; r++) if (peer_base[r]) cudaIpcCloseMemHandle(peer_base[r]);
   void *ptrs[] = {embed, wqkv, wo, wgu, wdown, lm_head, attn_norm, mlp_norm, final_norm, x, partial, logits, ar_buf,
                   attn_scratch, full_logits, gather_buf, cand_val, cand_val_all, cand_tok, cand_tok_all, cand_sum, cand_sum_all, xn, q, attn,
-                  act, d_out_tokens == h_out_tokens ? nullptr : d_out_tokens, kv_pool, kv8_pool, kv8_scale, piece_area, d_page_table, rope_cos, rope_sin, meta_dec.dev, meta_pre.dev, sym};
+                  act, d_out_tokens == h_out_tokens ? nullptr : d_out_tokens, kv_pool, kv8_pool, kv8_scale, piece_area, d_page_table, rope_cos, rope_sin, meta_dec.dev, meta_pre.dev, sym,
+                  f8_qkv.w, f8_qkv.scale, f8_o.w, f8_o.scale, f8_gu.w, f8_gu.scale, f8_down.w, f8_down.scale, f8_stage, xn8, xn_scale, attn8, attn_scale, act8, act_scale};
   for (void *p : ptrs) if (p) cudaFree(p);
   if (h_out_tokens) cudaFreeHost(h_out_tokens);
   if (h_page_table) cudaFreeHost(h_page_table);
@@ -402,6 +443,24 @@ bool Engine::tensor_slot(int kind, int layer, TensorSlot *o) {
     case DIS_T_WUP: s = {wgu + (l * 2 * inter_l + inter_l) * H, (size_t)inter_l, H, H, (size_t)tp_rank * inter_l, 0, (size_t)m.inter, H, false}; break;
     case DIS_T_WDOWN: s = {wdown + l * H * inter_l, H, (size_t)inter_l, (size_t)inter_l, 0, (size_t)tp_rank * inter_l, H, (size_t)m.inter, false}; break;
     default: return false;
+  }
+  if (f8) {  // (a fused weight's tensors start on a block of rows; the up's blocks follow the gate's)
+    F8Weight *f = nullptr;
+    size_t row = 0;
+    switch (kind) {
+      case DIS_T_WQ: f = &f8_qkv; break;
+      case DIS_T_WK: f = &f8_qkv; row = (size_t)qd_l; break;
+      case DIS_T_WV: f = &f8_qkv; row = (size_t)qd_l + kvd_l; break;
+      case DIS_T_WO: f = &f8_o; break;
+      case DIS_T_WGATE: f = &f8_gu; break;
+      case DIS_T_WUP: f = &f8_gu; row = (size_t)inter_l; break;
+      case DIS_T_WDOWN: f = &f8_down; break;
+    }
+    if (f) {
+      s.ptr = f8_stage;
+      s.w8 = f->w + (l * f->layer_rows + row) * s.cols;
+      s.scale8 = f->scale + l * f->layer_scales + (row + 127) / 128 * ((s.cols + 127) / 128);
+    }
   }
   *o = s;
   return true;
@@ -436,7 +495,12 @@ int Engine::load_tensor(int kind, int layer, const void *host, int dtype) {
         for (size_t c = 0; c < s.cols; c++) tmp[r * s.cols + c] = float_to_bf16_bits(f[c]);
       }
     }
-    ENG_CUDA(cudaMemcpy(s.ptr, tmp.data(), n * 2, cudaMemcpyHostToDevice));
+    if (!s.w8) ENG_CUDA(cudaMemcpy(s.ptr, tmp.data(), n * 2, cudaMemcpyHostToDevice));
+    else {  // (on the engine's stream: a plain copy may still be on its way when it returns, and this stream does not wait for it)
+      ENG_CUDA(cudaMemcpyAsync(s.ptr, tmp.data(), n * 2, cudaMemcpyHostToDevice, stream));
+      ENG_CUDA(launch_quant_weight_f8(static_cast<uint16_t *>(s.ptr), s.w8, s.scale8, (int)s.rows, (int)s.cols, stream));
+      ENG_CUDA(cudaStreamSynchronize(stream));  // the next tensor takes the same way
+    }
   }
   return DIS_OK;
 }
@@ -473,8 +537,9 @@ int Engine::load_synthetic(uint64_t seed) {
       RET_CUDA(launch_synth_bf16(tmp, n, seed, kind, pl ? layer : 0, amp, off, idx0, s.cols, s.full_cols, s.col0, stream));
       return launch_bf16_to_f32(tmp, static_cast<float *>(s.ptr), n, stream);
     }
-    return launch_synth_bf16(static_cast<uint16_t *>(s.ptr), n, seed, kind, pl ? layer : 0, amp, off, idx0, s.cols,
-                             s.full_cols, s.col0, stream);
+    RET_CUDA(launch_synth_bf16(static_cast<uint16_t *>(s.ptr), n, seed, kind, pl ? layer : 0, amp, off, idx0, s.cols,
+                               s.full_cols, s.col0, stream));
+    return s.w8 ? launch_quant_weight_f8(static_cast<uint16_t *>(s.ptr), s.w8, s.scale8, (int)s.rows, (int)s.cols, stream) : cudaSuccess;
   };
   for (int k : globals) ENG_CUDA(gen(k, 0));
   for (int l = 0; l < m.layers; l++)
@@ -492,6 +557,7 @@ int Engine::read_tensor(int kind, int layer, uint16_t *host, size_t *n) {
   if (!host || *n < need) { *n = need; return fail(DIS_ERR_INVALID_ARGUMENT, "read_tensor: buffer too small"); }
   *n = need;
   ENG_CUDA(cudaSetDevice(cfg.device));
+  if (s.w8) ENG_CUDA(launch_unquant_weight_f8(s.w8, s.scale8, static_cast<uint16_t *>(s.ptr), (int)s.rows, (int)s.cols, stream));
   ENG_CUDA(cudaStreamSynchronize(stream));
   if (s.f32) {
     std::vector<float> tmp(need);
@@ -682,6 +748,14 @@ cudaError_t Engine::linear_partial(const TmaMap *xmaps, const uint16_t *xptr, co
   return launch_gemm_partial(wmap, xmaps[tile_index(T)], partial, T, N, K, w_row0, s, stream);
 }
 
+// out = partial[T][N], one slice, of 8-bit rows and a layer's 8-bit weight
+cudaError_t Engine::linear_f8(const F8Weight &w, int layer, const TmaMap *xmaps, const float *xs, int T, int N, int K) {
+  const uint32_t tb = gemm_f8_token_box(T, N, K, false), fb = gemm_f8_feature_box(T, N, K, false);
+  kernel_launches++;
+  return launch_gemm_f8(w.map[fb == 64 ? 1 : 0], xmaps[tb == 32 ? 0 : tb == 64 ? 1 : 2], xs, w.scale + (size_t)layer * w.layer_scales, partial, false, T, N, K,
+                        (int)(layer * w.layer_rows), stream);
+}
+
 // Tensor parallel: sum the split-K slices, all-reduce over ranks; afterwards the data is ar_buf[T][H].
 cudaError_t Engine::allreduce_partials(int split, int T) {
   const long long n = (long long)T * m.hidden;
@@ -697,7 +771,8 @@ cudaError_t Engine::allreduce_partials(int split, int T) {
 
 // x (+)= the pending projection output (summed over split-K slices and, under tensor parallelism, over the
 // ranks); xn = bf16(RMSNorm(x) * gain).  With row_map only `rows` gathered rows are normalised (logits rows).
-cudaError_t Engine::consume_pending(const float *gain, const int *row_map, int rows, int T) {
+// to_f8: the rows leave in 8 bits (xn8, xn_scale) instead.
+cudaError_t Engine::consume_pending(const float *gain, const int *row_map, int rows, int T, bool to_f8) {
   const int H = m.hidden;
   if (pend_needs_ar) {
     // fused exchange over peer memory: split-K reduce + all-reduce + residual + norm in one kernel
@@ -706,13 +781,17 @@ cudaError_t Engine::consume_pending(const float *gain, const int *row_map, int r
                                    cur_meta->d<uint32_t>(cur_meta->o_arstep), (uint32_t)idx, idx & 1, T, H, m.rms_eps, stream));
     kernel_launches++;
     pend_needs_ar = false; pend_ptr = nullptr; pend_count = 0;
+    if (to_f8) {
+      kernel_launches++;
+      return launch_quant_f8(xn, xn8, xn_scale, rows, H, stream);
+    }
     if (!row_map) return cudaSuccess;
     kernel_launches++;  // x is complete: gather the rows that need logits
     return launch_add_rmsnorm(x, nullptr, nullptr, nullptr, 0, 0, gain, xn, row_map, rows, H, m.rms_eps, stream);
   }
   kernel_launches++;
-  const cudaError_t r = launch_add_rmsnorm(x, nullptr, nullptr, pend_ptr, pend_count, pend_str, gain, xn, row_map, rows, H,
-                                           m.rms_eps, stream);
+  const cudaError_t r = to_f8 ? launch_add_rmsnorm_f8(x, nullptr, nullptr, pend_ptr, pend_count, pend_str, gain, xn8, xn_scale, row_map, rows, H, m.rms_eps, stream)
+                              : launch_add_rmsnorm(x, nullptr, nullptr, pend_ptr, pend_count, pend_str, gain, xn, row_map, rows, H, m.rms_eps, stream);
   pend_ptr = nullptr; pend_count = 0;
   return r;
 }
@@ -744,7 +823,7 @@ int Engine::common_pages(int n, const int *slots) const {
 
 cudaError_t Engine::enqueue_layers(int T, int n_splits) {
   const int H = m.hidden, d = m.head_dim;
-  const bool gemv = (cfg.flags & DIS_FLAG_FORCE_GEMV) || T <= gemv_max_t;
+  const bool gemv = !f8 && ((cfg.flags & DIS_FLAG_FORCE_GEMV) || T <= gemv_max_t);
   const bool fused_ar = tp_size > 1 && tp_custom && (T <= ar_cap_rows || T <= ar_cap_big);  // exchange over peer memory, no NCCL kernel
   const bool pdl_ok = use_pdl && !profiling && (tp_size == 1 || fused_ar);
   // the PDL switch is thread-local state of the launch helper: whatever way this function is left, later
@@ -770,16 +849,18 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
     prof_mark(P_NORM);
     if (l == 0) {
       pdl_enabled() = false;  // the step's first kernel follows its metadata
-      RET_CUDA(launch_add_rmsnorm(x, tokens, embed, nullptr, 0, 0, attn_norm, xn, nullptr, T, H, m.rms_eps, stream));
+      if (f8) RET_CUDA(launch_add_rmsnorm_f8(x, tokens, embed, nullptr, 0, 0, attn_norm, xn8, xn_scale, nullptr, T, H, m.rms_eps, stream));
+      else RET_CUDA(launch_add_rmsnorm(x, tokens, embed, nullptr, 0, 0, attn_norm, xn, nullptr, T, H, m.rms_eps, stream));
       kernel_launches++;
     } else {
       pdl_enabled() = pdl_ok;
-      if (!skip(P_NORM)) RET_CUDA(consume_pending(attn_norm + (size_t)l * H, nullptr, T, T));
+      if (!skip(P_NORM)) RET_CUDA(consume_pending(attn_norm + (size_t)l * H, nullptr, T, T, f8));
     }
     pdl_enabled() = pdl_ok;
     int s_qkv = 1;
     prof_mark(P_QKV);
-    if (!skip(P_QKV)) RET_CUDA(linear_partial(xn_map, xn, wqkv_map, wqkv, l * nqkv_l, T, nqkv_l, H, &s_qkv));
+    if (f8) { if (!skip(P_QKV)) RET_CUDA(linear_f8(f8_qkv, l, xn8_map, xn_scale, T, nqkv_l, H)); }
+    else if (!skip(P_QKV)) RET_CUDA(linear_partial(xn_map, xn, wqkv_map, wqkv, l * nqkv_l, T, nqkv_l, H, &s_qkv));
     else s_qkv = gemm_pick_split_k(T, nqkv_l, H);
     const int pool_layer = kv8_pool ? 0 : l;
     uint16_t *pool = kv_pool + (size_t)pool_layer * kv_layer_stride;
@@ -833,13 +914,26 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
     }
     int s_o = 1;
     prof_mark(P_OPROJ);
-    if (!skip(P_OPROJ)) RET_CUDA(linear_partial(attn_map, attn, wo_map, wo, l * H, T, H, qd_l, &s_o));
+    if (f8) {
+      if (!skip(P_OPROJ)) {
+        RET_CUDA(launch_quant_f8(attn, attn8, attn_scale, T, qd_l, stream));
+        kernel_launches++;
+        RET_CUDA(linear_f8(f8_o, l, attn8_map, attn_scale, T, H, qd_l));
+      }
+    } else if (!skip(P_OPROJ)) RET_CUDA(linear_partial(attn_map, attn, wo_map, wo, l * H, T, H, qd_l, &s_o));
     else s_o = gemm_pick_split_k(T, H, qd_l);
     RET_CUDA(set_pending(s_o));
     prof_mark(P_NORM);
-    if (!skip(P_NORM)) RET_CUDA(consume_pending(mlp_norm + (size_t)l * H, nullptr, T, T));
+    if (!skip(P_NORM)) RET_CUDA(consume_pending(mlp_norm + (size_t)l * H, nullptr, T, T, f8));
     prof_mark(P_GATEUP);
-    if (gemv) {
+    if (f8) {
+      const uint32_t tb = gemm_f8_token_box(T, inter_l, H, true);
+      if (!skip(P_GATEUP)) {
+        RET_CUDA(launch_gemm_silu_f8(f8_gu.map[0], xn8_map[tb == 32 ? 0 : tb == 64 ? 1 : 2], xn_scale, f8_gu.scale + (size_t)l * f8_gu.layer_scales, act8, act_scale, T,
+                                     inter_l, H, (int)(l * f8_gu.layer_rows), stream));
+        kernel_launches++;
+      }
+    } else if (gemv) {
       RET_CUDA(launch_gemv_silu(xn, wgu + (size_t)l * 2 * inter_l * H, act, T, inter_l, H, stream));
       kernel_launches += (uint64_t)((T + kGemvMaxT - 1) / kGemvMaxT);
     } else if (use_persist && gemm_use_persist(T, inter_l, H, 1, true)) {
@@ -862,7 +956,8 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
     }
     int s_d = 1;
     prof_mark(P_DOWN);
-    if (!skip(P_DOWN)) RET_CUDA(linear_partial(act_map, act, wdown_map, wdown, l * H, T, H, inter_l, &s_d));
+    if (f8) { if (!skip(P_DOWN)) RET_CUDA(linear_f8(f8_down, l, act8_map, act_scale, T, H, inter_l)); }
+    else if (!skip(P_DOWN)) RET_CUDA(linear_partial(act_map, act, wdown_map, wdown, l * H, T, H, inter_l, &s_d));
     else s_d = gemm_pick_split_k(T, H, inter_l);
     RET_CUDA(set_pending(s_d));
   }

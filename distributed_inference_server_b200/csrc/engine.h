@@ -90,6 +90,19 @@ struct Engine {
   // weights
   uint16_t *embed = nullptr, *wqkv = nullptr, *wo = nullptr, *wgu = nullptr, *wdown = nullptr, *lm_head = nullptr;
   float *attn_norm = nullptr, *mlp_norm = nullptr, *final_norm = nullptr;
+  // DIS_FLAG_WEIGHTS_F8: the layers' projections in 8-bit floating point (f8.cuh) instead, all layers' rows one behind the other
+  struct F8Weight {
+    uint8_t *w = nullptr;
+    float *scale = nullptr;
+    size_t layer_rows = 0, layer_scales = 0;
+    TmaMap map[2];  // boxes of 128 and of 64 rows
+  };
+  bool f8 = false;
+  F8Weight f8_qkv, f8_o, f8_gu, f8_down;
+  uint16_t *f8_stage = nullptr;  // one tensor in bf16, on its way into 8 bits or back
+  uint8_t *xn8 = nullptr, *attn8 = nullptr, *act8 = nullptr;
+  float *xn_scale = nullptr, *attn_scale = nullptr, *act_scale = nullptr;
+  TmaMap xn8_map[3], attn8_map[3], act8_map[3];  // box rows 32 / 64 / 128
   TmaMap wqkv_map, wo_map, wgu_map, wgu_map128, wdown_map, lm_map;  // wgu_map: balanced tile height, wgu_map128: 128-row boxes
   // activations
   float *x = nullptr, *partial = nullptr, *logits = nullptr, *ar_buf = nullptr, *attn_scratch = nullptr;
@@ -172,7 +185,9 @@ struct Engine {
   bool rowmap_identity = true;  // decode: logits row i is token i
   int tp_export(uint8_t out[64]);
   int tp_import(const uint8_t *handles);
-  cudaError_t consume_pending(const float *gain, const int *row_map, int rows, int T);
+  cudaError_t consume_pending(const float *gain, const int *row_map, int rows, int T, bool to_f8 = false);
+  cudaError_t init_f8();
+  cudaError_t linear_f8(const F8Weight &w, int layer, const TmaMap *xmaps, const float *xs, int T, int N, int K);
 
   // layer-list decoders (stack.cu): the same sequences, pages, planner and sampler; prompt = the whole token history
   StackModel *stack = nullptr;
@@ -244,7 +259,7 @@ struct Engine {
   cudaError_t gather_full_logits(int R);
   int pick_attn_splits(int T, int max_ctx_in_batch) const;
   uint32_t finish_check(Sequence &s, uint32_t tok);
-  struct TensorSlot { void *ptr; size_t rows, cols, ld, row0, col0, full_rows, full_cols; bool f32; };
+  struct TensorSlot { void *ptr; size_t rows, cols, ld, row0, col0, full_rows, full_cols; bool f32; uint8_t *w8; float *scale8; };
   bool tensor_slot(int kind, int layer, TensorSlot *out);
 };
 

@@ -112,8 +112,8 @@ int Engine::init_stack(const dis_engine_config *c, const dis_stack_config *sc) {
   if (c->tp_size > 1) return fail(DIS_ERR_INVALID_ARGUMENT, "stack: tensor parallelism is not available for this family");
   if (c->flags & DIS_FLAG_PREFIX_CACHE)
     return fail(DIS_ERR_INVALID_ARGUMENT, "stack: the prefix cache cannot serve a family with recurrent state (a page does not hold it)");
-  if (c->flags & (DIS_FLAG_KV_INT8 | DIS_FLAG_ATTN_SHARED))
-    return fail(DIS_ERR_INVALID_ARGUMENT, "stack: DIS_FLAG_KV_INT8 and DIS_FLAG_ATTN_SHARED are for the Llama family");
+  if (c->flags & (DIS_FLAG_KV_INT8 | DIS_FLAG_ATTN_SHARED | DIS_FLAG_WEIGHTS_F8))
+    return fail(DIS_ERR_INVALID_ARGUMENT, "stack: DIS_FLAG_KV_INT8, DIS_FLAG_ATTN_SHARED and DIS_FLAG_WEIGHTS_F8 are for the Llama family");
   if (sc->compute_dtype != DIS_F32 && sc->compute_dtype != DIS_BF16) return fail(DIS_ERR_INVALID_ARGUMENT, "stack: compute_dtype");
   if (sc->canon_taps < 0 || sc->canon_taps > 16) return fail(DIS_ERR_INVALID_ARGUMENT, "stack: canon_taps must be 0..16");
   memset(&m, 0, sizeof(m));

@@ -75,8 +75,8 @@ typedef struct dis_model_config {
 } dis_model_config;
 
 /* Engine configuration: WorkerConfig (design.md:316-322) plus what it lacks for a GPU path.
- * `Quantization` (design.md:326-332) has no bf16 variant; this engine is bf16 weights / fp32
- * accumulate only. */
+ * `Quantization` (design.md:326-332) has no bf16 variant; this engine has bf16 weights, or 8-bit floating point ones
+ * (DIS_FLAG_WEIGHTS_F8), and fp32 sums. */
 #define DIS_FLAG_NO_GRAPH 1u   /* do not capture the decode step in a CUDA graph */
 #define DIS_FLAG_FORCE_GEMV 2u /* debugging: run every projection through the GEMV kernel */
 #define DIS_FLAG_NO_PDL 4u     /* launch the kernels of a step without programmatic dependent launch */
@@ -88,6 +88,12 @@ typedef struct dis_model_config {
 #define DIS_FLAG_ATTN_SHARED 32u /* decode steps read the pages that all of their sequences have in common once (dis_k_attn_shared), where that pays;
                                    such pages come from DIS_FLAG_PREFIX_CACHE.  Both flags need 1, 2, 4 or 8 query heads per kv head and are refused
                                    for layer-list decoders */
+#define DIS_FLAG_WEIGHTS_F8 64u  /* the layers' projections (q, k, v, o, gate, up, down) in 8-bit floating point with a scale for each block of 128 x 128
+                                   (see dis_k_gemm_f8): half the bytes of a decode step and twice the tensor rate of a prompt.  Tensors are loaded as ever
+                                   and turned into 8 bits on the way; dis_engine_read_tensor returns what they stand for, which bf16 holds exactly.  Their
+                                   inputs are rounded to 8 bits in blocks of 128 entries too; embeddings, norms, attention and the logits' head stay as they
+                                   are.  Needs hidden and inter / tp multiples of 16, n_heads * head_dim / tp and n_kv_heads * head_dim / tp multiples of 128,
+                                   and is refused with DIS_FLAG_FORCE_GEMV and for layer-list decoders */
 typedef struct dis_engine_config {
   dis_model_config model;
   int32_t device;              /* CUDA ordinal (WorkerConfig.gpu_layers has no meaning here) */
