@@ -455,15 +455,17 @@ static int gemm_f8_out(const char *me, const void *out, int out_dtype) {
 }
 static cudaError_t gemm_f8_call(const uint8_t *x8, const float *xs, const uint8_t *w8, const float *ws, void *out, int out_dtype, int T, int N, int K, cudaStream_t st) {
   dis::TmaMap wm, xm;
-  cudaError_t e = dis::make_f8_map(&wm, w8, (uint64_t)N, (uint64_t)K, dis::gemm_f8_feature_box(T, N, K, false));
-  if (e == cudaSuccess) e = dis::make_f8_map(&xm, x8, (uint64_t)T, (uint64_t)K, dis::gemm_f8_token_box(T, N, K, false));
+  const dis::F8Boxes box = dis::gemm_f8_boxes(T, N, K, false);
+  cudaError_t e = dis::make_f8_map(&wm, w8, (uint64_t)N, (uint64_t)K, box.feature_rows, box.depth);
+  if (e == cudaSuccess) e = dis::make_f8_map(&xm, x8, (uint64_t)T, (uint64_t)K, box.token_rows, box.depth);
   if (e != cudaSuccess) return e;
   return dis::launch_gemm_f8(wm, xm, xs, ws, out, out_dtype == DIS_BF16, T, N, K, 0, st);
 }
 static cudaError_t gemm_silu_f8_call(const uint8_t *x8, const float *xs, const uint8_t *wgu8, const float *wgus, uint8_t *h8, float *hs, int T, int I, int K, cudaStream_t st) {
   dis::TmaMap wm, xm;
-  cudaError_t e = dis::make_f8_map(&wm, wgu8, 2ull * I, (uint64_t)K, dis::gemm_f8_feature_box(T, I, K, true));
-  if (e == cudaSuccess) e = dis::make_f8_map(&xm, x8, (uint64_t)T, (uint64_t)K, dis::gemm_f8_token_box(T, I, K, true));
+  const dis::F8Boxes box = dis::gemm_f8_boxes(T, I, K, true);
+  cudaError_t e = dis::make_f8_map(&wm, wgu8, 2ull * I, (uint64_t)K, box.feature_rows, box.depth);
+  if (e == cudaSuccess) e = dis::make_f8_map(&xm, x8, (uint64_t)T, (uint64_t)K, box.token_rows, box.depth);
   if (e != cudaSuccess) return e;
   return dis::launch_gemm_silu_f8(wm, xm, xs, wgus, h8, hs, T, I, K, 0, st);
 }

@@ -299,6 +299,10 @@ int Engine::init(const dis_engine_config *c) {
   return DIS_OK;
 }
 
+// Which map of an 8-bit weight (F8Weight::map) and of 8-bit rows (xn8_map, ...) has the boxes that a product asks for
+static int f8_weight_map(const F8Boxes &b) { return b.feature_rows == 64 ? 2 : b.depth == 2 ? 1 : 0; }
+static int f8_token_map(const F8Boxes &b) { return b.depth == 2 ? 3 : b.token_rows == 32 ? 0 : b.token_rows == 64 ? 1 : 2; }
+
 // Weights and activations of DIS_FLAG_WEIGHTS_F8
 cudaError_t Engine::init_f8() {
   const size_t L = m.layers, H = m.hidden, cap = cap_tokens;
@@ -308,8 +312,10 @@ cudaError_t Engine::init_f8() {
     f.layer_scales = row_blocks * blocks(cols);
     RET_CUDA(dev_alloc(&f.w, L * rows * cols, &bytes_allocated));
     RET_CUDA(dev_alloc(&f.scale, L * f.layer_scales, &bytes_allocated));
-    RET_CUDA(make_f8_map(&f.map[0], f.w, L * rows, cols, 128));
-    return make_f8_map(&f.map[1], f.w, L * rows, cols, 64);
+    const uint32_t deep = cols % 128 == 0 ? 2 : 1;
+    RET_CUDA(make_f8_map(&f.map[0], f.w, L * rows, cols, 128, 1));
+    RET_CUDA(make_f8_map(&f.map[1], f.w, L * rows, cols, 128, deep));
+    return make_f8_map(&f.map[2], f.w, L * rows, cols, 64, deep);
   };
   RET_CUDA(weight(f8_qkv, nqkv_l, H, blocks(nqkv_l)));
   RET_CUDA(weight(f8_o, H, qd_l, blocks(H)));
@@ -319,8 +325,8 @@ cudaError_t Engine::init_f8() {
   auto rows = [&](uint8_t **x8, float **scale, TmaMap *maps, size_t cols) -> cudaError_t {
     RET_CUDA(dev_alloc(x8, cap * cols, &bytes_allocated));
     RET_CUDA(dev_alloc(scale, cap * blocks(cols), &bytes_allocated));
-    for (int i = 0; i < 3; i++) RET_CUDA(make_f8_map(&maps[i], *x8, cap, cols, 32u << i));
-    return cudaSuccess;
+    for (int i = 0; i < 3; i++) RET_CUDA(make_f8_map(&maps[i], *x8, cap, cols, 32u << i, 1));
+    return make_f8_map(&maps[3], *x8, cap, cols, 128, cols % 128 == 0 ? 2 : 1);
   };
   RET_CUDA(rows(&xn8, &xn_scale, xn8_map, H));
   RET_CUDA(rows(&attn8, &attn_scale, attn8_map, qd_l));
@@ -750,9 +756,9 @@ cudaError_t Engine::linear_partial(const TmaMap *xmaps, const uint16_t *xptr, co
 
 // out = partial[T][N], one slice, of 8-bit rows and a layer's 8-bit weight
 cudaError_t Engine::linear_f8(const F8Weight &w, int layer, const TmaMap *xmaps, const float *xs, int T, int N, int K) {
-  const uint32_t tb = gemm_f8_token_box(T, N, K, false), fb = gemm_f8_feature_box(T, N, K, false);
+  const F8Boxes box = gemm_f8_boxes(T, N, K, false);
   kernel_launches++;
-  return launch_gemm_f8(w.map[fb == 64 ? 1 : 0], xmaps[tb == 32 ? 0 : tb == 64 ? 1 : 2], xs, w.scale + (size_t)layer * w.layer_scales, partial, false, T, N, K,
+  return launch_gemm_f8(w.map[f8_weight_map(box)], xmaps[f8_token_map(box)], xs, w.scale + (size_t)layer * w.layer_scales, partial, false, T, N, K,
                         (int)(layer * w.layer_rows), stream);
 }
 
@@ -927,9 +933,9 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
     if (!skip(P_NORM)) RET_CUDA(consume_pending(mlp_norm + (size_t)l * H, nullptr, T, T, f8));
     prof_mark(P_GATEUP);
     if (f8) {
-      const uint32_t tb = gemm_f8_token_box(T, inter_l, H, true);
+      const F8Boxes box = gemm_f8_boxes(T, inter_l, H, true);
       if (!skip(P_GATEUP)) {
-        RET_CUDA(launch_gemm_silu_f8(f8_gu.map[0], xn8_map[tb == 32 ? 0 : tb == 64 ? 1 : 2], xn_scale, f8_gu.scale + (size_t)l * f8_gu.layer_scales, act8, act_scale, T,
+        RET_CUDA(launch_gemm_silu_f8(f8_gu.map[f8_weight_map(box)], xn8_map[f8_token_map(box)], xn_scale, f8_gu.scale + (size_t)l * f8_gu.layer_scales, act8, act_scale, T,
                                      inter_l, H, (int)(l * f8_gu.layer_rows), stream));
         kernel_launches++;
       }

@@ -95,14 +95,14 @@ struct Engine {
     uint8_t *w = nullptr;
     float *scale = nullptr;
     size_t layer_rows = 0, layer_scales = 0;
-    TmaMap map[2];  // boxes of 128 and of 64 rows
+    TmaMap map[3];  // as f8_weight_map picks
   };
   bool f8 = false;
   F8Weight f8_qkv, f8_o, f8_gu, f8_down;
   uint16_t *f8_stage = nullptr;  // one tensor in bf16, on its way into 8 bits or back
   uint8_t *xn8 = nullptr, *attn8 = nullptr, *act8 = nullptr;
   float *xn_scale = nullptr, *attn_scale = nullptr, *act_scale = nullptr;
-  TmaMap xn8_map[3], attn8_map[3], act8_map[3];  // box rows 32 / 64 / 128
+  TmaMap xn8_map[4], attn8_map[4], act8_map[4];  // as f8_token_map picks
   TmaMap wqkv_map, wo_map, wgu_map, wgu_map128, wdown_map, lm_map;  // wgu_map: balanced tile height, wgu_map128: 128-row boxes
   // activations
   float *x = nullptr, *partial = nullptr, *logits = nullptr, *ar_buf = nullptr, *attn_scratch = nullptr;

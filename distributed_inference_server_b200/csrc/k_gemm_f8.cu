@@ -14,7 +14,7 @@
 // Two kernels:
 //   tile  a CTA per 128 x 128 (gate-up: 128 x 128 + 128) tile and, where the tiles are few, a cluster of up to eight CTAs that share its K:
 //         each leaves its sums in its own shared memory, and after a cluster barrier every CTA finishes a share of the tokens.
-//   pair  two CTAs per 256 x 256 tile (cta_group::2), persistent, for many tokens: an SM brings 32 KB per block for 512 clocks of the
+//   pair  two CTAs per 256 x 256 (or 256 x 128) tile (cta_group::2), persistent, for many tokens: an SM brings 32 KB per block for 512 clocks of the
 //         tensor pipe, and reads its 128 x 256 sums from TMEM in the meantime.
 #include <cuda.h>
 
@@ -372,10 +372,10 @@ constexpr int kF8GroupBytes = kF8Group * 128 * 2 * 4;
 
 template <int BN>
 struct PairCfg {
-  static constexpr int kProducts = BN / 128, kBufs = 4 / kProducts;  // of a block; accumulators of each product
-  static constexpr int kFeatRows = BN / 2;                           // of one CTA
-  static constexpr int kStage = kF8Box + kFeatRows * kF8Block;       // one CTA's 128 token rows and its feature rows of a block
-  static constexpr int kStages = BN == 256 ? 6 : 8;
+  static constexpr int kProducts = BN / 128, kBufs = 4 / kProducts;   // of a block; accumulators of each product
+  static constexpr int kFeatBox = BN / 2 * kF8Block;                  // bytes of one CTA's feature rows of a block
+  static constexpr int kStage = 2 * kF8Box + 2 * kFeatBox;            // one CTA's part of two blocks: token rows, token rows, feature rows, feature rows
+  static constexpr int kStages = BN == 256 ? 3 : 4;
   static constexpr int kSmem = kStages * kStage + kF8Groups * kF8GroupBytes + 1024 + 256 + 1024;
 };
 
@@ -391,12 +391,20 @@ __device__ __forceinline__ void mbar_wait_soon(uint32_t bar, uint32_t parity) {
       : "memory");
   if (!ok) mbar_wait(bar, parity);
 }
+// Two blocks of a box's rows, {128 entries, rows, blocks} (make_f8_map with depth 2), one behind the other
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void *map, int c0, int c1, int c2, uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+      : "memory");
+}
 
 template <int kOut, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8PairThreads, 1)
 gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const float *__restrict__ xs,
                     const float *__restrict__ ws, void *__restrict__ out, float *__restrict__ out_scale, int T, int N, int K, int w_row0,
-                    int w_row_step, int tiles_n, int tiles_t, int t_fast, int wide) {
+                    int w_row_step, int tiles_n, int tiles_t, int t_fast, int deep, int wide) {
   using Cfg = PairCfg<BN>;
   constexpr bool kGated = kOut == kF8OutGated;
   constexpr int kTileN = kGated ? BN / 2 : BN;
@@ -425,7 +433,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&w_map);
     tma_prefetch_desc(&x_map);
-    for (int s = 0; s < Cfg::kStages; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), Cfg::kProducts); }
+    for (int s = 0; s < Cfg::kStages; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 2); }
     for (uint32_t i = 0; i < 4; i++) { mbar_init(acc_full(i), 1); mbar_init(acc_empty(i), 16 / Cfg::kProducts); }  // warps of both CTAs
     for (uint32_t g = 0; g < kF8Groups; g++) { mbar_init(f_full(g), 1); mbar_init(f_empty(g), 8); }
     fence_barrier_init();
@@ -452,12 +460,22 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
         uint32_t phase = 0;
         for (int tile = pair; tile < n_tiles; tile += pairs) {
           const int t0 = tile_t0(tile), wr = w_row0 + tile_n(tile) * kTileN + (int)rank * w_row_step;  // (gated: gate rows | up rows)
-          for (int kb = 0; kb < num_kb; kb++) {
-            mbar_wait(empty_bar(s), phase ^ 1u);  // passes on the first lap
-            if (rank == 0) mbar_expect_tx(full_bar(s), 2 * Cfg::kStage);
-            const uint32_t bar = cluster_bar(full_bar(s), 0), a = smem_base + s * Cfg::kStage;
-            tma_load_2d_pair(a, &x_map, kb * kF8Block, t0, bar, x_hint);
-            tma_load_2d_pair(a + kF8Box, &w_map, kb * kF8Block, wr, bar, w_hint);
+          for (int kb = 0; kb < num_kb; kb += 2) {
+            mbar_wait_soon(empty_bar(s), phase ^ 1u);  // passes on the first lap
+            const bool two = deep || kb + 1 < num_kb;  // (past K a box is zeros, as long as any other)
+            if (rank == 0) mbar_expect_tx(full_bar(s), two ? 2 * Cfg::kStage : Cfg::kStage);
+            const uint32_t bar = cluster_bar(full_bar(s), 0), a = smem_base + s * Cfg::kStage, w = a + 2 * kF8Box;
+            if (deep) {
+              tma_load_3d_pair(a, &x_map, 0, t0, kb, bar, x_hint);
+              tma_load_3d_pair(w, &w_map, 0, wr, kb, bar, w_hint);
+            } else {
+              tma_load_2d_pair(a, &x_map, kb * kF8Block, t0, bar, x_hint);
+              tma_load_2d_pair(w, &w_map, kb * kF8Block, wr, bar, w_hint);
+              if (two) {
+                tma_load_2d_pair(a + kF8Box, &x_map, (kb + 1) * kF8Block, t0, bar, x_hint);
+                tma_load_2d_pair(w + Cfg::kFeatBox, &w_map, (kb + 1) * kF8Block, wr, bar, w_hint);
+              }
+            }
             if (++s == Cfg::kStages) { s = 0; phase ^= 1u; }
           }
         }
@@ -509,22 +527,28 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
       int s = 0;
       for (int tile = pair; tile < n_tiles; tile += pairs)
         for (int kb = 0; kb < num_kb; kb++) {
+          const uint32_t second = kb & 1;  // of the stage's two blocks
+          const bool last = second || kb == num_kb - 1;
           if (BN == 256 || (buf & 1u) == mine) {
             const uint32_t h = BN == 256 ? mine : 0u, slot = buf * Cfg::kProducts + h;
-            mbar_wait_soon(full_bar(s), phase);
+            if (BN == 128 || !second) mbar_wait_soon(full_bar(s), phase);
             mbar_wait_soon(acc_empty(slot), aphase ^ 1u);  // both CTAs have taken this buffer (passes on first use)
             tc_fence_after();
             if (elect_one()) {
+              const uint32_t a = lo + second * (kF8Box >> 4), w = lo + ((2 * kF8Box + second * Cfg::kFeatBox + h * (kF8Box / 2)) >> 4);
 #pragma unroll
-              for (uint32_t k = 0; k < 4; k++)
-                umma_f8_pair(tmem_base + slot * 128u, lo + 2 * k, lo + ((kF8Box + h * (kF8Box / 2)) >> 4) + 2 * k, idesc, k > 0 ? 1u : 0u);
+              for (uint32_t k = 0; k < 4; k++) umma_f8_pair(tmem_base + slot * 128u, a + 2 * k, w + 2 * k, idesc, k > 0 ? 1u : 0u);
               umma_commit_pair(acc_full(slot));
-              umma_commit_pair(empty_bar(s));
+              // A stage is empty after two commits: of both warps (256 columns) or of both blocks, whoever issued them (128)
+              if (BN == 256 ? last : true) umma_commit_pair(empty_bar(s));
+              if (BN == 128 && last && !second) umma_commit_pair(empty_bar(s));
             }
             __syncwarp();
           }
-          lo += Cfg::kStage >> 4;
-          if (++s == Cfg::kStages) { s = 0; phase ^= 1u; lo = lo0; }
+          if (last) {
+            lo += Cfg::kStage >> 4;
+            if (++s == Cfg::kStages) { s = 0; phase ^= 1u; lo = lo0; }
+          }
           if (++buf == Cfg::kBufs) { buf = 0; aphase ^= 1u; }
         }
     }
@@ -697,6 +721,10 @@ int tile_cost(int T, int N, int K) {
   const long long cost = 600 + (split > 1 ? 100 : 0) + 60 * per * rounds;
   return cost > 0x7fffffff ? 0x7fffffff : (int)cost;
 }
+// Blocks that a load of the pair kernel brings: two where rows hold whole blocks only (past the end of a row that does not, the second would be
+// the next row's start).  A thread's wait, expectation and two loads take it 0.37 us, as long as a block's MMAs, whatever the boxes' size.
+uint32_t f8_depth(int K) { return K % kF8Block == 0 ? 2u : 1u; }
+
 // Columns of a pair's tile.  (Gated: 256, a tile is a block of 128 features under one scale.)  us with 128 / 256: 4096 x 4096, 512 tokens 13.8 / 18.0, 1024
 // tokens 21.5 / 20.4.
 int pair_f8_columns(int T, int N, int K, bool gated) { return gated || pair_f8_cost(T, N, K, 256) <= pair_f8_cost(T, N, K, 128) ? 256 : 128; }
@@ -720,8 +748,8 @@ cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float
   const int pairs = n_tiles < kNumSMs / 2 ? (int)n_tiles : kNumSMs / 2;
   const int t_fast = (long long)(kOut == kF8OutGated ? 2 : 1) * N > (long long)T ? 1 : 0;  // as gemm_pair_kernel: the smaller operand stays in L2
   return launch_k(gemm_f8_pair_kernel<kOut, BN>, dim3(2 * pairs), dim3(kF8PairThreads), (size_t)Cfg::kSmem, st, *reinterpret_cast<const CUtensorMap *>(&w_map),
-                  *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, T, N, K, w_row0, kOut == kF8OutGated ? N : Cfg::kFeatRows, tiles_n, tiles_t,
-                  t_fast, wide);
+                  *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, T, N, K, w_row0, kOut == kF8OutGated ? N : BN / 2, tiles_n, tiles_t,
+                  t_fast, f8_depth(K) == 2, wide);
 }
 
 }  // namespace
@@ -734,9 +762,9 @@ bool gemm_f8_in_pairs(int T, int N, int K, bool gated) {
   const int narrow = pair_f8_cost(T, N, K, 128), wide = pair_f8_cost(T, N, K, 256);
   return (narrow < wide ? narrow : wide) < tile_cost(T, N, K);
 }
-uint32_t gemm_f8_token_box(int T, int N, int K, bool gated) { return gemm_f8_in_pairs(T, N, K, gated) ? 128u : (uint32_t)tile_tokens(T); }
-uint32_t gemm_f8_feature_box(int T, int N, int K, bool gated) {
-  return gemm_f8_in_pairs(T, N, K, gated) && pair_f8_columns(T, N, K, gated) == 128 ? 64u : 128u;
+F8Boxes gemm_f8_boxes(int T, int N, int K, bool gated) {
+  if (!gemm_f8_in_pairs(T, N, K, gated)) return {(uint32_t)tile_tokens(T), 128u, 1u};
+  return {128u, pair_f8_columns(T, N, K, gated) == 128 ? 64u : 128u, f8_depth(K)};
 }
 
 cudaError_t launch_gemm_f8(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, bool bf16, int T, int N, int K, int w_row0,

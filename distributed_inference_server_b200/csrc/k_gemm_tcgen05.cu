@@ -249,8 +249,20 @@ static cudaError_t make_map(TmaMap *out, const void *base, uint64_t rows, uint64
 cudaError_t make_tma_map_2d(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
   return make_map(out, base, rows, cols, box_rows, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2);
 }
-cudaError_t make_f8_map(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
-  return make_map(out, base, rows, cols, box_rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
+cudaError_t make_f8_map(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t depth) {
+  if (depth == 1) return make_map(out, base, rows, cols, box_rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
+  // {128 entries, rows, blocks of 128 entries}: a box of `depth` blocks lands as that many boxes one behind the other
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) { set_last_error("cuTensorMapEncodeTiled is not available from this driver"); return cudaErrorNotSupported; }
+  if (cols % 128 != 0 || ((uintptr_t)base & 15u) || box_rows == 0 || box_rows > 256) { set_last_error("TMA map: rows of whole blocks of 128, base 16-byte aligned, box rows 1..256"); return cudaErrorInvalidValue; }
+  const cuuint64_t dims[3] = {128, rows, cols / 128};
+  const cuuint64_t strides[2] = {cols, 128};
+  const cuuint32_t box[3] = {128, box_rows, depth};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(reinterpret_cast<CUtensorMap *>(out), CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { set_last_error("cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r)); return cudaErrorInvalidValue; }
+  return cudaSuccess;
 }
 
 // UMMA N (token tile): 32 / 64 for decode batches (HBM-bound), 128 and 256 for prefill (the wider the token tile,

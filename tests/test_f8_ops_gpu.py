@@ -192,7 +192,7 @@ def sums_off(xv, wv):
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("T,N,K", [(1, 4096, 4096), (1, 1, 16), (2, 130, 272), (31, 1001, 1040), (32, 6144, 4096), (33, 256, 128), (64, 512, 2048), (65, 2560, 2048),
                                    (77, 1001, 1040), (128, 128, 14336), (129, 300, 400), (256, 4096, 1024), (257, 512, 512), (300, 1001, 1040), (513, 260, 144),
-                                   (1000, 2048, 5632), (2100, 4096, 256), (1, 20000, 128), (5, 128, 28672), (700, 8, 16)])
+                                   (1000, 2048, 5632), (2100, 4096, 256), (2100, 5001, 656), (1300, 8200, 1040), (3000, 4096, 1936), (1, 20000, 128), (5, 128, 28672), (700, 8, 16)])
 def test_product(T, N, K, bf16):
     g = gen(T + 3 * N + K)
     xq, xs, xv = rows_in_8_bits(rows(g, T, K).double())
@@ -237,7 +237,7 @@ def silu64(g):
 
 
 @pytest.mark.parametrize("T,I,K", [(1, 14336, 4096), (1, 16, 16), (3, 144, 272), (19, 720, 272), (32, 5632, 2048), (33, 128, 4096), (64, 1040, 512), (100, 720, 400), (128, 1792, 1024),
-                                   (256, 256, 640), (257, 720, 272), (600, 5632, 2048), (1025, 144, 128), (300, 16, 16)])
+                                   (256, 256, 640), (257, 720, 272), (600, 5632, 2048), (1025, 144, 128), (1025, 3600, 1040), (300, 16, 16)])
 def test_gate_up_product(T, I, K):
     g = gen(T + 3 * I + K)
     xq, xs, xv = rows_in_8_bits(rows(g, T, K).double())
