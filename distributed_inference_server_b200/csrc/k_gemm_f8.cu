@@ -71,7 +71,8 @@ __device__ __forceinline__ float2 pair_of(uint64_t s) {
   return r;
 }
 
-// The scales of a thread's token and of its columns' weight rows, fetched ahead: the token's four blocks at a time, the weight's 32, one
+// The scales of a thread's token and of its columns' weight rows, fetched ahead (from L2, where the kernel ahead has left them; an SM's own cache may
+// still hold what a kernel before that one read there): the token's four blocks at a time, the weight's 32, one
 // per lane (they are the same for the whole warp).  Blocks are asked for in order from begin()'s first on.
 template <int kW>
 struct Scales {
@@ -80,12 +81,12 @@ struct Scales {
   float x[4], x_next[4], w[kW], w_next[kW];
   __device__ __forceinline__ void fetch_x(int b) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) x_next[i] = t < T && b + i < end ? xs[(size_t)(b + i) * T + t] : 0.f;
+    for (int i = 0; i < 4; i++) x_next[i] = t < T && b + i < end ? __ldcg(xs + (size_t)(b + i) * T + t) : 0.f;
   }
   __device__ __forceinline__ void fetch_w(int b) {
     const int l = b + (int)(threadIdx.x & 31);
 #pragma unroll
-    for (int j = 0; j < kW; j++) w_next[j] = l < end && ws[j] ? ws[j][l] : 0.f;
+    for (int j = 0; j < kW; j++) w_next[j] = l < end ? __ldcg(ws[j] + l) : 0.f;
   }
   // i: blocks since begin(); returns the factors of block first + i
   __device__ __forceinline__ void get(int first, int i, float (&f)[kW]) {
@@ -503,9 +504,9 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
             for (int i = 0; i < 2; i++) {
               const int at_kb = min(kb + k + i, num_kb - 1);
 #pragma unroll
-              for (int j = 0; j < 4; j++) x[i][j] = t0 + 32 * j < T ? xs[(size_t)at_kb * T + t0 + 32 * j] : 0.f;
-              a[i] = w0[at_kb];
-              c[i] = w1[at_kb];
+              for (int j = 0; j < 4; j++) x[i][j] = t0 + 32 * j < T ? __ldcg(xs + (size_t)at_kb * T + t0 + 32 * j) : 0.f;
+              a[i] = __ldcg(w0 + at_kb);
+              c[i] = __ldcg(w1 + at_kb);
             }
             if (k == 0) mbar_wait(f_empty(g), phase ^ 1u);  // passes on the first lap
 #pragma unroll
@@ -706,12 +707,12 @@ cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *x
 }
 
 // What a product takes behind its launch, in hundredths of a microsecond, fitted to ten shapes from 1024 x 1024 to 10240 x 8192 and 8192 x 28672 at
-// 128 to 1024 tokens: in pairs 25 and 37 per block for every round of tiles of 128 and of 256 columns, in tiles 60 per block of a slice for every
+// 128 to 1024 tokens: in pairs 21.5 and 37 per block for every round of tiles of 128 and of 256 columns, in tiles 60 per block of a slice for every
 // round of CTAs.
 int pair_f8_cost(int T, int N, int K, int columns) {
   const long long tiles = (long long)((N + columns - 1) / columns) * ((T + 255) / 256), num_kb = (K + kF8Block - 1) / kF8Block;
   const long long rounds = (tiles + kNumSMs / 2 - 1) / (kNumSMs / 2);
-  const long long cost = columns == 128 ? 350 + 25 * num_kb * rounds : 400 + 37 * num_kb * rounds;
+  const long long cost = columns == 128 ? 350 + 43 * num_kb * rounds / 2 : 400 + 37 * num_kb * rounds;
   return cost > 0x7fffffff ? 0x7fffffff : (int)cost;
 }
 int tile_cost(int T, int N, int K) {
@@ -725,8 +726,8 @@ int tile_cost(int T, int N, int K) {
 // the next row's start).  A thread's wait, expectation and two loads take it 0.37 us, as long as a block's MMAs, whatever the boxes' size.
 uint32_t f8_depth(int K) { return K % kF8Block == 0 ? 2u : 1u; }
 
-// Columns of a pair's tile.  (Gated: 256, a tile is a block of 128 features under one scale.)  us with 128 / 256: 4096 x 4096, 512 tokens 13.8 / 18.0, 1024
-// tokens 21.5 / 20.4.
+// Columns of a pair's tile.  (Gated: 256, a tile is a block of 128 features under one scale.)  us with 128 / 256: 4096 x 4096, 512 tokens 11.9 / 18.0, 1024
+// tokens 19.3 / 18.6.
 int pair_f8_columns(int T, int N, int K, bool gated) { return gated || pair_f8_cost(T, N, K, 256) <= pair_f8_cost(T, N, K, 128) ? 256 : 128; }
 
 template <int kOut, int BN>

@@ -23,7 +23,7 @@ quant_f8_kernel(const uint16_t *__restrict__ x, uint8_t *__restrict__ x8, float 
     const int k = b * kF8Block + part;
     const bool in = t < T && k < K;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (in) v = ld_stream_16(x + (size_t)t * K + k);
+    if (in) v = __ldcg(reinterpret_cast<const uint4 *>(x + (size_t)t * K + k));
     const float2 p0 = bf16x2_to_float2(v.x), p1 = bf16x2_to_float2(v.y), p2 = bf16x2_to_float2(v.z), p3 = bf16x2_to_float2(v.w);
     uint32_t top = max(f8_top4(p0.x, p0.y, p1.x, p1.y), f8_top4(p2.x, p2.y, p3.x, p3.y));
 #pragma unroll
