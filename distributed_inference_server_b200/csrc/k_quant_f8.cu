@@ -11,28 +11,37 @@ namespace {
 constexpr int kQuantThreads = 256;
 constexpr int kQuantRows = kQuantThreads / 16;  // 16 lanes take a block of a row, 8 entries each
 
-// grid.x: groups of kQuantRows rows, grid.y: shares of the blocks
+// grid.x: groups of kQuantRows rows, grid.y: shares of the blocks.  Four blocks' loads are on their way at once: 64 KB an SM (with two, 8192 x 6000
+// took 35 us, 4.2 TB/s).
 __global__ void __launch_bounds__(kQuantThreads)
 quant_f8_kernel(const uint16_t *__restrict__ x, uint8_t *__restrict__ x8, float *__restrict__ scale, int T, int K, int per) {
   pdl_launch_dependents();
   pdl_wait();
+  constexpr int kAtOnce = 4;
   const int t = blockIdx.x * kQuantRows + (threadIdx.x >> 4), part = (threadIdx.x & 15) * 8;
   const int blocks = (K + kF8Block - 1) / kF8Block, b1 = min(blocks, ((int)blockIdx.y + 1) * per);
-#pragma unroll 2
-  for (int b = blockIdx.y * per; b < b1; b++) {
-    const int k = b * kF8Block + part;
-    const bool in = t < T && k < K;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (in) v = __ldcg(reinterpret_cast<const uint4 *>(x + (size_t)t * K + k));
-    const float2 p0 = bf16x2_to_float2(v.x), p1 = bf16x2_to_float2(v.y), p2 = bf16x2_to_float2(v.z), p3 = bf16x2_to_float2(v.w);
-    uint32_t top = max(f8_top4(p0.x, p0.y, p1.x, p1.y), f8_top4(p2.x, p2.y, p3.x, p3.y));
+  for (int b0 = blockIdx.y * per; b0 < b1; b0 += kAtOnce) {
+    uint4 v[kAtOnce];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float s = f8_scale(top), r = f8_inverse(s);
-    if (in) {
-      const uint2 o = make_uint2(f8_pack4(p0.x * r, p0.y * r, p1.x * r, p1.y * r), f8_pack4(p2.x * r, p2.y * r, p3.x * r, p3.y * r));
-      *reinterpret_cast<uint2 *>(x8 + (size_t)t * K + k) = o;
-      if (part == 0) scale[(size_t)b * T + t] = s;
+    for (int j = 0; j < kAtOnce; j++) {
+      const int k = (b0 + j) * kF8Block + part;
+      v[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (t < T && b0 + j < b1 && k < K) v[j] = __ldcg(reinterpret_cast<const uint4 *>(x + (size_t)t * K + k));
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) {
+      if (b0 + j >= b1) break;
+      const float2 p0 = bf16x2_to_float2(v[j].x), p1 = bf16x2_to_float2(v[j].y), p2 = bf16x2_to_float2(v[j].z), p3 = bf16x2_to_float2(v[j].w);
+      uint32_t top = max(f8_top4(p0.x, p0.y, p1.x, p1.y), f8_top4(p2.x, p2.y, p3.x, p3.y));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float s = f8_scale(top), r = f8_inverse(s);
+      const int k = (b0 + j) * kF8Block + part;
+      if (t < T && k < K) {
+        const uint2 o = make_uint2(f8_pack4(p0.x * r, p0.y * r, p1.x * r, p1.y * r), f8_pack4(p2.x * r, p2.y * r, p3.x * r, p3.y * r));
+        *reinterpret_cast<uint2 *>(x8 + (size_t)t * K + k) = o;
+        if (part == 0) scale[(size_t)(b0 + j) * T + t] = s;
+      }
     }
   }
 }
@@ -84,55 +93,74 @@ __global__ void unquant_weight_f8_kernel(const uint8_t *__restrict__ w8, const f
 }
 
 // add_rmsnorm (k_elementwise.cu) whose rows leave in 8 bits: a CTA per row, and a warp per block of 128 entries, four a lane, so that a
-// block's maximum is one warp reduction.  The normed row is not rounded to bf16 on its way.
+// block's maximum is one warp reduction.  The normed row is not rounded to bf16 on its way.  A thread keeps its kGroups groups of four entries in
+// registers from the sum to the store, all of their loads on their way at once.
+template <int kGroups>
 __global__ void __launch_bounds__(1024)
 add_rmsnorm_f8_kernel(float *__restrict__ x, const uint32_t *__restrict__ tokens, const uint16_t *__restrict__ embed, const float *__restrict__ partial,
                       int n_partial, long long partial_stride, const float *__restrict__ gain, uint8_t *__restrict__ x8, float *__restrict__ scale,
                       const int *__restrict__ row_map, int T, int H, float eps) {
   __shared__ float red[32];
-  extern __shared__ float row[];  // H floats (only used when a thread owns more than one group)
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = blockDim.x * 4;
   pdl_launch_dependents();
   pdl_wait();
   const int src = row_map ? row_map[t] : t;
-  const int step = blockDim.x * 4;
-  const bool single = H <= step;
-  float ss = 0.f;
-  float4 keep = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = threadIdx.x * 4; i < H; i += step) {
-    float4 v;
-    if (tokens) {
-      const uint2 e = *reinterpret_cast<const uint2 *>(embed + (size_t)tokens[src] * H + i);
-      const float2 a = bf16x2_to_float2(e.x), b = bf16x2_to_float2(e.y);
-      v = make_float4(a.x, a.y, b.x, b.y);
-    } else {
-      v = *reinterpret_cast<const float4 *>(x + (size_t)src * H + i);
-      const float *pp = partial + (size_t)src * H + i;
-#pragma unroll 4
-      for (int s = 0; s < n_partial; s++) {
-        const float4 p = *reinterpret_cast<const float4 *>(pp + (size_t)s * partial_stride);
-        v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
+  float4 v[kGroups];
+  if (tokens) {
+    const uint16_t *row = embed + (size_t)tokens[src] * H;
+#pragma unroll
+    for (int j = 0; j < kGroups; j++) {
+      const int i = threadIdx.x * 4 + j * step;
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < H) {
+        const uint2 e = *reinterpret_cast<const uint2 *>(row + i);
+        const float2 a = bf16x2_to_float2(e.x), b = bf16x2_to_float2(e.y);
+        v[j] = make_float4(a.x, a.y, b.x, b.y);
       }
     }
-    if (!row_map) *reinterpret_cast<float4 *>(x + (size_t)t * H + i) = v;
-    if (single) keep = v; else *reinterpret_cast<float4 *>(row + i) = v;
-    ss += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+  } else {
+    const float *row = x + (size_t)src * H;
+#pragma unroll
+    for (int j = 0; j < kGroups; j++) {
+      const int i = threadIdx.x * 4 + j * step;
+      v[j] = i < H ? *reinterpret_cast<const float4 *>(row + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const float *pp = partial + (size_t)src * H;
+#pragma unroll(kGroups == 1 ? 4 : 1)
+    for (int s = 0; s < n_partial; s++, pp += partial_stride) {
+#pragma unroll
+      for (int j = 0; j < kGroups; j++) {
+        const int i = threadIdx.x * 4 + j * step;
+        if (i < H) {
+          const float4 p = *reinterpret_cast<const float4 *>(pp + i);
+          v[j].x += p.x; v[j].y += p.y; v[j].z += p.z; v[j].w += p.w;
+        }
+      }
+    }
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < kGroups; j++) {
+    const int i = threadIdx.x * 4 + j * step;
+    if (!row_map && i < H) *reinterpret_cast<float4 *>(x + (size_t)t * H + i) = v[j];
+    ss += v[j].x * v[j].x + v[j].y * v[j].y + v[j].z * v[j].z + v[j].w * v[j].w;
   }
   ss = warp_sum(ss);
   if (lane == 0) red[warp] = ss;
   __syncthreads();
   ss = warp_sum(lane < (int)(blockDim.x >> 5) ? red[lane] : 0.f);
   const float inv = rsqrtf(ss / (float)H + eps);
-  for (int b = warp; b * kF8Block < H; b += blockDim.x >> 5) {
-    const int i = b * kF8Block + lane * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < kGroups; j++) {
+    const int i = threadIdx.x * 4 + j * step, b = i / kF8Block;
+    if (b * kF8Block >= H) break;  // (for the whole warp)
+    float4 n = make_float4(0.f, 0.f, 0.f, 0.f);
     if (i < H) {
-      v = single ? keep : *reinterpret_cast<const float4 *>(row + i);
       const float4 g = *reinterpret_cast<const float4 *>(gain + i);
-      v = make_float4(v.x * inv * g.x, v.y * inv * g.y, v.z * inv * g.z, v.w * inv * g.w);
+      n = make_float4(v[j].x * inv * g.x, v[j].y * inv * g.y, v[j].z * inv * g.z, v[j].w * inv * g.w);
     }
-    const float s = f8_scale(__reduce_max_sync(0xffffffffu, f8_top4(v.x, v.y, v.z, v.w))), r = f8_inverse(s);
-    if (i < H) *reinterpret_cast<uint32_t *>(x8 + (size_t)t * H + i) = f8_pack4(v.x * r, v.y * r, v.z * r, v.w * r);
+    const float s = f8_scale(__reduce_max_sync(0xffffffffu, f8_top4(n.x, n.y, n.z, n.w))), r = f8_inverse(s);
+    if (i < H) *reinterpret_cast<uint32_t *>(x8 + (size_t)t * H + i) = f8_pack4(n.x * r, n.y * r, n.z * r, n.w * r);
     if (lane == 0) scale[(size_t)b * T + t] = s;
   }
 }
@@ -166,15 +194,16 @@ cudaError_t launch_add_rmsnorm_f8(float *x, const uint32_t *tokens, const uint16
                                   const float *gain, uint8_t *x8, float *scale, const int *row_map, int T, int H, float eps, cudaStream_t st) {
   if (T <= 0) return cudaSuccess;
   if (H % 4 != 0 || H * 4 > 200 * 1024) { set_last_error("add_rmsnorm_f8: H must be a multiple of 4 and <= 51200"); return cudaErrorInvalidValue; }
-  int threads = (H / 4 + 31) / 32 * 32;
+  // Few rows: as many threads as a row takes, up to 1024.  Many: 256 and eight groups each, so that an SM has rows in different phases beside each
+  // other (as add_rmsnorm).
+  const int quads = H / 4;
+  int threads = (quads + 31) / 32 * 32;
+  if (T >= 512 && threads > 256) threads = quads <= 8 * 256 ? 256 : (quads + 8 * 32 - 1) / (8 * 32) * 32;
   threads = threads > 1024 ? 1024 : threads;
-  if (T >= 512 && threads > 256) threads = 256;  // as add_rmsnorm: rows in different phases beside each other
-  const size_t smem = H <= threads * 4 ? 0 : (size_t)H * sizeof(float);
-  static DeviceOnce once;
-  if (smem > 48 * 1024)
-    DIS_CUDA_TRY(once.run([&] { return cudaFuncSetAttribute(add_rmsnorm_f8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); }));
-  return launch_k(add_rmsnorm_f8_kernel, dim3(T), dim3(threads), smem, st, x, tokens, embed, partial, n_partial, partial_stride, gain, x8, scale, row_map, T, H,
-                  eps);
+  const int groups = (quads + threads - 1) / threads;
+  auto f = groups == 1 ? add_rmsnorm_f8_kernel<1> : groups == 2 ? add_rmsnorm_f8_kernel<2> : groups <= 4 ? add_rmsnorm_f8_kernel<4>
+           : groups <= 8 ? add_rmsnorm_f8_kernel<8> : add_rmsnorm_f8_kernel<16>;  // (16 * 1024 * 4 > 51200)
+  return launch_k(f, dim3(T), dim3(threads), 0, st, x, tokens, embed, partial, n_partial, partial_stride, gain, x8, scale, row_map, T, H, eps);
 }
 
 }  // namespace dis

@@ -150,7 +150,7 @@ def near_8_bits(x8, s, want, off):
 
 
 @pytest.mark.parametrize("T,H,n_partial,how", [(1, 4096, 4, "add"), (32, 4096, 1, "add"), (5, 272, 3, "add"), (700, 2048, 2, "add"), (3, 8192, 8, "add"), (2, 16, 1, "add"),
-                                               (40, 4096, 0, "embed"), (600, 272, 0, "embed"), (7, 1040, 2, "map"), (520, 8192, 0, "map")])
+                                               (40, 4096, 0, "embed"), (2, 51200, 1, "add"), (513, 20000, 1, "add"), (513, 6160, 2, "add"), (513, 12288, 1, "embed"), (1, 12288, 3, "add"), (600, 272, 0, "embed"), (7, 1040, 2, "map"), (520, 8192, 0, "map")])
 def test_norm_into_8_bits(T, H, n_partial, how):
     g = gen(T + H)
     rows_in = 2 * T if how == "map" else T
