@@ -706,26 +706,22 @@ cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *x
                           w_row0, split, tile_t, stages, bar_off, weights_first, wide);
 }
 
-// What a product takes behind its launch, in hundredths of a microsecond, fitted to ten shapes from 1024 x 1024 to 10240 x 8192 and 8192 x 28672 at
-// 128 to 1024 tokens: in pairs 21.5 and 37 per block for every round of tiles of 128 and of 256 columns, in tiles 60 per block of a slice for every
-// round of CTAs.
+// What a product takes, in hundredths of a microsecond, fitted to ten shapes from 1024 x 1024 to 10240 x 8192 and 8192 x 28672 at 128 to 4096 tokens:
+// in pairs a start and an end for every round of tiles, and 20 (128 columns) or 34 (256; 39 with several rounds, at the power limit) per block; in
+// tiles 60 per block of a slice for every round of CTAs, and the tokens' sums that the slices exchange.
 int pair_f8_cost(int T, int N, int K, int columns) {
   const long long tiles = (long long)((N + columns - 1) / columns) * ((T + 255) / 256), num_kb = (K + kF8Block - 1) / kF8Block;
   const long long rounds = (tiles + kNumSMs / 2 - 1) / (kNumSMs / 2);
-  const long long cost = columns == 128 ? 350 + 43 * num_kb * rounds / 2 : 400 + 37 * num_kb * rounds;
+  const long long cost = columns == 128 ? 230 + rounds * (300 + 20 * num_kb) : 300 + rounds * (400 + (rounds > 1 ? 39 : 34) * num_kb);
   return cost > 0x7fffffff ? 0x7fffffff : (int)cost;
 }
 int tile_cost(int T, int N, int K) {
   const int split = tile_split(T, N, K, false), tile_t = tile_tokens(T);
   const long long ctas = (long long)((N + 127) / 128) * ((T + tile_t - 1) / tile_t) * split;
   const long long per = ((K + kF8Block - 1) / kF8Block + split - 1) / split, rounds = (ctas + 2 * kNumSMs - 1) / (2 * kNumSMs);
-  const long long cost = 600 + (split > 1 ? 100 : 0) + 60 * per * rounds;
+  const long long cost = 500 + (split > 1 ? 100 : 0) + 60 * per * rounds + (T - 128ll) * 50 / 64;
   return cost > 0x7fffffff ? 0x7fffffff : (int)cost;
 }
-// Blocks that a load of the pair kernel brings: two where rows hold whole blocks only (past the end of a row that does not, the second would be
-// the next row's start).  A thread's wait, expectation and two loads take it 0.37 us, as long as a block's MMAs, whatever the boxes' size.
-uint32_t f8_depth(int K) { return K % kF8Block == 0 ? 2u : 1u; }
-
 // Columns of a pair's tile.  (Gated: 256, a tile is a block of 128 features under one scale.)  us with 128 / 256: 4096 x 4096, 512 tokens 11.9 / 18.0, 1024
 // tokens 19.3 / 18.6.
 int pair_f8_columns(int T, int N, int K, bool gated) { return gated || pair_f8_cost(T, N, K, 256) <= pair_f8_cost(T, N, K, 128) ? 256 : 128; }
@@ -755,9 +751,9 @@ cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float
 
 }  // namespace
 
-// Which products run in pairs.  Up to 128 tokens none: a pair's tile is half empty (4096 x 14336, 128 tokens: 18.9 us in tiles, 31.4 in pairs; gate-up
+// Which products run in pairs.  Up to 128 tokens none: a pair's tile is half empty (4096 x 14336, 128 tokens: 18.9 us in tiles, 27.7 in pairs; gate-up
 // 14336 x 4096, 128 tokens 30.6 and 35.3).  Gate-up products from there on (129 tokens: 49.5 and 35.1; 1024 x 1024, 129 tokens 11.0 and 9.8), plain ones
-// where the estimates say so (8192 x 8192, 200 tokens 24.0 and 21.2; but 2048 x 5632, 192 tokens 11.4 and 15.6).
+// where the estimates say so (8192 x 8192, 200 tokens 24.0 and 20.3; but 2048 x 5632, 192 tokens 11.4 and 13.6).
 bool gemm_f8_in_pairs(int T, int N, int K, bool gated) {
   if (T <= 128 || gated) return T > 128;
   const int narrow = pair_f8_cost(T, N, K, 128), wide = pair_f8_cost(T, N, K, 256);
