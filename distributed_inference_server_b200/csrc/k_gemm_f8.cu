@@ -722,6 +722,10 @@ int tile_cost(int T, int N, int K) {
   const long long cost = 500 + (split > 1 ? 100 : 0) + 60 * per * rounds + (T - 128ll) * 50 / 64;
   return cost > 0x7fffffff ? 0x7fffffff : (int)cost;
 }
+// Blocks that a load of the pair kernel brings: two where rows hold whole blocks only (past the end of a row that does not, the second would be
+// the next row's start).  A thread's wait, expectation and two loads take it 0.37 us, as long as a block's MMAs, whatever the boxes' size.
+uint32_t f8_depth(int K) { return K % kF8Block == 0 ? 2u : 1u; }
+
 // Columns of a pair's tile.  (Gated: 256, a tile is a block of 128 features under one scale.)  us with 128 / 256: 4096 x 4096, 512 tokens 11.9 / 18.0, 1024
 // tokens 19.3 / 18.6.
 int pair_f8_columns(int T, int N, int K, bool gated) { return gated || pair_f8_cost(T, N, K, 256) <= pair_f8_cost(T, N, K, 128) ? 256 : 128; }
