@@ -405,7 +405,10 @@ __device__ __forceinline__ void mbar_wait_soon(uint32_t bar, uint32_t parity) {
       : "memory");
   if (!ok) mbar_wait(bar, parity);
 }
-// Two blocks of a box's rows, {128 entries, rows, blocks} (make_f8_map with depth 2), one behind the other
+// Two blocks of a box's rows, {128 entries, rows, blocks} (make_f8_map with depth 2), one behind the other; the same into L2 only
+__device__ __forceinline__ void tma_prefetch_3d(const void *map, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void *map, int c0, int c1, int c2, uint32_t bar, uint64_t policy) {
   asm volatile(
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
@@ -452,6 +455,16 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
     for (uint32_t g = 0; g < kF8Groups; g++) { mbar_init(f_full(g), 1); mbar_init(f_empty(g), 8); }
     fence_barrier_init();
     fence_proxy_async();
+    // One round of tiles: the first weight rows, as far as L2, where what the kernel ahead may still write arrives too (gate-up 5632 x 2048, 200 tokens
+    // 14.4 -> 13.5 us; of several rounds it took a hundredth).
+    const int wr = w_row0 + tile_n(pair) * kTileN + (int)rank * w_row_step;
+    for (int kb = 0; n_tiles <= pairs && kb < num_kb && kb < 2 * Cfg::kStages; kb += 2) {
+      if (deep) tma_prefetch_3d(&w_map, 0, wr, kb);
+      else {
+        tma_prefetch_2d(&w_map, kb * kF8Block, wr);
+        if (kb + 1 < num_kb) tma_prefetch_2d(&w_map, (kb + 1) * kF8Block, wr);
+      }
+    }
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
