@@ -126,6 +126,7 @@ PROTOTYPES = {
     "dis_last_error": (C.c_char_p, []),
     "dis_engine_last_error": (C.c_char_p, [vp]),
     "dis_engine_load_tensor": (C.c_int, [vp, C.c_int, C.c_int, vp, C.c_int]),
+    "dis_engine_load_tensor_f8": (C.c_int, [vp, C.c_int, C.c_int, vp, vp]),
     "dis_engine_load_synthetic": (C.c_int, [vp, C.c_uint64]),
     "dis_engine_read_tensor": (C.c_int, [vp, C.c_int, C.c_int, vp, C.POINTER(C.c_size_t)]),
     "dis_engine_finalize": (C.c_int, [vp]),

@@ -78,6 +78,11 @@ int dis_engine_load_tensor(dis_engine *e, int kind, int layer, const void *host,
   LOCKED(e);
   return e->eng.load_tensor(kind, layer, host, dtype);
 }
+int dis_engine_load_tensor_f8(dis_engine *e, int kind, int layer, const uint8_t *host, const float *scale) {
+  if (int rc = guard_null(e)) return rc;
+  LOCKED(e);
+  return e->eng.load_tensor_f8(kind, layer, host, scale);
+}
 int dis_engine_load_synthetic(dis_engine *e, uint64_t seed) {
   if (int rc = guard_null(e)) return rc;
   LOCKED(e);

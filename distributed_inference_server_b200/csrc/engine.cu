@@ -511,6 +511,23 @@ int Engine::load_tensor(int kind, int layer, const void *host, int dtype) {
   return DIS_OK;
 }
 
+// A projection that is in 8 bits already, with its own scales
+int Engine::load_tensor_f8(int kind, int layer, const uint8_t *host, const float *scale) {
+  if (shut) return fail(DIS_ERR_SHUTDOWN, "engine is shut down");
+  if (!f8) return fail(DIS_ERR_INVALID_ARGUMENT, "load_tensor_f8: the engine was made without DIS_FLAG_WEIGHTS_F8");
+  if (!host || !scale) return fail(DIS_ERR_INVALID_ARGUMENT, "load_tensor_f8: null host pointer");
+  TensorSlot s;
+  if (!tensor_slot(kind, layer, &s) || !s.w8) return fail(DIS_ERR_INVALID_ARGUMENT, "load_tensor_f8: bad tensor kind or layer (the layers' projections are in 8 bits)");
+  if (s.row0 % 128 || s.col0 % 128) return fail(DIS_ERR_INVALID_ARGUMENT, "load_tensor_f8: this rank's part of the tensor starts inside a block of 128");
+  auto blocks = [](size_t n) { return (n + 127) / 128; };
+  ENG_CUDA(cudaSetDevice(cfg.device));
+  ENG_CUDA(cudaMemcpy2DAsync(s.w8, s.cols, host + s.row0 * s.full_cols + s.col0, s.full_cols, s.cols, s.rows, cudaMemcpyHostToDevice, stream));
+  const size_t row = blocks(s.full_cols) * sizeof(float), mine = blocks(s.cols) * sizeof(float);
+  ENG_CUDA(cudaMemcpy2DAsync(s.scale8, mine, scale + s.row0 / 128 * blocks(s.full_cols) + s.col0 / 128, row, mine, blocks(s.rows), cudaMemcpyHostToDevice, stream));
+  ENG_CUDA(cudaStreamSynchronize(stream));
+  return DIS_OK;
+}
+
 // amplitude / offset convention of the synthetic model (independently restated in the oracle)
 static void synth_params(const dis_model_config &m, int kind, float *amp, float *off) {
   const float a = 0.034641016f;  // 0.02 * sqrt(3): uniform(-a, a) has std 0.02

@@ -232,6 +232,7 @@ struct Engine {
   int fail(int code, const std::string &msg);
   int init(const dis_engine_config *c);
   int load_tensor(int kind, int layer, const void *host, int dtype);
+  int load_tensor_f8(int kind, int layer, const uint8_t *host, const float *scale);
   int load_synthetic(uint64_t seed);
   int read_tensor(int kind, int layer, uint16_t *host, size_t *n);
   int finalize();

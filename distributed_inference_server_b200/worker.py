@@ -205,6 +205,13 @@ class Engine:
             raise TypeError("load_tensor: float32 values or uint16 bf16 bit patterns")
         self._check(self.lib.dis_engine_load_tensor(self.h, kind, layer, arr.ctypes.data, dt))
 
+    def load_tensor_f8(self, kind: int, layer: int, arr: np.ndarray, scale: np.ndarray):
+        """A projection in 8 bits: e4m3 bit patterns [rows][cols] and fp32 scales of its blocks of 128 x 128 (FLAG_WEIGHTS_F8)."""
+        if arr.dtype != np.uint8 or scale.dtype != np.float32 or arr.ndim != 2 or scale.shape != tuple(-(-n // 128) for n in arr.shape):
+            raise TypeError("load_tensor_f8: uint8 e4m3 bit patterns [rows][cols] and a float32 scale for each block of 128 x 128")
+        arr, scale = np.ascontiguousarray(arr), np.ascontiguousarray(scale)
+        self._check(self.lib.dis_engine_load_tensor_f8(self.h, kind, layer, arr.ctypes.data, scale.ctypes.data))
+
     def load_named(self, name: str, arr: np.ndarray, shape=None):
         """A tensor of a layer-list model by its name in the model file: float32 values or uint16 bf16 bit patterns."""
         shape = tuple(arr.shape if shape is None else shape)

@@ -151,6 +151,10 @@ DIS_API const char *dis_engine_last_error(dis_engine *e);
  * over as a full, unsharded [out,in] row-major matrix and the engine keeps its tensor-parallel
  * slice.  `layer` is ignored for EMBED / FINAL_NORM / LM_HEAD. */
 DIS_API int dis_engine_load_tensor(dis_engine *e, int kind, int layer, const void *host, int dtype);
+/* A projection that is in 8 bits already, for an engine with DIS_FLAG_WEIGHTS_F8: the whole tensor, e4m3 [rows][cols], and its scales, fp32
+ * [ceil(rows / 128)][ceil(cols / 128)], any numbers; an entry stands for the product.  Under tensor parallelism a rank's part has to start on a block of
+ * 128 in both directions.  dis_engine_read_tensor returns the products rounded to bf16. */
+DIS_API int dis_engine_load_tensor_f8(dis_engine *e, int kind, int layer, const uint8_t *host, const float *scale);
 /* Random-init weights generated on the device from a counter-based hash (benchmarks, tests). */
 DIS_API int dis_engine_load_synthetic(dis_engine *e, uint64_t seed);
 /* Copy the engine's (sharded) copy of a tensor back as bf16 bit patterns; *n_elems in = capacity. */

@@ -108,6 +108,49 @@ def test_weights_are_what_their_8_bits_stand_for(how):
     e.close()
 
 
+def test_weights_that_are_in_8_bits_already():
+    """Tensors of a checkpoint in 8 bits with scales of its own (max / 448, no powers of two) give the logits of what they stand for, and read back as that."""
+    ref = RestatedF8(WIDE, 5)
+    m = O.Oracle(WIDE, act_round=True)
+    m.fill_synthetic(5, True)
+    e = Engine(WorkerConfig(to_engine_shape(WIDE), max_batch=8, kv_pages=64, page_size=16, max_step_tokens=256, flags=B.FLAG_WEIGHTS_F8))
+    for kind, layer, a in m.tensors():
+        a = torch.from_numpy(np.array(a, np.float32))
+        if kind not in (O.WQ, O.WK, O.WV, O.WO, O.WGATE, O.WUP, O.WDOWN):
+            e.load_tensor(kind, layer, a.numpy())
+            continue
+        n, k = a.shape
+        pad = torch.nn.functional.pad(a, (0, -k % 128, 0, -n % 128))
+        b = pad.view(-1, 128, pad.shape[1] // 128, 128)
+        s = b.abs().amax((1, 3)) / 448
+        q = (b / s[:, None, :, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+        value = (q.float() * s[:, None, :, None]).view(pad.shape)[:n, :k].contiguous()
+        e.load_tensor_f8(kind, layer, q.view(pad.shape)[:n, :k].contiguous().view(torch.uint8).numpy(), s.numpy())
+        assert np.array_equal(e.read_tensor(kind, layer), bits(value).reshape(-1)), (kind, layer)
+        ref.t[kind, layer] = value
+    e.finalize()
+    rng = np.random.default_rng(6)
+    prompts = [rng.integers(0, WIDE.vocab, n).tolist() for n in (12, 200)]
+    _, out, logits = follow(e, prompts, 3)
+    for i, p in enumerate(prompts):
+        want = ref.logits(p + out[i])
+        for k in range(3):
+            assert rel_err(logits[k][i], want[len(p) + k]) <= tol(WIDE), (i, k)
+    q = np.zeros((WIDE.hidden, WIDE.inter), np.uint8)
+    s = np.zeros((-(-WIDE.hidden // 128), -(-WIDE.inter // 128)), np.float32)
+    for kind, layer in ((O.EMBED, 0), (O.LM_HEAD, 0), (O.ATTN_NORM, 0), (O.WDOWN, 2), (O.WDOWN, -1), (77, 0)):
+        with pytest.raises(WorkerError):
+            e.load_tensor_f8(kind, layer, q, s)
+    with pytest.raises(TypeError):
+        e.load_tensor_f8(O.WDOWN, 0, q, s[:, 1:])
+    e.close()
+    e = make_engine(WIDE, seed=1)
+    with pytest.raises(WorkerError) as err:
+        e.load_tensor_f8(O.WDOWN, 0, q, s)
+    assert "DIS_FLAG_WEIGHTS_F8" in str(err.value)
+    e.close()
+
+
 def test_f8_engine_mixed_passes():
     """Prompts read in chunks beside running sequences: the restatement's choices."""
     rng = np.random.default_rng(2)
