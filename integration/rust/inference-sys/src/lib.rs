@@ -7,6 +7,7 @@ pub const DIS_OK: c_int = 0;
 pub const DIS_FLAG_PREFIX_CACHE: u32 = 8;
 pub const DIS_FLAG_KV_INT8: u32 = 16;
 pub const DIS_FLAG_ATTN_SHARED: u32 = 32;
+pub const DIS_FLAG_WEIGHTS_F8: u32 = 64;   // the layers' projections in 8-bit floating point
 
 #[repr(C)]
 #[derive(Clone, Copy, Default)]
