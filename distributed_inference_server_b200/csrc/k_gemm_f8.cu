@@ -390,13 +390,17 @@ static_assert(128 * kF8PairRegsLow + 256 * kF8PairRegsHigh <= kF8PairThreads * k
 constexpr int kF8Group = 4, kF8Groups = 4;                  // blocks whose factors are made together; such groups kept
 constexpr int kF8GroupBytes = kF8Group * 128 * 2 * 4;
 
+// Where a warp turns 32 tokens x 16 words from a token a lane to lanes side by side, [token][17 words]; of a gated tile, the tokens' largest magnitudes
+constexpr int kF8TurnRow = 17 * 4, kF8TurnWarp = 32 * kF8TurnRow, kF8Turn = 8 * kF8TurnWarp;
+
 template <int BN>
 struct PairCfg {
   static constexpr int kProducts = BN / 128, kBufs = 4 / kProducts;   // of a block; accumulators of each product
   static constexpr int kFeatBox = BN / 2 * kF8Block;                  // bytes of one CTA's feature rows of a block
   static constexpr int kStage = 2 * kF8Box + 2 * kFeatBox;            // one CTA's part of two blocks: token rows, token rows, feature rows, feature rows
   static constexpr int kStages = BN == 256 ? 3 : 4;
-  static constexpr int kSmem = kStages * kStage + kF8Groups * kF8GroupBytes + 1024 + 256 + 1024;
+  static constexpr int kSmem = kStages * kStage + kF8Groups * kF8GroupBytes + 1024 + 256 + kF8Turn;
+  static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 };
 
 enum { kF8OutF32 = 0, kF8OutBf16 = 1, kF8OutGated = 2 };
@@ -423,6 +427,55 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void *map, 
       : "memory");
 }
 
+// Rows of `out` that start anywhere: a warp's 32 tokens (from `first` on) by 16 or 32 features, which lie a token a lane, are turned so that lanes side by
+// side store what lies side by side.  (A lane that stores its own token's 16, 32 rows at once, writes every sector eight times: 5000 x 4143, K 512, 228 us
+// against the 20 of 4144 columns; 36 turned.)  out: the first of the features in token 0's row; n: that feature.
+__device__ __forceinline__ void turn_f32(uint32_t mine, const uint32_t (&v)[16], float *out, int first, int T, int n, int N) {
+  const int lane = threadIdx.x & 31, col = lane & 15;
+#pragma unroll
+  for (int i = 0; i < 16; i++) asm volatile("st.shared.b32 [%0], %1;" ::"r"(mine + (uint32_t)lane * kF8TurnRow + 4u * i), "r"(v[i]) : "memory");
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const int row = 2 * i + (lane >> 4);
+    float x;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(mine + (uint32_t)row * kF8TurnRow + 4u * col) : "memory");
+    if (first + row < T && n + col < N) out[(size_t)(first + row) * N + col] = x;
+  }
+  __syncwarp();
+}
+// The same with two features in a word.  A row that starts in the middle of a word has its first and last feature by themselves, and words in between
+// from two halves.
+__device__ __forceinline__ void turn_bf16(uint32_t mine, const uint32_t (&p)[16], uint16_t *out, int first, int T, int n, int N) {
+  const int lane = threadIdx.x & 31, l = lane & 15;
+#pragma unroll
+  for (int i = 0; i < 16; i++) asm volatile("st.shared.b32 [%0], %1;" ::"r"(mine + (uint32_t)lane * kF8TurnRow + 4u * i), "r"(p[i]) : "memory");
+  __syncwarp();
+  const int many = min(N - n, 32);  // features that the row still has here
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const int row = 2 * i + (lane >> 4);
+    uint32_t a, b;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(a) : "r"(mine + (uint32_t)row * kF8TurnRow + 4u * l) : "memory");
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(b) : "r"(mine + (uint32_t)row * kF8TurnRow + 4u * min(l + 1, 15)) : "memory");
+    uint16_t *o = out + (size_t)(first + row) * N;
+    const int off = (int)((uintptr_t)o >> 1) & 1, e = 2 * l + off;
+    if (first + row < T && e + 1 < many) *reinterpret_cast<uint32_t *>(o + e) = off ? __funnelshift_r(a, b, 16) : a;
+  }
+  if (first + lane < T) {  // a lane its token's single ones
+    uint16_t *o = out + (size_t)(first + lane) * N;
+    const int off = (int)((uintptr_t)o >> 1) & 1;
+    auto single = [&](int e) {
+      uint16_t v;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(mine + (uint32_t)lane * kF8TurnRow + 2u * e) : "memory");
+      o[e] = v;
+    };
+    if (off) single(0);
+    if ((many - off) & 1) single(many - 1);
+  }
+  __syncwarp();
+}
+
 template <int kOut, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8PairThreads, 1)
 gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const float *__restrict__ xs,
@@ -442,7 +495,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   auto f_full = [&](uint32_t g) { return bar_base + 8u * (2 * Cfg::kStages + 8 + g); };
   auto f_empty = [&](uint32_t g) { return bar_base + 8u * (2 * Cfg::kStages + 8 + kF8Groups + g); };
   const uint32_t tmem_slot = bar_base + 8u * (2 * Cfg::kStages + 8 + 2 * kF8Groups);
-  const uint32_t tops = bar_base + 256u;  // [128 tokens][2 halves] largest magnitudes of a gated tile
+  const uint32_t turn = bar_base + 256u, tops = turn;  // (tops: [128 tokens][2 halves])
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   uint32_t rank;
@@ -657,35 +710,45 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
           }
           if (half == 0) out_scale[(size_t)tile_n(tile) * T + t] = s;
         }
-      } else if (t < T) {
+      } else {
+        // 32 features at a time: twice of the first 128, twice of the second
+        const int first = t - lane;  // the warp's tokens: first + [0, 32)
+        const uint32_t mine = turn + (uint32_t)(warp - 4) * kF8TurnWarp;
 #pragma unroll
-        for (int c = 0; c < BN / 32; c++) {  // 16 features at a time: four times of the first 128, four of the second
-          const int n = n0 + 16 * c + (c >= 4 ? 64 : 0);
-          uint32_t v[16];
+        for (int c = 0; c < BN / 64; c++) {
+          const int n = n0 + 32 * c + (c >= 2 ? 64 : 0);
+          if (n >= N) continue;
+          if constexpr (kOut == kF8OutF32) {
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float2 a = pair_of(sums[8 * c + i]);
-            v[2 * i] = __float_as_uint(a.x);
-            v[2 * i + 1] = __float_as_uint(a.y);
-          }
-          if (kOut == kF8OutF32) {
-            float *o = static_cast<float *>(out) + (size_t)t * N + n;
-            if (wide && n + 16 <= N) { st_32(o, v); st_32(o + 8, v + 8); }
-            else
+            for (int h = 0; h < 2; h++) {
+              uint32_t v[16];
 #pragma unroll
-              for (int i = 0; i < 16; i++)
-                if (n + i < N) o[i] = __uint_as_float(v[i]);
+              for (int i = 0; i < 8; i++) {
+                const float2 a = pair_of(sums[16 * c + 8 * h + i]);
+                v[2 * i] = __float_as_uint(a.x);
+                v[2 * i + 1] = __float_as_uint(a.y);
+              }
+              const int m = n + 16 * h;
+              if (wide && m + 16 <= N) {
+                float *o = static_cast<float *>(out) + (size_t)t * N + m;
+                if (t < T) { st_32(o, v); st_32(o + 8, v + 8); }
+              } else {
+                turn_f32(mine, v, static_cast<float *>(out) + m, first, T, m, N);
+              }
+            }
           } else {
-            uint16_t *o = static_cast<uint16_t *>(out) + (size_t)t * N + n;
-            if (wide && n + 16 <= N) {
-              uint32_t p[8];
+            uint32_t p[16];
 #pragma unroll
-              for (int i = 0; i < 8; i++) p[i] = float2_to_bf16x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-              st_32(o, p);
-            } else
-#pragma unroll
-              for (int i = 0; i < 16; i++)
-                if (n + i < N) o[i] = float_to_bf16_bits(__uint_as_float(v[i]));
+            for (int i = 0; i < 16; i++) {
+              const float2 a = pair_of(sums[16 * c + i]);
+              p[i] = float2_to_bf16x2(a.x, a.y);
+            }
+            if (wide && n + 32 <= N) {
+              uint16_t *o = static_cast<uint16_t *>(out) + (size_t)t * N + n;
+              if (t < T) { st_32(o, p); st_32(o + 16, p + 8); }
+            } else {
+              turn_bf16(mine, p, static_cast<uint16_t *>(out) + n, first, T, n, N);
+            }
           }
         }
       }

@@ -12,10 +12,11 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("T,N,K", [(300, 640, 384), (2100, 5008, 384), (2100, 5008, 128), (129, 144, 128), (255, 256, 640), (511, 272, 16), (1300, 8192, 1152), (2048, 8192, 144),
-                                   (257, 20000, 256), (16, 128, 384), (128, 1000, 896)])
+                                   (257, 20000, 256), (16, 128, 384), (128, 1000, 896), (300, 1001, 384), (700, 33, 640), (2100, 5003, 272), (257, 129, 16), (1025, 4143, 384)])
 @pytest.mark.parametrize("bf16,by", [(False, 1), (True, 1), (True, 8), (False, 4)])
 def test_outputs_that_start_anywhere(T, N, K, bf16, by):
-    """Rows of N multiples of 16 whose output starts `by` elements behind a boundary: element stores, or the narrower vectors; odd and even numbers of blocks."""
+    """Outputs that start `by` elements behind a boundary, rows of odd and even lengths: narrower vectors, words that two features share, single elements; odd and even numbers of
+    blocks."""
     g = gen(T + N + K)
     xq, xs, xv = rows_in_8_bits(rows(g, T, K).double())
     wq, ws, wv = weight(g, N, K)
