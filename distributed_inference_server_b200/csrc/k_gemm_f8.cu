@@ -801,13 +801,17 @@ cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *x
                           w_row0, split, tile_t, stages, bar_off, weights_first, wide);
 }
 
+// Blocks that a load of the pair kernel brings: two where rows hold whole blocks only (past the end of a row that does not, the second would be
+// the next row's start).  A thread's wait, expectation and two loads take it 0.37 us, as long as a block's MMAs, whatever the boxes' size.
+uint32_t f8_depth(int K) { return K % kF8Block == 0 ? 2u : 1u; }
+
 // What a product takes, in hundredths of a microsecond, fitted to ten shapes from 1024 x 1024 to 10240 x 8192 and 8192 x 28672 at 128 to 4096 tokens:
-// in pairs a start and an end for every round of tiles, and 20 (128 columns) or 34 (256; 39 with several rounds, at the power limit) per block; in
+// in pairs a start and an end for every round of tiles, and 20 (128 columns; 25 a block a load) or 34 (256; 39 with several rounds, at the power limit) per block; in
 // tiles 60 per block of a slice for every round of CTAs, and the tokens' sums that the slices exchange.
 int pair_f8_cost(int T, int N, int K, int columns) {
   const long long tiles = (long long)((N + columns - 1) / columns) * ((T + 255) / 256), num_kb = (K + kF8Block - 1) / kF8Block;
   const long long rounds = (tiles + kNumSMs / 2 - 1) / (kNumSMs / 2);
-  const long long cost = columns == 128 ? 230 + rounds * (300 + 20 * num_kb) : 300 + rounds * (400 + (rounds > 1 ? 39 : 34) * num_kb);
+  const long long cost = columns == 128 ? 230 + rounds * (300 + (f8_depth(K) == 2 ? 20 : 25) * num_kb) : 300 + rounds * (400 + (rounds > 1 ? 39 : 34) * num_kb);
   return cost > 0x7fffffff ? 0x7fffffff : (int)cost;
 }
 int tile_cost(int T, int N, int K) {
@@ -817,10 +821,6 @@ int tile_cost(int T, int N, int K) {
   const long long cost = 500 + (split > 1 ? 100 : 0) + 60 * per * rounds + (T - 128ll) * 50 / 64;
   return cost > 0x7fffffff ? 0x7fffffff : (int)cost;
 }
-// Blocks that a load of the pair kernel brings: two where rows hold whole blocks only (past the end of a row that does not, the second would be
-// the next row's start).  A thread's wait, expectation and two loads take it 0.37 us, as long as a block's MMAs, whatever the boxes' size.
-uint32_t f8_depth(int K) { return K % kF8Block == 0 ? 2u : 1u; }
-
 // Columns of a pair's tile.  (Gated: 256, a tile is a block of 128 features under one scale.)  us with 128 / 256: 4096 x 4096, 512 tokens 11.9 / 18.0, 1024
 // tokens 19.3 / 18.6.
 int pair_f8_columns(int T, int N, int K, bool gated) { return gated || pair_f8_cost(T, N, K, 256) <= pair_f8_cost(T, N, K, 128) ? 256 : 128; }
