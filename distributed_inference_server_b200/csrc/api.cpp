@@ -464,7 +464,7 @@ static cudaError_t gemm_f8_call(const uint8_t *x8, const float *xs, const uint8_
   cudaError_t e = dis::make_f8_map(&wm, w8, (uint64_t)N, (uint64_t)K, box.feature_rows, box.depth);
   if (e == cudaSuccess) e = dis::make_f8_map(&xm, x8, (uint64_t)T, (uint64_t)K, box.token_rows, box.depth);
   if (e != cudaSuccess) return e;
-  return dis::launch_gemm_f8(wm, xm, xs, ws, out, out_dtype == DIS_BF16, T, N, K, 0, st);
+  return dis::launch_gemm_f8(wm, xm, x8, w8, xs, ws, out, out_dtype == DIS_BF16, T, N, K, 0, st);
 }
 static cudaError_t gemm_silu_f8_call(const uint8_t *x8, const float *xs, const uint8_t *wgu8, const float *wgus, uint8_t *h8, float *hs, int T, int I, int K, cudaStream_t st) {
   dis::TmaMap wm, xm;
@@ -472,7 +472,7 @@ static cudaError_t gemm_silu_f8_call(const uint8_t *x8, const float *xs, const u
   cudaError_t e = dis::make_f8_map(&wm, wgu8, 2ull * I, (uint64_t)K, box.feature_rows, box.depth);
   if (e == cudaSuccess) e = dis::make_f8_map(&xm, x8, (uint64_t)T, (uint64_t)K, box.token_rows, box.depth);
   if (e != cudaSuccess) return e;
-  return dis::launch_gemm_silu_f8(wm, xm, xs, wgus, h8, hs, T, I, K, 0, st);
+  return dis::launch_gemm_silu_f8(wm, xm, x8, wgu8, xs, wgus, h8, hs, T, I, K, 0, st);
 }
 
 int dis_k_gemm_f8(const uint8_t *x8, const float *xs, const uint8_t *w8, const float *ws, void *out, int32_t out_dtype, int32_t T, int32_t N, int32_t K,

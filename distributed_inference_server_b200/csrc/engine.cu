@@ -772,10 +772,10 @@ cudaError_t Engine::linear_partial(const TmaMap *xmaps, const uint16_t *xptr, co
 }
 
 // out = partial[T][N], one slice, of 8-bit rows and a layer's 8-bit weight
-cudaError_t Engine::linear_f8(const F8Weight &w, int layer, const TmaMap *xmaps, const float *xs, int T, int N, int K) {
+cudaError_t Engine::linear_f8(const F8Weight &w, int layer, const TmaMap *xmaps, const uint8_t *x8, const float *xs, int T, int N, int K) {
   const F8Boxes box = gemm_f8_boxes(T, N, K, false);
   kernel_launches++;
-  return launch_gemm_f8(w.map[f8_weight_map(box)], xmaps[f8_token_map(box)], xs, w.scale + (size_t)layer * w.layer_scales, partial, false, T, N, K,
+  return launch_gemm_f8(w.map[f8_weight_map(box)], xmaps[f8_token_map(box)], x8, w.w, xs, w.scale + (size_t)layer * w.layer_scales, partial, false, T, N, K,
                         (int)(layer * w.layer_rows), stream);
 }
 
@@ -882,7 +882,7 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
     pdl_enabled() = pdl_ok;
     int s_qkv = 1;
     prof_mark(P_QKV);
-    if (f8) { if (!skip(P_QKV)) RET_CUDA(linear_f8(f8_qkv, l, xn8_map, xn_scale, T, nqkv_l, H)); }
+    if (f8) { if (!skip(P_QKV)) RET_CUDA(linear_f8(f8_qkv, l, xn8_map, xn8, xn_scale, T, nqkv_l, H)); }
     else if (!skip(P_QKV)) RET_CUDA(linear_partial(xn_map, xn, wqkv_map, wqkv, l * nqkv_l, T, nqkv_l, H, &s_qkv));
     else s_qkv = gemm_pick_split_k(T, nqkv_l, H);
     const int pool_layer = kv8_pool ? 0 : l;
@@ -941,7 +941,7 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
       if (!skip(P_OPROJ)) {
         RET_CUDA(launch_quant_f8(attn, attn8, attn_scale, T, qd_l, stream));
         kernel_launches++;
-        RET_CUDA(linear_f8(f8_o, l, attn8_map, attn_scale, T, H, qd_l));
+        RET_CUDA(linear_f8(f8_o, l, attn8_map, attn8, attn_scale, T, H, qd_l));
       }
     } else if (!skip(P_OPROJ)) RET_CUDA(linear_partial(attn_map, attn, wo_map, wo, l * H, T, H, qd_l, &s_o));
     else s_o = gemm_pick_split_k(T, H, qd_l);
@@ -952,7 +952,7 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
     if (f8) {
       const F8Boxes box = gemm_f8_boxes(T, inter_l, H, true);
       if (!skip(P_GATEUP)) {
-        RET_CUDA(launch_gemm_silu_f8(f8_gu.map[f8_weight_map(box)], xn8_map[f8_token_map(box)], xn_scale, f8_gu.scale + (size_t)l * f8_gu.layer_scales, act8, act_scale, T,
+        RET_CUDA(launch_gemm_silu_f8(f8_gu.map[f8_weight_map(box)], xn8_map[f8_token_map(box)], xn8, f8_gu.w, xn_scale, f8_gu.scale + (size_t)l * f8_gu.layer_scales, act8, act_scale, T,
                                      inter_l, H, (int)(l * f8_gu.layer_rows), stream));
         kernel_launches++;
       }
@@ -979,7 +979,7 @@ cudaError_t Engine::enqueue_layers(int T, int n_splits) {
     }
     int s_d = 1;
     prof_mark(P_DOWN);
-    if (f8) { if (!skip(P_DOWN)) RET_CUDA(linear_f8(f8_down, l, act8_map, act_scale, T, H, inter_l)); }
+    if (f8) { if (!skip(P_DOWN)) RET_CUDA(linear_f8(f8_down, l, act8_map, act8, act_scale, T, H, inter_l)); }
     else if (!skip(P_DOWN)) RET_CUDA(linear_partial(act_map, act, wdown_map, wdown, l * H, T, H, inter_l, &s_d));
     else s_d = gemm_pick_split_k(T, H, inter_l);
     RET_CUDA(set_pending(s_d));

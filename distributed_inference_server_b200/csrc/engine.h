@@ -187,7 +187,7 @@ struct Engine {
   int tp_import(const uint8_t *handles);
   cudaError_t consume_pending(const float *gain, const int *row_map, int rows, int T, bool to_f8 = false);
   cudaError_t init_f8();
-  cudaError_t linear_f8(const F8Weight &w, int layer, const TmaMap *xmaps, const float *xs, int T, int N, int K);
+  cudaError_t linear_f8(const F8Weight &w, int layer, const TmaMap *xmaps, const uint8_t *x8, const float *xs, int T, int N, int K);
 
   // layer-list decoders (stack.cu): the same sequences, pages, planner and sampler; prompt = the whole token history
   StackModel *stack = nullptr;

@@ -17,6 +17,7 @@
 //   pair  two CTAs per 256 x 256 (or 256 x 128) tile (cta_group::2), persistent, for many tokens: an SM brings 32 KB per block for 512 clocks of the
 //         tensor pipe, and reads its 128 x 256 sums from TMEM in the meantime.
 #include <cuda.h>
+#include <cuda_fp16.h>
 
 #include "f8.cuh"
 #include "kernels.h"
@@ -71,6 +72,24 @@ __device__ __forceinline__ float2 pair_of(uint64_t s) {
   return r;
 }
 
+// Weight scales are any numbers, and a token's times one of them need not be a number: as a factor it would make NaN of a block of zeros.  A block's sum is 0 or
+// at least 2^-18, so what it is under two such scales is a number only if it is 0 or their product below 2^146.  No rows and weights that were turned into 8
+// bits here come near it, so there are two ways out that cost the others next to nothing: gate-up tiles hold their sums in units of 2^24 from the first such
+// block on, their factors, x w 2^-24, end at the largest number (with which any sum but 0 becomes infinite); elsewhere redo_token.
+constexpr float kF8Largest = 3.40282347e38f, kF8Unit = 16777216.f;
+__device__ __forceinline__ bool f8_too_large(float x, float w) { return fabsf(x * w) > kF8Largest && fabsf(x) <= kF8Largest && fabsf(w) <= kF8Largest; }
+__device__ __forceinline__ float f8_factor_in_units(float x, float w) {
+  const float f = fabsf(x) > fabsf(w) ? x * (1.f / kF8Unit) * w : w * (1.f / kF8Unit) * x;
+  return fabsf(x) <= kF8Largest && fabsf(w) <= kF8Largest ? fminf(fmaxf(f, -kF8Largest), kF8Largest) : f;
+}
+template <int kPairs>
+__device__ __forceinline__ void times(uint64_t (&sums)[kPairs], float by) {
+  uint64_t f;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "f"(by));
+#pragma unroll
+  for (int i = 0; i < kPairs; i++) asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(sums[i]) : "l"(f));
+}
+
 // The scales of a thread's token and of its columns' weight rows, fetched ahead (from L2, where the kernel ahead has left them; an SM's own cache may
 // still hold what a kernel before that one read there): the token's four blocks at a time, the weight's 32, one
 // per lane (they are the same for the whole warp).
@@ -90,6 +109,23 @@ struct Scales {
     const int l = first + (i + (int)(threadIdx.x & 31)) * step;
 #pragma unroll
     for (int j = 0; j < kW; j++) w_next[j] = l < end ? __ldcg(ws[j] + l) : 0.f;
+  }
+  // The factors of the i-th block, for sums in units or not.  True if they have to be (for any thread of the warp)
+  __device__ __forceinline__ bool get_in_units(int i, bool in_units, float (&f)[kW]) {
+    get(i, f);
+    bool large = false;
+#pragma unroll
+    for (int j = 0; j < kW; j++) large |= fabsf(f[j]) > kF8Largest;
+    if (!in_units && !__any_sync(0xffffffffu, large)) return false;
+    const float a = (i & 2) ? ((i & 1) ? x[3] : x[2]) : ((i & 1) ? x[1] : x[0]);
+    large = false;
+#pragma unroll
+    for (int j = 0; j < kW; j++) large |= f8_too_large(a, __shfl_sync(0xffffffffu, w[j], i & 31));
+    in_units |= __any_sync(0xffffffffu, large);
+    if (in_units)
+#pragma unroll
+      for (int j = 0; j < kW; j++) f[j] = f8_factor_in_units(a, __shfl_sync(0xffffffffu, w[j], i & 31));
+    return in_units;
   }
   // The factors of the i-th block
   __device__ __forceinline__ void get(int i, float (&f)[kW]) {
@@ -156,9 +192,75 @@ __device__ __forceinline__ void store4(const TileOut &o, int t, int n, const flo
         if (n + i < o.N) p[i] = v[i];
   }
 }
+
+// The rows of tokens with a factor that is too large (see kF8Largest) are taken from memory once more, their blocks added in 64 bits: 0.3 ms for a token's 128
+// features at a K of 4096.
+struct F8Memory {
+  const uint8_t *x8, *w8;  // (w8: the call's first row)
+  const float *xs, *ws;
+  int K;
+};
+__device__ __forceinline__ float dot16(uint4 a, uint4 b, float sum) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    uint32_t p, q;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(p) : "h"((uint16_t)(x[i >> 1] >> (i & 1) * 16)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(q) : "h"((uint16_t)(w[i >> 1] >> (i & 1) * 16)));
+    const float2 u = __half22float2(*reinterpret_cast<__half2 *>(&p)), v = __half22float2(*reinterpret_cast<__half2 *>(&q));
+    sum = fmaf(u.x, v.x, sum);
+    sum = fmaf(u.y, v.y, sum);
+  }
+  return sum;
+}
+// A warp: token t's 128 features from o.n0 on, four a lane, if one of the factors there is too large to be a number
+template <bool kGated>
+__device__ __forceinline__ void redo_token(const F8Memory &m, const TileOut &o, int t) {
+  const int lane = threadIdx.x & 31, num_kb = (m.K + kF8Block - 1) / kF8Block, block = o.n0 / kF8Block, ups = (o.N + kF8Block - 1) / kF8Block;
+  bool large = false;
+  for (int kb = lane; kb < num_kb; kb += 32) {
+    const float x = __ldcg(m.xs + (size_t)kb * o.T + t), w = __ldcg(m.ws + (size_t)block * num_kb + kb);
+    large |= f8_too_large(x, w) || (kGated && f8_too_large(x, __ldcg(m.ws + (size_t)(ups + block) * num_kb + kb)));
+  }
+  if (!__any_sync(0xffffffffu, large)) return;
+  auto sum = [&](int n, int up) {
+    const uint8_t *x = m.x8 + (size_t)t * m.K, *w = m.w8 + ((size_t)up * o.N + n) * m.K;
+    const float *ws = m.ws + (size_t)(up * ups + block) * num_kb;
+    double y = 0.;
+#pragma unroll 1
+    for (int kb = 0; kb < num_kb; kb++) {
+      float s = 0.f;
+#pragma unroll 1
+      for (int k = kb * kF8Block; k < min(m.K, (kb + 1) * kF8Block); k += 16)
+        s = dot16(__ldcg(reinterpret_cast<const uint4 *>(x + k)), __ldcg(reinterpret_cast<const uint4 *>(w + k)), s);
+      y += (double)__ldcg(m.xs + (size_t)kb * o.T + t) * (double)__ldcg(ws + kb) * (double)s;
+    }
+    return (float)y;
+  };
+  const int n0 = o.n0 + lane * 4;
+  if (kGated) {
+    auto h = [&](int n) { return silu(sum(n, 0)) * sum(n, 1); };
+    uint32_t top = 0;
+#pragma unroll 1
+    for (int n = n0; n < min(n0 + 4, o.N); n++) top = max(top, f8_bits(h(n)));
+    const float s = f8_scale(__reduce_max_sync(0xffffffffu, top)), q = f8_inverse(s);
+#pragma unroll 1
+    for (int n = n0; n < min(n0 + 4, o.N); n++) static_cast<uint8_t *>(o.out)[(size_t)t * o.N + n] = (uint8_t)f8_pack4(h(n) * q, 0.f, 0.f, 0.f);
+    if (lane == 0) o.scale[(size_t)block * o.T + t] = s;
+  } else {
+#pragma unroll 1
+    for (int n = n0; n < min(n0 + 4, o.N); n++) {
+      const float y = sum(n, 0);
+      if (o.bf16) static_cast<uint16_t *>(o.out)[(size_t)t * o.N + n] = float_to_bf16_bits(y);
+      else static_cast<float *>(o.out)[(size_t)t * o.N + n] = y;
+    }
+  }
+}
+
 template <bool kGated, int kLd>
-__device__ __forceinline__ void finish_tokens(uint32_t base, int rows, int first, int step, int split, const TileOut &o) {
+__device__ __forceinline__ bool finish_tokens(uint32_t base, int rows, int first, int step, int split, const TileOut &o) {
   const int lane = threadIdx.x & 31;
+  float top = 0.f;
   for (int r0 = first; r0 < rows; r0 += 4 * step) {
     float a[4][4], b[4][4];
 #pragma unroll
@@ -180,6 +282,8 @@ __device__ __forceinline__ void finish_tokens(uint32_t base, int rows, int first
     }
     const int n = o.n0 + lane * 4;
 #pragma unroll
+    for (int j = 0; j < 4 && !kGated; j++) top = max_mag(max_mag(top, a[j][0], a[j][1]), a[j][2], a[j][3]);
+#pragma unroll
     for (int j = 0; j < 4; j++) {
       const int t = o.t0 + r0 + j * step;
       if (r0 + j * step >= rows) break;
@@ -194,6 +298,7 @@ __device__ __forceinline__ void finish_tokens(uint32_t base, int rows, int first
       }
     }
   }
+  return __any_sync(0xffffffffu, !(top <= kF8Largest));
 }
 // A thread's sums to its token's row: 64 columns from col on (sums: 32 pairs)
 __device__ __forceinline__ void put_sums(uint32_t row, int col, const uint64_t *sums) {
@@ -224,8 +329,9 @@ struct TileCfg {
 template <bool kGated>
 __global__ void __launch_bounds__(kF8Threads, kGated ? 1 : 2)
 gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const float *__restrict__ xs,
-                    const float *__restrict__ ws, void *__restrict__ out, float *__restrict__ out_scale, int out_bf16, int T, int N, int K,
-                    int w_row0, int split, int tile_t, int stages, uint32_t bar_off, int weights_first, int wide) {
+                    const float *__restrict__ ws, const uint8_t *__restrict__ x8, const uint8_t *__restrict__ w8, void *__restrict__ out,
+                    float *__restrict__ out_scale, int out_bf16, int T, int N, int K, int w_row0, int split, int tile_t, int stages, uint32_t bar_off,
+                    int weights_first, int wide) {
   using Cfg = TileCfg<kGated>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -330,9 +436,17 @@ gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
     for (int i = 0; i < Cfg::kCols / 4; i++) sums[i] = 0;
     const uint32_t cols = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 64;
     uint32_t buf = 0, aphase = 0;
+    bool in_units = false;  // (gated; plain tiles see to it at their end, which spilled registers here: 14336 x 4096, 1 / 128 tokens 21.9 / 27.3 us, in units 21.6 / 26.6)
     for (int kb = kb0, i = 0; kb < kb1; kb += kb_step, i++) {
       float f[kGated ? 2 : 1];
-      sc.get(kGated ? i : kb - kb0, f);
+      if constexpr (kGated) {
+        if (sc.get_in_units(i, in_units, f) && !in_units) {
+          in_units = true;
+          times(sums, 1.f / kF8Unit);
+        }
+      } else {
+        sc.get(kb - kb0, f);
+      }
       mbar_wait(acc_full(buf), aphase);
       tc_fence_after();
       constexpr int CH = 16, kChunks = Cfg::kCols / 2 / CH;  // (32 columns at a time cost registers that two CTAs an SM do not have)
@@ -351,6 +465,7 @@ gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
       aphase ^= buf;
       buf ^= 1u;
     }
+    if (kGated && in_units) times(sums, kF8Unit);
     // The last MMAs have read the ring: the tokens' sums take its place
     if (r < rows) {
       const uint32_t row = smem_base + (uint32_t)(r * Cfg::kLd) * 4u;
@@ -367,8 +482,19 @@ gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
 
   // every CTA of the cluster finishes a share of the tokens
   const TileOut o{out, out_scale, T, N, t0, n0, wide, out_bf16};
-  finish_tokens<kGated, Cfg::kLd>(smem_base, rows, slice + split * warp, split * (kF8Threads / 32), split, o);
+  const bool odd = finish_tokens<kGated, Cfg::kLd>(smem_base, rows, slice + split * warp, split * (kF8Threads / 32), split, o);
   if (split > 1) cluster_meet();  // no CTA leaves while another reads its sums
+  if (!kGated && odd) {  // an infinite factor leaves no number behind (and so do other things)
+    auto anew = [](int v) { int r; asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v)); return r; };  // (nothing of this is worth a register in the loop above)
+    const int sp = anew(split), tt = anew(tile_t), TT = anew(T);
+    int bx, by, tid;
+    asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(bx));
+    asm volatile("mov.u32 %0, %%ctaid.y;" : "=r"(by));
+    asm volatile("mov.u32 %0, %%tid.x;" : "=r"(tid));
+    const TileOut again{out, out_scale, TT, anew(N), 0, bx / sp * 128, 0, anew(out_bf16)};
+#pragma unroll 1
+    for (int r = bx % sp + sp * (tid >> 5); r < min(tt, TT - by * tt); r += sp * (kF8Threads / 32)) redo_token<false>(F8Memory{x8, w8, xs, ws, anew(K)}, again, by * tt + r);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ pair kernel
@@ -380,15 +506,17 @@ gemm_f8_tile_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
 // for half the MMAs of 32.
 // Three warpgroups.  Warp 0 TMA.  Warps 1 and 3 MMA: two waits, four MMAs and their commits take one warp as long as a block's MMAs take, so
 // each issues one of a block's two products (128 columns: every second block).  Warp 2 the products of both scales, [block][token][two] in
-// shared memory, four blocks at a time: fetched and multiplied by the sums' warps themselves they cost a fifth of the kernel's time (8192^3 of
+// shared memory, in groups of four blocks: fetched and multiplied by the sums' warps themselves they cost a fifth of the kernel's time (8192^3 of
 // one value: 392 us against 329 without any).  Warpgroups 1 and 2 the sums, BN / 2 columns a thread in registers, which the first
 // warpgroup leaves them (setmaxnreg).
 constexpr int kF8PairThreads = 384;
-constexpr int kF8PairRegs = 168, kF8PairRegsLow = 40, kF8PairRegsHigh = 232;  // at launch, of the first warpgroup, of the others
+constexpr int kF8PairRegs = 168, kF8PairRegsLow = 56, kF8PairRegsHigh = 224;  // at launch, of the first warpgroup, of the others
 static_assert(128 * kF8PairRegsLow + 256 * kF8PairRegsHigh <= kF8PairThreads * kF8PairRegs, "more registers than the block is launched with");
 
 constexpr int kF8Group = 4, kF8Groups = 4;                  // blocks whose factors are made together; such groups kept
 constexpr int kF8GroupBytes = kF8Group * 128 * 2 * 4;
+// Behind the barriers, a bit a tile of the CTA's, from the 257th on shared with the one 256 tiles earlier: whether one of its factors is no number
+constexpr int kF8Large = 208, kF8LargeWords = 8;
 
 // Where a warp turns 32 tokens x 16 words from a token a lane to lanes side by side, [token][17 words]; of a gated tile, the tokens' largest magnitudes
 constexpr int kF8TurnRow = 17 * 4, kF8TurnWarp = 32 * kF8TurnRow, kF8Turn = 8 * kF8TurnWarp;
@@ -401,6 +529,7 @@ struct PairCfg {
   static constexpr int kStages = BN == 256 ? 3 : 4;
   static constexpr int kSmem = kStages * kStage + kF8Groups * kF8GroupBytes + 1024 + 256 + kF8Turn;
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
+  static_assert(8 * (2 * kStages + 8 + 2 * kF8Groups) + 4 <= kF8Large && kF8Large + 4 * kF8LargeWords <= 256, "barriers, the address of tensor memory, words");
 };
 
 enum { kF8OutF32 = 0, kF8OutBf16 = 1, kF8OutGated = 2 };
@@ -479,8 +608,8 @@ __device__ __forceinline__ void turn_bf16(uint32_t mine, const uint32_t (&p)[16]
 template <int kOut, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8PairThreads, 1)
 gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const float *__restrict__ xs,
-                    const float *__restrict__ ws, void *__restrict__ out, float *__restrict__ out_scale, int T, int N, int K, int w_row0,
-                    int w_row_step, int tiles_n, int tiles_t, int t_fast, int deep, int wide) {
+                    const float *__restrict__ ws, const uint8_t *__restrict__ x8, const uint8_t *__restrict__ w8, void *__restrict__ out,
+                    float *__restrict__ out_scale, int T, int N, int K, int w_row0, int w_row_step, int tiles_n, int tiles_t, int t_fast, int deep, int wide) {
   using Cfg = PairCfg<BN>;
   constexpr bool kGated = kOut == kF8OutGated;
   constexpr int kTileN = kGated ? BN / 2 : BN;
@@ -495,6 +624,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   auto f_full = [&](uint32_t g) { return bar_base + 8u * (2 * Cfg::kStages + 8 + g); };
   auto f_empty = [&](uint32_t g) { return bar_base + 8u * (2 * Cfg::kStages + 8 + kF8Groups + g); };
   const uint32_t tmem_slot = bar_base + 8u * (2 * Cfg::kStages + 8 + 2 * kF8Groups);
+  const uint32_t large_at = bar_base + kF8Large;
   const uint32_t turn = bar_base + 256u, tops = turn;  // (tops: [128 tokens][2 halves])
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
@@ -512,6 +642,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
     for (int s = 0; s < Cfg::kStages; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 2); }
     for (uint32_t i = 0; i < 4; i++) { mbar_init(acc_full(i), 1); mbar_init(acc_empty(i), 16 / Cfg::kProducts); }  // warps of both CTAs
     for (uint32_t g = 0; g < kF8Groups; g++) { mbar_init(f_full(g), 1); mbar_init(f_empty(g), 8); }
+    for (uint32_t i = 0; i < kF8LargeWords; i++) asm volatile("st.shared.u32 [%0], 0;" ::"r"(large_at + 4u * i) : "memory");
     fence_barrier_init();
     fence_proxy_async();
     // One round of tiles: the first weight rows, as far as L2, where what the kernel ahead may still write arrives too (gate-up 5632 x 2048, 200 tokens
@@ -573,36 +704,49 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
       }
       __syncwarp();
     } else if (warp == 2) {
-      // Factors of four tokens a lane, two blocks' scales on their way at a time
+      // Factors of four tokens a lane, two blocks at a time, the next two's scales on their way meanwhile (fetched when they are needed, with the comparison
+      // below: 4096 x 14336, 512 tokens 33.9 us)
       pdl_wait();
       const int blocks_n = (N + 127) / 128;
-      uint32_t g = 0, phase = 0;
-      for (int tile = pair; tile < n_tiles; tile += pairs) {
+      uint32_t g = 0, phase = 0, tiles = 0;
+      for (int tile = pair; tile < n_tiles; tile += pairs, tiles++) {
         const int t0 = tile_t0(tile) + lane, b = tile_n(tile) * (kTileN / 128), b2 = kGated ? blocks_n + b : b + 1;
         const float *w0 = ws + (size_t)b * num_kb, *w1 = BN == 256 && (kGated || b2 < blocks_n) ? ws + (size_t)b2 * num_kb : w0;  // (columns past N: whatever)
-        for (int kb = 0; kb < num_kb; kb += kF8Group) {
-          const uint32_t at = factors + g * (uint32_t)kF8GroupBytes + (uint32_t)lane * 8u;
+        struct Two { float x[2][4], a[2], c[2]; } now, next;
+        auto fetch = [&](int kb, Two &v) {
 #pragma unroll
-          for (int k = 0; k < kF8Group; k += 2) {
-            float x[2][4], a[2], c[2];
+          for (int i = 0; i < 2; i++) {
+            const int at_kb = min(kb + i, num_kb - 1);
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-              const int at_kb = min(kb + k + i, num_kb - 1);
-#pragma unroll
-              for (int j = 0; j < 4; j++) x[i][j] = t0 + 32 * j < T ? __ldcg(xs + (size_t)at_kb * T + t0 + 32 * j) : 0.f;
-              a[i] = __ldcg(w0 + at_kb);
-              c[i] = __ldcg(w1 + at_kb);
-            }
-            if (k == 0) mbar_wait(f_empty(g), phase ^ 1u);  // passes on the first lap
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-              for (int j = 0; j < 4; j++)
-                asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + (k + i) * 1024u + j * 256u), "f"(x[i][j] * a[i]), "f"(x[i][j] * c[i]) : "memory");
+            for (int j = 0; j < 4; j++) v.x[i][j] = t0 + 32 * j < T ? __ldcg(xs + (size_t)at_kb * T + t0 + 32 * j) : 0.f;
+            v.a[i] = __ldcg(w0 + at_kb);
+            v.c[i] = __ldcg(w1 + at_kb);
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(f_full(g));
-          if (++g == kF8Groups) { g = 0; phase ^= 1u; }
+        };
+        bool large = false;
+        fetch(0, now);
+#pragma unroll 2
+        for (int kb = 0; kb < num_kb; kb += 2) {
+          const uint32_t at = factors + g * (uint32_t)kF8GroupBytes + (kb & (kF8Group - 1)) * 1024u + (uint32_t)lane * 8u;
+          fetch(kb + 2, next);
+          if ((kb & 2) == 0) mbar_wait(f_empty(g), phase ^ 1u);  // passes on the first lap
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + i * 1024u + j * 256u), "f"(now.x[i][j] * now.a[i]), "f"(now.x[i][j] * now.c[i]) : "memory");
+            large |= fmaxf(fmaxf(fabsf(now.x[i][0]), fabsf(now.x[i][1])), fmaxf(fabsf(now.x[i][2]), fabsf(now.x[i][3]))) * fmaxf(fabsf(now.a[i]), fabsf(now.c[i])) > kF8Largest;
+          }
+          if (kb + 2 >= num_kb) {
+            large = __any_sync(0xffffffffu, large);
+            if (large && lane == 0) asm volatile("red.shared.or.b32 [%0], %1;" ::"r"(large_at + (tiles >> 5 & (kF8LargeWords - 1)) * 4u), "r"(1u << (tiles & 31)) : "memory");
+          }
+          if ((kb & 2) || kb + 2 >= num_kb) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(f_full(g));
+            if (++g == kF8Groups) { g = 0; phase ^= 1u; }
+          }
+          now = next;
         }
       }
     } else if (rank == 0) {
@@ -637,6 +781,21 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
           }
           if (++buf == Cfg::kBufs) { buf = 0; aphase ^= 1u; }
         }
+    }
+    // Tiles with a factor that is no number, behind all others.  (In the sums' warps, within their loop or behind it, it cost every tile: 4096 x 14336, 512 tokens
+    // 30 -> 32 to 37 us.)
+    asm volatile("bar.sync 15, 384;" ::: "memory");
+    pdl_wait();  // (not all of these warps have been there)
+    uint32_t tiles = 0;
+    for (int tile = pair; tile < n_tiles; tile += pairs, tiles++) {
+      uint32_t large;
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(large) : "r"(large_at + (tiles >> 5 & (kF8LargeWords - 1)) * 4u) : "memory");
+      if (large >> (tiles & 31) & 1u)
+#pragma unroll 1
+        for (int n0 = tile_n(tile) * kTileN; n0 < min((tile_n(tile) + 1) * kTileN, N); n0 += kF8Block)
+#pragma unroll 1
+          for (int t = tile_t0(tile) + warp; t < min(tile_t0(tile) + 128, T); t += 4)
+            redo_token<kGated>(F8Memory{x8, w8, xs, ws, K}, TileOut{out, out_scale, T, N, 0, n0, 0, kOut == kF8OutBf16}, t);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8PairRegsHigh));
@@ -753,6 +912,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
         }
       }
     }
+    asm volatile("bar.arrive 15, 384;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -779,8 +939,8 @@ int tile_split(int T, int N, int K, bool gated) {
 }
 
 template <bool kGated>
-cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int out_bf16, int T, int N,
-                        int K, int w_row0, int wide, cudaStream_t st) {
+cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, const uint8_t *x8, const uint8_t *w8, void *out,
+                        float *out_scale, int out_bf16, int T, int N, int K, int w_row0, int wide, cudaStream_t st) {
   using Cfg = TileCfg<kGated>;
   static DeviceOnce once;
   DIS_CUDA_TRY(once.run([&] { return cudaFuncSetAttribute(gemm_f8_tile_kernel<kGated>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8MaxSmem); }));
@@ -797,7 +957,7 @@ cudaError_t tile_launch(const TmaMap &w_map, const TmaMap &x_map, const float *x
   const int smem = (int)bar_off + kTileRest;
   const int weights_first = !(pdl_enabled() && !pdl_weights_settled());
   return launch_k_cluster(gemm_f8_tile_kernel<kGated>, dim3(tiles_n * split, tiles_t), dim3(kF8Threads), (size_t)smem, st, split,
-                          *reinterpret_cast<const CUtensorMap *>(&w_map), *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, out_bf16, T, N, K,
+                          *reinterpret_cast<const CUtensorMap *>(&w_map), *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, x8, w8 + (size_t)w_row0 * K, out, out_scale, out_bf16, T, N, K,
                           w_row0, split, tile_t, stages, bar_off, weights_first, wide);
 }
 
@@ -826,8 +986,8 @@ int tile_cost(int T, int N, int K) {
 int pair_f8_columns(int T, int N, int K, bool gated) { return gated || pair_f8_cost(T, N, K, 256) <= pair_f8_cost(T, N, K, 128) ? 256 : 128; }
 
 template <int kOut, int BN>
-cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, float *out_scale, int T, int N, int K,
-                           int w_row0, int wide, cudaStream_t st) {
+cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, const uint8_t *x8, const uint8_t *w8, void *out,
+                           float *out_scale, int T, int N, int K, int w_row0, int wide, cudaStream_t st) {
   using Cfg = PairCfg<BN>;
   static DeviceOnce once;
   DIS_CUDA_TRY(once.run([&] {
@@ -844,7 +1004,7 @@ cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float
   const int pairs = n_tiles < kNumSMs / 2 ? (int)n_tiles : kNumSMs / 2;
   const int t_fast = (long long)(kOut == kF8OutGated ? 2 : 1) * N > (long long)T ? 1 : 0;  // as gemm_pair_kernel: the smaller operand stays in L2
   return launch_k(gemm_f8_pair_kernel<kOut, BN>, dim3(2 * pairs), dim3(kF8PairThreads), (size_t)Cfg::kSmem, st, *reinterpret_cast<const CUtensorMap *>(&w_map),
-                  *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, out, out_scale, T, N, K, w_row0, kOut == kF8OutGated ? N : BN / 2, tiles_n, tiles_t,
+                  *reinterpret_cast<const CUtensorMap *>(&x_map), xs, ws, x8, w8 + (size_t)w_row0 * K, out, out_scale, T, N, K, w_row0, kOut == kF8OutGated ? N : BN / 2, tiles_n, tiles_t,
                   t_fast, f8_depth(K) == 2, wide);
 }
 
@@ -863,8 +1023,8 @@ F8Boxes gemm_f8_boxes(int T, int N, int K, bool gated) {
   return {128u, pair_f8_columns(T, N, K, gated) == 128 ? 64u : 128u, f8_depth(K)};
 }
 
-cudaError_t launch_gemm_f8(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, bool bf16, int T, int N, int K, int w_row0,
-                           cudaStream_t st) {
+cudaError_t launch_gemm_f8(const TmaMap &w_map, const TmaMap &x_map, const uint8_t *x8, const uint8_t *w8, const float *xs, const float *ws, void *out, bool bf16, int T,
+                           int N, int K, int w_row0, cudaStream_t st) {
   if (T <= 0 || N <= 0) return cudaSuccess;
   const uintptr_t at = (uintptr_t)out;
   if (gemm_f8_in_pairs(T, N, K, false)) {
@@ -872,18 +1032,18 @@ cudaError_t launch_gemm_f8(const TmaMap &w_map, const TmaMap &x_map, const float
     const bool narrow = pair_f8_columns(T, N, K, false) == 128;
     auto f = bf16 ? (narrow ? pair_f8_launch<kF8OutBf16, 128> : pair_f8_launch<kF8OutBf16, 256>)
                   : (narrow ? pair_f8_launch<kF8OutF32, 128> : pair_f8_launch<kF8OutF32, 256>);
-    return f(w_map, x_map, xs, ws, out, nullptr, T, N, K, w_row0, wide, st);
+    return f(w_map, x_map, xs, ws, x8, w8, out, nullptr, T, N, K, w_row0, wide, st);
   }
   const int wide = N % 4 == 0 && (at & (bf16 ? 7u : 15u)) == 0;
-  return tile_launch<false>(w_map, x_map, xs, ws, out, nullptr, bf16 ? 1 : 0, T, N, K, w_row0, wide, st);
+  return tile_launch<false>(w_map, x_map, xs, ws, x8, w8, out, nullptr, bf16 ? 1 : 0, T, N, K, w_row0, wide, st);
 }
 
 // h = silu(gate) * up in 8 bits; gate rows at w_row0, up rows at w_row0 + I; ws: the gate's blocks, then the up's
-cudaError_t launch_gemm_silu_f8(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, uint8_t *h8, float *hs, int T, int I, int K,
+cudaError_t launch_gemm_silu_f8(const TmaMap &w_map, const TmaMap &x_map, const uint8_t *x8, const uint8_t *w8, const float *xs, const float *ws, uint8_t *h8, float *hs, int T, int I, int K,
                                 int w_row0, cudaStream_t st) {
   if (T <= 0 || I <= 0) return cudaSuccess;
-  if (gemm_f8_in_pairs(T, I, K, true)) return pair_f8_launch<kF8OutGated, 256>(w_map, x_map, xs, ws, h8, hs, T, I, K, w_row0, 0, st);
-  return tile_launch<true>(w_map, x_map, xs, ws, h8, hs, 0, T, I, K, w_row0, 0, st);
+  if (gemm_f8_in_pairs(T, I, K, true)) return pair_f8_launch<kF8OutGated, 256>(w_map, x_map, xs, ws, x8, w8, h8, hs, T, I, K, w_row0, 0, st);
+  return tile_launch<true>(w_map, x_map, xs, ws, x8, w8, h8, hs, 0, T, I, K, w_row0, 0, st);
 }
 
 }  // namespace dis

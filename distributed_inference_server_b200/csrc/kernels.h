@@ -177,14 +177,14 @@ cudaError_t launch_unquant_weight_f8(const uint8_t *w8, const float *scale, uint
 cudaError_t launch_add_rmsnorm_f8(float *x, const uint32_t *tokens, const uint16_t *embed, const float *partial, int n_partial, long long partial_stride,
                                   const float *gain, uint8_t *x8, float *scale, const int *row_map, int T, int H, float eps, cudaStream_t st);
 
-// k_gemm_f8.cu : products of them.  w_map, x_map: make_f8_map with the boxes that gemm_f8_boxes() names for the call's sizes; w_row0: first row of W's map.
+// k_gemm_f8.cu : products of them.  w_map, x_map: make_f8_map of w8 and x8 with the boxes that gemm_f8_boxes() names for the call's sizes; w_row0: first row of W's map.
 struct F8Boxes { uint32_t token_rows, feature_rows, depth; };  // rows of a box; blocks of 128 entries that one holds
 F8Boxes gemm_f8_boxes(int T, int N, int K, bool gated);
 cudaError_t make_f8_map(TmaMap *out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t depth);
 bool gemm_f8_in_pairs(int T, int N, int K, bool gated);
-cudaError_t launch_gemm_f8(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, void *out, bool bf16, int T, int N, int K, int w_row0,
+cudaError_t launch_gemm_f8(const TmaMap &w_map, const TmaMap &x_map, const uint8_t *x8, const uint8_t *w8, const float *xs, const float *ws, void *out, bool bf16, int T, int N, int K, int w_row0,
                            cudaStream_t st);
-cudaError_t launch_gemm_silu_f8(const TmaMap &w_map, const TmaMap &x_map, const float *xs, const float *ws, uint8_t *h8, float *hs, int T, int I, int K,
+cudaError_t launch_gemm_silu_f8(const TmaMap &w_map, const TmaMap &x_map, const uint8_t *x8, const uint8_t *w8, const float *xs, const float *ws, uint8_t *h8, float *hs, int T, int I, int K,
                                 int w_row0, cudaStream_t st);
 
 }  // namespace dis
