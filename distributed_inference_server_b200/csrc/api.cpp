@@ -407,6 +407,7 @@ static int f8_shape(const char *who, int rows, long long n, int k) {
   if (rows < 0) what = "a negative number of rows";
   else if (rows > 65535 * 32) what = "more than 65535 * 32 rows";
   else if (k < 16 || k % 16) what = "rows must hold a positive multiple of 16 entries";
+  else if (k > 1 << 30) what = "rows of more than 2^30 entries";
   else if (n < 0 || n > 65535ll * 128) what = "a weight has 1 to 65535 * 128 rows";
   if (!what) return DIS_OK;
   dis::set_last_error(std::string(who) + ": " + what);
@@ -415,8 +416,8 @@ static int f8_shape(const char *who, int rows, long long n, int k) {
 
 int dis_k_quant_f8(const uint16_t *x, uint8_t *x8, float *scale, int32_t T, int32_t K, void *stream) {
   static const char *me = "quant_f8";
-  if (int rc = need_gpu()) return rc;
   if (int rc = f8_shape(me, T, 0, K)) return rc;
+  if (int rc = need_gpu()) return rc;
   if (T == 0) return DIS_OK;
   if (!x || !x8 || !scale) return cache_refuse(me, "null pointer");
   if (off(x, 16) || off(x8, 16) || off(scale, 4)) return cache_refuse(me, "x and x8 start on 16 bytes, the scales on 4");
@@ -425,8 +426,8 @@ int dis_k_quant_f8(const uint16_t *x, uint8_t *x8, float *scale, int32_t T, int3
 }
 int dis_k_quant_weight_f8(const uint16_t *w, uint8_t *w8, float *scale, int32_t N, int32_t K, void *stream) {
   static const char *me = "quant_weight_f8";
-  if (int rc = need_gpu()) return rc;
   if (int rc = f8_shape(me, 0, N, K)) return rc;
+  if (int rc = need_gpu()) return rc;
   if (N == 0) return DIS_OK;
   if (!w || !w8 || !scale) return cache_refuse(me, "null pointer");
   if (off(w, 16) || off(w8, 16) || off(scale, 4)) return cache_refuse(me, "w and w8 start on 16 bytes, the scales on 4");
@@ -436,8 +437,8 @@ int dis_k_quant_weight_f8(const uint16_t *w, uint8_t *w8, float *scale, int32_t 
 int dis_k_add_rmsnorm_f8(float *x, const uint32_t *tokens, const uint16_t *embed, const float *partial, int32_t n_partial, int64_t partial_stride,
                          const float *gain, uint8_t *x8, float *scale, const int32_t *row_map, int32_t T, int32_t H, float eps, void *stream) {
   static const char *me = "add_rmsnorm_f8";
-  if (int rc = need_gpu()) return rc;
   if (int rc = f8_shape(me, T, 0, H)) return rc;
+  if (int rc = need_gpu()) return rc;
   if (H > 51200) return cache_refuse(me, "rows of more than 51200 entries");
   if (n_partial < 0) return cache_refuse(me, "a negative number of partial sums");
   if (T == 0) return DIS_OK;
@@ -478,8 +479,8 @@ static cudaError_t gemm_silu_f8_call(const uint8_t *x8, const float *xs, const u
 int dis_k_gemm_f8(const uint8_t *x8, const float *xs, const uint8_t *w8, const float *ws, void *out, int32_t out_dtype, int32_t T, int32_t N, int32_t K,
                   void *stream) {
   static const char *me = "gemm_f8";
-  if (int rc = need_gpu()) return rc;
   if (int rc = f8_shape(me, T, N, K)) return rc;
+  if (int rc = need_gpu()) return rc;
   if (T == 0 || N == 0) return DIS_OK;
   if (int rc = gemm_f8_checks(me, x8, xs, w8, ws, out)) return rc;
   if (int rc = gemm_f8_out(me, out, out_dtype)) return rc;
@@ -489,8 +490,8 @@ int dis_k_gemm_f8(const uint8_t *x8, const float *xs, const uint8_t *w8, const f
 int dis_k_gemm_silu_f8(const uint8_t *x8, const float *xs, const uint8_t *wgu8, const float *wgus, uint8_t *h8, float *hs, int32_t T, int32_t I, int32_t K,
                        void *stream) {
   static const char *me = "gemm_silu_f8";
-  if (int rc = need_gpu()) return rc;
   if (int rc = f8_shape(me, T, I, K)) return rc;
+  if (int rc = need_gpu()) return rc;
   if (I % 16) return cache_refuse(me, "the inner size must be a multiple of 16");
   if (T == 0 || I == 0) return DIS_OK;
   if (int rc = gemm_f8_checks(me, x8, xs, wgu8, wgus, h8)) return rc;
@@ -501,9 +502,9 @@ int dis_k_gemm_silu_f8(const uint8_t *x8, const float *xs, const uint8_t *wgu8, 
 int dis_k_ffn_f8(const uint16_t *x, const uint8_t *wgu8, const float *wgus, const uint8_t *wd8, const float *wds, uint8_t *x8, float *xs, uint8_t *h8,
                  float *hs, void *out, int32_t out_dtype, int32_t T, int32_t H, int32_t I, void *stream) {
   static const char *me = "ffn_f8";
-  if (int rc = need_gpu()) return rc;
   if (int rc = f8_shape(me, T, I, H)) return rc;
   if (int rc = f8_shape(me, T, H, I)) return rc;
+  if (int rc = need_gpu()) return rc;
   if (T == 0) return DIS_OK;
   if (!x || off(x, 16)) return cache_refuse(me, "x must be there and start on 16 bytes");
   if (int rc = gemm_f8_checks(me, x8, xs, wgu8, wgus, h8)) return rc;

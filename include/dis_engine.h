@@ -466,9 +466,10 @@ DIS_API int dis_k_attn_shared_in_common(int32_t T, int32_t n_heads, int32_t n_kv
  * [ceil(N / 128)][ceil(K / 128)], any fp32 number (as checkpoints hold them, or from dis_k_quant_weight_f8); a fused gate-up weight [2][I][K]
  * has the gate's blocks, then the up's: 2 ceil(I / 128) rows of scales.  Sums are fp32: a block's 128 products by the tensor cores, their sums times both
  * scales added by fp32 FMAs, right to fp32's rounding and 2^-101 a block; results do not change from call to call.  Two scales whose product is no fp32
- * number, though each is, cost time (their token's features are computed without the tensor cores), not the result.  K is a positive multiple of 16 (its last block may be shorter), I too; N and T
- * are any.  Sizes that do not fit, null pointers and starts off the boundaries given are refused with DIS_ERR_INVALID_ARGUMENT before anything is
- * launched.  8-bit rows and bf16 inputs start on 16 bytes.  T = 0 or N = 0 is a call without work. */
+ * number, though each is, cost time (their token's features are computed without the tensor cores), not the result.  K is a positive multiple of 16 (its
+ * last block may be shorter) and at most 2^30, I a multiple of 16; N and I are at most 65535 * 128, T 65535 * 32.  Sizes that do not fit, null pointers and
+ * starts off the boundaries given are refused with DIS_ERR_INVALID_ARGUMENT before anything is launched.  8-bit rows and bf16 inputs start on 16 bytes.
+ * T = 0 or N = 0 is a call without work. */
 
 /* bf16 rows [T][K] into 8 bits */
 DIS_API int dis_k_quant_f8(const uint16_t *x, uint8_t *x8, float *scale, int32_t T, int32_t K, void *stream);
