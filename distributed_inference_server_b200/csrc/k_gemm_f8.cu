@@ -90,8 +90,8 @@ __device__ __forceinline__ void times(uint64_t (&sums)[kPairs], float by) {
   for (int i = 0; i < kPairs; i++) asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(sums[i]) : "l"(f));
 }
 
-// The scales of a thread's token and of its columns' weight rows, fetched ahead (from L2, where the kernel ahead has left them; an SM's own cache may
-// still hold what a kernel before that one read there): the token's four blocks at a time, the weight's 32, one
+// The scales of a thread's token and of its columns' weight rows, fetched ahead (from L2, where the kernel ahead has left them, perhaps while this one was
+// there already, which the read-only path is not made for): the token's four blocks at a time, the weight's 32, one
 // per lane (they are the same for the whole warp).
 template <int kW>
 struct Scales {

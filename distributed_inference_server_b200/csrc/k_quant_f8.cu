@@ -60,7 +60,7 @@ quant_weight_f8_kernel(const uint16_t *__restrict__ w, uint8_t *__restrict__ w8,
 #pragma unroll
   for (int i = 0; i < 16; i++) {
     v[i] = make_uint2(0u, 0u);
-    if (n0 + i < N && k < K) v[i] = *reinterpret_cast<const uint2 *>(w + (size_t)(n0 + i) * K + k);
+    if (n0 + i < N && k < K) v[i] = __ldcg(reinterpret_cast<const uint2 *>(w + (size_t)(n0 + i) * K + k));
     const float2 a = bf16x2_to_float2(v[i].x), b = bf16x2_to_float2(v[i].y);
     top = max(top, f8_top4(a.x, a.y, b.x, b.y));
   }
@@ -92,6 +92,14 @@ __global__ void unquant_weight_f8_kernel(const uint8_t *__restrict__ w8, const f
   }
 }
 
+// A load that the SM's own cache serves, which rows of an SM share, and not the read-only path: that is for what does not change while a kernel lives, and the
+// kernel in front may still write what this one reads.  (The gain from L2: 8192 rows of 8192 139 us against 130.)
+__device__ __forceinline__ float4 ld_coherent(const float *p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 // add_rmsnorm (k_elementwise.cu) whose rows leave in 8 bits: a CTA per row, and a warp per block of 128 entries, four a lane, so that a
 // block's maximum is one warp reduction.  The normed row is not rounded to bf16 on its way.  A thread keeps its kGroups groups of four entries in
 // registers from the sum to the store, all of their loads on their way at once.
@@ -104,16 +112,16 @@ add_rmsnorm_f8_kernel(float *__restrict__ x, const uint32_t *__restrict__ tokens
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = blockDim.x * 4;
   pdl_launch_dependents();
   pdl_wait();
-  const int src = row_map ? row_map[t] : t;
+  const int src = row_map ? __ldcg(row_map + t) : t;
   float4 v[kGroups];
   if (tokens) {
-    const uint16_t *row = embed + (size_t)tokens[src] * H;
+    const uint16_t *row = embed + (size_t)__ldcg(tokens + src) * H;
 #pragma unroll
     for (int j = 0; j < kGroups; j++) {
       const int i = threadIdx.x * 4 + j * step;
       v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i < H) {
-        const uint2 e = *reinterpret_cast<const uint2 *>(row + i);
+        const uint2 e = __ldcg(reinterpret_cast<const uint2 *>(row + i));
         const float2 a = bf16x2_to_float2(e.x), b = bf16x2_to_float2(e.y);
         v[j] = make_float4(a.x, a.y, b.x, b.y);
       }
@@ -123,7 +131,7 @@ add_rmsnorm_f8_kernel(float *__restrict__ x, const uint32_t *__restrict__ tokens
 #pragma unroll
     for (int j = 0; j < kGroups; j++) {
       const int i = threadIdx.x * 4 + j * step;
-      v[j] = i < H ? *reinterpret_cast<const float4 *>(row + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[j] = i < H ? __ldcg(reinterpret_cast<const float4 *>(row + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     const float *pp = partial + (size_t)src * H;
 #pragma unroll(kGroups == 1 ? 4 : 1)
@@ -132,7 +140,7 @@ add_rmsnorm_f8_kernel(float *__restrict__ x, const uint32_t *__restrict__ tokens
       for (int j = 0; j < kGroups; j++) {
         const int i = threadIdx.x * 4 + j * step;
         if (i < H) {
-          const float4 p = *reinterpret_cast<const float4 *>(pp + i);
+          const float4 p = __ldcg(reinterpret_cast<const float4 *>(pp + i));
           v[j].x += p.x; v[j].y += p.y; v[j].z += p.z; v[j].w += p.w;
         }
       }
@@ -156,7 +164,7 @@ add_rmsnorm_f8_kernel(float *__restrict__ x, const uint32_t *__restrict__ tokens
     if (b * kF8Block >= H) break;  // (for the whole warp)
     float4 n = make_float4(0.f, 0.f, 0.f, 0.f);
     if (i < H) {
-      const float4 g = *reinterpret_cast<const float4 *>(gain + i);
+      const float4 g = ld_coherent(gain + i);
       n = make_float4(v[j].x * inv * g.x, v[j].y * inv * g.y, v[j].z * inv * g.z, v[j].w * inv * g.w);
     }
     const float s = f8_scale(__reduce_max_sync(0xffffffffu, f8_top4(n.x, n.y, n.z, n.w))), r = f8_inverse(s);
