@@ -13,7 +13,7 @@ import ctypes as C
 import enum
 import uuid
 from dataclasses import dataclass, field
-from typing import Callable, List, Optional, Sequence
+from typing import Callable, List, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -36,6 +36,12 @@ class ModelShape:
     def c(self) -> B.ModelConfig:
         return B.ModelConfig(self.vocab, self.hidden, self.layers, self.n_heads, self.n_kv_heads, self.head_dim,
                              self.inter, self.max_ctx, self.rope_theta, self.rms_eps)
+
+    def projection(self, kind: int) -> Optional[Tuple[int, int]]:
+        """(rows, cols) of a layer's projection, unsharded; None for other tensors."""
+        q, kv = self.n_heads * self.head_dim, self.n_kv_heads * self.head_dim
+        return {B.T_WQ: (q, self.hidden), B.T_WK: (kv, self.hidden), B.T_WV: (kv, self.hidden), B.T_WO: (self.hidden, q),
+                B.T_WGATE: (self.inter, self.hidden), B.T_WUP: (self.inter, self.hidden), B.T_WDOWN: (self.hidden, self.inter)}.get(kind)
 
 
 TINYLLAMA = ModelShape(32000, 2048, 22, 32, 4, 64, 5632, 2048, 10000.0, 1e-5)
@@ -176,6 +182,7 @@ class Engine:
             self.h = None
             raise WorkerError(_KIND[rc], self.lib.dis_last_error().decode())
         self.vocab = cfg.stack.vocab if cfg.stack is not None else cfg.model.vocab
+        self.shape = cfg.model if cfg.stack is None else None
 
     def _check(self, rc: int):
         if rc != B.OK:
@@ -206,9 +213,12 @@ class Engine:
         self._check(self.lib.dis_engine_load_tensor(self.h, kind, layer, arr.ctypes.data, dt))
 
     def load_tensor_f8(self, kind: int, layer: int, arr: np.ndarray, scale: np.ndarray):
-        """A projection in 8 bits: e4m3 bit patterns [rows][cols] and fp32 scales of its blocks of 128 x 128 (FLAG_WEIGHTS_F8)."""
+        """A projection in 8 bits, the whole tensor: e4m3 bit patterns [rows][cols] and fp32 scales of its blocks of 128 x 128 (FLAG_WEIGHTS_F8)."""
         if arr.dtype != np.uint8 or scale.dtype != np.float32 or arr.ndim != 2 or scale.shape != tuple(-(-n // 128) for n in arr.shape):
             raise TypeError("load_tensor_f8: uint8 e4m3 bit patterns [rows][cols] and a float32 scale for each block of 128 x 128")
+        want = self.shape.projection(kind) if self.shape is not None else None  # (the engine refuses other kinds before it reads)
+        if want is not None and arr.shape != want:
+            raise TypeError(f"load_tensor_f8: the tensor is {want[0]} x {want[1]}, the array {arr.shape[0]} x {arr.shape[1]}")
         arr, scale = np.ascontiguousarray(arr), np.ascontiguousarray(scale)
         self._check(self.lib.dis_engine_load_tensor_f8(self.h, kind, layer, arr.ctypes.data, scale.ctypes.data))
 
