@@ -79,6 +79,8 @@ extern "C" {
     pub fn dis_engine_destroy(e: *mut dis_engine) -> c_int;
     pub fn dis_engine_last_error(e: *mut dis_engine) -> *const c_char;
     pub fn dis_engine_load_tensor(e: *mut dis_engine, kind: c_int, layer: c_int, host: *const c_void, dtype: c_int) -> c_int;
+    /// DIS_FLAG_WEIGHTS_F8: a projection that is in 8 bits already, e4m3 bytes and the scales of its blocks of 128 x 128.
+    pub fn dis_engine_load_tensor_f8(e: *mut dis_engine, kind: c_int, layer: c_int, host: *const u8, scale: *const f32) -> c_int;
     pub fn dis_engine_load_synthetic(e: *mut dis_engine, seed: u64) -> c_int;
     pub fn dis_engine_finalize(e: *mut dis_engine) -> c_int;
     pub fn dis_engine_seq_add(e: *mut dis_engine, prompt: *const u32, n: i32, p: *const dis_sampling_params, slot: *mut i32) -> c_int;
