@@ -994,7 +994,10 @@ cudaError_t pair_f8_launch(const TmaMap &w_map, const TmaMap &x_map, const float
     // a block launched with fewer registers would wait for those that its warpgroups ask for
     cudaFuncAttributes at;
     cudaError_t e = cudaFuncGetAttributes(&at, gemm_f8_pair_kernel<kOut, BN>);
-    if (e == cudaSuccess && at.numRegs != kF8PairRegs) e = cudaErrorInvalidKernelImage;
+    if (e == cudaSuccess && at.numRegs < kF8PairRegs) {
+      set_last_error("gemm_f8: built with " + std::to_string(at.numRegs) + " registers a thread for the pair kernel, which divides up " + std::to_string(kF8PairRegs));
+      e = cudaErrorInvalidKernelImage;
+    }
     return e == cudaSuccess ? cudaFuncSetAttribute(gemm_f8_pair_kernel<kOut, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem) : e;
   }));
   const int feats = kOut == kF8OutGated ? BN / 2 : BN;
