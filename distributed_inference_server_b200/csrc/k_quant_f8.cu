@@ -101,8 +101,9 @@ __device__ __forceinline__ float4 ld_coherent(const float *p) {
 }
 
 // add_rmsnorm (k_elementwise.cu) whose rows leave in 8 bits: a CTA per row, and a warp per block of 128 entries, four a lane, so that a
-// block's maximum is one warp reduction.  The normed row is not rounded to bf16 on its way.  A thread keeps its kGroups groups of four entries in
-// registers from the sum to the store, all of their loads on their way at once.
+// block's maximum is one warp reduction.  The normed row is not rounded to bf16 on its way.  A thread keeps its kGroups groups of four entries from the sum to
+// the store, all of their loads on their way at once: in registers up to eight, while sixteen (rows of more than 32768 entries) spill 904 bytes to
+// local memory, which L1 holds.
 template <int kGroups>
 __global__ void __launch_bounds__(1024)
 add_rmsnorm_f8_kernel(float *__restrict__ x, const uint32_t *__restrict__ tokens, const uint16_t *__restrict__ embed, const float *__restrict__ partial,

@@ -92,7 +92,7 @@ typedef struct dis_model_config {
                                    (see dis_k_gemm_f8): half the bytes of a decode step and twice the tensor rate of a prompt.  Tensors are loaded as ever
                                    and turned into 8 bits on the way; dis_engine_read_tensor returns what they stand for, which bf16 holds exactly.  Their
                                    inputs are rounded to 8 bits in blocks of 128 entries too; embeddings, norms, attention and the logits' head stay as they
-                                   are.  Needs hidden and inter / tp multiples of 16, n_heads * head_dim / tp and n_kv_heads * head_dim / tp multiples of 128,
+                                   are.  One tensor's place in bf16 is kept for loading and reading back.  Needs hidden and inter / tp multiples of 16, n_heads * head_dim / tp and n_kv_heads * head_dim / tp multiples of 128,
                                    and is refused with DIS_FLAG_FORCE_GEMV and for layer-list decoders */
 typedef struct dis_engine_config {
   dis_model_config model;
@@ -153,7 +153,8 @@ DIS_API const char *dis_engine_last_error(dis_engine *e);
 DIS_API int dis_engine_load_tensor(dis_engine *e, int kind, int layer, const void *host, int dtype);
 /* A projection that is in 8 bits already, for an engine with DIS_FLAG_WEIGHTS_F8: the whole tensor, e4m3 [rows][cols], and its scales, fp32
  * [ceil(rows / 128)][ceil(cols / 128)], any numbers; an entry stands for the product.  Under tensor parallelism a rank's part has to start on a block of
- * 128 in both directions.  dis_engine_read_tensor returns the products rounded to bf16. */
+ * 128 in both directions.  The host reads the file: this library's own model readers take fp32 and bf16 tensors only.  dis_engine_read_tensor returns
+ * the products as fp32 numbers rounded to bf16. */
 DIS_API int dis_engine_load_tensor_f8(dis_engine *e, int kind, int layer, const uint8_t *host, const float *scale);
 /* Random-init weights generated on the device from a counter-based hash (benchmarks, tests). */
 DIS_API int dis_engine_load_synthetic(dis_engine *e, uint64_t seed);
@@ -463,7 +464,7 @@ DIS_API int dis_k_attn_shared_in_common(int32_t T, int32_t n_heads, int32_t n_kv
  * Rows of activations [T][K] in 8 bits: e4m3 values x8 and one fp32 scale for each 128 entries, scale [ceil(K / 128)][T]; an entry stands for x8 s.
  * What is written here has s = 2^ceil(log2(max|x| / 448)), not below 2^-126, and x8 = x / s rounded to the nearest value, ties to even; a block
  * with an infinity or NaN has the scale NaN, and whatever takes it is NaN.  Weights [N][K] have one scale for each block of 128 x 128, scale
- * [ceil(N / 128)][ceil(K / 128)], any fp32 number (as checkpoints hold them, or from dis_k_quant_weight_f8); a fused gate-up weight [2][I][K]
+ * [ceil(N / 128)][ceil(K / 128)], any fp32 numbers, or the powers of two of dis_k_quant_weight_f8; a fused gate-up weight [2][I][K]
  * has the gate's blocks, then the up's: 2 ceil(I / 128) rows of scales.  Sums are fp32: a block's 128 products by the tensor cores, their sums times both
  * scales added by fp32 FMAs, right to fp32's rounding and 2^-101 a block; results do not change from call to call.  Two scales whose product is no fp32
  * number, though each is, cost time (their token's features are computed without the tensor cores), not the result.  K is a positive multiple of 16 (its
@@ -483,7 +484,8 @@ DIS_API int dis_k_add_rmsnorm_f8(float *x, const uint32_t *tokens, const uint16_
 /* out[t][n] = sum_k x[t][k] w[n][k]; out_dtype DIS_F32 or DIS_BF16 */
 DIS_API int dis_k_gemm_f8(const uint8_t *x8, const float *xs, const uint8_t *w8, const float *ws, void *out, int32_t out_dtype, int32_t T, int32_t N,
                           int32_t K, void *stream);
-/* The gate-up product of a feed-forward block, h = silu(x Wgate^T) (x Wup^T), itself turned into 8 bits: h8 [T][I], hs [ceil(I / 128)][T] */
+/* The gate-up product of a feed-forward block, h = silu(x Wgate^T) (x Wup^T), itself turned into 8 bits: h8 [T][I], hs [ceil(I / 128)][T].  A silu below
+ * 10^-36 (of gates below -87.3) counts as 0. */
 DIS_API int dis_k_gemm_silu_f8(const uint8_t *x8, const float *xs, const uint8_t *wgu8, const float *wgus, uint8_t *h8, float *hs, int32_t T, int32_t I,
                                int32_t K, void *stream);
 /* A whole feed-forward block in one call: x bf16 [T][H] into x8, xs; the gate-up product into h8, hs; out [T][H] = h Wdown^T, wd8 [H][I].  x8 [T][H], xs
