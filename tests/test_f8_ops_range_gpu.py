@@ -142,3 +142,39 @@ def test_what_is_no_number_stays_none(T, N, K):
     rest = ~lost
     rest[kind == 1, 128:256] = False
     assert torch.equal(out[rest], clean[rest])
+
+
+def test_wild_tokens_among_many_tiles():
+    """More than 256 tiles a CTA, which note what they have to look at again in 256 bits; captured, and replayed with other tokens."""
+    T, N, K = 40000, 32000, 16
+    g = gen(7)
+    x8, w8 = some(g, T, K), some(g, N, K)
+    xs = (torch.rand(1, T, generator=g, device=DEV) + 0.5) * 2.0 ** -60
+    ws = (torch.rand(blocks(N), 1, generator=g, device=DEV) + 0.5) * 2.0 ** 60
+    out = torch.empty(T, N, dtype=torch.bfloat16, device=DEV)
+    x, s = x8.clone(), xs.clone()
+
+    def call(stream):
+        check(lib().dis_k_gemm_f8(ptr(x), ptr(s), ptr(w8), ptr(ws), ptr(out), B.BF16, T, N, K, stream.cuda_stream))
+
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    call(st)
+    st.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        call(torch.cuda.current_stream())
+    for wild in ((5, T - 1), (), (0, 255, 256, 20001)):
+        x.copy_(x8)
+        s.copy_(xs)
+        out.fill_(float("nan"))
+        for t in wild:
+            x[t], s[0, t] = 0, 2.0 ** 100
+        graph.replay()
+        sync()
+        assert bool(out.isfinite().all())
+        for t in (0, 5, 128, 256, 20001, T - 1):
+            xv, wv = values(x[t:t + 1], s[:, t:t + 1], False), values(w8, ws, True)
+            want, bound = xv @ wv.T, off(xv, wv)
+            bound = bound + (want.abs() + bound) * 2.0 ** -8
+            assert bool(((out[t:t + 1].double() - want).abs() <= bound).all()), t
